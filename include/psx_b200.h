@@ -49,8 +49,10 @@ typedef enum psx_row_status {
                                 path holds; nothing was drawn for this row.  Only where the whole row is
                                 not at hand (the vocabulary-sharded merge): with the row on the GPU such a
                                 row is decided from the row itself */
-    PSX_ROW_DEVICE_TIMEOUT = 32 /* a bounded device-side wait (a bulk copy of a piece of the row into
+    PSX_ROW_DEVICE_TIMEOUT = 32, /* a bounded device-side wait (a bulk copy of a piece of the row into
                                 shared memory) ran out; nothing was drawn for this row */
+    PSX_ROW_CACHE_FULL = 64,  /* psx_b200_store_cache_8bit: the row's new positions do not fit; none was stored */
+    PSX_ROW_BAD_OFFSETS = 65  /* psx_b200_store_cache_8bit: the row's offsets or its filled length make no sense; nothing was stored */
 } psx_row_status;
 
 /* GenerationConfig (include/pulsatrix/generation.hpp:29-52) without the loop fields, plus the
@@ -76,6 +78,9 @@ typedef struct psx_row_diag {
     double draw_margin;   /* min |u - edge| over the two CDF edges of the chosen bucket */
     double top_p_margin;  /* min |cumulative - (1 - top_p)| seen by the top-p walk */
 } psx_row_diag;
+
+/* Element types of the entry points that take more than fp32. */
+typedef enum psx_dtype { PSX_FLOAT32 = 0, PSX_BFLOAT16 = 1, PSX_FLOAT16 = 2 } psx_dtype;
 
 typedef struct psx_ctx psx_ctx;
 
@@ -331,6 +336,85 @@ PSX_API psx_status psx_b200_decode_attention(psx_ctx* ctx, void* stream, const f
                                              const float* key_keep, float* context, int64_t batch, int64_t heads,
                                              int64_t kv_heads, int64_t q_len, int64_t head_dim, int64_t cached, int64_t max_len,
                                              float scale, int32_t causal, int64_t window, int32_t* status);
+
+/* Beam search's step over a whole batch (no counterpart in the reference, whose Generate() has no beams): of all
+ * (beam, token) pairs of a group of `beams` rows, the `keep` with the largest score + log-probability,
+ *     value(b, v) = (scores[b] - log sum_w exp(logits[b][w])) + logits[b][v]     in double precision,
+ * best first; of equal values the lowest beam's, then the lowest token's.  What offers nothing: logits of -inf (tokens that
+ * psx_b200_process_logits removed), beams whose score is -inf (before the first step all but the first), and the other tokens
+ * of a finished beam, which offers finished_token at its own score.  Places that no candidate is left for get -inf, -1, -1.
+ *   logits       device fp32, row g * beams + b at logits + row * row_stride (row_stride >= vocab)
+ *   scores       device fp32 (groups * beams): the beams' scores so far
+ *   finished     device bytes (groups * beams), non-zero: the beam has ended; may be NULL
+ *   out_scores   device fp32 (groups, keep), the values rounded once (below the lowest float: that)
+ *   parents      device int64 (groups, keep): the beam continued, 0 .. beams - 1, as psx_b200_reorder_states takes it
+ *   tokens       device int64 (groups, keep)
+ *   group_status device int32 (groups), may be NULL: PSX_ROW_OK; PSX_ROW_NON_FINITE: a NaN or +inf among the logits of a beam
+ *                that is alive and not finished, or among the scores (all places are -inf, -1, -1); PSX_ROW_ALL_REMOVED: nothing
+ *                is left at all
+ * keep may be larger than beams (twice as many leave enough when finished ones are set aside).  Limits: beams <= 64,
+ * keep <= 128, vocab <= 2^30 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; the outputs must not overlap the inputs.
+ * The context's scratch grows to groups * beams * (vocab / 2048) * (keep * 8 + 16) bytes at most; inside a stream capture it
+ * cannot grow (PSX_ERR_UNSUPPORTED): make a call of that size before. */
+PSX_API psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream, const float* logits, int64_t groups, int64_t beams, int64_t vocab,
+                                        int64_t row_stride, const float* scores, const uint8_t* finished, int64_t finished_token,
+                                        int64_t keep, float* out_scores, int64_t* parents, int64_t* tokens, int32_t* group_status);
+
+/* One state of every beam: (groups * beams, heads, positions) of position_bytes each, contiguous.  A cache of keys or values
+ * is (rows, kv_heads, max_len) of head_dim elements; a state without positions has heads = positions = 1.  tokens_per_position:
+ * how many tokens a position belongs to (1; a block's length for psx_cache_8bit's scales). */
+typedef struct psx_beam_state {
+    void* data;
+    int64_t heads, positions, position_bytes, tokens_per_position;
+} psx_beam_state;
+
+/* States that follow their beams, in place: row j of every group becomes what row parents[j] of the group was, in all of
+ * `count` states.  parents: device int64 (groups, beams), in any order and with repetitions; a row whose parent lies outside
+ * 0 .. beams - 1 stays as it is.  lengths: device int64 (groups * beams), tokens that each row holds before the call; the first
+ * ceil(lengths[parent] / tokens_per_position) positions are taken over and what lies behind them in the row is left as it was;
+ * NULL: all positions.  `states` is a host array, read during the call.  The states must overlap neither each other nor
+ * parents or lengths (PSX_ERR_BAD_ARGUMENT).  Limit: beams <= 64 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`. */
+PSX_API psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream, const psx_beam_state* states, int64_t count, int64_t groups,
+                                           int64_t beams, const int64_t* parents, const int64_t* lengths);
+
+/* A cache of keys and values in 8 bits: codes in e4m3 (1 sign, 4 exponent and 3 fraction bits, largest 448, no infinities),
+ * (batch, kv_heads, max_len, head_dim), and a scale for every `block` positions of a (row, kv head): (batch, kv_heads,
+ * ceil(max_len / block)) fp32.  An element's value is its code times its block's scale.  A quarter of the bytes of the fp32
+ * cache.  All device pointers, codes 16-byte aligned; block is 16, 32 or 64, head_dim a multiple of 16 up to 256, batch <= 4096
+ * (else PSX_ERR_UNSUPPORTED). */
+typedef struct psx_cache_8bit {
+    uint8_t* key_codes;
+    float* key_scales;
+    uint8_t* value_codes;
+    float* value_scales;
+    int64_t batch, kv_heads, max_len, head_dim, block;
+} psx_cache_8bit;
+
+/* Appends new positions to such a cache (KVCache::append, src/kv_cache.cpp, in 8 bits): prompts, or the one position of a
+ * decoding step.  keys, values: device, `dtype`, (total, kv_heads, head_dim) with the positions of all rows one row behind the
+ * other, a position at keys + i * key_stride elements (a slice of a wider projection will do; 16-byte aligned for fp32 and
+ * 8-byte for the others, strides multiples of four).  Row b's are offsets[b] .. offsets[b + 1] (device int64, batch + 1) and become
+ * positions cached[b] onwards (device int64, batch).
+ * A block's scale is the least power of two 2^e, e >= -100, at which 448 * 2^e reaches the largest finite magnitude of its new
+ * elements, or the scale that the block has where that is larger and the block holds cached positions; codes are
+ * value / scale rounded to the nearest, ties to even; infinities become the largest code, NaN stays NaN.  Where a partly filled
+ * block's scale grows, its codes are brought to the new one (exact but for codes that fall below 2^-6).  Nothing else is written.
+ * row_status: device int32 (batch), may be NULL: PSX_ROW_OK, PSX_ROW_CACHE_FULL or PSX_ROW_BAD_OFFSETS (such a row is left alone). */
+PSX_API psx_status psx_b200_store_cache_8bit(psx_ctx* ctx, void* stream, const psx_cache_8bit* cache, const void* keys, const void* values,
+                                             int32_t dtype, int64_t total, int64_t key_stride, int64_t value_stride, const int64_t* offsets,
+                                             const int64_t* cached, int32_t* row_status);
+
+/* psx_b200_decode_attention over a cache in 8 bits, for rows of different lengths: q and context are `dtype` (batch, heads,
+ * q_len, head_dim), contiguous, 16-byte aligned; row b sees positions 0 .. lengths[b] - 1 (device int64; outside 0 .. max_len:
+ * the nearer end), its q_len new positions being the last of them (already stored).  New position i is position
+ * p = lengths[b] - q_len + i: with `causal` it sees no key j > p and, with window > 0, no key j + window <= p.  A query that sees
+ * nothing has the context 0.  Positions that no query of a row sees are not read.  Softmax statistics and sums are floats; codes
+ * are exact in the products, queries and weights carry 11 bits (bf16, fp16) or 22 (fp32).
+ * Limits: (heads / kv_heads) * q_len <= 16, <= 8 where head_dim > 128 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; scratch
+ * in a stream capture as psx_b200_beam_select. */
+PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, const void* q, int32_t dtype, const psx_cache_8bit* cache,
+                                                  const int64_t* lengths, void* context, int64_t heads, int64_t q_len, float scale,
+                                                  int32_t causal, int64_t window);
 
 /* Replace DeviceBackend::softmax_rows, logsumexp_rows and gather_rows
  * (include/pulsatrix/device_backend.hpp:456,465,596; CUDA implementations src/cuda_backend.cu with

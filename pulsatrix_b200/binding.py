@@ -9,7 +9,7 @@ from pathlib import Path
 import numpy as np
 
 PACKAGE = Path(__file__).resolve().parent
-ROW_OK, ROW_NON_FINITE, ROW_ALL_REMOVED, ROW_TOO_WIDE, ROW_DEVICE_TIMEOUT = 0, 4, 5, 16, 32
+ROW_OK, ROW_NON_FINITE, ROW_ALL_REMOVED, ROW_TOO_WIDE, ROW_DEVICE_TIMEOUT, ROW_CACHE_FULL, ROW_BAD_OFFSETS = 0, 4, 5, 16, 32, 64, 65
 OK, ERR_BAD_ARGUMENT, ERR_CUDA, ERR_ROW_FAILED, ERR_UNSUPPORTED = range(5)
 
 EXPORTS = [
@@ -20,6 +20,7 @@ EXPORTS = [
     "psx_b200_exchange_handle_bytes", "psx_b200_exchange_create", "psx_b200_exchange_open", "psx_b200_exchange_destroy",
     "psx_b200_exchange_sample", "psx_b200_exchange_results", "psx_b200_exchange_test_wait",
     "psx_b200_top_k_rows", "psx_b200_lm_head_logits", "psx_b200_lm_head_sample_rows", "psx_b200_softmax_rows", "psx_b200_logsumexp_rows", "psx_b200_gather_rows", "psx_b200_decode_attention",
+    "psx_b200_beam_select", "psx_b200_reorder_states", "psx_b200_store_cache_8bit", "psx_b200_decode_attention_8bit",
     "psx_uniforms_mt19937_64", "psx_uniforms_portable",
 ]
 
@@ -68,6 +69,21 @@ class RowDiag(C.Structure):
 
 ROW_DIAG_DTYPE = np.dtype({"names": ["candidates", "survivors", "draw_margin", "top_p_margin"],
                            "formats": ["<i4", "<i4", "<f8", "<f8"], "itemsize": C.sizeof(RowDiag)})
+
+
+class BeamState(C.Structure):
+    """psx_beam_state."""
+
+    _fields_ = [("data", C.c_void_p), ("heads", C.c_int64), ("positions", C.c_int64), ("position_bytes", C.c_int64),
+                ("tokens_per_position", C.c_int64)]
+
+
+class Cache8bitLayout(C.Structure):
+    """psx_cache_8bit."""
+
+    _fields_ = [("key_codes", C.c_void_p), ("key_scales", C.c_void_p), ("value_codes", C.c_void_p), ("value_scales", C.c_void_p),
+                ("batch", C.c_int64), ("kv_heads", C.c_int64), ("max_len", C.c_int64), ("head_dim", C.c_int64), ("block", C.c_int64)]
+
 
 _lib = None
 _native = None  # the per-step calls without ctypes (host/python_calls.cpp); bound to the same library
@@ -134,6 +150,10 @@ def library():
         lib.psx_b200_gather_rows.argtypes = [ptr, ptr, ptr, ptr, ptr, C.c_size_t, C.c_size_t]
         lib.psx_b200_decode_attention.argtypes = [ptr, ptr, ptr, ptr, ptr, ptr, ptr, i64, i64, i64, i64, i64, i64, i64, C.c_float, C.c_int32,
                                                   i64, ptr]
+        lib.psx_b200_beam_select.argtypes = [ptr, ptr, ptr, i64, i64, i64, i64, ptr, ptr, i64, i64, ptr, ptr, ptr, ptr]
+        lib.psx_b200_reorder_states.argtypes = [ptr, ptr, ptr, i64, i64, i64, ptr, ptr]
+        lib.psx_b200_store_cache_8bit.argtypes = [ptr, ptr, ptr, ptr, ptr, C.c_int32, i64, i64, i64, ptr, ptr, ptr]
+        lib.psx_b200_decode_attention_8bit.argtypes = [ptr, ptr, ptr, C.c_int32, ptr, ptr, ptr, i64, i64, C.c_float, C.c_int32, i64]
         lib.psx_uniforms_mt19937_64.argtypes = [ptr, i64, ptr]
         lib.psx_uniforms_portable.argtypes = [ptr, i64, ptr]
         from . import _native as native
@@ -220,6 +240,55 @@ def sample_rows_static(logits, history_ids, history_offsets, config, uniforms, t
         _ptr(history_ids), _ptr(history_offsets), C.addressof(config), _ptr(uniforms), _ptr(tokens), _ptr(log_probs), _ptr(status))
     if status_code:
         _check(status_code)
+
+
+def _dtype_code(tensor):
+    """The psx_dtype of a tensor."""
+    import torch
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(tensor.dtype)
+    if code is None:
+        raise TypeError(f"float32, bfloat16 or float16 is expected, got {tensor.dtype}")
+    return code
+
+
+def _need(condition, message):
+    if not condition:
+        raise ValueError(message)
+
+
+class Cache8bit:
+    """A cache of keys and values in 8 bits (psx_cache_8bit) over tensors of the caller's: codes (batch, kv_heads, max_len,
+    head_dim), torch.float8_e4m3fn or uint8, and float32 scales (batch, kv_heads, ceil(max_len / block)), all contiguous."""
+
+    def __init__(self, key_codes, key_scales, value_codes, value_scales, block=32):
+        import torch
+        _need(key_codes.dim() == 4 and block > 0, "codes are (batch, kv_heads, max_len, head_dim)")
+        batch, kv_heads, max_len, head_dim = key_codes.shape
+        for codes in (key_codes, value_codes):
+            _need(codes.shape == key_codes.shape and codes.is_contiguous() and codes.dtype in (torch.float8_e4m3fn, torch.uint8),
+                  "codes are contiguous float8_e4m3fn or uint8 tensors of one shape")
+        for scales in (key_scales, value_scales):
+            _need(tuple(scales.shape) == (batch, kv_heads, -(-max_len // block)) and scales.is_contiguous() and scales.dtype == torch.float32,
+                  "scales are contiguous float32 tensors, one for every `block` positions")
+        _need(len({t.get_device() for t in (key_codes, key_scales, value_codes, value_scales)}) == 1, "a cache lies on one device")
+        self.key_codes, self.key_scales, self.value_codes, self.value_scales = key_codes, key_scales, value_codes, value_scales
+        self.batch, self.kv_heads, self.max_len, self.head_dim, self.block = batch, kv_heads, max_len, head_dim, block
+        self.device = key_codes.get_device()
+        self._layout = Cache8bitLayout(key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(), value_scales.data_ptr(), batch,
+                                       kv_heads, max_len, head_dim, block)
+        self._address = C.addressof(self._layout)
+
+    @classmethod
+    def empty(cls, batch, kv_heads, max_len, head_dim, block=32, device="cuda"):
+        """One with nothing in it yet."""
+        import torch
+        codes = [torch.zeros((batch, kv_heads, max_len, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+        scales = [torch.zeros((batch, kv_heads, -(-max_len // block)), dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(codes[0], scales[0], codes[1], scales[1], block)
+
+    def states(self):
+        """Its tensors as Context.reorder_states takes them."""
+        return [(self.key_codes, 1), (self.key_scales, self.block), (self.value_codes, 1), (self.value_scales, self.block)]
 
 
 class Context:
@@ -465,6 +534,98 @@ class Context:
                                         values.data_ptr(), _ptr(key_keep), context.data_ptr(), batch, heads, kv_heads, q_len, head_dim,
                                         cached, max_len, float(scale), int(bool(causal)), window, status.data_ptr()))
         return context, status
+
+    # ---- beams, states that follow them, the cache in 8 bits ---------------------------------------------
+    def _here(self, *tensors):
+        for t in tensors:
+            if t is not None and t.get_device() != self.device:
+                raise ValueError(f"tensors on cuda:{self.device} are expected, got one on {t.device}")
+
+    def beam_select(self, logits, scores, beams, keep, finished=None, finished_token=0, vocab=None, stream=None):
+        """Beam search's selection (psx_b200_beam_select).  logits: cuda float32 (groups * beams, vocab), rows contiguous; scores:
+        float32 (groups * beams); finished: bool or uint8 (groups * beams) or None.  Returns {"scores", "parents", "tokens"} of
+        shape (groups, keep) and "status" (groups)."""
+        import torch
+        rows = logits.shape[0]
+        vocab = logits.shape[1] if vocab is None else vocab
+        _need(beams > 0 and rows % beams == 0, "logits hold `beams` rows per group")
+        _need(logits.dtype == torch.float32 and scores.dtype == torch.float32, "logits and scores are float32")
+        _need(0 < vocab <= logits.shape[1] and (rows == 0 or logits.stride(1) == 1), "a row's logits are contiguous")
+        _need(scores.numel() == rows and scores.is_contiguous(), "one score per row")
+        if finished is not None:
+            _need(finished.numel() == rows and finished.is_contiguous() and finished.element_size() == 1, "one byte per row says what is finished")
+        self._here(logits, scores, finished)
+        groups = rows // beams
+        stream = _stream_of(logits) if stream is None else stream
+        shape, device = (groups, max(keep, 0)), logits.device
+        out = {"scores": torch.empty(shape, dtype=torch.float32, device=device), "parents": torch.empty(shape, dtype=torch.int64, device=device),
+               "tokens": torch.empty(shape, dtype=torch.int64, device=device), "status": torch.empty(groups, dtype=torch.int32, device=device)}
+        _check(_native.beam_select(self._handle, stream, logits.data_ptr(), groups, beams, vocab, logits.stride(0) if rows > 1 else logits.shape[1],
+                                   scores.data_ptr(), _ptr(finished), finished_token, keep, out["scores"].data_ptr(), out["parents"].data_ptr(),
+                                   out["tokens"].data_ptr(), out["status"].data_ptr()))
+        return out
+
+    def reorder_states(self, parents, states, lengths=None, stream=None):
+        """Rows of states that follow their beams, in place (psx_b200_reorder_states).  parents: int64 (groups, beams), row
+        numbers within the group; states: tensors (groups * beams, heads, positions, ...), contiguous, each alone or as (tensor,
+        tokens per position); lengths: int64 (groups * beams), the tokens that each row holds before, or None for all positions."""
+        import torch
+        _need(parents.dim() == 2 and parents.dtype == torch.int64 and parents.is_contiguous(), "parents are contiguous int64 (groups, beams)")
+        groups, beams = parents.shape
+        described = (BeamState * len(states))()
+        for entry, state in zip(described, states):
+            tensor, per = state if isinstance(state, (tuple, list)) else (state, 1)
+            _need(tensor.dim() >= 3 and tensor.shape[0] == groups * beams and tensor.is_contiguous(),
+                  "a state is a contiguous (groups * beams, heads, positions, ...) tensor")
+            self._here(tensor)
+            size = tensor.element_size()
+            for n in tensor.shape[3:]:
+                size *= n
+            if size == 0:  # (nothing to move)
+                entry.data, entry.heads, entry.positions, entry.position_bytes, entry.tokens_per_position = None, 0, 0, 1, 1
+                continue
+            entry.data, entry.heads, entry.positions = tensor.data_ptr(), tensor.shape[1], tensor.shape[2]
+            entry.position_bytes, entry.tokens_per_position = size, per
+        if lengths is not None:
+            _need(lengths.dtype == torch.int64 and lengths.numel() == groups * beams and lengths.is_contiguous(), "one int64 length per row")
+        self._here(parents, lengths)
+        _check(_native.reorder_states(self._handle, _stream_of(parents) if stream is None else stream, C.addressof(described), len(states), groups,
+                                      beams, parents.data_ptr(), _ptr(lengths)))
+
+    def store_cache_8bit(self, cache, keys, values, offsets, cached, stream=None):
+        """Appends new positions to a Cache8bit (psx_b200_store_cache_8bit).  keys, values: float32, bfloat16 or float16 (total,
+        kv_heads, head_dim), the rows' new positions one row behind the other, heads and dimensions contiguous; offsets: int64
+        (batch + 1); cached: int64 (batch), the positions held before.  Returns the rows' statuses, int32 (batch)."""
+        import torch
+        _need(keys.dim() == 3 and keys.shape == values.shape and keys.dtype == values.dtype and tuple(keys.shape[1:]) == (cache.kv_heads, cache.head_dim),
+              "keys and values are (total, kv_heads, head_dim) of one type")
+        for t in (keys, values):
+            _need(t.shape[0] == 0 or (t.stride(2) == 1 and t.stride(1) == cache.head_dim), "heads and dimensions of a position are contiguous")
+        _need(offsets.dtype == torch.int64 and offsets.numel() == cache.batch + 1 and offsets.is_contiguous(), "offsets are int64 (batch + 1)")
+        _need(cached.dtype == torch.int64 and cached.numel() == cache.batch and cached.is_contiguous(), "cached is int64 (batch)")
+        self._here(cache.key_codes, keys, values, offsets, cached)
+        total, width = keys.shape[0], cache.kv_heads * cache.head_dim
+        status = torch.empty(cache.batch, dtype=torch.int32, device=offsets.device)
+        _check(_native.store_cache_8bit(self._handle, _stream_of(keys) if stream is None else stream, cache._address, keys.data_ptr(), values.data_ptr(),
+                                        _dtype_code(keys), total, keys.stride(0) if total > 1 else width, values.stride(0) if total > 1 else width,
+                                        offsets.data_ptr(), cached.data_ptr(), status.data_ptr()))
+        return status
+
+    def decode_attention_8bit(self, q, cache, lengths, scale=None, causal=True, window=0, stream=None):
+        """Attention of the new positions over a Cache8bit (psx_b200_decode_attention_8bit).  q: float32, bfloat16 or float16
+        (batch, heads, q_len, head_dim); lengths: int64 (batch), the positions that each row sees, the new ones among them.
+        Returns the context, like q."""
+        import torch
+        batch, heads, q_len, head_dim = q.shape
+        _need(batch == cache.batch and head_dim == cache.head_dim and q.is_contiguous(), "q is a contiguous (batch, heads, q_len, head_dim) as the cache")
+        _need(lengths.dtype == torch.int64 and lengths.numel() == batch and lengths.is_contiguous(), "lengths are int64 (batch)")
+        self._here(q, cache.key_codes, lengths)
+        if scale is None:
+            scale = 1.0 / float(np.sqrt(np.float32(head_dim)))
+        context = torch.empty_like(q)
+        _check(_native.decode_attention_8bit(self._handle, _stream_of(q) if stream is None else stream, q.data_ptr(), _dtype_code(q), cache._address,
+                                             lengths.data_ptr(), context.data_ptr(), heads, q_len, float(scale), int(bool(causal)), window))
+        return context
 
     # ---- vocabulary-sharded -----------------------------------------------------------------------------
     def shard_record_bytes(self, config) -> int:

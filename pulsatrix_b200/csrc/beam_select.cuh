@@ -1,0 +1,45 @@
+// Launch interface of the selection over beams and vocabulary (beam_select.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace psx {
+
+constexpr int kMostKept = 128;         // candidates per group
+constexpr int kMostSelectBeams = 64;
+
+struct BeamPart {        // what the first kernel leaves of a part of a row
+    double sum;          // of exp(logit - top) over the part
+    float top;           // the part's largest logit; -inf: none
+    int32_t not_finite;  // it holds a NaN or +inf
+};
+
+struct BeamEntry {
+    float logit;
+    int32_t token;
+};
+
+struct BeamSelectParams {
+    const float* logits;      // (groups * beams, vocab), row r at logits + r * row_stride
+    const float* scores;      // (groups * beams): the beams' scores so far
+    const uint8_t* finished;  // (groups * beams) or null
+    float* out_scores;        // (groups, keep)
+    int64_t* parents;         // (groups, keep): the beam that a candidate continues, 0 .. beams - 1
+    int64_t* tokens;          // (groups, keep)
+    int32_t* group_status;    // (groups) or null
+    int64_t groups, row_stride, finished_token;
+    int32_t beams, vocab, keep;
+    int32_t parts;            // of a row
+    int32_t values;           // logits per thread of a part's block: 8 or 32
+    int32_t aligned;          // every row starts on a 16-byte boundary and is a multiple of four long
+    BeamPart* part_stats;     // (groups * beams, parts)
+    BeamEntry* entries;       // (groups * beams, parts, keep), best first
+};
+
+// parts, values and aligned, from the sizes and pointers.
+void plan_beam_select(BeamSelectParams& p, int sm_count);
+cudaError_t launch_beam_select(const BeamSelectParams& p, cudaStream_t stream);
+
+}  // namespace psx

@@ -11,15 +11,21 @@
 #include <string>
 #include <vector>
 
+#include "beam_select.cuh"
+#include "decode_attention_8bit.cuh"
+#include "elements.cuh"
 #include "lm_head.cuh"
 #include "merge_rows.cuh"
 #include "peer_exchange.cuh"
 #include "decode_attention.cuh"
 #include "process_rows.cuh"
+#include "reorder_states.cuh"
+#include "row_prefix.cuh"
 #include "row_ops.cuh"
 #include "sample_plan.cuh"
 #include "scan_rows.cuh"
 #include "shard_records.cuh"
+#include "store_cache_8bit.cuh"
 #include "topk_rows.cuh"
 #include "whole_rows.cuh"
 
@@ -83,6 +89,9 @@ struct psx_ctx {
     cudaEvent_t ring_done[kRingSlots] = {};  // the copy out of (or into) a slot has finished
     // staging of the sharded path
     Buffer shard_uniform_scratch;
+    // Scratch that captured graphs may hold: what it outgrows stays allocated until the context goes (see reserve_kept).
+    Buffer beam_scratch, attention_8bit_pieces, attention_8bit_arrived;
+    std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
     bool timing = false;
     std::vector<cudaEvent_t> timing_events;
@@ -103,6 +112,40 @@ psx_status reserve(Buffer& b, size_t bytes) {
     b.bytes = want;
     return PSX_OK;
 }
+
+// The same for scratch whose address a captured graph may replay: what is outgrown is kept (each is a quarter larger than what
+// asked for it, at least), and inside a capture nothing is allocated.  `grown`: whether the memory is new.
+psx_status reserve_kept(psx_ctx* ctx, cudaStream_t stream, Buffer& b, size_t bytes, bool* grown = nullptr) {
+    if (grown) *grown = false;
+    if (bytes <= b.bytes) return PSX_OK;
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    PSX_CUDA(cudaStreamIsCapturing(stream, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone) {
+        return fail(PSX_ERR_UNSUPPORTED, "psx_b200: the context's scratch cannot grow inside a stream capture: make a call of this size before");
+    }
+    const size_t want = std::max(bytes + bytes / 4 + 256, 2 * b.bytes);
+    void* ptr = nullptr;
+    PSX_CUDA(cudaMalloc(&ptr, want));
+    if (b.ptr) ctx->outgrown.push_back(b.ptr);
+    b.ptr = ptr;
+    b.bytes = want;
+    if (grown) *grown = true;
+    return PSX_OK;
+}
+
+// The context's device for the length of a call.
+struct OnDevice {
+    int before = -1;
+    cudaError_t error;
+    explicit OnDevice(int device) {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != device) error = cudaSetDevice(device);
+        else if (error == cudaSuccess) before = -1;  // (nothing to put back)
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
 
 // A host entry point from its first copy on.  The staged inputs are being copied in by transfers just enqueued, so no promise about
 // inputs holds meanwhile; and however the call ends, nothing is in flight in the staging memory afterwards.
@@ -379,9 +422,10 @@ void psx_b200_ctx_destroy(psx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Buffer* b : {&ctx->stats[0], &ctx->stats[1], &ctx->part_counts[0], &ctx->part_counts[1], &ctx->candidates[0], &ctx->candidates[1], &ctx->banned, &ctx->sort_keys, &ctx->head_logits, &ctx->attention_partial, &ctx->surv_cols, &ctx->surv_vals,
                       &ctx->surv_counts, &ctx->pl_tokens, &ctx->pl_log_probs, &ctx->pl_status, &ctx->h_logits, &ctx->h_inputs,
-                      &ctx->h_results, &ctx->shard_uniform_scratch}) {
+                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived}) {
         if (b->ptr) cudaFree(b->ptr);
     }
+    for (void* p : ctx->outgrown) cudaFree(p);
     for (Buffer* b : {&ctx->pinned_inputs, &ctx->pinned_results, &ctx->pinned_ring}) {
         if (b->ptr) cudaFreeHost(b->ptr);
     }
@@ -1095,6 +1139,185 @@ psx_status psx_b200_decode_attention(psx_ctx* ctx, void* stream_ptr, const float
     }
     PSX_CUDA(psx::launch_decode_attention(p, stream));
     ctx->launches += p.splits > 1 ? 2 : 1;
+    return PSX_OK;
+}
+
+// ---- beams, states that follow them, the cache in 8 bits -----------------------------------------------------------------
+
+psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream_ptr, const float* logits, int64_t groups, int64_t beams, int64_t vocab,
+                                int64_t row_stride, const float* scores, const uint8_t* finished, int64_t finished_token, int64_t keep,
+                                float* out_scores, int64_t* parents, int64_t* tokens, int32_t* group_status) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    if (groups < 0 || beams <= 0 || vocab <= 0 || keep <= 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: beam sizes must be positive");
+    if (row_stride < vocab) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: row_stride is smaller than the vocabulary");
+    if (finished && (finished_token < 0 || finished_token >= vocab)) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: finished_token is not in the vocabulary");
+    }
+    if (groups == 0) return PSX_OK;
+    if (!logits || !scores || !out_scores || !parents || !tokens) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (beams > psx::kMostSelectBeams || keep > psx::kMostKept || vocab > (int64_t(1) << 30) || groups > 0x7fffffff / beams) {
+        return fail(PSX_ERR_UNSUPPORTED, "psx_b200: beam selection takes at most 64 beams, 128 candidates per group and 2^30 tokens");
+    }
+    psx::BeamSelectParams p{};
+    p.logits = logits; p.scores = scores; p.finished = finished; p.out_scores = out_scores; p.parents = parents; p.tokens = tokens;
+    p.group_status = group_status; p.groups = groups; p.row_stride = row_stride; p.finished_token = finished_token;
+    p.beams = (int32_t)beams; p.vocab = (int32_t)vocab; p.keep = (int32_t)keep;
+    psx::plan_beam_select(p, ctx->sm_count);
+    const int64_t lists = groups * beams * p.parts;
+    if (lists > 0x7fffffff || beams * p.parts * keep > 0x7fffffff) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    const size_t stats_bytes = (size_t)lists * sizeof(psx::BeamPart);
+    if (psx_status s = reserve_kept(ctx, stream, ctx->beam_scratch, stats_bytes + (size_t)(lists * keep) * sizeof(psx::BeamEntry))) return s;
+    p.part_stats = static_cast<psx::BeamPart*>(ctx->beam_scratch.ptr);
+    p.entries = reinterpret_cast<psx::BeamEntry*>(static_cast<char*>(ctx->beam_scratch.ptr) + stats_bytes);
+    PSX_CUDA(psx::launch_beam_select(p, stream));
+    ctx->launches += 2;
+    return PSX_OK;
+}
+
+psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream_ptr, const psx_beam_state* states, int64_t count, int64_t groups,
+                                   int64_t beams, const int64_t* parents, const int64_t* lengths) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    if (count < 0 || groups < 0 || beams <= 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: beam sizes must be positive");
+    if (count == 0 || groups == 0) return PSX_OK;
+    if (!states || !parents) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (beams > psx::kMostBeams) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: states follow at most 64 beams");
+    if (groups > 0x7fffffff / beams) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
+    // The bytes that the call touches, none of them twice.
+    std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+    for (int64_t i = 0; i < count; ++i) {
+        const psx_beam_state& s = states[i];
+        if (s.heads < 0 || s.positions < 0 || s.position_bytes <= 0 || s.tokens_per_position <= 0) {
+            return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: state sizes must be positive");
+        }
+        const __int128 bytes = (__int128)groups * beams * s.heads * s.positions * s.position_bytes;
+        if (s.heads > 0x7fffffff || s.positions > ((int64_t)1 << 40) || s.position_bytes > ((int64_t)1 << 40) || bytes > ((__int128)1 << 48)) {
+            return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a state is larger than any memory");
+        }
+        if (bytes == 0) continue;
+        if (!s.data) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+        const uintptr_t at = reinterpret_cast<uintptr_t>(s.data);
+        ranges.emplace_back(at, at + (uintptr_t)bytes);
+    }
+    const size_t rows_bytes = (size_t)(groups * beams) * sizeof(int64_t);
+    ranges.emplace_back(reinterpret_cast<uintptr_t>(parents), reinterpret_cast<uintptr_t>(parents) + rows_bytes);
+    if (lengths) ranges.emplace_back(reinterpret_cast<uintptr_t>(lengths), reinterpret_cast<uintptr_t>(lengths) + rows_bytes);
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i) {
+        if (ranges[i].first < ranges[i - 1].second) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: states overlap each other, parents or lengths");
+    }
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    psx::ReorderParams p{};
+    p.beams = (int32_t)beams; p.groups = groups; p.parents = parents; p.lengths = lengths;
+    for (int64_t i = 0; i < count; ++i) {
+        const psx_beam_state& s = states[i];
+        if (s.heads > 0 && s.positions > 0) {
+            p.states[p.count++] = {static_cast<char*>(s.data), s.heads, s.positions, s.position_bytes, s.tokens_per_position, 0, 0, 0};
+        }
+        if (p.count == psx::kStatesPerLaunch || (i + 1 == count && p.count > 0)) {
+            const cudaError_t e = psx::launch_reorder_states(p, ctx->sm_count, static_cast<cudaStream_t>(stream_ptr));
+            if (e == cudaErrorInvalidValue) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many heads of states for one call");
+            PSX_CUDA(e);
+            ctx->launches += 1;
+            p.count = 0;
+        }
+    }
+    return PSX_OK;
+}
+
+namespace {
+psx_status check_cache_8bit(const psx_cache_8bit* c, psx::Cache8bitView* view) {
+    if (!c) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (c->batch < 0 || c->kv_heads <= 0 || c->max_len <= 0 || c->head_dim <= 0 || c->block <= 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: cache sizes must be positive");
+    }
+    if ((c->block != 16 && c->block != 32 && c->block != 64) || c->head_dim % 16 != 0 || c->head_dim > 256 || c->batch > psx::kMostPrefixRows ||
+        c->kv_heads > 65536 || c->max_len > ((int64_t)1 << 36) || std::max<int64_t>(c->batch, 1) * c->kv_heads > 0x7fffffff / (c->max_len / 16 + 1)) {
+        return fail(PSX_ERR_UNSUPPORTED,
+                    "psx_b200: a cache in 8 bits has blocks of 16, 32 or 64 positions, a head dimension that is a multiple of 16 up to 256, "
+                    "at most 4096 rows and 2^31 blocks of 16 positions");
+    }
+    if (c->batch > 0 && (!c->key_codes || !c->key_scales || !c->value_codes || !c->value_scales)) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    }
+    if ((reinterpret_cast<uintptr_t>(c->key_codes) | reinterpret_cast<uintptr_t>(c->value_codes)) % 16 != 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the cache must start on a 16-byte boundary");
+    }
+    *view = {c->key_codes, c->key_scales, c->value_codes, c->value_scales, c->batch, c->max_len, (c->max_len + c->block - 1) / c->block,
+             (int32_t)c->kv_heads, (int32_t)c->head_dim, (int32_t)c->block};
+    return PSX_OK;
+}
+}  // namespace
+
+psx_status psx_b200_store_cache_8bit(psx_ctx* ctx, void* stream_ptr, const psx_cache_8bit* cache, const void* keys, const void* values,
+                                     int32_t dtype, int64_t total, int64_t key_stride, int64_t value_stride, const int64_t* offsets,
+                                     const int64_t* cached, int32_t* row_status) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    psx::StoreCacheParams p{};
+    if (psx_status s = check_cache_8bit(cache, &p.cache)) return s;
+    if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
+    if (total < 0 || total > 0x7fffffff) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the number of new positions is out of range");
+    if (p.cache.batch == 0) return PSX_OK;
+    if (!offsets || !cached || (total > 0 && (!keys || !values))) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    const int64_t width = cache->kv_heads * cache->head_dim;
+    if (key_stride < width || value_stride < width || key_stride % 4 != 0 || value_stride % 4 != 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a position's stride is at least kv_heads * head_dim and a multiple of four");
+    }
+    if ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % (4 * psx::element_bytes(dtype)) != 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: keys and values must start on a boundary of four elements");
+    }
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    p.keys = keys; p.values = values; p.offsets = offsets; p.cached = cached; p.row_status = row_status; p.total = total;
+    p.key_stride = key_stride; p.value_stride = value_stride; p.type = dtype;
+    PSX_CUDA(psx::launch_store_cache_8bit(p, ctx->sm_count, static_cast<cudaStream_t>(stream_ptr)));
+    ctx->launches += 1;
+    return PSX_OK;
+}
+
+psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const void* q, int32_t dtype, const psx_cache_8bit* cache,
+                                          const int64_t* lengths, void* context, int64_t heads, int64_t q_len, float scale, int32_t causal,
+                                          int64_t window) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    psx::Attention8bitParams p{};
+    if (psx_status s = check_cache_8bit(cache, &p.cache)) return s;
+    if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
+    if (heads <= 0 || q_len <= 0 || window < 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: attention sizes must be positive");
+    if (heads % cache->kv_heads != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: heads must be a multiple of kv_heads");
+    const int64_t group = heads / cache->kv_heads, most = cache->head_dim > 128 ? 8 : 16;
+    if (group > most || q_len > most || group * q_len > most) {
+        return fail(PSX_ERR_UNSUPPORTED,
+                    "psx_b200: attention over the cache in 8 bits takes at most 16 query rows per kv head (group x new positions), 8 beyond a "
+                    "head dimension of 128");
+    }
+    if (p.cache.batch == 0) return PSX_OK;
+    if (!q || !lengths || !context) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(context) % 16 != 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: queries and context must start on a 16-byte boundary");
+    }
+    p.q = q; p.context = context; p.lengths = lengths; p.heads = (int32_t)heads; p.group = (int32_t)group; p.q_len = (int32_t)q_len;
+    p.rows = (int32_t)(group * q_len); p.type = dtype; p.causal = causal ? 1 : 0; p.scale = scale;
+    p.window = std::min(window, cache->max_len);  // (a wider one hides nothing more, and sums with it stay in range)
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    p.grid = psx::attention_8bit_grid(p, ctx->sm_count);
+    bool grown;
+    const size_t counters = (size_t)(cache->batch * cache->kv_heads) * sizeof(int32_t);
+    if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;
+    if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_arrived, counters, &grown)) return s;
+    if (grown) {
+        const cudaError_t e = cudaMemsetAsync(ctx->attention_8bit_arrived.ptr, 0, ctx->attention_8bit_arrived.bytes, stream);
+        if (e != cudaSuccess) ctx->attention_8bit_arrived.bytes = 0;  // (counters that are not zero are not used)
+        PSX_CUDA(e);
+    }
+    p.partial = static_cast<float*>(ctx->attention_8bit_pieces.ptr);
+    p.arrived = static_cast<int32_t*>(ctx->attention_8bit_arrived.ptr);
+    PSX_CUDA(psx::launch_decode_attention_8bit(p, stream));
+    ctx->launches += 1;
     return PSX_OK;
 }
 

@@ -1,0 +1,508 @@
+// Attention of the new positions over a cache held in 8 bits, in one pass over the cache.
+//
+// For a query row q and cached position j with codes k_j, v_j and block scales a_j, b_j:
+//     s_j = scale * a_j * (q . k_j),   context = sum_j exp(s_j) b_j v_j / sum_j exp(s_j)   over the positions that the row sees.
+//
+// Codes become halves exactly, so both products run as half matrix instructions (m16n8k16, float accumulators) in the
+// transposed form: 16 positions by 8 query rows, then 16 dimensions by 8 query rows.  The query rows of a kv head (group x
+// new positions, up to 16) are the narrow side, which wastes nothing at 8 rows; the codes are converted once for all of them.
+// A query row is brought to a power of two near 1 and rounded to halves (bf16 and fp16 queries lose nothing but bits below 2^-24 of
+// their largest element); an fp32 row is a half and the half that is left, two instructions each, some 22 bits.  Weights:
+// the running maximum M is taken over s_j + log2(b_j), so that w_j = exp(s_j - M) b_j is at most 1 whatever the scales; it is
+// rounded to halves (2^-11, below the rounding of a bf16 or fp16 context; for fp32 contexts again two halves).  Maxima, sums
+// and contexts are floats.
+//
+// The cached positions of all (row, kv head) pairs lie on one axis, in tiles of 32, and every block takes an equal share of it:
+// lengths that differ from row to row leave no SM idle, and one long row is spread over all of them.  A pair that several
+// blocks share leaves a piece per block; the last block to arrive joins them, in order.  Inside a block each of four warps
+// takes every fourth tile, with its own three stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no
+// warp waits for another until the end of a pair.  Bound by HBM: 2 bytes per position, head dimension and kv head.
+#include "decode_attention_8bit.cuh"
+
+#include <algorithm>
+
+#include "elements.cuh"
+#include "once_per_device.hpp"
+#include "row_prefix.cuh"
+
+namespace psx {
+namespace {
+
+constexpr int kThreads = 128, kWarps = 4, kTile = 32;
+constexpr int kLeastShare = 2 * kWarps;  // tiles: shorter pieces cost more in joining than they gain (see the launch)
+constexpr float kNone = -__builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+
+__host__ __device__ constexpr int stages_of(int dims) { return dims > 128 ? 2 : 3; }
+__host__ __device__ constexpr int stage_bytes(int dims) { return 2 * kTile * dims + 16; }  // keys, values, two scales each
+__host__ __device__ constexpr size_t shared_of(int dims) { return (size_t)kWarps * stages_of(dims) * stage_bytes(dims); }
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+template <int pending>
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(pending) : "memory"); }
+
+__device__ __forceinline__ void multiply(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t halves(float low, float high) {
+    const __half2 h = __floats2half2_rn(low, high);
+    uint32_t r;
+    __builtin_memcpy(&r, &h, 4);
+    return r;
+}
+// What the halves leave of the two floats, as halves.
+__device__ __forceinline__ uint32_t halves_left(float low, float high, uint32_t taken) {
+    __half2 h;
+    __builtin_memcpy(&h, &taken, 4);
+    const float2 t = __half22float2(h);
+    return halves(low - t.x, high - t.y);
+}
+
+// Chunk (16 codes) `chunk` of row `row` of a stage lies at this chunk of the row: eight rows' chunks of one column lie in
+// different banks, and so do four neighbouring chunks of two neighbouring rows.
+template <int dims>
+__device__ __forceinline__ int placed(int row, int chunk) {
+    if constexpr (dims == 64) return chunk ^ ((row >> 1) & 3);
+    else return chunk ^ (((row & 1) << 2) | ((row >> 1) & 3));
+}
+
+// Bounds of what query rows see, in positions.
+struct Sight {
+    int64_t length, first_own;  // the position of the first new one
+    int64_t window;
+    bool causal;
+    __device__ __forceinline__ int64_t last(int i) const { return causal ? first_own + i : length - 1; }
+    __device__ __forceinline__ int64_t first(int i) const { return causal && window > 0 ? first_own + i - window + 1 : 0; }
+    __device__ __forceinline__ int64_t first_tile() const { return max(first(0), (int64_t)0) / kTile; }
+    __device__ __forceinline__ int64_t end_tile() const { return max(length + kTile - 1, (int64_t)0) / kTile; }
+};
+
+__device__ __forceinline__ Sight sight_of(const Attention8bitParams& p, int64_t row) {
+    const int64_t length = min(max(p.lengths[row], (int64_t)0), p.cache.max_len);
+    return {length, length - p.q_len, p.window, p.causal != 0};
+}
+
+template <class T, int dims, int tiles_of_rows>
+__global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const __grid_constant__ Attention8bitParams p) {
+    constexpr bool precise = sizeof(T) == 4;
+    constexpr int kStages = stages_of(dims), kStageBytes = stage_bytes(dims), kSegments = dims / 64, kBlocks = dims / 16;
+    constexpr int kRows = 8 * tiles_of_rows;
+    extern __shared__ __align__(16) uint8_t shared[];
+    int* prefix = reinterpret_cast<int*>(shared + shared_of(dims));
+    __shared__ int carry[kWarps];
+    __shared__ float tops[kWarps][kRows], totals[kWarps][kRows];
+    __shared__ int is_last;
+    const Cache8bitView& c = p.cache;
+    const int batch = (int)c.batch, head_dim = c.head_dim, chunks = head_dim / 16;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, gid = lane / 4, tig = lane % 4;
+    uint8_t* stages = shared + warp * kStages * kStageBytes;
+    const uint32_t stages_at = shared_address(stages);
+    const int shift = 31 - __clz(c.block);
+
+    sum_of_rows(batch, prefix, carry, [&](int row) {
+        const Sight s = sight_of(p, row);
+        return (int)max(s.end_tile() - s.first_tile(), (int64_t)0) * c.kv_heads;
+    });
+    const int all = prefix[batch];
+    const int share = max((int)(((int64_t)all + gridDim.x - 1) / gridDim.x), kLeastShare);
+    // Rows that see nothing have no tiles, hence no block: their context is zero.
+    for (int64_t row = blockIdx.x; row < batch; row += gridDim.x) {
+        if (prefix[row + 1] != prefix[row]) continue;
+        T* out = static_cast<T*>(p.context) + row * p.heads * p.q_len * head_dim;
+        for (int i = threadIdx.x; i < p.heads * p.q_len * head_dim; i += kThreads) out[i] = from_float<T>(0.0f);
+    }
+    int64_t at = (int64_t)blockIdx.x * share;
+    const int64_t stop = min(at + share, (int64_t)all);
+    int row = at < stop ? row_of_item(prefix, batch, (int)at) : 0;
+    while (at < stop) {
+        while (prefix[row + 1] <= at) ++row;
+        const Sight sight = sight_of(p, row);
+        const int tiles = (prefix[row + 1] - prefix[row]) / c.kv_heads;
+        const int head = (int)(at - prefix[row]) / tiles, from_tile = (int)(at - prefix[row]) % tiles;
+        const int to_tile = (int)min((int64_t)tiles, from_tile + (stop - at));
+        const int64_t pair = (int64_t)row * c.kv_heads + head, tile0 = sight.first_tile();
+        const uint8_t* keys = c.key_codes + pair * c.max_len * head_dim;
+        const uint8_t* values = c.value_codes + pair * c.max_len * head_dim;
+        const float* key_scales = c.key_scales + pair * c.blocks;
+        const float* value_scales = c.value_scales + pair * c.blocks;
+
+        const int64_t seen = max(sight.first(0), (int64_t)0);  // no row sees a position before this one
+        const auto fetch = [&](int tile, int stage) {  // positions that no row sees arrive as zeros, whatever the cache holds there
+            const int64_t position = (tile0 + tile) * kTile;
+            const uint32_t to = stages_at + stage * kStageBytes;
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) {
+                const int index = i * 32 + lane, r = index / kBlocks, chunk = index % kBlocks;
+                if (chunk < chunks) {
+                    const bool there = position + r < sight.length && position + r >= seen;
+                    const int64_t offset = there ? (position + r) * head_dim + chunk * 16 : 0;
+                    const uint32_t place = r * dims + placed<dims>(r, chunk) * 16;
+                    copy16(to + place, keys + offset, there);
+                    copy16(to + kTile * dims + place, values + offset, there);
+                }
+            }
+            if (lane < 4) {  // the scales of the tile's two halves, keys' then values'
+                const int64_t first = position + lane % 2 * 16;
+                const bool there = first < sight.length;
+                copy4(to + 2 * kTile * dims + lane * 4, (lane < 2 ? key_scales : value_scales) + (there ? first >> shift : 0), there);
+            }
+        };
+        int fetched = from_tile + warp;
+#pragma unroll
+        for (int s = 0; s < kStages - 1; ++s) {
+            if (fetched < to_tile) fetch(fetched, s);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            fetched += kWarps;
+        }
+
+        // The query rows as the right-hand operand: lane (gid, tig) holds row gid's dimensions 16 tig .. 16 tig + 15 of every 64.
+        uint32_t qh[tiles_of_rows][kSegments][4][2], ql[precise ? tiles_of_rows : 1][precise ? kSegments : 1][4][2];
+        float row_scale[tiles_of_rows][2];  // of the score rows that this lane holds: rows 2 tig and 2 tig + 1
+        const T* q = static_cast<const T*>(p.q) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+#pragma unroll
+        for (int n = 0; n < tiles_of_rows; ++n) {
+            const int r = n * 8 + gid;
+            float x[kSegments][16];
+            float largest = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSegments; ++s) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = s * 64 + tig * 16 + i;
+                    float4 four = make_float4(0, 0, 0, 0);
+                    if (r < p.rows && d < head_dim) four = load_four(q + (int64_t)r * head_dim + d);
+                    x[s][i] = four.x, x[s][i + 1] = four.y, x[s][i + 2] = four.z, x[s][i + 3] = four.w;
+                    largest = fmaxf(largest, fmaxf(fmaxf(fabsf(four.x), fabsf(four.y)), fmaxf(fabsf(four.z), fabsf(four.w))));
+                }
+            }
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            // 2^-e with largest = m 2^e, 1 <= m < 2 (kept where it and its inverse are normal numbers)
+            const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int s = 0; s < kSegments; ++s) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float low = x[s][4 * w + 2 * h] * down, high = x[s][4 * w + 2 * h + 1] * down;
+                        qh[n][s][w][h] = halves(low, high);
+                        if constexpr (precise) ql[n][s][w][h] = halves_left(low, high, qh[n][s][w][h]);
+                    }
+                }
+            }
+            const float factor = up * (p.scale * kLog2e);
+            row_scale[n][0] = __shfl_sync(0xffffffffu, factor, 8 * tig);      // (row 2 tig is lanes 8 tig .. 8 tig + 3)
+            row_scale[n][1] = __shfl_sync(0xffffffffu, factor, 8 * tig + 4);
+        }
+
+        float out[tiles_of_rows][kBlocks][4], top[tiles_of_rows][2], total[tiles_of_rows][2];
+#pragma unroll
+        for (int n = 0; n < tiles_of_rows; ++n) {
+            top[n][0] = top[n][1] = kNone;
+            total[n][0] = total[n][1] = 0.0f;
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
+        }
+        // Positions that every row sees need no mask.
+        const int64_t all_from = sight.first(p.q_len - 1), all_to = sight.last(0);
+
+        int stage = 0;
+        for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
+            copies_done<kStages - 2>();
+            __syncwarp();
+            {
+                const int next = stage == 0 ? kStages - 1 : stage - 1;  // the stage that the tile before this one used
+                if (fetched < to_tile) fetch(fetched, next);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                fetched += kWarps;
+            }
+            const uint8_t* k_stage = stages + stage * kStageBytes;
+            const float* scales = reinterpret_cast<const float*>(k_stage + 2 * kTile * dims);
+            const int64_t position = (tile0 + tile) * kTile;
+            float score[tiles_of_rows][2][4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                for (int n = 0; n < tiles_of_rows; ++n) score[n][half][0] = score[n][half][1] = score[n][half][2] = score[n][half][3] = 0.0f;
+                const int r0 = half * 16 + gid, r1 = r0 + 8;
+#pragma unroll
+                for (int s = 0; s < kSegments; ++s) {
+                    const int chunk = s * 4 + tig;
+                    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                    if (chunk < chunks) {
+                        a = *reinterpret_cast<const uint4*>(k_stage + r0 * dims + placed<dims>(r0, chunk) * 16);
+                        b = *reinterpret_cast<const uint4*>(k_stage + r1 * dims + placed<dims>(r1, chunk) * 16);
+                    }
+                    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t a0 = codes_to_halves(aw[w]), a1 = codes_to_halves(bw[w]);
+                        const uint32_t a2 = codes_to_halves(aw[w] >> 16), a3 = codes_to_halves(bw[w] >> 16);
+#pragma unroll
+                        for (int n = 0; n < tiles_of_rows; ++n) {
+                            if constexpr (precise) multiply(score[n][half], a0, a1, a2, a3, ql[n][s][w][0], ql[n][s][w][1]);
+                            multiply(score[n][half], a0, a1, a2, a3, qh[n][s][w][0], qh[n][s][w][1]);
+                        }
+                    }
+                }
+            }
+            // score[n][half][2 o + i]: position half * 16 + 8 o + gid, query row 8 n + 2 tig + i
+            float value_scale[2], value_log[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float key_scale = scales[half];
+                value_scale[half] = scales[2 + half];
+                value_log[half] = __log2f(fmaxf(value_scale[half], 0x1p-100f));
+#pragma unroll
+                for (int n = 0; n < tiles_of_rows; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) score[n][half][i] *= key_scale * row_scale[n][i & 1];
+                }
+            }
+            if (position < all_from || position + kTile - 1 > all_to) {
+#pragma unroll
+                for (int n = 0; n < tiles_of_rows; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int own = (n * 8 + 2 * tig + i) % p.q_len;
+                        const int64_t first = sight.first(own), last = sight.last(own);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) {
+                                const int64_t j = position + half * 16 + o * 8 + gid;
+                                if (j < first || j > last) score[n][half][2 * o + i] = kNone;
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < tiles_of_rows; ++n) {
+                float high[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    high[i] = fmaxf(fmaxf(score[n][0][i], score[n][0][2 + i]) + value_log[0], fmaxf(score[n][1][i], score[n][1][2 + i]) + value_log[1]);
+#pragma unroll
+                    for (int step = 4; step < 32; step *= 2) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], step));
+                }
+                if (__any_sync(0xffffffffu, high[0] > top[n][0] || high[1] > top[n][1])) {
+                    float less[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float next = fmaxf(top[n][i], high[i]);
+                        less[i] = next > kNone ? exp2_approx(top[n][i] - next) : 1.0f;
+                        top[n][i] = next;
+                        total[n][i] *= less[i];
+                    }
+#pragma unroll
+                    for (int m = 0; m < kBlocks; ++m) {
+                        out[n][m][0] *= less[0], out[n][m][1] *= less[1];
+                        out[n][m][2] *= less[0], out[n][m][3] *= less[1];
+                    }
+                }
+            }
+            // Weights, rounded to halves and turned round: lane (gid, tig) then holds query row gid's weights of positions 2 tig, 2 tig + 1.
+            uint32_t wh[tiles_of_rows][2][2], wl[precise ? tiles_of_rows : 1][2][2];
+#pragma unroll
+            for (int n = 0; n < tiles_of_rows; ++n) {
+                const float t0 = top[n][0] > kNone ? top[n][0] : 0.0f, t1 = top[n][1] > kNone ? top[n][1] : 0.0f;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) {
+                        const float e0 = exp2_approx(score[n][half][2 * o] - t0), e1 = exp2_approx(score[n][half][2 * o + 1] - t1);
+                        total[n][0] += e0;
+                        total[n][1] += e1;
+                        const float w0 = e0 * value_scale[half], w1 = e1 * value_scale[half];
+                        const uint32_t taken = halves(w0, w1);
+                        wh[n][half][o] = transposed(taken);
+                        if constexpr (precise) wl[n][half][o] = transposed(halves_left(w0, w1, taken));
+                    }
+                }
+            }
+            // The values come as 8 x 8 matrices of code pairs, turned round: lane (gid, tig) gets dimensions 2 gid, 2 gid + 1 of
+            // positions 2 tig and 2 tig + 1; dimension 2 gid is row gid of the left-hand operand, 2 gid + 1 row gid + 8.
+            const uint32_t v_at = stages_at + stage * kStageBytes + kTile * dims;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = half * 16 + lane % 16;
+#pragma unroll
+                for (int m = 0; m < kBlocks; m += 2) {
+                    if (m < chunks) {
+                        uint32_t x[4];
+                        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                            : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                            : "r"(v_at + r * dims + placed<dims>(r, m + lane / 16) * 16)
+                            : "memory");
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t low = __byte_perm(x[2 * i], 0, 0x3120), high = __byte_perm(x[2 * i + 1], 0, 0x3120);
+                            const uint32_t a0 = codes_to_halves(low), a1 = codes_to_halves(low >> 16);
+                            const uint32_t a2 = codes_to_halves(high), a3 = codes_to_halves(high >> 16);
+#pragma unroll
+                            for (int n = 0; n < tiles_of_rows; ++n) {
+                                if constexpr (precise) multiply(out[n][m + i], a0, a1, a2, a3, wl[n][half][0], wl[n][half][1]);
+                                multiply(out[n][m + i], a0, a1, a2, a3, wh[n][half][0], wh[n][half][1]);
+                            }
+                        }
+                    }
+                }
+            }
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+        copies_done<0>();
+
+        // The four warps' results meet in shared memory.  (The stages are free: every warp has read its own.)
+#pragma unroll
+        for (int n = 0; n < tiles_of_rows; ++n) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int step = 4; step < 32; step *= 2) total[n][i] += __shfl_xor_sync(0xffffffffu, total[n][i], step);
+                if (gid == 0) {
+                    tops[warp][n * 8 + 2 * tig + i] = top[n][i];
+                    totals[warp][n * 8 + 2 * tig + i] = total[n][i];
+                }
+            }
+        }
+        __syncthreads();
+        float* meet = reinterpret_cast<float*>(shared);  // (warp, row, dimension)
+#pragma unroll
+        for (int n = 0; n < tiles_of_rows; ++n) {
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = n * 8 + 2 * tig + (i & 1), d = m * 16 + 2 * gid + (i >> 1);
+                    meet[(warp * kRows + r) * dims + d] = out[n][m][i];
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = from_tile == 0 && to_tile == tiles;
+        T* context = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+        const int piece_floats = kRows * (dims + 2);
+        float* piece = p.partial + ((int64_t)blockIdx.x * 2 + (at == (int64_t)blockIdx.x * share ? 0 : 1)) * piece_floats;
+        for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) {
+            const int r = i / head_dim, d = i % head_dim;
+            float high = kNone, sum = 0.0f, value = 0.0f;
+            for (int w = 0; w < kWarps; ++w) high = fmaxf(high, tops[w][r]);
+            for (int w = 0; w < kWarps; ++w) {
+                if (totals[w][r] == 0.0f) continue;  // (a warp without a position that the row sees)
+                const float less = exp2_approx(tops[w][r] - high);
+                sum += totals[w][r] * less;
+                value += meet[(w * kRows + r) * dims + d] * less;
+            }
+            if (whole) {
+                context[i] = from_float<T>(sum == 0.0f ? 0.0f : value / sum);
+            } else {
+                __stcg(piece + r * (dims + 2) + d, value);
+                if (d == 0) {
+                    __stcg(piece + r * (dims + 2) + dims, high);
+                    __stcg(piece + r * (dims + 2) + dims + 1, sum);
+                }
+            }
+        }
+        if (!whole) {
+            const int64_t begin = prefix[row] + (int64_t)head * tiles, end = begin + tiles;
+            const int64_t first = begin / share, last = (end - 1) / share;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                is_last = atomicAdd(p.arrived + pair, 1) == (int)(last - first);
+                if (is_last) p.arrived[pair] = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (is_last) {
+                const auto piece_of = [&](int64_t block) {
+                    return p.partial + (block * 2 + (block == first && begin != block * share ? 1 : 0)) * piece_floats;
+                };
+                for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) {
+                    const int r = i / head_dim, d = i % head_dim;
+                    float high = kNone, sum = 0.0f, value = 0.0f;
+                    for (int64_t b = first; b <= last; ++b) high = fmaxf(high, __ldcg(piece_of(b) + r * (dims + 2) + dims));
+                    for (int64_t b = first; b <= last; ++b) {
+                        const float* from = piece_of(b) + r * (dims + 2);
+                        const float part = __ldcg(from + dims + 1);
+                        if (part == 0.0f) continue;
+                        const float less = exp2_approx(__ldcg(from + dims) - high);
+                        sum += part * less;
+                        value += __ldcg(from + d) * less;
+                    }
+                    context[i] = from_float<T>(sum == 0.0f ? 0.0f : value / sum);
+                }
+            }
+        }
+        at += to_tile - from_tile;
+        __syncthreads();  // (shared memory is free for the next pair)
+    }
+}
+
+template <class T, int dims, int tiles_of_rows>
+cudaError_t launch(const Attention8bitParams& p, cudaStream_t stream) {
+    static OncePerDevice raised;
+    const auto kernel = decode_attention_8bit_kernel<T, dims, tiles_of_rows>;
+    int device = 0;
+    if (const cudaError_t e = cudaGetDevice(&device)) return e;
+    const cudaError_t e = raised.run(device, [&] {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(shared_of(dims) + (kMostPrefixRows + 1) * sizeof(int)));
+    });
+    if (e != cudaSuccess) return e;
+    const size_t shared = shared_of(dims) + (size_t)(p.cache.batch + 1) * sizeof(int);
+    kernel<<<(unsigned)p.grid, kThreads, shared, stream>>>(p);
+    return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_type(const Attention8bitParams& p, cudaStream_t stream) {
+    const int dims = p.cache.head_dim;
+    if (dims > 128) return launch<T, 256, 1>(p, stream);
+    if (dims > 64) return p.rows <= 8 ? launch<T, 128, 1>(p, stream) : launch<T, 128, 2>(p, stream);
+    return p.rows <= 8 ? launch<T, 64, 1>(p, stream) : launch<T, 64, 2>(p, stream);
+}
+
+int padded_dims(const Attention8bitParams& p) { return p.cache.head_dim > 128 ? 256 : p.cache.head_dim > 64 ? 128 : 64; }
+
+}  // namespace
+
+int attention_8bit_grid(const Attention8bitParams& p, int sm_count) {
+    // As many blocks as the GPU holds at once (shared memory: 227 KB of an SM), no more than there are least shares.
+    const int dims = padded_dims(p);
+    const int resident = dims == 256 ? 1 : dims == 128 ? 2 : 4;
+    const int64_t tiles = p.cache.batch * p.cache.kv_heads * ((p.cache.max_len + kTile - 1) / kTile);
+    return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count * resident, (tiles + kLeastShare - 1) / kLeastShare));
+}
+
+size_t attention_8bit_partial_bytes(const Attention8bitParams& p) {
+    const int rows = p.rows <= 8 ? 8 : 16;
+    return (size_t)p.grid * 2 * rows * (padded_dims(p) + 2) * sizeof(float);
+}
+
+cudaError_t launch_decode_attention_8bit(const Attention8bitParams& p, cudaStream_t stream) {
+    if (p.rows > 16 || p.cache.head_dim > 256 || (p.cache.head_dim > 128 && p.rows > 8)) return cudaErrorInvalidValue;
+    if (p.type == kFloat32) return launch_type<float>(p, stream);
+    if (p.type == kBfloat16) return launch_type<__nv_bfloat16>(p, stream);
+    return launch_type<__half>(p, stream);
+}
+
+}  // namespace psx

@@ -116,3 +116,14 @@ def test_settings_are_a_ctypes_structure(lib):
         with pytest.raises(TypeError):
             psx.sample_rows_static(Rows(), None, None, refused, None, None, None, None, stream=0)
     psx.sample_rows_static(Rows(), None, None, psx.SamplingConfig.make(do_sample=False), None, None, None, None, stream=0)
+
+
+def test_beam_and_cache_entry_points_check_their_arguments_before_touching_a_gpu(lib):
+    # no context: nothing is read, nothing is launched
+    state, cache = binding.BeamState(), binding.Cache8bitLayout()
+    assert lib.psx_b200_beam_select(None, None, None, 1, 1, 1, 1, None, None, 0, 1, None, None, None, None) == binding.ERR_BAD_ARGUMENT
+    assert lib.psx_b200_reorder_states(None, None, C.addressof(state), 1, 1, 1, None, None) == binding.ERR_BAD_ARGUMENT
+    assert lib.psx_b200_store_cache_8bit(None, None, C.addressof(cache), None, None, 0, 0, 0, 0, None, None, None) == binding.ERR_BAD_ARGUMENT
+    assert lib.psx_b200_decode_attention_8bit(None, None, None, 0, C.addressof(cache), None, None, 1, 1, 1.0, 1, 0) == binding.ERR_BAD_ARGUMENT
+    # as a C compiler lays out psx_beam_state and psx_cache_8bit
+    assert C.sizeof(binding.BeamState) == 40 and C.sizeof(binding.Cache8bitLayout) == 72
