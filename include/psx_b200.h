@@ -416,6 +416,27 @@ PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, co
                                                   const int64_t* lengths, void* context, int64_t heads, int64_t q_len, float scale,
                                                   int32_t causal, int64_t window);
 
+/* Attention of whole prompts, for sequences of different lengths packed one behind the other: what psx_b200_decode_attention does
+ * for a few new positions and declines for many (src/multihead_attention_module.cpp:443-480, forward(), without padding).  q:
+ * device, `dtype`, (total_q, heads, head_dim), a position at q + i * q_stride elements, its heads contiguous; k, v: (total_k,
+ * kv_heads, head_dim), likewise (slices of one projection will do); query head h reads kv head h / (heads / kv_heads).  Sequence
+ * b has queries q_offsets[b] .. q_offsets[b + 1] and keys k_offsets[b] .. k_offsets[b + 1] (device int64, batch + 1, ascending); with
+ * more keys than queries the queries are the last positions (a prompt that continues a cached prefix).  Query i of n, with m
+ * keys, is position p = m - n + i: with `causal` it sees no key j > p and, with window > 0, no key j + window <= p.  A query that
+ * sees nothing gets 0.  out: (total_q, heads, head_dim), contiguous; rows that belong to no sequence are left as they were.
+ * Products run on the tensor cores with float accumulators.  bf16 and fp16: weights are rounded to that type; fp32: every
+ * factor as three bf16 parts, so that products are exact to about 2^-24 (an infinity counts as NaN).  Keys and values of other
+ * sequences, finite or not, have no influence; a NaN among a sequence's own values reaches the queries of the 128 positions
+ * around it that do not see it, too.
+ * All pointers 16-byte aligned, strides a multiple of 16 bytes.  Limits: head_dim a multiple of 8 up to 128, batch <= 4096, total_q
+ * and total_k <= 2^29 (else PSX_ERR_UNSUPPORTED).  status (device, may be null, the caller's to zero): bit 0 is set if a bounded
+ * device-side wait ran out (psx_b200_ctx_set_wait_limit).  Asynchronous on `stream`; fp32 takes scratch of 1.5 times the
+ * operands' bytes (in a stream capture as psx_b200_beam_select). */
+PSX_API psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream, int32_t dtype, const void* q, const void* k, const void* v, void* out,
+                                             int64_t total_q, int64_t total_k, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                             const int64_t* q_offsets, const int64_t* k_offsets, int64_t batch, int64_t heads,
+                                             int64_t kv_heads, int64_t head_dim, float scale, int32_t causal, int64_t window, int32_t* status);
+
 /* Replace DeviceBackend::softmax_rows, logsumexp_rows and gather_rows
  * (include/pulsatrix/device_backend.hpp:456,465,596; CUDA implementations src/cuda_backend.cu with
  * the kernels src/gpu_kernels.cuh:315-365,665; CPU semantics src/cpu_backend.cpp:292-338,459-466)

@@ -20,7 +20,7 @@ EXPORTS = [
     "psx_b200_exchange_handle_bytes", "psx_b200_exchange_create", "psx_b200_exchange_open", "psx_b200_exchange_destroy",
     "psx_b200_exchange_sample", "psx_b200_exchange_results", "psx_b200_exchange_test_wait",
     "psx_b200_top_k_rows", "psx_b200_lm_head_logits", "psx_b200_lm_head_sample_rows", "psx_b200_softmax_rows", "psx_b200_logsumexp_rows", "psx_b200_gather_rows", "psx_b200_decode_attention",
-    "psx_b200_beam_select", "psx_b200_reorder_states", "psx_b200_store_cache_8bit", "psx_b200_decode_attention_8bit",
+    "psx_b200_beam_select", "psx_b200_reorder_states", "psx_b200_store_cache_8bit", "psx_b200_decode_attention_8bit", "psx_b200_prompt_attention",
     "psx_uniforms_mt19937_64", "psx_uniforms_portable",
 ]
 
@@ -154,6 +154,8 @@ def library():
         lib.psx_b200_reorder_states.argtypes = [ptr, ptr, ptr, i64, i64, i64, ptr, ptr]
         lib.psx_b200_store_cache_8bit.argtypes = [ptr, ptr, ptr, ptr, ptr, C.c_int32, i64, i64, i64, ptr, ptr, ptr]
         lib.psx_b200_decode_attention_8bit.argtypes = [ptr, ptr, ptr, C.c_int32, ptr, ptr, ptr, i64, i64, C.c_float, C.c_int32, i64]
+        lib.psx_b200_prompt_attention.argtypes = [ptr, ptr, C.c_int32, ptr, ptr, ptr, ptr, i64, i64, i64, i64, i64, ptr, ptr, i64, i64, i64, i64,
+                                                  C.c_float, C.c_int32, i64, ptr]
         lib.psx_uniforms_mt19937_64.argtypes = [ptr, i64, ptr]
         lib.psx_uniforms_portable.argtypes = [ptr, i64, ptr]
         from . import _native as native
@@ -626,6 +628,34 @@ class Context:
         _check(_native.decode_attention_8bit(self._handle, _stream_of(q) if stream is None else stream, q.data_ptr(), _dtype_code(q), cache._address,
                                              lengths.data_ptr(), context.data_ptr(), heads, q_len, float(scale), int(bool(causal)), window))
         return context
+
+    def prompt_attention(self, q, k, v, q_offsets, k_offsets=None, scale=None, causal=True, window=0, out=None, stream=None):
+        """Attention of whole prompts, packed one behind the other (psx_b200_prompt_attention).  q: float32, bfloat16 or float16
+        (total_q, heads, head_dim); k, v: (total_k, kv_heads, head_dim); heads and dimensions of a position contiguous; q_offsets,
+        k_offsets: int64 (batch + 1), the latter the same as q_offsets if None.  Returns the context, (total_q, heads, head_dim)
+        (`out` if given: rows of no sequence keep what they hold), and a one-element int32 status tensor."""
+        import torch
+        k_offsets = q_offsets if k_offsets is None else k_offsets
+        total_q, heads, head_dim = q.shape
+        total_k, kv_heads = k.shape[0], k.shape[1]
+        _need(k.shape == v.shape and k.shape[2] == head_dim and q.dtype == k.dtype == v.dtype, "q, k and v are of one type and head dimension")
+        strides = []
+        for t, width in ((q, heads * head_dim), (k, kv_heads * head_dim), (v, kv_heads * head_dim)):
+            _need(t.shape[0] == 0 or (t.stride(2) == 1 and (t.stride(1) == head_dim or t.shape[1] == 1)), "heads and dimensions of a position are contiguous")
+            strides.append(t.stride(0) if t.shape[0] > 1 else width)
+        _need(q_offsets.dtype == torch.int64 and q_offsets.is_contiguous() and q_offsets.numel() > 0, "offsets are int64 (batch + 1)")
+        _need(k_offsets.dtype == torch.int64 and k_offsets.is_contiguous() and k_offsets.numel() == q_offsets.numel(), "offsets are int64 (batch + 1)")
+        if out is None:
+            out = torch.empty((total_q, heads, head_dim), dtype=q.dtype, device=q.device)
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out is contiguous and of q's shape and type")
+        self._here(q, k, v, out, q_offsets, k_offsets)
+        if scale is None:
+            scale = 1.0 / float(np.sqrt(np.float32(head_dim)))
+        status = _zeroed_word(q.device, stream)
+        _check(_native.prompt_attention(self._handle, _stream_of(q) if stream is None else stream, _dtype_code(q), q.data_ptr(), k.data_ptr(),
+                                        v.data_ptr(), out.data_ptr(), total_q, total_k, *strides, q_offsets.data_ptr(), k_offsets.data_ptr(),
+                                        q_offsets.numel() - 1, heads, kv_heads, head_dim, float(scale), int(bool(causal)), window, status.data_ptr()))
+        return out, status
 
     # ---- vocabulary-sharded -----------------------------------------------------------------------------
     def shard_record_bytes(self, config) -> int:

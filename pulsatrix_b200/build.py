@@ -17,7 +17,7 @@ PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libpsx_b200.so"
 SOURCES = ["c_abi.cu", "scan_rows.cu", "merge_rows.cu", "whole_rows.cu", "topk_rows.cu", "shard_records.cu", "peer_exchange.cu", "no_alloc.cu", "read_floor.cu", "process_rows.cu", "row_ops.cu", "lm_head.cu", "decode_attention.cu",
-           "beam_select.cu", "reorder_states.cu", "store_cache_8bit.cu", "decode_attention_8bit.cu"]
+           "beam_select.cu", "reorder_states.cu", "store_cache_8bit.cu", "decode_attention_8bit.cu", "prompt_attention.cu"]
 HOST_SOURCES = ["determinism.cpp", "sampler.cpp", "backend.cpp", "generation.cpp"]  # the C++ API over the C ABI
 PYTHON_CALLS = PACKAGE / "_native.so"  # the per-step calls as a CPython extension module (host/python_calls.cpp)
 CPP_TEST = PACKAGE.parent / "tests" / "cpp" / "host_api_test"

@@ -19,6 +19,7 @@
 #include "peer_exchange.cuh"
 #include "decode_attention.cuh"
 #include "process_rows.cuh"
+#include "prompt_attention.cuh"
 #include "reorder_states.cuh"
 #include "row_prefix.cuh"
 #include "row_ops.cuh"
@@ -90,7 +91,7 @@ struct psx_ctx {
     // staging of the sharded path
     Buffer shard_uniform_scratch;
     // Scratch that captured graphs may hold: what it outgrows stays allocated until the context goes (see reserve_kept).
-    Buffer beam_scratch, attention_8bit_pieces, attention_8bit_arrived;
+    Buffer beam_scratch, attention_8bit_pieces, attention_8bit_arrived, prompt_parts;
     std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
     bool timing = false;
@@ -422,7 +423,7 @@ void psx_b200_ctx_destroy(psx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Buffer* b : {&ctx->stats[0], &ctx->stats[1], &ctx->part_counts[0], &ctx->part_counts[1], &ctx->candidates[0], &ctx->candidates[1], &ctx->banned, &ctx->sort_keys, &ctx->head_logits, &ctx->attention_partial, &ctx->surv_cols, &ctx->surv_vals,
                       &ctx->surv_counts, &ctx->pl_tokens, &ctx->pl_log_probs, &ctx->pl_status, &ctx->h_logits, &ctx->h_inputs,
-                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived}) {
+                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts}) {
         if (b->ptr) cudaFree(b->ptr);
     }
     for (void* p : ctx->outgrown) cudaFree(p);
@@ -1318,6 +1319,51 @@ psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const 
     p.arrived = static_cast<int32_t*>(ctx->attention_8bit_arrived.ptr);
     PSX_CUDA(psx::launch_decode_attention_8bit(p, stream));
     ctx->launches += 1;
+    return PSX_OK;
+}
+
+psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dtype, const void* q, const void* k, const void* v, void* out,
+                                     int64_t total_q, int64_t total_k, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                                     const int64_t* q_offsets, const int64_t* k_offsets, int64_t batch, int64_t heads, int64_t kv_heads,
+                                     int64_t head_dim, float scale, int32_t causal, int64_t window, int32_t* status) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
+    if (batch < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || total_q < 0 || total_k < 0 || window < 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: attention sizes must be positive");
+    }
+    if (heads % kv_heads != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: heads must be a multiple of kv_heads");
+    if (!std::isfinite(scale)) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the score scale must be finite");
+    if (head_dim % 8 != 0 || head_dim > 128 || batch > psx::kMostPrefixRows || total_q > (1 << 29) || total_k > (1 << 29) || heads > 65536 ||
+        (total_q / 128 + batch) * heads > 0x7fffffff) {
+        return fail(PSX_ERR_UNSUPPORTED,
+                    "psx_b200: attention of prompts takes a head dimension that is a multiple of 8 up to 128, at most 4096 sequences and 2^29 positions");
+    }
+    if (q_stride < heads * head_dim || k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a position's stride is at least its heads times head_dim");
+    }
+    if (batch == 0 || total_q == 0) return PSX_OK;
+    if (!q || !out || !q_offsets || !k_offsets || (total_k > 0 && (!k || !v))) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    const uintptr_t lies = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                           reinterpret_cast<uintptr_t>(out) | (uintptr_t)((q_stride | k_stride | v_stride) * psx::element_bytes(dtype));
+    if (lies % 16 != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: operands and their positions must start on 16-byte boundaries");
+    psx::PromptAttentionParams p{};
+    p.q = q; p.k = k; p.v = v; p.out = out; p.q_offsets = q_offsets; p.k_offsets = k_offsets; p.status = status; p.total_q = total_q; p.total_k = total_k;
+    p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride;
+    p.window = std::min<int64_t>(window, 1 << 30);  // (a wider one hides nothing more, and sums with it stay in range)
+    p.wait_limit_ns = ctx->wait_limit_ns; p.batch = (int32_t)batch; p.heads = (int32_t)heads; p.kv_heads = (int32_t)kv_heads;
+    p.head_dim = (int32_t)head_dim; p.type = dtype; p.causal = causal ? 1 : 0; p.scale = scale; p.extra_bytes = ctx->test_short_copy ? 16 : 0;
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    if (dtype == psx::kFloat32) {
+        if (psx_status s = reserve_kept(ctx, stream, ctx->prompt_parts, psx::prompt_split_bytes(p))) return s;
+        p.split = ctx->prompt_parts.ptr;
+    }
+    int launches = 0;
+    const cudaError_t e = psx::launch_prompt_attention(p, stream, &launches);
+    ctx->launches += launches;
+    if (e == cudaErrorNotSupported) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: the driver has no tensor maps");
+    PSX_CUDA(e);
     return PSX_OK;
 }
 

@@ -1,0 +1,568 @@
+// Attention of whole prompts, packed one behind the other: per sequence and head softmax(scale q k^T, masked) v, on the
+// fifth-generation tensor cores, without the scores in memory.
+//
+// A CTA takes `tiles` tiles of 128 queries of one (sequence, head) and goes through the keys that they see in blocks.  One thread
+// asks for copies (tiled, 128-byte swizzle), one thread issues the products, and a warpgroup per tile turns scores into weights, a
+// thread per query: it loads its row of scores from tensor memory, keeps the running maximum and sum in registers (no
+// exchange between threads), and writes the weights back to tensor memory, from where they are the left operand of the second
+// product.  The context stays in tensor memory; it is rescaled only where a row's maximum has grown by more than 2^8 since
+// the last time (weights are then up to 2^8 instead of 1, which costs no precision).
+//
+// 16-bit operands: two tiles, blocks of 128 keys, two stages of keys and of values; while the tensor core works for one tile the
+// other tile's warpgroup works on its scores; a tile's weights take its scores' place.  Weights are rounded to the operands'
+// type, the error of which is of the size of the context's own rounding.  Bound by the exponentials (16 a clock and SM) and
+// the products about alike.
+//
+// fp32 operands: every number is split into three bf16 parts that add up to it (8 bits of the fraction each), and a product is the
+// six products of parts that reach fp32's precision, the small ones first; a split kernel writes the parts ahead of time.
+// One tile, blocks of 64 keys; the scores have two places and the weights' parts one of their own, so that the next block's
+// scores are formed while this block's weights are.  Six bf16 products are still several times faster than the FP32 pipes.
+//
+// Rows behind a sequence's last key in a block belong to other sequences: their scores are masked, and their values are set to zero in
+// shared memory, so that a NaN there is not seen here.
+#include "prompt_attention.cuh"
+
+#include <algorithm>
+
+#include "elements.cuh"
+#include "once_per_device.hpp"
+#include "row_prefix.cuh"
+#include "tensor_core.cuh"
+
+namespace psx {
+namespace {
+
+constexpr float kNone = -__builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTileRows = 128;
+constexpr float kMostGrowth = 8.0f;  // of a row's maximum, in powers of two, before its context is rescaled
+
+template <int dims_, int parts_>
+struct Shape {
+    static constexpr int dims = dims_, parts = parts_;  // the head dimension, rounded up to 64 or 128
+    static constexpr int tiles = parts == 1 ? 2 : 1;
+    static constexpr int block = parts == 1 ? 128 : 64;
+    static constexpr int stages = parts == 1 ? (dims == 64 ? 4 : 2) : (dims == 64 ? 2 : 1);
+    static constexpr int threads = tiles * 128 + 64;  // the warpgroups, the copying warp, the issuing warp
+    static constexpr int slabs = dims / 64;            // a tile lies in slabs of 64 columns, rows of 128 bytes
+    static constexpr int q_part = kTileRows * dims * 2, q_bytes = parts * q_part;
+    static constexpr int k_part = block * dims * 2, k_bytes = parts * k_part;  // (of the values too)
+    static constexpr int shared = tiles * q_bytes + 2 * stages * k_bytes;
+    // Tensor memory: scores (two places for each tile, or one that the weights share), weights' parts, contexts.
+    static constexpr int score_at = 0;
+    static constexpr int weight_at = parts == 1 ? 0 : 2 * block;
+    static constexpr int weight_part = block / 2;
+    static constexpr int context_at = parts == 1 ? tiles * block : 256;
+    static_assert(weight_at + parts * weight_part <= 256 && context_at + tiles * dims <= 512);
+};
+
+struct alignas(64) PromptLaunch {
+    CUtensorMap q_map, k_map, v_map;
+    PromptAttentionParams p;
+    int32_t steps;  // of 16 dimensions
+    int32_t dims16;  // the head dimension, rounded up to 16
+};
+
+// What a tile of queries sees: key j where first(i) <= j < end(i), i the query's number in its sequence.
+struct Sight {
+    int64_t keys, ahead;  // keys of the sequence; keys before the first query's own position
+    int64_t window;
+    bool causal;
+    __device__ __forceinline__ int64_t end(int64_t i) const { return causal ? min(keys, i + ahead + 1) : keys; }
+    __device__ __forceinline__ int64_t first(int64_t i) const { return causal && window > 0 ? max(i + ahead + 1 - window, (int64_t)0) : 0; }
+};
+
+__device__ __forceinline__ uint32_t pack(float low, float high, __nv_bfloat16) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack(float low, float high, __half) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
+    return r;
+}
+
+// Elem: the type of the products' operands (bf16 for the parts of fp32); Out: the type of the context.
+template <class Elem, class Out, class S>
+__global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const __grid_constant__ PromptLaunch launch) {
+    extern __shared__ uint8_t raw_shared[];
+    __shared__ uint64_t q_full, k_full[S::stages], k_empty[S::stages], v_full[S::stages], v_empty[S::stages];
+    __shared__ uint64_t score_full[2], weight_full[2], context_full[2], drained;
+    __shared__ uint32_t tensor_at;
+    __shared__ uint32_t give_up;
+    __shared__ int carry[32];
+    const PromptAttentionParams& p = launch.p;
+    uint8_t* shared = raw_shared + ((1024 - (smem_address(raw_shared) & 1023)) & 1023);
+    int* prefix = reinterpret_cast<int*>(shared + S::shared);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    constexpr int kCopyWarp = S::tiles * 4, kIssueWarp = S::tiles * 4 + 1;
+    constexpr int kRows = S::tiles * kTileRows;
+
+    const auto queries_of = [&](int b) { return max(min(p.q_offsets[b + 1], p.total_q) - max(p.q_offsets[b], (int64_t)0), (int64_t)0); };
+    sum_of_rows(p.batch, prefix, carry, [&](int b) { return (int)((queries_of(b) + kRows - 1) / kRows); });
+    const int group_of_rows = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+    if (group_of_rows >= prefix[p.batch]) return;
+    const int b = row_of_item(prefix, p.batch, group_of_rows);
+    const int64_t queries = queries_of(b), q_begin = max(p.q_offsets[b], (int64_t)0), k_begin = max(p.k_offsets[b], (int64_t)0);
+    const int64_t keys = max(min(p.k_offsets[b + 1], p.total_k) - k_begin, (int64_t)0);
+    const Sight sight{keys, keys - queries, p.window, p.causal != 0};
+    // The last queries see the most keys: they come first, so that the short work is left for the end.
+    const int64_t row0 = (int64_t)(prefix[b + 1] - 1 - group_of_rows) * kRows;
+    if (row0 < 0 || row0 >= queries) return;  // (offsets that make no sense)
+    int64_t ends[S::tiles];
+    int64_t begin = sight.first(row0) / S::block;  // blocks of keys, for all tiles
+    int counts[S::tiles], most = 0;
+#pragma unroll
+    for (int t = 0; t < S::tiles; ++t) {
+        const int64_t first_row = row0 + t * kTileRows, last_row = min(first_row + kTileRows, queries) - 1;
+        ends[t] = last_row < first_row ? 0 : max(sight.end(last_row), (int64_t)0);
+        counts[t] = (int)max((ends[t] + S::block - 1) / S::block - begin, (int64_t)0);
+        most = max(most, counts[t]);
+    }
+
+    if (threadIdx.x == 0) {
+        barrier_init(&q_full, 1);
+        for (int s = 0; s < S::stages; ++s) {
+            barrier_init(&k_full[s], 1);
+            barrier_init(&k_empty[s], 1);
+            barrier_init(&v_full[s], 1);
+            barrier_init(&v_empty[s], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            barrier_init(&score_full[t], 1);
+            barrier_init(&weight_full[t], 128);
+            barrier_init(&context_full[t], 1);
+        }
+        barrier_init(&drained, 1);
+        barrier_init_fence();
+        give_up = 0;
+    }
+    if (warp == kIssueWarp) tensor_allocate(&tensor_at, 512);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = tensor_at;
+    const auto wait_alone = [&](uint64_t* bar, uint32_t parity) {
+        if (barrier_wait_bounded(bar, parity, p.wait_limit_ns, &give_up)) return true;
+        *(volatile uint32_t*)&give_up = 1;
+        return false;
+    };
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {  // (a warp goes on as a whole or not at all)
+        return __all_sync(0xffffffffu, wait_alone(bar, parity)) != 0;
+    };
+    const uint32_t q_at = smem_address(shared), k_at = q_at + S::tiles * S::q_bytes, v_at = k_at + S::stages * S::k_bytes;
+
+    if (warp == kCopyWarp) {
+        if (lane == 0 && most > 0) {
+            const int kv_head = head / (p.heads / p.kv_heads);
+            const auto fetch = [&](uint32_t to, int rows, const CUtensorMap* map, int y, int64_t z, int64_t total, uint64_t* bar) {
+                for (int part = 0; part < S::parts; ++part) {
+                    for (int slab = 0; slab < S::slabs; ++slab) {
+                        if (slab * 64 >= p.head_dim) continue;
+                        tiled_copy_to_shared(to + (part * S::slabs + slab) * rows * 128, map, slab * 64, y, (int)(part * total + z), bar);
+                    }
+                }
+            };
+            const uint32_t filled = (uint32_t)min(S::slabs, (p.head_dim + 63) / 64) * 128 * S::parts;  // bytes per row that arrive
+            uint32_t q_bytes = 0;
+            for (int t = 0; t < S::tiles; ++t) q_bytes += counts[t] > 0 ? kTileRows * filled : 0;
+            barrier_expect_bytes(&q_full, q_bytes);
+            for (int t = 0; t < S::tiles; ++t) {
+                if (counts[t] > 0) fetch(q_at + t * S::q_bytes, kTileRows, &launch.q_map, head, q_begin + row0 + t * kTileRows, p.total_q, &q_full);
+            }
+            int asked = 0;
+            bool fine = true;
+            for (; asked < most && fine; ++asked) {
+                const int s = asked % S::stages, round = asked / S::stages;
+                const int64_t z = k_begin + (begin + asked) * S::block;
+                if (round > 0 && !(fine = wait_alone(&k_empty[s], (round - 1) & 1))) break;
+                barrier_expect_bytes(&k_full[s], S::block * filled + p.extra_bytes);
+                fetch(k_at + s * S::k_bytes, S::block, &launch.k_map, kv_head, z, p.total_k, &k_full[s]);
+                if (round > 0 && !(fine = wait_alone(&v_empty[s], (round - 1) & 1))) {
+                    barrier_wait_bounded(&k_full[s], round & 1, p.wait_limit_ns);
+                    break;
+                }
+                barrier_expect_bytes(&v_full[s], S::block * filled);
+                fetch(v_at + s * S::k_bytes, S::block, &launch.v_map, kv_head, z, p.total_k, &v_full[s]);
+            }
+            // Nothing is on its way into shared memory when the CTA ends.  (Without a failure every copy has been waited for.)
+            if (*(volatile uint32_t*)&give_up || !fine) {
+                barrier_wait_bounded(&q_full, 0, p.wait_limit_ns);
+                for (int i = max(asked - S::stages, 0); i < asked; ++i) {
+                    barrier_wait_bounded(&k_full[i % S::stages], (i / S::stages) & 1, p.wait_limit_ns);
+                    barrier_wait_bounded(&v_full[i % S::stages], (i / S::stages) & 1, p.wait_limit_ns);
+                }
+            }
+        }
+    } else if (warp == kIssueWarp) {
+        constexpr bool bfloat = __is_same(Elem, __nv_bfloat16);
+        const uint32_t score_kind = product_descriptor(bfloat, false, kTileRows, S::block);
+        const uint32_t context_kind = product_descriptor(bfloat, true, kTileRows, launch.dims16);
+        const auto score = [&](int t, int s, int place) {  // S = Q K^T of a tile and a stage of keys
+            bool add = false;
+            for (int sum = S::parts - 1; sum >= 0; --sum) {  // (the smallest products first)
+                for (int part = 0; part <= sum; ++part) {
+                    for (int step = 0; step < launch.steps; ++step) {
+                        const uint32_t inside = step % 4 * 32;
+                        const uint32_t a = q_at + t * S::q_bytes + part * S::q_part + step / 4 * (kTileRows * 128) + inside;
+                        const uint32_t c = k_at + s * S::k_bytes + (sum - part) * S::k_part + step / 4 * (S::block * 128) + inside;
+                        product_of_shared(tensor + place, operand_descriptor(a, 16, 1024), operand_descriptor(c, 16, 1024), score_kind, add);
+                        add = true;
+                    }
+                }
+            }
+        };
+        const auto weigh = [&](int t, int s, bool add) {  // O += P V
+            for (int sum = S::parts - 1; sum >= 0; --sum) {
+                for (int part = 0; part <= sum; ++part) {
+                    for (int step = 0; step < S::block / 16; ++step) {
+                        const uint32_t a = tensor + S::weight_at + t * S::block + part * S::weight_part + step * 8;
+                        const uint32_t c = v_at + s * S::k_bytes + (sum - part) * S::k_part + step * (16 * 128);
+                        product_of_tensor(tensor + S::context_at + t * S::dims, a, operand_descriptor(c, S::block * 128, 1024), context_kind, add);
+                        add = true;
+                    }
+                }
+            }
+        };
+        // Values behind the sequence's last key become zeros, by the whole warp, when their block has arrived.
+        const auto clear_tail = [&](int c, int s) {
+            const int64_t real = keys - (begin + c) * S::block;
+            if (real >= S::block) return;
+            const int rows = S::block - (int)real;
+            for (int slab = 0; slab < S::parts * S::slabs; ++slab) {
+                uint4* row = reinterpret_cast<uint4*>(shared + (v_at - q_at) + s * S::k_bytes + slab * (S::block * 128) + real * 128);
+                for (int i = lane; i < rows * 8; i += 32) row[i] = make_uint4(0, 0, 0, 0);
+            }
+            shared_writes_before_async();
+            __syncwarp();
+        };
+        const auto arrive = [&](uint64_t* bar) {
+            if (lane == 0) products_arrive(bar);
+        };
+        const auto stage_wait = [&](uint64_t* full, int c) { return wait(&full[c % S::stages], (c / S::stages) & 1); };
+        bool fine = most == 0 || (wait(&q_full, 0) && stage_wait(k_full, 0));
+        if (most > 0 && fine) {
+            tensor_fence_after();
+            if constexpr (S::tiles == 2) {
+                for (int t = 0; t < 2; ++t) {
+                    if (counts[t] == 0) continue;
+                    if (lane == 0) score(t, 0, S::score_at + t * S::block);
+                    arrive(&score_full[t]);
+                }
+                arrive(&k_empty[0]);
+                for (int c = 0; c < most && fine; ++c) {
+                    fine = stage_wait(v_full, c);
+                    if (!fine) break;
+                    clear_tail(c, c % S::stages);
+                    bool next = false;  // the next block's keys are there
+                    for (int t = 0; t < 2 && fine; ++t) {
+                        if (c >= counts[t]) continue;
+                        fine = wait(&weight_full[t], c & 1);
+                        if (!fine) break;
+                        tensor_fence_after();
+                        if (lane == 0) weigh(t, c % S::stages, c > 0);
+                        if (c + 1 == counts[t]) {
+                            arrive(&context_full[t]);
+                            continue;
+                        }
+                        if (!next) fine = next = stage_wait(k_full, c + 1);
+                        if (!fine) break;
+                        if (lane == 0) score(t, (c + 1) % S::stages, S::score_at + t * S::block);
+                        arrive(&score_full[t]);
+                    }
+                    arrive(&v_empty[c % S::stages]);
+                    if (next) arrive(&k_empty[(c + 1) % S::stages]);
+                }
+            } else {
+                if (lane == 0) score(0, 0, S::score_at);
+                arrive(&score_full[0]);
+                arrive(&k_empty[0]);
+                for (int c = 0; c < most && fine; ++c) {
+                    if (c + 1 < most) {  // (the place of block c - 1's scores: its weights are complete, hence read)
+                        fine = stage_wait(k_full, c + 1);
+                        if (!fine) break;
+                        if (lane == 0) score(0, (c + 1) % S::stages, S::score_at + ((c + 1) & 1) * S::block);
+                        arrive(&score_full[(c + 1) & 1]);
+                        arrive(&k_empty[(c + 1) % S::stages]);
+                    }
+                    fine = stage_wait(v_full, c);
+                    if (!fine) break;
+                    clear_tail(c, c % S::stages);
+                    fine = wait(&weight_full[0], c & 1);
+                    if (!fine) break;
+                    tensor_fence_after();
+                    if (lane == 0) weigh(0, c % S::stages, c > 0);
+                    arrive(&context_full[0]);
+                    arrive(&v_empty[c % S::stages]);
+                }
+            }
+        }
+        // Every product has ended before tensor memory is given back.
+        arrive(&drained);
+        barrier_wait_bounded(&drained, 0, p.wait_limit_ns);
+    } else {
+        const int t = warp / 4;
+        const int64_t row = row0 + t * kTileRows + (warp % 4) * 32 + lane;  // this thread's query
+        const uint32_t lanes = tensor + ((uint32_t)(warp % 4) << 21);        // (32 lanes further: bits 16 up)
+        const uint32_t context_at = lanes + S::context_at + t * S::dims;
+        const int64_t end = sight.end(row), first = sight.first(row);
+        // What all queries of the warp see needs no mask.
+        const int64_t warp_row = row - lane, all_end = sight.end(warp_row), all_first = sight.first(min(warp_row + 31, max(queries - 1, (int64_t)0)));
+        const int count = counts[t];
+        const float scale = p.scale * kLog2e;
+        const float factor = fabsf(scale) < 1e-37f ? copysignf(1e-37f, scale) : scale;  // (masked scores times it stay infinite)
+        const bool turned = factor < 0.0f;  // the lowest score weighs most
+        const float masked = turned ? -kNone : kNone;
+        float top = masked, total = 0.0f;   // of the scores before the factor
+        bool fine = true;
+        for (int c = 0; c < count; ++c) {
+            const int place = S::tiles == 2 ? t : c & 1;
+            fine = wait(&score_full[place], S::tiles == 2 ? c & 1 : (c / 2) & 1);
+            if (!fine) break;
+            tensor_fence_after();
+            float x[S::block];
+#pragma unroll
+            for (int i = 0; i < S::block; i += 32) tensor_load32(lanes + S::score_at + place * S::block + i, x + i);
+            tensor_loads_done();
+            const int64_t key = (begin + c) * S::block;
+            if (key < all_first || key + S::block > all_end) {
+                const int low = (int)min(max(first - key, (int64_t)0), (int64_t)S::block), high = (int)min(max(end - key, (int64_t)0), (int64_t)S::block);
+#pragma unroll
+                for (int i = 0; i < S::block; ++i) x[i] = i >= low && i < high ? x[i] : masked;
+            }
+            float best = x[0];
+            if (turned) {
+#pragma unroll
+                for (int i = 1; i < S::block; ++i) best = fminf(best, x[i]);
+            } else {
+                float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int i = 4; i < S::block; i += 4) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], x[i + k]);
+                }
+                best = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            }
+            // The reference point moves only where the weights would grow beyond 2^8.
+            const float grown = top == masked ? (best == masked ? 0.0f : -kNone) : (best - top) * factor;
+            const bool moves = grown > kMostGrowth;
+            float less = 1.0f;
+            if (moves) {
+                less = top == masked ? 0.0f : exp2_approx(-grown);
+                top = best;
+                total *= less;
+            }
+            if constexpr (S::tiles == 1) {  // the products that read this tile's weights and write its context have ended
+                if (c > 0) {
+                    fine = wait(&context_full[0], (c - 1) & 1);
+                    if (!fine) break;
+                    tensor_fence_after();
+                }
+            }
+            if (c > 0 && __any_sync(0xffffffffu, moves)) {
+                for (int i = 0; i < launch.dims16; i += 32) {
+                    float o[32];
+                    tensor_load32(context_at + i, o);
+                    tensor_loads_done();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] *= less;
+                    tensor_store32(context_at + i, reinterpret_cast<const uint32_t*>(o));
+                }
+            }
+            const float offset = top == masked ? 0.0f : -top * factor;
+            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < S::block; i += 32) {
+                uint32_t packed[S::parts][16];
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    float w0 = exp2_approx(fmaf(x[i + k], factor, offset)), w1 = exp2_approx(fmaf(x[i + k + 1], factor, offset));
+                    sums[k & 2] += w0;
+                    sums[(k & 2) + 1] += w1;
+#pragma unroll
+                    for (int part = 0; part < S::parts; ++part) {
+                        const uint32_t two = pack(w0, w1, Elem{});
+                        packed[part][k / 2] = two;
+                        if (part + 1 < S::parts) {  // (bf16: what is left is exact)
+                            w0 -= __uint_as_float(two << 16);
+                            w1 -= __uint_as_float(two & 0xffff0000u);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int part = 0; part < S::parts; ++part) {
+                    tensor_store16(lanes + S::weight_at + t * S::block + part * S::weight_part + i / 2, packed[part]);
+                }
+            }
+            total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            tensor_stores_done();
+            tensor_fence_before();
+            barrier_arrive(&weight_full[t]);
+        }
+        if (count > 0 && fine) {
+            fine = wait(&context_full[t], S::tiles == 2 ? 0 : (count - 1) & 1);
+            tensor_fence_after();
+        }
+        if (fine) {
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+            Out* out = static_cast<Out*>(p.out) + ((q_begin + row) * p.heads + head) * p.head_dim;
+            for (int i = 0; i < p.head_dim; i += 32) {
+                float o[32];
+                if (count > 0) {
+                    tensor_load32(context_at + i, o);
+                    tensor_loads_done();
+                }
+                if (row < queries) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        if (i + k >= p.head_dim) break;
+                        if constexpr (sizeof(Out) == 4) {
+                            float4 a = make_float4(o[k] * inverse, o[k + 1] * inverse, o[k + 2] * inverse, o[k + 3] * inverse);
+                            float4 c = make_float4(o[k + 4] * inverse, o[k + 5] * inverse, o[k + 6] * inverse, o[k + 7] * inverse);
+                            if (total == 0.0f) a = c = make_float4(0, 0, 0, 0);
+                            reinterpret_cast<float4*>(out + i + k)[0] = a;
+                            reinterpret_cast<float4*>(out + i + k)[1] = c;
+                        } else {
+                            uint4 a = make_uint4(pack(o[k] * inverse, o[k + 1] * inverse, Elem{}), pack(o[k + 2] * inverse, o[k + 3] * inverse, Elem{}),
+                                                 pack(o[k + 4] * inverse, o[k + 5] * inverse, Elem{}), pack(o[k + 6] * inverse, o[k + 7] * inverse, Elem{}));
+                            if (total == 0.0f) a = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(out + i + k) = a;
+                        }
+                    }
+                }
+            }
+        }
+        tensor_fence_before();
+    }
+    __syncthreads();
+    if (warp == kIssueWarp) {
+        tensor_fence_after();
+        tensor_free(tensor, 512);
+    }
+    if (threadIdx.x == 0 && give_up && p.status) atomicOr(p.status, 1);
+}
+
+// Each fp32 number as three bf16 numbers that add up to it, (part, position, head, dimension).
+__global__ void split_kernel(const float* from, __nv_bfloat16* to, int64_t positions, int64_t stride, int width) {
+    const int64_t fours = positions * (width / 4), all = positions * width;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < fours; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t position = i / (width / 4), at = i % (width / 4) * 4;
+        const float4 four = *reinterpret_cast<const float4*>(from + position * stride + at);
+        float x[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            __nv_bfloat16 h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool finite = fabsf(x[k]) < -kNone;
+                h[k] = __float2bfloat16_rn(x[k]);
+                if (finite && !(fabsf(__bfloat162float(h[k])) < -kNone)) h[k] = __float2bfloat16_rz(x[k]);  // (the largest floats)
+                x[k] = finite ? x[k] - __bfloat162float(h[k]) : 0.0f;
+            }
+            *reinterpret_cast<uint2*>(to + part * all + position * width + at) = *reinterpret_cast<const uint2*>(h);
+        }
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+    static const EncodeTiled found = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &result) != cudaSuccess ||
+            result != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return found;
+}
+
+// (dimension, head, position): boxes of 64 dimensions of one head and `rows` positions.
+bool encode(CUtensorMap* map, bool bfloat, const void* at, int64_t positions, int64_t stride, int heads, int head_dim, int rows) {
+    const cuuint64_t sizes[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)std::max<int64_t>(positions, 1)};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)rows}, steps[3] = {1, 1, 1};
+    return encoder()(map, bfloat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(at), sizes, strides, box, steps,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class Elem, class Out, class S>
+cudaError_t launch(const PromptAttentionParams& p, cudaStream_t stream, int* launches) {
+    constexpr bool bfloat = __is_same(Elem, __nv_bfloat16);
+    static OncePerDevice raised;
+    const auto kernel = prompt_attention_kernel<Elem, Out, S>;
+    // 1024 bytes to start on a boundary of that.  More than half of an SM's, so that a CTA has the tensor memory for itself.
+    const size_t shared = S::shared + 1024 + (size_t)(p.batch + 1) * sizeof(int);
+    static_assert(S::shared > 114 << 10);
+    int device = 0;
+    if (const cudaError_t e = cudaGetDevice(&device)) return e;
+    const cudaError_t e = raised.run(device, [&] {
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(S::shared + 1024 + (kMostPrefixRows + 1) * sizeof(int)));
+    });
+    if (e != cudaSuccess) return e;
+    PromptLaunch l;
+    l.p = p;
+    l.steps = (p.head_dim + 15) / 16;
+    l.dims16 = l.steps * 16;
+    const void *q = p.q, *k = p.k, *v = p.v;
+    int64_t q_rows = p.total_q, k_rows = p.total_k, q_stride = p.q_stride, k_stride = p.k_stride, v_stride = p.v_stride;
+    if constexpr (S::parts == 3) {
+        auto* to = static_cast<__nv_bfloat16*>(p.split);
+        const auto split = [&](const void* from, int64_t positions, int64_t stride, int heads) {
+            const int width = heads * p.head_dim;
+            __nv_bfloat16* parts = to;
+            to += 3 * positions * width;
+            if (positions > 0) {
+                const int64_t blocks = (positions * (width / 4) + 255) / 256;
+                split_kernel<<<(unsigned)std::min<int64_t>(blocks, 148 * 8), 256, 0, stream>>>(static_cast<const float*>(from), parts, positions, stride, width);
+                ++*launches;
+            }
+            return parts;
+        };
+        q = split(p.q, p.total_q, p.q_stride, p.heads);
+        k = split(p.k, p.total_k, p.k_stride, p.kv_heads);
+        v = split(p.v, p.total_k, p.v_stride, p.kv_heads);
+        q_rows *= 3, k_rows *= 3;
+        q_stride = (int64_t)p.heads * p.head_dim;
+        k_stride = v_stride = (int64_t)p.kv_heads * p.head_dim;
+    }
+    if (p.total_k == 0) k = v = q, k_stride = v_stride = (int64_t)p.kv_heads * p.head_dim;  // (never read)
+    if (!encode(&l.q_map, bfloat, q, q_rows, q_stride, p.heads, p.head_dim, kTileRows) ||
+        !encode(&l.k_map, bfloat, k, k_rows, k_stride, p.kv_heads, p.head_dim, S::block) ||
+        !encode(&l.v_map, bfloat, v, k_rows, v_stride, p.kv_heads, p.head_dim, S::block)) {
+        return cudaErrorInvalidValue;
+    }
+    const int64_t row_groups = p.total_q / (S::tiles * kTileRows) + p.batch;  // no more than these
+    kernel<<<(unsigned)(row_groups * p.heads), S::threads, shared, stream>>>(l);
+    ++*launches;
+    return cudaGetLastError();
+}
+
+template <class Elem, class Out, int parts>
+cudaError_t launch_dims(const PromptAttentionParams& p, cudaStream_t stream, int* launches) {
+    if (p.head_dim <= 64) return launch<Elem, Out, Shape<64, parts>>(p, stream, launches);
+    return launch<Elem, Out, Shape<128, parts>>(p, stream, launches);
+}
+
+}  // namespace
+
+size_t prompt_split_bytes(const PromptAttentionParams& p) {
+    if (p.type != kFloat32) return 0;
+    return (size_t)6 * p.head_dim * (p.total_q * p.heads + 2 * p.total_k * p.kv_heads);
+}
+
+cudaError_t launch_prompt_attention(const PromptAttentionParams& p, cudaStream_t stream, int* launches) {
+    *launches = 0;
+    if (!encoder()) return cudaErrorNotSupported;
+    if (p.type == kFloat32) return launch_dims<__nv_bfloat16, float, 3>(p, stream, launches);
+    if (p.type == kBfloat16) return launch_dims<__nv_bfloat16, __nv_bfloat16, 1>(p, stream, launches);
+    return launch_dims<__half, __half, 1>(p, stream, launches);
+}
+
+}  // namespace psx

@@ -80,7 +80,8 @@ PyObject* invoke(psx_status (*fn)(A...), PyObject* const* args, Py_ssize_t count
 #define PSX_CALLS(X)                                                                                                     \
     X(sample_rows) X(sample_rows_static) X(sample_rows_host) X(process_logits_host) X(shard_scan) X(shard_merge_rows)   \
     X(exchange_sample) X(top_k_rows) X(lm_head_logits) X(lm_head_sample_rows) X(softmax_rows) X(logsumexp_rows)         \
-    X(gather_rows) X(decode_attention) X(beam_select) X(reorder_states) X(store_cache_8bit) X(decode_attention_8bit)
+    X(gather_rows) X(decode_attention) X(beam_select) X(reorder_states) X(store_cache_8bit) X(decode_attention_8bit)    \
+    X(prompt_attention)
 
 #define PSX_DEFINE(name)                                                                                         \
     decltype(&psx_b200_##name) g_##name = nullptr;                                                               \

@@ -127,3 +127,4 @@ def test_beam_and_cache_entry_points_check_their_arguments_before_touching_a_gpu
     assert lib.psx_b200_decode_attention_8bit(None, None, None, 0, C.addressof(cache), None, None, 1, 1, 1.0, 1, 0) == binding.ERR_BAD_ARGUMENT
     # as a C compiler lays out psx_beam_state and psx_cache_8bit
     assert C.sizeof(binding.BeamState) == 40 and C.sizeof(binding.Cache8bitLayout) == 72
+    assert lib.psx_b200_prompt_attention(None, None, 0, None, None, None, None, 0, 0, 0, 0, 0, None, None, 0, 1, 1, 8, 1.0, 1, 0, None) == binding.ERR_BAD_ARGUMENT

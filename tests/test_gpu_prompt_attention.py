@@ -1,0 +1,235 @@
+"""Attention of whole prompts (psx_b200_prompt_attention) against the formula in double precision.
+
+Tolerance: a score is a sum of head_dim products in float, off by sqrt(head_dim) * 2^-23 or so of the sum of its terms' sizes
+(fp32 operands: the dropped products of parts add 2^-23 of it), and twice a factor's rounding; a weight is off by that, by 2^-22 of the
+exponential and by its rounding to the operands' type (half a step; fp32: 2^-24); a context by twice its weights' error and
+its sums', times the largest value, plus half a step of its own."""
+import numpy as np
+import pytest
+
+import gpu_harness as gh
+import pulsatrix_b200 as psx
+
+pytestmark = pytest.mark.gpu
+HALF_STEP = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}
+
+
+def _attention(q, k, v, q_at, k_at, scale, causal, window):
+    """(context, nan where no sequence is; per element the slack that its sequence's sizes give)"""
+    heads, kv_heads = q.shape[1], k.shape[1]
+    out, most, value = np.full(q.shape, np.nan), np.zeros(q.shape[0]), np.zeros(q.shape[0])
+    for b in range(len(q_at) - 1):
+        n, m = q_at[b + 1] - q_at[b], k_at[b + 1] - k_at[b]
+        if n <= 0:
+            continue
+        rows = slice(q_at[b], q_at[b + 1])
+        out[rows] = 0
+        if m <= 0:
+            continue
+        place, j = m - n + np.arange(n)[:, None], np.arange(m)[None, :]
+        seen = j <= place if causal else np.ones((n, m), dtype=bool)
+        if causal and window:
+            seen &= j > place - window
+        for h in range(heads):
+            kk, vv = k[k_at[b]:k_at[b + 1], h // (heads // kv_heads)], v[k_at[b]:k_at[b + 1], h // (heads // kv_heads)]
+            s = np.where(seen, q[rows, h] @ kk.T * scale, -np.inf)
+            w = np.exp(s - np.where(seen.any(1), s.max(1), 0)[:, None])
+            total = w.sum(1, keepdims=True)
+            out[rows, h] = (w / np.where(total > 0, total, 1)) @ vv
+            most[rows] = np.maximum(most[rows], (np.abs(q[rows, h]) @ np.abs(kk).T).max(1) * abs(scale))
+            value[rows] = np.maximum(value[rows], np.abs(vv).max())
+    return out, most, value
+
+
+def _slack(dtype, most, value, head_dim, keys):
+    score = most * (2 * np.sqrt(head_dim) + 4) * 2.0 ** -23
+    weight = 2 * score + 2.0 ** -21 + 2 * HALF_STEP[dtype] + (np.sqrt(keys) + 8) * 2.0 ** -23
+    return (weight * value)[:, None, None]
+
+
+def _tensor(x, dtype):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).to(getattr(torch, dtype)).cuda()
+
+
+def _check(dtype, q_lens, k_lens, heads, kv_heads, head_dim, causal=True, window=0, scale=None, seed=0, lead=0, behind=0, ctx=None, size=1.0):
+    """lead, behind: positions before the first sequence and behind the last one, that belong to none."""
+    import torch
+    rng = np.random.RandomState(seed + head_dim + sum(q_lens))
+    q_at, k_at = (lead + np.concatenate([[0], np.cumsum(n)]).astype(np.int64) for n in (q_lens, k_lens))
+    q, k, v = (_tensor(rng.randn(n[-1] + behind, h, head_dim) * s, dtype) for n, h, s in ((q_at, heads, size), (k_at, kv_heads, size), (k_at, kv_heads, 1.0)))
+    clean = [x.double().cpu().numpy() for x in (q, k, v)]
+    for x, n in ((q, q_at), (k, k_at), (v, k_at)):  # what belongs to no sequence
+        x[:lead] = float("nan")
+        x[n[-1]:] = float("inf")
+    out = torch.full_like(q, 7.0)
+    got, status = (ctx or gh.ctx()).prompt_attention(q, k, v, torch.from_numpy(q_at).cuda(), torch.from_numpy(k_at).cuda(), causal=causal, window=window,
+                                                     scale=scale, out=out)
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0
+    want, most, value = _attention(*clean, q_at, k_at, head_dim ** -0.5 if scale is None else scale, causal, window)
+    got = got.double().cpu().numpy()
+    none = np.isnan(want)
+    assert (got[none] == 7.0).all()
+    slack = _slack(dtype, most, value, head_dim, max(k_lens)) + HALF_STEP[dtype] * np.abs(want)
+    bad = ~(np.abs(got - want) <= slack) & ~none
+    assert not bad.any(), (np.argwhere(bad)[:5], np.abs(got - want)[bad][:5], slack[bad][:5])
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("head_dim", [64, 128, 96, 80, 8, 72])
+def test_one_block(dtype, head_dim):
+    _check(dtype, [100], [100], 2, 1, head_dim)
+    _check(dtype, [128], [64], 1, 1, head_dim, causal=False)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("head_dim", [64, 128, 88])
+@pytest.mark.parametrize("length", [1, 2, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300, 511, 700])
+def test_every_length(dtype, head_dim, length):
+    _check(dtype, [length], [length], 2, 2, head_dim)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (6, 2), (8, 1), (5, 5)])
+def test_packed_sequences_and_head_layouts(dtype, heads, kv_heads):
+    _check(dtype, [130, 1, 0, 300, 17, 256, 64], [130, 1, 0, 300, 17, 256, 64], heads, kv_heads, 64, lead=3, behind=70)
+    _check(dtype, [5, 200, 33], [205, 200, 600], heads, kv_heads, 128, behind=200)     # prompts that continue a prefix
+    _check(dtype, [300, 140, 9], [100, 0, 8], heads, kv_heads, 64)                       # queries before the first key see nothing
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("causal,window", [(False, 0), (False, 9), (True, 1), (True, 50), (True, 128), (True, 129), (True, 300), (True, 2 ** 50)])
+def test_masks(dtype, causal, window):
+    _check(dtype, [500, 77, 260], [500, 300, 260], 2, 1, 64, causal=causal, window=window, seed=window % 100)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_scales_and_scores_of_every_size(dtype):
+    for scale in (0.0, -0.125, 1e-30, 2.0):
+        _check(dtype, [200], [200], 2, 1, 64, scale=scale, seed=3)
+    _check(dtype, [300], [300], 1, 1, 128, size=6.0)   # scores of some hundred: maxima that grow from block to block
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_long_prompts(dtype):
+    _check(dtype, [2500, 1111], [2500, 1500], 2, 1, 128)
+
+
+def test_many_short_sequences():
+    rng = np.random.RandomState(8)
+    lens = rng.randint(0, 40, 700).tolist()
+    _check("bfloat16", lens, lens, 3, 1, 64)
+    _check("float32", lens[:300], lens[:300], 2, 2, 64)
+
+
+def test_slices_of_one_projection():
+    import torch
+    rng = np.random.RandomState(9)
+    for dtype in ("bfloat16", "float32"):
+        wide = _tensor(rng.randn(333, 4 + 2 + 2, 64), dtype)
+        q, k, v = wide[:, :4], wide[:, 4:6], wide[:, 6:]
+        at = torch.tensor([0, 33, 333], device="cuda")
+        a, _ = gh.ctx().prompt_attention(q, k, v, at)
+        b, _ = gh.ctx().prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), at)
+        assert (a == b).all()
+
+
+def test_a_nan_stays_in_its_sequence():
+    import torch
+    rng = np.random.RandomState(10)
+    for dtype in ("bfloat16", "float32"):
+        q, k, v = (_tensor(rng.randn(300, 2, 64), dtype) for _ in range(3))
+        at = torch.tensor([0, 100, 200, 300], device="cuda")
+        want, _ = gh.ctx().prompt_attention(q, k, v, at)
+        for x in (q, k, v):
+            x[150:200] = float("nan")
+        got, _ = gh.ctx().prompt_attention(q, k, v, at)
+        assert (got[:100] == want[:100]).all() and (got[200:] == want[200:]).all() and got[150:200].isnan().all()
+
+
+def test_the_same_call_gives_the_same_bits_and_graphs_replay():
+    import torch
+    rng = np.random.RandomState(11)
+    for dtype in ("bfloat16", "float32"):
+        ctx = psx.Context(0)
+        q, k, v = (_tensor(rng.randn(900, h, 64), dtype) for h in (4, 2, 2))
+        at = torch.tensor([0, 300, 900], device="cuda")
+        first = ctx.prompt_attention(q, k, v, at)[0].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, status = ctx.prompt_attention(q, k, v, at)
+        big = _tensor(rng.randn(3000, 4, 64), dtype)
+        ctx.prompt_attention(big, big, big, torch.tensor([0, 3000], device="cuda"))  # (the scratch grows)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert (out == first).all() and int(status) == 0
+        at.copy_(torch.tensor([0, 10, 800]))
+        want = ctx.prompt_attention(q, k, v, at)[0]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (out[:800] == want[:800]).all()
+
+
+def test_another_stream_and_the_device_stays():
+    import torch
+    s = torch.cuda.Stream()
+    q = torch.randn(200, 2, 64, device="cuda").bfloat16()
+    at = torch.tensor([0, 200], device="cuda")
+    want = gh.ctx().prompt_attention(q, q, q, at)[0]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        got = gh.ctx().prompt_attention(q, q, q, at)[0]
+    s.synchronize()
+    assert (got == want).all()
+
+
+def test_a_wait_that_runs_out_is_reported():
+    import torch
+    for dtype in ("bfloat16", "float32"):
+        ctx = psx.Context(0)
+        q = torch.randn(1000, 2, 64, device="cuda").to(getattr(torch, dtype))
+        at = torch.tensor([0, 1000], device="cuda")
+        want = ctx.prompt_attention(q, q, q, at)[0]
+        ctx.set_wait_limit(20_000_000)
+        ctx.test_short_copy(True)
+        assert int(ctx.prompt_attention(q, q, q, at)[1].cpu()) == 1
+        ctx.test_short_copy(False)
+        got, status = ctx.prompt_attention(q, q, q, at)
+        assert int(status.cpu()) == 0 and (got == want).all()
+
+
+def test_refusals():
+    import torch
+    ctx = gh.ctx()
+    at = torch.tensor([0, 4], device="cuda")
+
+    def call(heads=2, kv_heads=1, head_dim=64, dtype=torch.bfloat16, offsets=at, **kw):
+        q, k = torch.zeros(4, heads, head_dim, dtype=dtype, device="cuda"), torch.zeros(4, kv_heads, head_dim, dtype=dtype, device="cuda")
+        return ctx.prompt_attention(q, k, k, offsets, **kw)
+
+    for status, kw in ((psx.ERR_BAD_ARGUMENT, dict(heads=3, kv_heads=2)), (psx.ERR_UNSUPPORTED, dict(head_dim=136)), (psx.ERR_UNSUPPORTED, dict(head_dim=20, dtype=torch.float32)),
+                       (psx.ERR_BAD_ARGUMENT, dict(scale=float("inf"))), (psx.ERR_BAD_ARGUMENT, dict(window=-1)),
+                       (psx.ERR_UNSUPPORTED, dict(offsets=torch.zeros(4098, dtype=torch.int64, device="cuda")))):
+        with pytest.raises(psx.PsxError) as e:
+            call(**kw)
+        assert e.value.status == status
+    with pytest.raises(TypeError):
+        call(dtype=torch.float64)
+    for kw in (dict(offsets=at.int()), dict(k_offsets=at[:1]), dict(out=torch.zeros(4, 2, 64, device="cuda"))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    flat = torch.zeros(4 * 128 + 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(psx.PsxError) as e:  # a base that is not on a 16-byte boundary
+        x = flat[1:1 + 4 * 128].view(4, 2, 64)
+        ctx.prompt_attention(x, x, x, at)
+    assert e.value.status == psx.ERR_BAD_ARGUMENT
+    q = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    assert ctx.prompt_attention(q, q, q, torch.tensor([0, 0], device="cuda"))[0].shape == (0, 2, 64)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    out, _ = ctx.prompt_attention(x, q, q, torch.tensor([0, 3], device="cuda"), torch.tensor([0, 0], device="cuda"))  # no keys at all
+    assert (out == 0).all()
