@@ -2,7 +2,9 @@
 call goes through the C ABI into the CUDA kernels."""
 from __future__ import annotations
 
+import array
 import ctypes as C
+import math
 import os
 from pathlib import Path
 
@@ -244,18 +246,26 @@ def sample_rows_static(logits, history_ids, history_offsets, config, uniforms, t
         _check(status_code)
 
 
+_torch = None
+_DTYPES = {}  # torch dtype -> psx_dtype
+
+
+def _torch_module():
+    """torch, imported by the first call that needs it (and looked up once: a call takes a few microseconds altogether)."""
+    global _torch
+    if _torch is None:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+        _torch = torch
+    return _torch
+
+
 def _dtype_code(tensor):
     """The psx_dtype of a tensor."""
-    import torch
-    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(tensor.dtype)
+    code = _DTYPES.get(tensor.dtype)
     if code is None:
         raise TypeError(f"float32, bfloat16 or float16 is expected, got {tensor.dtype}")
     return code
-
-
-def _need(condition, message):
-    if not condition:
-        raise ValueError(message)
 
 
 class Cache8bit:
@@ -263,19 +273,23 @@ class Cache8bit:
     head_dim), torch.float8_e4m3fn or uint8, and float32 scales (batch, kv_heads, ceil(max_len / block)), all contiguous."""
 
     def __init__(self, key_codes, key_scales, value_codes, value_scales, block=32):
-        import torch
-        _need(key_codes.dim() == 4 and block > 0, "codes are (batch, kv_heads, max_len, head_dim)")
-        batch, kv_heads, max_len, head_dim = key_codes.shape
-        for codes in (key_codes, value_codes):
-            _need(codes.shape == key_codes.shape and codes.is_contiguous() and codes.dtype in (torch.float8_e4m3fn, torch.uint8),
-                  "codes are contiguous float8_e4m3fn or uint8 tensors of one shape")
-        for scales in (key_scales, value_scales):
-            _need(tuple(scales.shape) == (batch, kv_heads, -(-max_len // block)) and scales.is_contiguous() and scales.dtype == torch.float32,
-                  "scales are contiguous float32 tensors, one for every `block` positions")
-        _need(len({t.get_device() for t in (key_codes, key_scales, value_codes, value_scales)}) == 1, "a cache lies on one device")
+        torch = _torch or _torch_module()
+        shape = key_codes.shape
+        if len(shape) != 4 or block <= 0:
+            raise ValueError("codes are (batch, kv_heads, max_len, head_dim)")
+        batch, kv_heads, max_len, head_dim = shape
+        if not (value_codes.shape == shape and key_codes.is_contiguous() and value_codes.is_contiguous() and
+                key_codes.dtype in (torch.float8_e4m3fn, torch.uint8) and value_codes.dtype in (torch.float8_e4m3fn, torch.uint8)):
+            raise ValueError("codes are contiguous float8_e4m3fn or uint8 tensors of one shape")
+        scales = (batch, kv_heads, -(-max_len // block))
+        if not (key_scales.shape == scales and value_scales.shape == scales and key_scales.is_contiguous() and value_scales.is_contiguous() and
+                key_scales.dtype is torch.float32 and value_scales.dtype is torch.float32):
+            raise ValueError("scales are contiguous float32 tensors, one for every `block` positions")
+        self.device = device = key_codes.get_device()
+        if not device == key_scales.get_device() == value_codes.get_device() == value_scales.get_device():
+            raise ValueError("a cache lies on one device")
         self.key_codes, self.key_scales, self.value_codes, self.value_scales = key_codes, key_scales, value_codes, value_scales
         self.batch, self.kv_heads, self.max_len, self.head_dim, self.block = batch, kv_heads, max_len, head_dim, block
-        self.device = key_codes.get_device()
         self._layout = Cache8bitLayout(key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(), value_scales.data_ptr(), batch,
                                        kv_heads, max_len, head_dim, block)
         self._address = C.addressof(self._layout)
@@ -537,96 +551,125 @@ class Context:
                                         cached, max_len, float(scale), int(bool(causal)), window, status.data_ptr()))
         return context, status
 
-    # ---- beams, states that follow them, the cache in 8 bits ---------------------------------------------
+    # ---- beams, states that follow them, the cache in 8 bits, prompts -------------------------------------
+    def _elsewhere(self, tensor):
+        return ValueError(f"tensors on cuda:{self.device} are expected, got one on {tensor.device}")
+
     def _here(self, *tensors):
         for t in tensors:
-            if t is not None and t.get_device() != self.device:
-                raise ValueError(f"tensors on cuda:{self.device} are expected, got one on {t.device}")
+            if t.get_device() != self.device:
+                raise self._elsewhere(t)
 
     def beam_select(self, logits, scores, beams, keep, finished=None, finished_token=0, vocab=None, stream=None):
         """Beam search's selection (psx_b200_beam_select).  logits: cuda float32 (groups * beams, vocab), rows contiguous; scores:
         float32 (groups * beams); finished: bool or uint8 (groups * beams) or None.  Returns {"scores", "parents", "tokens"} of
         shape (groups, keep) and "status" (groups)."""
-        import torch
-        rows = logits.shape[0]
-        vocab = logits.shape[1] if vocab is None else vocab
-        _need(beams > 0 and rows % beams == 0, "logits hold `beams` rows per group")
-        _need(logits.dtype == torch.float32 and scores.dtype == torch.float32, "logits and scores are float32")
-        _need(0 < vocab <= logits.shape[1] and (rows == 0 or logits.stride(1) == 1), "a row's logits are contiguous")
-        _need(scores.numel() == rows and scores.is_contiguous(), "one score per row")
+        torch = _torch or _torch_module()
+        rows, columns = logits.shape
+        vocab = columns if vocab is None else vocab
+        if beams <= 0 or rows % beams or not 0 < vocab <= columns:
+            raise ValueError("logits hold `beams` rows per group, of `vocab` columns at least")
+        if not (logits.dtype is torch.float32 and scores.dtype is torch.float32 and scores.numel() == rows and scores.is_contiguous()):
+            raise ValueError("logits are float32, and so are the scores, one per row")
+        row_stride, column_stride = logits.stride()
+        if rows == 1:
+            row_stride = columns
+        if column_stride != 1 and rows:
+            raise ValueError("a row's logits are contiguous")
+        self._here(logits, scores)
         if finished is not None:
-            _need(finished.numel() == rows and finished.is_contiguous() and finished.element_size() == 1, "one byte per row says what is finished")
-        self._here(logits, scores, finished)
+            if not (finished.numel() == rows and finished.is_contiguous() and finished.element_size() == 1):
+                raise ValueError("one byte per row says what is finished")
+            self._here(finished)
         groups = rows // beams
         stream = _stream_of(logits) if stream is None else stream
         shape, device = (groups, max(keep, 0)), logits.device
-        out = {"scores": torch.empty(shape, dtype=torch.float32, device=device), "parents": torch.empty(shape, dtype=torch.int64, device=device),
-               "tokens": torch.empty(shape, dtype=torch.int64, device=device), "status": torch.empty(groups, dtype=torch.int32, device=device)}
-        _check(_native.beam_select(self._handle, stream, logits.data_ptr(), groups, beams, vocab, logits.stride(0) if rows > 1 else logits.shape[1],
-                                   scores.data_ptr(), _ptr(finished), finished_token, keep, out["scores"].data_ptr(), out["parents"].data_ptr(),
-                                   out["tokens"].data_ptr(), out["status"].data_ptr()))
-        return out
+        out_scores, parents = torch.empty(shape, device=device, dtype=torch.float32), torch.empty(shape, dtype=torch.int64, device=device)
+        tokens, status = torch.empty_like(parents), torch.empty(groups, dtype=torch.int32, device=device)
+        code = _native.beam_select(self._handle, stream, logits.data_ptr(), groups, beams, vocab, row_stride, scores.data_ptr(),
+                                   None if finished is None else finished.data_ptr(), finished_token, keep, out_scores.data_ptr(),
+                                   parents.data_ptr(), tokens.data_ptr(), status.data_ptr())
+        if code:
+            _check(code)
+        return {"scores": out_scores, "parents": parents, "tokens": tokens, "status": status}
 
     def reorder_states(self, parents, states, lengths=None, stream=None):
         """Rows of states that follow their beams, in place (psx_b200_reorder_states).  parents: int64 (groups, beams), row
         numbers within the group; states: tensors (groups * beams, heads, positions, ...), contiguous, each alone or as (tensor,
         tokens per position); lengths: int64 (groups * beams), the tokens that each row holds before, or None for all positions."""
-        import torch
-        _need(parents.dim() == 2 and parents.dtype == torch.int64 and parents.is_contiguous(), "parents are contiguous int64 (groups, beams)")
+        torch = _torch or _torch_module()
+        if not (parents.dim() == 2 and parents.dtype is torch.int64 and parents.is_contiguous()):
+            raise ValueError("parents are contiguous int64 (groups, beams)")
         groups, beams = parents.shape
-        described = (BeamState * len(states))()
-        for entry, state in zip(described, states):
-            tensor, per = state if isinstance(state, (tuple, list)) else (state, 1)
-            _need(tensor.dim() >= 3 and tensor.shape[0] == groups * beams and tensor.is_contiguous(),
-                  "a state is a contiguous (groups * beams, heads, positions, ...) tensor")
-            self._here(tensor)
-            size = tensor.element_size()
-            for n in tensor.shape[3:]:
-                size *= n
-            if size == 0:  # (nothing to move)
-                entry.data, entry.heads, entry.positions, entry.position_bytes, entry.tokens_per_position = None, 0, 0, 1, 1
-                continue
-            entry.data, entry.heads, entry.positions = tensor.data_ptr(), tensor.shape[1], tensor.shape[2]
-            entry.position_bytes, entry.tokens_per_position = size, per
+        rows, here = groups * beams, self.device
+        described = []  # (psx_beam_state: five words)
+        for state in states:
+            tensor, per = state if type(state) in (tuple, list) else (state, 1)
+            shape = tensor.shape
+            if len(shape) < 3 or shape[0] != rows or not tensor.is_contiguous():
+                raise ValueError("a state is a contiguous (groups * beams, heads, positions, ...) tensor")
+            if tensor.get_device() != here:
+                raise self._elsewhere(tensor)
+            heads, positions = shape[1], shape[2]
+            size = tensor.element_size() * (shape[3] if len(shape) == 4 else math.prod(shape[3:]))
+            described += (tensor.data_ptr(), heads, positions, size, per) if size else (0, 0, 0, 1, 1)  # (nothing to move)
+        described = array.array("q", described)
         if lengths is not None:
-            _need(lengths.dtype == torch.int64 and lengths.numel() == groups * beams and lengths.is_contiguous(), "one int64 length per row")
-        self._here(parents, lengths)
-        _check(_native.reorder_states(self._handle, _stream_of(parents) if stream is None else stream, C.addressof(described), len(states), groups,
-                                      beams, parents.data_ptr(), _ptr(lengths)))
+            if not (lengths.dtype is torch.int64 and lengths.numel() == rows and lengths.is_contiguous()):
+                raise ValueError("one int64 length per row")
+            self._here(lengths)
+        self._here(parents)
+        code = _native.reorder_states(self._handle, _stream_of(parents) if stream is None else stream, described.buffer_info()[0], len(states), groups,
+                                      beams, parents.data_ptr(), None if lengths is None else lengths.data_ptr())
+        if code:
+            _check(code)
 
     def store_cache_8bit(self, cache, keys, values, offsets, cached, stream=None):
         """Appends new positions to a Cache8bit (psx_b200_store_cache_8bit).  keys, values: float32, bfloat16 or float16 (total,
         kv_heads, head_dim), the rows' new positions one row behind the other, heads and dimensions contiguous; offsets: int64
         (batch + 1); cached: int64 (batch), the positions held before.  Returns the rows' statuses, int32 (batch)."""
-        import torch
-        _need(keys.dim() == 3 and keys.shape == values.shape and keys.dtype == values.dtype and tuple(keys.shape[1:]) == (cache.kv_heads, cache.head_dim),
-              "keys and values are (total, kv_heads, head_dim) of one type")
-        for t in (keys, values):
-            _need(t.shape[0] == 0 or (t.stride(2) == 1 and t.stride(1) == cache.head_dim), "heads and dimensions of a position are contiguous")
-        _need(offsets.dtype == torch.int64 and offsets.numel() == cache.batch + 1 and offsets.is_contiguous(), "offsets are int64 (batch + 1)")
-        _need(cached.dtype == torch.int64 and cached.numel() == cache.batch and cached.is_contiguous(), "cached is int64 (batch)")
-        self._here(cache.key_codes, keys, values, offsets, cached)
-        total, width = keys.shape[0], cache.kv_heads * cache.head_dim
-        status = torch.empty(cache.batch, dtype=torch.int32, device=offsets.device)
-        _check(_native.store_cache_8bit(self._handle, _stream_of(keys) if stream is None else stream, cache._address, keys.data_ptr(), values.data_ptr(),
-                                        _dtype_code(keys), total, keys.stride(0) if total > 1 else width, values.stride(0) if total > 1 else width,
-                                        offsets.data_ptr(), cached.data_ptr(), status.data_ptr()))
+        torch = _torch or _torch_module()
+        shape, kv_heads, head_dim, batch = keys.shape, cache.kv_heads, cache.head_dim, cache.batch
+        total = shape[0]
+        if not (shape == (total, kv_heads, head_dim) and values.shape == shape and keys.dtype is values.dtype):
+            raise ValueError("keys and values are (total, kv_heads, head_dim) of one type")
+        key_stride, value_stride = keys.stride(), values.stride()
+        if total and not (key_stride[2] == value_stride[2] == 1 and (kv_heads == 1 or key_stride[1] == value_stride[1] == head_dim)):
+            raise ValueError("heads and dimensions of a position are contiguous")
+        if not (offsets.dtype is torch.int64 and offsets.numel() == batch + 1 and offsets.is_contiguous() and
+                cached.dtype is torch.int64 and cached.numel() == batch and cached.is_contiguous()):
+            raise ValueError("offsets are int64 (batch + 1), cached is int64 (batch)")
+        here = self.device
+        if not (cache.device == here == keys.get_device() == values.get_device() == offsets.get_device() == cached.get_device()):
+            self._here(cache.key_codes, keys, values, offsets, cached)
+        status = torch.empty(batch, dtype=torch.int32, device=offsets.device)
+        width = kv_heads * head_dim
+        code = _native.store_cache_8bit(self._handle, _stream_of(keys) if stream is None else stream, cache._address, keys.data_ptr(), values.data_ptr(),
+                                        _dtype_code(keys), total, key_stride[0] if total > 1 else width, value_stride[0] if total > 1 else width,
+                                        offsets.data_ptr(), cached.data_ptr(), status.data_ptr())
+        if code:
+            _check(code)
         return status
 
     def decode_attention_8bit(self, q, cache, lengths, scale=None, causal=True, window=0, stream=None):
         """Attention of the new positions over a Cache8bit (psx_b200_decode_attention_8bit).  q: float32, bfloat16 or float16
         (batch, heads, q_len, head_dim); lengths: int64 (batch), the positions that each row sees, the new ones among them.
         Returns the context, like q."""
-        import torch
+        torch = _torch or _torch_module()
         batch, heads, q_len, head_dim = q.shape
-        _need(batch == cache.batch and head_dim == cache.head_dim and q.is_contiguous(), "q is a contiguous (batch, heads, q_len, head_dim) as the cache")
-        _need(lengths.dtype == torch.int64 and lengths.numel() == batch and lengths.is_contiguous(), "lengths are int64 (batch)")
-        self._here(q, cache.key_codes, lengths)
+        if not (batch == cache.batch and head_dim == cache.head_dim and q.is_contiguous()):
+            raise ValueError("q is a contiguous (batch, heads, q_len, head_dim) as the cache")
+        if not (lengths.dtype is torch.int64 and lengths.numel() == batch and lengths.is_contiguous()):
+            raise ValueError("lengths are int64 (batch)")
+        if not (cache.device == self.device == q.get_device() == lengths.get_device()):
+            self._here(q, cache.key_codes, lengths)
         if scale is None:
-            scale = 1.0 / float(np.sqrt(np.float32(head_dim)))
+            scale = head_dim ** -0.5
         context = torch.empty_like(q)
-        _check(_native.decode_attention_8bit(self._handle, _stream_of(q) if stream is None else stream, q.data_ptr(), _dtype_code(q), cache._address,
-                                             lengths.data_ptr(), context.data_ptr(), heads, q_len, float(scale), int(bool(causal)), window))
+        code = _native.decode_attention_8bit(self._handle, _stream_of(q) if stream is None else stream, q.data_ptr(), _dtype_code(q), cache._address,
+                                             lengths.data_ptr(), context.data_ptr(), heads, q_len, scale, 1 if causal else 0, window)
+        if code:
+            _check(code)
         return context
 
     def prompt_attention(self, q, k, v, q_offsets, k_offsets=None, scale=None, causal=True, window=0, out=None, stream=None):
@@ -634,27 +677,39 @@ class Context:
         (total_q, heads, head_dim); k, v: (total_k, kv_heads, head_dim); heads and dimensions of a position contiguous; q_offsets,
         k_offsets: int64 (batch + 1), the latter the same as q_offsets if None.  Returns the context, (total_q, heads, head_dim)
         (`out` if given: rows of no sequence keep what they hold), and a one-element int32 status tensor."""
-        import torch
-        k_offsets = q_offsets if k_offsets is None else k_offsets
-        total_q, heads, head_dim = q.shape
-        total_k, kv_heads = k.shape[0], k.shape[1]
-        _need(k.shape == v.shape and k.shape[2] == head_dim and q.dtype == k.dtype == v.dtype, "q, k and v are of one type and head dimension")
-        strides = []
-        for t, width in ((q, heads * head_dim), (k, kv_heads * head_dim), (v, kv_heads * head_dim)):
-            _need(t.shape[0] == 0 or (t.stride(2) == 1 and (t.stride(1) == head_dim or t.shape[1] == 1)), "heads and dimensions of a position are contiguous")
-            strides.append(t.stride(0) if t.shape[0] > 1 else width)
-        _need(q_offsets.dtype == torch.int64 and q_offsets.is_contiguous() and q_offsets.numel() > 0, "offsets are int64 (batch + 1)")
-        _need(k_offsets.dtype == torch.int64 and k_offsets.is_contiguous() and k_offsets.numel() == q_offsets.numel(), "offsets are int64 (batch + 1)")
+        torch = _torch or _torch_module()
+        if k_offsets is None:
+            k_offsets = q_offsets
+        q_shape, k_shape = q.shape, k.shape
+        total_q, heads, head_dim = q_shape
+        total_k, kv_heads, k_dim = k_shape
+        if not (v.shape == k_shape and k_dim == head_dim and q.dtype is k.dtype is v.dtype):
+            raise ValueError("q, k and v are of one type and head dimension")
+        q_stride, k_stride, v_stride = q.stride(), k.stride(), v.stride()
+        if not ((total_q == 0 or (q_stride[2] == 1 and (heads == 1 or q_stride[1] == head_dim))) and
+                (total_k == 0 or (k_stride[2] == v_stride[2] == 1 and (kv_heads == 1 or k_stride[1] == v_stride[1] == head_dim)))):
+            raise ValueError("heads and dimensions of a position are contiguous")
+        batch = q_offsets.numel() - 1
+        if not (q_offsets.dtype is k_offsets.dtype is torch.int64 and batch >= 0 and k_offsets.numel() == batch + 1 and q_offsets.is_contiguous() and
+                k_offsets.is_contiguous()):
+            raise ValueError("offsets are int64 (batch + 1)")
         if out is None:
-            out = torch.empty((total_q, heads, head_dim), dtype=q.dtype, device=q.device)
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out is contiguous and of q's shape and type")
-        self._here(q, k, v, out, q_offsets, k_offsets)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q_shape, dtype=q.dtype, device=q.device)
+        elif not (out.shape == q_shape and out.dtype is q.dtype and out.is_contiguous()):
+            raise ValueError("out is contiguous and of q's shape and type")
+        here = self.device
+        if not (q.get_device() == here == k.get_device() == v.get_device() == q_offsets.get_device() == k_offsets.get_device() == out.get_device()):
+            self._here(q, k, v, out, q_offsets, k_offsets)
         if scale is None:
-            scale = 1.0 / float(np.sqrt(np.float32(head_dim)))
-        status = _zeroed_word(q.device, stream)
-        _check(_native.prompt_attention(self._handle, _stream_of(q) if stream is None else stream, _dtype_code(q), q.data_ptr(), k.data_ptr(),
-                                        v.data_ptr(), out.data_ptr(), total_q, total_k, *strides, q_offsets.data_ptr(), k_offsets.data_ptr(),
-                                        q_offsets.numel() - 1, heads, kv_heads, head_dim, float(scale), int(bool(causal)), window, status.data_ptr()))
+            scale = head_dim ** -0.5
+        status = torch.empty(1, dtype=torch.int32, device=q.device)
+        code = _native.prompt_attention(self._handle, _stream_of(q) if stream is None else stream, _dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                        out.data_ptr(), total_q, total_k, q_stride[0] if total_q > 1 else heads * head_dim,
+                                        k_stride[0] if total_k > 1 else kv_heads * head_dim, v_stride[0] if total_k > 1 else kv_heads * head_dim,
+                                        q_offsets.data_ptr(), k_offsets.data_ptr(), batch, heads, kv_heads, head_dim, scale, 1 if causal else 0, window,
+                                        status.data_ptr())
+        if code:
+            _check(code)
         return out, status
 
     # ---- vocabulary-sharded -----------------------------------------------------------------------------

@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPartList = 1024, kGroupList = 1024;
+constexpr int kHeldEntries = 12;  // per thread of the second kernel: 8 beams of 19 parts with 16 each in all
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -202,6 +203,15 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
     const int64_t group = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, keep = p.keep;
     if (threadIdx.x == 0) listed = 0, not_finite = 0;
+    // The first entries of every thread are asked for ahead of the normalisers, and kept.
+    const BeamEntry* entries = p.entries + group * p.beams * p.parts * keep;
+    const int per_beam = p.parts * keep, all = p.beams * per_beam;
+    BeamEntry held[kHeldEntries];
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) {
+        const int e = i * kThreads + threadIdx.x;
+        held[i] = e < all ? entries[e] : BeamEntry{kNone, -1};
+    }
     __syncthreads();
     for (int b = warp; b < p.beams; b += kWarps) {
         const int64_t row = group * p.beams + b;
@@ -229,16 +239,20 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
         }
     }
     __syncthreads();
-    const BeamEntry* entries = p.entries + group * p.beams * p.parts * keep;
-    const int per_beam = p.parts * keep, all = p.beams * per_beam;
-    const auto candidate = [&](int e) {
-        const BeamEntry entry = entries[e];
+    const auto candidate_of = [&](int e, BeamEntry entry) {
         const int b = e / per_beam;
         return Candidate{base[b] + (double)entry.logit, (uint64_t)b << 32 | (uint32_t)entry.token};
     };
+    const auto candidate = [&](int e) { return candidate_of(e, entries[e]); };
+    constexpr int kHeld = kHeldEntries * kThreads;
     float largest = kNone;
+#pragma unroll
+    for (int i = 0; i < kHeldEntries; ++i) {
+        const int e = i * kThreads + threadIdx.x;
+        if (e < all) largest = fmaxf(largest, as_float(candidate_of(e, held[i]).value));
+    }
 #pragma unroll 4
-    for (int e = threadIdx.x; e < all; e += kThreads) largest = fmaxf(largest, as_float(candidate(e).value));
+    for (int e = kHeld + threadIdx.x; e < all; e += kThreads) largest = fmaxf(largest, as_float(candidate(e).value));
     const uint32_t mine = warp_bound(largest, keep, nullptr);
     if (lane == 0) bounds[warp] = mine;
     __syncthreads();
@@ -247,13 +261,18 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
     const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
     // (rounding to float keeps the order: what is at or above the bound in double is so in float)
     if (largest >= bound && largest > kNone) {
-        for (int e = threadIdx.x; e < all; e += kThreads) {
-            const Candidate c = candidate(e);
+        const auto offer = [&](const Candidate& c) {
             if (c.value > (double)kNone && as_float(c.value) >= bound) {
                 const int at = atomicAdd(&listed, 1);
                 if (at < kGroupList) list[at] = c;
             }
+        };
+#pragma unroll
+        for (int i = 0; i < kHeldEntries; ++i) {
+            const int e = i * kThreads + threadIdx.x;
+            if (e < all) offer(candidate_of(e, held[i]));
         }
+        for (int e = kHeld + threadIdx.x; e < all; e += kThreads) offer(candidate(e));
     }
     __syncthreads();
     const int count = listed;

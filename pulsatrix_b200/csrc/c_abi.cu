@@ -1341,7 +1341,14 @@ psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dty
     if (q_stride < heads * head_dim || k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim) {
         return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a position's stride is at least its heads times head_dim");
     }
-    if (batch == 0 || total_q == 0) return PSX_OK;
+    if (batch == 0 || total_q == 0) {
+        if (status) {
+            const OnDevice device(ctx->device);
+            PSX_CUDA(device.error);
+            PSX_CUDA(cudaMemsetAsync(status, 0, sizeof(int32_t), static_cast<cudaStream_t>(stream_ptr)));
+        }
+        return PSX_OK;
+    }
     if (!q || !out || !q_offsets || !k_offsets || (total_k > 0 && (!k || !v))) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
     const uintptr_t lies = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                            reinterpret_cast<uintptr_t>(out) | (uintptr_t)((q_stride | k_stride | v_stride) * psx::element_bytes(dtype));
@@ -1359,6 +1366,7 @@ psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dty
         if (psx_status s = reserve_kept(ctx, stream, ctx->prompt_parts, psx::prompt_split_bytes(p))) return s;
         p.split = ctx->prompt_parts.ptr;
     }
+    if (status) PSX_CUDA(cudaMemsetAsync(status, 0, sizeof(int32_t), stream));
     int launches = 0;
     const cudaError_t e = psx::launch_prompt_attention(p, stream, &launches);
     ctx->launches += launches;

@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
         __syncthreads();
         const bool whole = from_tile == 0 && to_tile == tiles;
         T* context = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
-        const int piece_floats = kRows * (dims + 2);
+        const int piece_floats = kRows * (dims + 4);
         float* piece = p.partial + ((int64_t)blockIdx.x * 2 + (at == (int64_t)blockIdx.x * share ? 0 : 1)) * piece_floats;
         for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) {
             const int r = i / head_dim, d = i % head_dim;
@@ -415,10 +415,10 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
             if (whole) {
                 context[i] = from_float<T>(sum == 0.0f ? 0.0f : value / sum);
             } else {
-                __stcg(piece + r * (dims + 2) + d, value);
+                __stcg(piece + r * (dims + 4) + d, value);
                 if (d == 0) {
-                    __stcg(piece + r * (dims + 2) + dims, high);
-                    __stcg(piece + r * (dims + 2) + dims + 1, sum);
+                    __stcg(piece + r * (dims + 4) + dims, high);
+                    __stcg(piece + r * (dims + 4) + dims + 1, sum);
                 }
             }
         }
@@ -434,22 +434,46 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
             }
             __syncthreads();
             if (is_last) {
-                const auto piece_of = [&](int64_t block) {
-                    return p.partial + (block * 2 + (block == first && begin != block * share ? 1 : 0)) * piece_floats;
-                };
-                for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) {
-                    const int r = i / head_dim, d = i % head_dim;
-                    float high = kNone, sum = 0.0f, value = 0.0f;
-                    for (int64_t b = first; b <= last; ++b) high = fmaxf(high, __ldcg(piece_of(b) + r * (dims + 2) + dims));
-                    for (int64_t b = first; b <= last; ++b) {
-                        const float* from = piece_of(b) + r * (dims + 2);
-                        const float part = __ldcg(from + dims + 1);
-                        if (part == 0.0f) continue;
-                        const float less = exp2_approx(__ldcg(from + dims) - high);
-                        sum += part * less;
-                        value += __ldcg(from + d) * less;
+                const int pieces = (int)(last - first) + 1;
+                const float* base = p.partial + first * 2 * piece_floats;  // (the first piece is its block's second one unless it starts it)
+                const int skip = begin != first * share ? piece_floats : 0;
+                float* less = reinterpret_cast<float*>(shared);  // (piece, row): what a piece's sums count for
+                for (int i = threadIdx.x; i < pieces * p.rows; i += kThreads) {
+                    const int b = i / p.rows, r = i % p.rows;
+                    less[i] = __ldcg(base + (b == 0 ? skip : (int64_t)b * 2 * piece_floats) + r * (dims + 4) + dims);
+                }
+                __syncthreads();
+                for (int r = warp; r < p.rows; r += kWarps) {
+                    float high = kNone, sum = 0.0f;
+                    for (int b = lane; b < pieces; b += 32) high = fmaxf(high, less[b * p.rows + r]);
+#pragma unroll
+                    for (int step = 16; step > 0; step /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, step));
+                    for (int b = lane; b < pieces; b += 32) {
+                        const float mine = less[b * p.rows + r];
+                        const float factor = mine > kNone ? exp2_approx(mine - high) : 0.0f;
+                        less[b * p.rows + r] = factor;
+                        sum += factor * __ldcg(base + (b == 0 ? skip : (int64_t)b * 2 * piece_floats) + r * (dims + 4) + dims + 1);
                     }
-                    context[i] = from_float<T>(sum == 0.0f ? 0.0f : value / sum);
+#pragma unroll
+                    for (int step = 16; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+                    if (lane == 0) totals[0][r] = sum;
+                }
+                __syncthreads();
+                const int fours = head_dim / 4;
+                for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
+                    const int r = i / fours, d = i % fours * 4;
+                    const float* from = base + r * (dims + 4) + d;
+                    float4 value = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+                    for (int b = 0; b < pieces; ++b) {
+                        const float4 part = __ldcg(reinterpret_cast<const float4*>(from + (b == 0 ? skip : (int64_t)b * 2 * piece_floats)));
+                        const float factor = less[b * p.rows + r];
+                        value.x += part.x * factor, value.y += part.y * factor, value.z += part.z * factor, value.w += part.w * factor;
+                    }
+                    const float inverse = totals[0][r] == 0.0f ? 0.0f : 1.0f / totals[0][r];
+                    T* to = context + r * head_dim + d;
+                    to[0] = from_float<T>(value.x * inverse), to[1] = from_float<T>(value.y * inverse);
+                    to[2] = from_float<T>(value.z * inverse), to[3] = from_float<T>(value.w * inverse);
                 }
             }
         }
@@ -495,7 +519,7 @@ int attention_8bit_grid(const Attention8bitParams& p, int sm_count) {
 
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p) {
     const int rows = p.rows <= 8 ? 8 : 16;
-    return (size_t)p.grid * 2 * rows * (padded_dims(p) + 2) * sizeof(float);
+    return (size_t)p.grid * 2 * rows * (padded_dims(p) + 4) * sizeof(float);
 }
 
 cudaError_t launch_decode_attention_8bit(const Attention8bitParams& p, cudaStream_t stream) {
