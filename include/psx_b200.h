@@ -354,7 +354,7 @@ PSX_API psx_status psx_b200_decode_attention(psx_ctx* ctx, void* stream, const f
  *                is left at all
  * keep may be larger than beams (twice as many leave enough when finished ones are set aside).  Limits: beams <= 64,
  * keep <= 128, vocab <= 2^30 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; the outputs must not overlap the inputs.
- * The context's scratch grows to groups * beams * (vocab / 2048) * (keep * 8 + 16) bytes at most; inside a stream capture it
+ * The context's scratch grows to groups * beams * (vocab / 1024) * (keep * 8 + 16) bytes at most; inside a stream capture it
  * cannot grow (PSX_ERR_UNSUPPORTED): make a call of that size before. */
 PSX_API psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream, const float* logits, int64_t groups, int64_t beams, int64_t vocab,
                                         int64_t row_stride, const float* scores, const uint8_t* finished, int64_t finished_token,
@@ -392,8 +392,8 @@ typedef struct psx_cache_8bit {
 
 /* Appends new positions to such a cache (KVCache::append, src/kv_cache.cpp, in 8 bits): prompts, or the one position of a
  * decoding step.  keys, values: device, `dtype`, (total, kv_heads, head_dim) with the positions of all rows one row behind the
- * other, a position at keys + i * key_stride elements (a slice of a wider projection will do; 16-byte aligned for fp32 and
- * 8-byte for the others, strides multiples of four).  Row b's are offsets[b] .. offsets[b + 1] (device int64, batch + 1) and become
+ * other, a position at keys + i * key_stride elements (a slice of a wider projection will do; positions start on
+ * 16-byte boundaries).  Row b's are offsets[b] .. offsets[b + 1] (device int64, batch + 1) and become
  * positions cached[b] onwards (device int64, batch).
  * A block's scale is the least power of two 2^e, e >= -100, at which 448 * 2^e reaches the largest finite magnitude of its new
  * elements, or the scale that the block has where that is larger and the block holds cached positions; codes are

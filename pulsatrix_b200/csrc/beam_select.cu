@@ -2,19 +2,20 @@
 //
 //     value(b, v) = (score_b - log sum_w exp(l_bw)) + l_bv        (double precision; ties: the lowest b, then the lowest v)
 //
-// First kernel, a block per part of a row (8192 logits, or 2048 where those would leave SMs idle): the logits are read once,
-// into registers; the part leaves its maximum, its sum of exponentials and its `keep` best logits in order.  Within a row the
-// order by value is the order by logit, so nothing else of the part can be among the group's best.  The `keep` best are found
-// without sorting the part: every warp gives the n-th largest of its lanes' maxima, n = ceil(keep / 8), and the smallest of
-// those over the eight warps is a bound that at least `keep` logits reach; what reaches it goes on a list (some more than
-// `keep`), and an entry's place is the number of keys above its own.  A list that overflows (thousands of equal logits) is
-// replaced by `keep` sweeps over the registers.  Bound by HBM: 4 bytes per logit.
+// First kernel, a block per part of a row: the logits are read once, in chunks of 16 per thread (4 where that would leave SMs
+// idle) with the next chunk on its way, a running maximum and sum per thread; the part leaves its maximum, its sum of
+// exponentials and its `keep` best logits in order.  Within a row the order by value is the order by logit, so nothing else of
+// the part can be among the group's best.  The `keep` best are found without sorting the part: every warp gives the n-th
+// largest of its lanes' maxima, n = ceil(keep / 8), and the smallest of those over the eight warps is a bound that at least
+// `keep` logits reach.  The few chunks whose maximum reaches it are read again, out of L2, and what reaches it goes on a list
+// (some more than `keep`); an entry's place is the number of keys above its own.  A list that overflows (thousands of equal
+// logits) is replaced by `keep` sweeps over those chunks.  Bound by HBM: 4 bytes per logit.
 //
 // Second kernel, a block per group: the rows' normalisers from the parts' sums, then the same selection over the parts' lists.
 // It is launched early and waits for the first kernel's end.
 //
-// The exponentials are summed in float over a thread's 8 or 32 logits, relative to the warp's maximum, and in double from
-// there on, in an order that depends on columns alone: equal rows have equal normalisers, so that their candidates tie.
+// The exponentials are summed in float over a thread's logits, relative to its maximum so far, and in double from there on, in
+// an order that depends on columns alone: equal rows have equal normalisers, so that their candidates tie.
 #include "beam_select.cuh"
 
 #include <algorithm>
@@ -25,8 +26,9 @@ namespace psx {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMostChunks = 8;  // of a part
 constexpr int kPartList = 1024, kGroupList = 1024;
-constexpr int kHeldEntries = 12;  // per thread of the second kernel: 8 beams of 19 parts with 16 each in all
+constexpr int kHeldEntries = 8;  // per thread of the second kernel
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -64,16 +66,30 @@ __device__ __forceinline__ uint64_t block_max(uint64_t key, uint64_t* shared) {
     return key;
 }
 
+// {a, b} + {x, x} and {a, b} * {x, x}, each rounded as alone.
+__device__ __forceinline__ float2 add_pair(float2 a, float2 x) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, x, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tadd.rn.f32x2 r, a, x;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(x.x), "f"(x.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 x) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, x, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tmul.rn.f32x2 r, a, x;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(x.x), "f"(x.y));
+    return r;
+}
+
 template <int values, bool aligned>
-__global__ void __launch_bounds__(kThreads) beam_parts_kernel(const __grid_constant__ BeamSelectParams p) {
-    constexpr int kPart = kThreads * values;
+__global__ void __launch_bounds__(kThreads, 4) beam_parts_kernel(const __grid_constant__ BeamSelectParams p) {
+    constexpr int kChunk = kThreads * values;
     __shared__ uint64_t list[kPartList], best_of[kWarps];
     __shared__ uint32_t bounds[kWarps], tops[kWarps];
     __shared__ double sums[kWarps];
-    __shared__ int listed, not_finite;
+    __shared__ int listed;
     const int64_t part_row = blockIdx.x;
     const int64_t row = part_row / p.parts;
-    const int part = (int)(part_row % p.parts), keep = p.keep, first = part * kPart;
+    const int part = (int)(part_row % p.parts), keep = p.keep, begin = part * p.chunks * kChunk, end = min(begin + p.chunks * kChunk, p.vocab);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     BeamEntry* entries = p.entries + part_row * keep;
     const float score = p.scores[row];
@@ -87,73 +103,97 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const __grid_const
         asm volatile("griddepcontrol.launch_dependents;");
         return;
     }
-    if (threadIdx.x == 0) listed = 0, not_finite = 0;
+    if (threadIdx.x == 0) listed = 0;
 
-    float v[values];
     const float* from = p.logits + row * p.row_stride;
-    // Column of a thread's j-th logit: fours of neighbours where the rows are aligned, neighbours on neighbouring lanes else.
-    const auto column = [&](int j) {
-        return aligned ? first + j / 4 * (kThreads * 4) + (int)threadIdx.x * 4 + j % 4 : first + j * kThreads + (int)threadIdx.x;
+    // Column of a thread's j-th logit of a chunk: fours of neighbours where the rows are aligned, neighbours on neighbouring lanes else.
+    const auto column = [&](int chunk, int j) {
+        return begin + chunk * kChunk + (aligned ? j / 4 * (kThreads * 4) + (int)threadIdx.x * 4 + j % 4 : j * kThreads + (int)threadIdx.x);
     };
-    if constexpr (aligned) {
+    const auto load = [&](int chunk, float (&v)[values], auto read) {
+        if constexpr (aligned) {
 #pragma unroll
-        for (int j = 0; j < values; j += 4) {
-            float4 x = make_float4(kNone, kNone, kNone, kNone);
-            if (column(j) < p.vocab) x = __ldcs(reinterpret_cast<const float4*>(from + column(j)));
-            v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
+            for (int j = 0; j < values; j += 4) {
+                float4 x = make_float4(kNone, kNone, kNone, kNone);
+                if (column(chunk, j) < end) x = read(reinterpret_cast<const float4*>(from + column(chunk, j)));
+                v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < values; ++j) v[j] = column(chunk, j) < end ? read(from + column(chunk, j)) : kNone;
         }
-    } else {
+    };
+    const auto stream = [](auto* at) { return __ldcs(at); };
+    const auto again = [](auto* at) { return __ldcg(at); };
+
+    // The running maximum and sum of this thread, and the maximum of each of its chunks; the next chunk is on its way meanwhile.
+    float v[2][values], chunk_top[kMostChunks], top = kNone, sum = 0.0f;
+    load(0, v[0], stream);
 #pragma unroll
-        for (int j = 0; j < values; ++j) v[j] = column(j) < p.vocab ? __ldcs(from + column(j)) : kNone;
-    }
-    float largest = kNone;
-    bool wrong = false;
+    for (int c = 0; c < kMostChunks; ++c) {
+        chunk_top[c] = kNone;
+        if (c < p.chunks) {
+            if (c + 1 < kMostChunks && c + 1 < p.chunks) load(c + 1, v[(c + 1) % 2], stream);
+            const float(&x)[values] = v[c % 2];
+            float high[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-    for (int j = 0; j < values; ++j) {
-        largest = fmaxf(largest, v[j]);
-        wrong |= !(v[j] < -kNone);
-    }
-    uint32_t top_key;
-    const uint32_t mine = warp_bound(largest, keep, &top_key);
-    const float top = from_ordered(top_key);
-    float sum = 0.0f;
-    if (top > kNone) {
+            for (int j = 4; j < values; j += 4) {
 #pragma unroll
-        for (int j = 0; j < values; ++j) sum += exp2_approx((v[j] - top) * kLog2e);
+                for (int k = 0; k < 4; ++k) high[k] = fmaxf(high[k], x[j + k]);
+            }
+            chunk_top[c] = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+            const float next = fmaxf(top, chunk_top[c]), level = next > kNone ? next : 0.0f;
+            float2 part_sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+#pragma unroll
+            for (int j = 0; j < values; j += 2) {
+                const float2 d = mul_pair(add_pair(make_float2(x[j], x[j + 1]), make_float2(-level, -level)), make_float2(kLog2e, kLog2e));
+                part_sum[j / 2 % 2] = add_pair(part_sum[j / 2 % 2], make_float2(exp2_approx(d.x), exp2_approx(d.y)));
+            }
+            sum = sum * exp2_approx((top - level) * kLog2e) + ((part_sum[0].x + part_sum[0].y) + (part_sum[1].x + part_sum[1].y));
+            top = next;
+        }
     }
-    double total = sum;
+    // (A NaN or +inf among the logits makes the sum NaN: the maximum passes over a NaN, and inf - inf is one.)
+    uint32_t warp_top_key;
+    const uint32_t mine = warp_bound(top, keep, &warp_top_key);
+    const float warp_level = from_ordered(warp_top_key);
+    double total = sum * exp2_approx((top - (warp_level > kNone ? warp_level : 0.0f)) * kLog2e);
 #pragma unroll
     for (int step = 16; step > 0; step /= 2) total += __shfl_xor_sync(0xffffffffu, total, step);
     if (lane == 0) {
         bounds[warp] = mine;
-        tops[warp] = top_key;
+        tops[warp] = warp_top_key;
         sums[warp] = total;
     }
-    const bool any_wrong = __any_sync(0xffffffffu, wrong);
     __syncthreads();
-    if (any_wrong && lane == 0) not_finite = 1;
     uint32_t bound_key = bounds[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) bound_key = min(bound_key, bounds[w]);
     const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
-    if (largest >= bound && largest > kNone) {
+    uint32_t hits = 0;  // the chunks that reach the bound; they are read again, out of L2
+#pragma unroll
+    for (int c = 0; c < kMostChunks; ++c) hits |= (chunk_top[c] >= bound && chunk_top[c] > kNone) ? 1u << c : 0u;
+    for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
+        const int c = __ffs(rest) - 1;
+        load(c, v[0], again);
 #pragma unroll
         for (int j = 0; j < values; ++j) {
-            if (v[j] >= bound && v[j] > kNone) {
+            if (v[0][j] >= bound && v[0][j] > kNone) {
                 const int at = atomicAdd(&listed, 1);
-                if (at < kPartList) list[at] = entry_key(v[j], column(j));
+                if (at < kPartList) list[at] = entry_key(v[0][j], column(c, j));
             }
         }
     }
     __syncthreads();
     const int count = listed;
-    if (threadIdx.x < 32) {  // the part's record
+    if (warp == kWarps - 1) {  // the part's record
         const float warp_top = lane < kWarps ? from_ordered(tops[lane]) : kNone;
         float part_top = warp_top;
         for (int step = 16; step > 0; step /= 2) part_top = fmaxf(part_top, __shfl_xor_sync(0xffffffffu, part_top, step));
-        double part_sum = lane < kWarps && warp_top > kNone ? sums[lane] * exp((double)warp_top - (double)part_top) : 0.0;
+        const float level = part_top > kNone ? part_top : 0.0f;
+        double part_sum = lane < kWarps ? sums[lane] * exp((double)warp_top - (double)level) : 0.0;
         for (int step = 16; step > 0; step /= 2) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, step);
-        if (lane == 0) p.part_stats[part_row] = {part_sum, part_top, not_finite};
+        if (lane == 0) p.part_stats[part_row] = {part_sum, part_top, part_sum != part_sum};
     }
     int placed = min(count, keep);
     if (count <= kPartList) {
@@ -167,10 +207,14 @@ __global__ void __launch_bounds__(kThreads) beam_parts_kernel(const __grid_const
         uint64_t last = ~0ull;
         for (placed = 0; placed < keep; ++placed) {
             uint64_t best = 0;
+            for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
+                const int c = __ffs(rest) - 1;
+                load(c, v[0], again);
 #pragma unroll
-            for (int j = 0; j < values; ++j) {
-                const uint64_t key = v[j] > kNone ? entry_key(v[j], column(j)) : 0;
-                if (key < last) best = max(best, key);
+                for (int j = 0; j < values; ++j) {
+                    const uint64_t key = v[0][j] > kNone ? entry_key(v[0][j], column(c, j)) : 0;
+                    if (key < last) best = max(best, key);
+                }
             }
             best = block_max(best, best_of);
             if (best == 0) break;
@@ -203,14 +247,22 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
     const int64_t group = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, keep = p.keep;
     if (threadIdx.x == 0) listed = 0, not_finite = 0;
-    // The first entries of every thread are asked for ahead of the normalisers, and kept.
+    // The lists' first entries, the best of all lists, then the second ones and so on, are asked for ahead of the normalisers and
+    // kept.  Every eight neighbours go to the eight warps in an order that changes: the bound is good where each warp has its
+    // share of the best, and one beam's lists are neighbours.
     const BeamEntry* entries = p.entries + group * p.beams * p.parts * keep;
-    const int per_beam = p.parts * keep, all = p.beams * per_beam;
+    const int lists = p.beams * p.parts;
+    constexpr int kHeld = kHeldEntries * kThreads;
+    const int all_held = min(lists * keep, kHeld);
+    const auto place_of = [&](int i) {
+        const uint32_t y = i * 32 + lane;
+        return (int)(y * 8 + ((warp + (y * 2654435761u >> 29)) & 7));
+    };
     BeamEntry held[kHeldEntries];
 #pragma unroll
     for (int i = 0; i < kHeldEntries; ++i) {
-        const int e = i * kThreads + threadIdx.x;
-        held[i] = e < all ? entries[e] : BeamEntry{kNone, -1};
+        const int x = place_of(i);
+        held[i] = x < all_held ? entries[x % lists * keep + x / lists] : BeamEntry{kNone, -1};
     }
     __syncthreads();
     for (int b = warp; b < p.beams; b += kWarps) {
@@ -239,20 +291,16 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
         }
     }
     __syncthreads();
-    const auto candidate_of = [&](int e, BeamEntry entry) {
-        const int b = e / per_beam;
+    const auto candidate_of = [&](int of_list, BeamEntry entry) {
+        const int b = of_list / p.parts;
         return Candidate{base[b] + (double)entry.logit, (uint64_t)b << 32 | (uint32_t)entry.token};
     };
-    const auto candidate = [&](int e) { return candidate_of(e, entries[e]); };
-    constexpr int kHeld = kHeldEntries * kThreads;
     float largest = kNone;
 #pragma unroll
     for (int i = 0; i < kHeldEntries; ++i) {
-        const int e = i * kThreads + threadIdx.x;
-        if (e < all) largest = fmaxf(largest, as_float(candidate_of(e, held[i]).value));
+        const int x = place_of(i);
+        if (x < all_held) largest = fmaxf(largest, as_float(candidate_of(x % lists, held[i]).value));
     }
-#pragma unroll 4
-    for (int e = kHeld + threadIdx.x; e < all; e += kThreads) largest = fmaxf(largest, as_float(candidate(e).value));
     const uint32_t mine = warp_bound(largest, keep, nullptr);
     if (lane == 0) bounds[warp] = mine;
     __syncthreads();
@@ -260,19 +308,24 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
     for (int w = 1; w < kWarps; ++w) bound_key = min(bound_key, bounds[w]);
     const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
     // (rounding to float keeps the order: what is at or above the bound in double is so in float)
+    const auto offer = [&](const Candidate& c) {
+        if (!(c.value > (double)kNone && as_float(c.value) >= bound)) return false;
+        const int at = atomicAdd(&listed, 1);
+        if (at < kGroupList) list[at] = c;
+        return true;
+    };
     if (largest >= bound && largest > kNone) {
-        const auto offer = [&](const Candidate& c) {
-            if (c.value > (double)kNone && as_float(c.value) >= bound) {
-                const int at = atomicAdd(&listed, 1);
-                if (at < kGroupList) list[at] = c;
-            }
-        };
 #pragma unroll
         for (int i = 0; i < kHeldEntries; ++i) {
-            const int e = i * kThreads + threadIdx.x;
-            if (e < all) offer(candidate_of(e, held[i]));
+            const int x = place_of(i);
+            if (x < all_held) offer(candidate_of(x % lists, held[i]));
         }
-        for (int e = kHeld + threadIdx.x; e < all; e += kThreads) offer(candidate(e));
+    }
+    if (all_held < lists * keep) {  // lists are in order: each from where it is not held on, as far as it reaches the bound
+        for (int q = threadIdx.x; q < lists; q += kThreads) {
+            for (int slot = max(kHeld - q + lists - 1, 0) / lists; slot < keep && offer(candidate_of(q, entries[q * keep + slot])); ++slot) {
+            }
+        }
     }
     __syncthreads();
     const int count = listed;
@@ -296,8 +349,8 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
         Candidate last{(double)-kNone, 0};
         for (placed = 0; placed < keep; ++placed) {
             Candidate best{(double)kNone, ~0ull};
-            for (int e = threadIdx.x; e < all; e += kThreads) {
-                const Candidate c = candidate(e);
+            for (int e = threadIdx.x; e < lists * keep; e += kThreads) {
+                const Candidate c = candidate_of(e / keep, entries[e]);
                 if (ahead(last, c) && ahead(c, best)) best = c;
             }
             for (int step = 16; step > 0; step /= 2) {
@@ -327,20 +380,26 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
 
 void plan_beam_select(BeamSelectParams& p, int sm_count) {
     const int64_t rows = p.groups * p.beams;
-    // 32 logits per thread keep enough loads in flight; with fewer blocks than SMs the shorter parts spread the row further.
-    p.values = rows * ((p.vocab + kThreads * 32 - 1) / (kThreads * 32)) < sm_count ? 8 : 32;
-    p.parts = (p.vocab + kThreads * p.values - 1) / (kThreads * p.values);
+    // Long parts cost least per logit (what a part costs besides is shared by up to eight chunks of 4096); where they would be
+    // fewer than the GPU holds at once, shorter ones spread the rows further.
+    const auto chunks = [&](int values) { return (p.vocab + kThreads * values - 1) / (kThreads * values); };
+    p.values = rows * chunks(16) < sm_count ? 4 : 16;
+    const int all = chunks(p.values);
+    p.chunks = kMostChunks;
+    while (p.chunks > 1 && rows * ((all + p.chunks - 1) / p.chunks) < 2 * sm_count) --p.chunks;
+    p.parts = (all + p.chunks - 1) / p.chunks;
+    p.chunks = (all + p.parts - 1) / p.parts;  // (no part much shorter than the others)
     p.aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.row_stride % 4 == 0 && p.vocab % 4 == 0;
 }
 
 cudaError_t launch_beam_select(const BeamSelectParams& p, cudaStream_t stream) {
     const unsigned blocks = (unsigned)(p.groups * p.beams * p.parts);
-    if (p.values == 8) {
-        if (p.aligned) beam_parts_kernel<8, true><<<blocks, kThreads, 0, stream>>>(p);
-        else beam_parts_kernel<8, false><<<blocks, kThreads, 0, stream>>>(p);
+    if (p.values == 4) {
+        if (p.aligned) beam_parts_kernel<4, true><<<blocks, kThreads, 0, stream>>>(p);
+        else beam_parts_kernel<4, false><<<blocks, kThreads, 0, stream>>>(p);
     } else {
-        if (p.aligned) beam_parts_kernel<32, true><<<blocks, kThreads, 0, stream>>>(p);
-        else beam_parts_kernel<32, false><<<blocks, kThreads, 0, stream>>>(p);
+        if (p.aligned) beam_parts_kernel<16, true><<<blocks, kThreads, 0, stream>>>(p);
+        else beam_parts_kernel<16, false><<<blocks, kThreads, 0, stream>>>(p);
     }
     if (const cudaError_t e = cudaGetLastError()) return e;
     cudaLaunchConfig_t config{};

@@ -32,13 +32,14 @@ struct BeamSelectParams {
     int64_t groups, row_stride, finished_token;
     int32_t beams, vocab, keep;
     int32_t parts;            // of a row
-    int32_t values;           // logits per thread of a part's block: 8 or 32
+    int32_t values;           // logits per thread of a chunk: 4 or 16
+    int32_t chunks;           // of a part, 1 to 8
     int32_t aligned;          // every row starts on a 16-byte boundary and is a multiple of four long
     BeamPart* part_stats;     // (groups * beams, parts)
     BeamEntry* entries;       // (groups * beams, parts, keep), best first
 };
 
-// parts, values and aligned, from the sizes and pointers.
+// parts, values, chunks and aligned, from the sizes and pointers.
 void plan_beam_select(BeamSelectParams& p, int sm_count);
 cudaError_t launch_beam_select(const BeamSelectParams& p, cudaStream_t stream);
 

@@ -1260,16 +1260,18 @@ psx_status psx_b200_store_cache_8bit(psx_ctx* ctx, void* stream_ptr, const psx_c
     psx::StoreCacheParams p{};
     if (psx_status s = check_cache_8bit(cache, &p.cache)) return s;
     if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
-    if (total < 0 || total > 0x7fffffff) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the number of new positions is out of range");
+    if (total < 0 || (total / cache->block + 2 * cache->batch) * cache->kv_heads > 0x3fffffff) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the number of new positions is out of range");
+    }
     if (p.cache.batch == 0) return PSX_OK;
     if (!offsets || !cached || (total > 0 && (!keys || !values))) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
     const int64_t width = cache->kv_heads * cache->head_dim;
-    if (key_stride < width || value_stride < width || key_stride % 4 != 0 || value_stride % 4 != 0) {
-        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a position's stride is at least kv_heads * head_dim and a multiple of four");
+    if (key_stride < width || value_stride < width) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a position's stride is at least its heads times head_dim");
     }
-    if ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % (4 * psx::element_bytes(dtype)) != 0) {
-        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: keys and values must start on a boundary of four elements");
-    }
+    const uintptr_t lies = reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values) |
+                           (uintptr_t)((key_stride | value_stride) * psx::element_bytes(dtype));
+    if (lies % 16 != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: keys and values and their positions must start on 16-byte boundaries");
     const OnDevice device(ctx->device);
     PSX_CUDA(device.error);
     p.keys = keys; p.values = values; p.offsets = offsets; p.cached = cached; p.row_status = row_status; p.total = total;

@@ -8,34 +8,37 @@ namespace psx {
 
 constexpr int64_t kMostPrefixRows = 4096;  // (prefix[] is 16 KB of shared memory then)
 
-// prefix[0] = 0, prefix[r + 1] = prefix[r] + count(r) for r < rows; `carry`: shared, one int per warp and one more.  All
+// prefix[0] = 0, prefix[r + 1] = prefix[r] + count(r) for r < rows; `carry`: shared, one int per warp.  All
 // threads of the block (whole warps, 32 at most) call it; the sums are readable by all of them afterwards.
 template <class Count>
 __device__ __forceinline__ void sum_of_rows(int rows, int* prefix, int* carry, Count count) {
     const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (threadIdx.x == 0) prefix[0] = 0;
-    int before = 0;
-    for (int base = 0; base < rows; base += blockDim.x) {
-        const int row = base + threadIdx.x;
-        int sum = row < rows ? count(row) : 0;
+    // Every thread takes neighbouring rows, so that the lengths of many rows are on their way at once.
+    const int each = (rows + (int)blockDim.x - 1) / (int)blockDim.x, first = min((int)threadIdx.x * each, rows), end = min(first + each, rows);
+    int mine = 0;
+#pragma unroll 4
+    for (int row = first; row < end; ++row) mine += count(row);
+    int sum = mine;
 #pragma unroll
-        for (int step = 1; step < 32; step *= 2) {
-            const int other = __shfl_up_sync(0xffffffffu, sum, step);
-            if (lane >= step) sum += other;
-        }
-        if (lane == 31) carry[warp] = sum;
-        __syncthreads();
-        int mine = before, all = before;
-        for (int w = 0; w < warps; ++w) {
-            const int c = carry[w];
-            if (w < warp) mine += c;
-            all += c;
-        }
-        if (row < rows) prefix[row + 1] = mine + sum;
-        before = all;
-        __syncthreads();
+    for (int step = 1; step < 32; step *= 2) {
+        const int other = __shfl_up_sync(0xffffffffu, sum, step);
+        if (lane >= step) sum += other;
     }
-    if (rows == 0) __syncthreads();
+    if (lane == 31) carry[warp] = sum;
+    __syncthreads();
+    int before = sum - mine;
+    for (int w = 0; w < warps; ++w) before += w < warp ? carry[w] : 0;
+    if (threadIdx.x == 0) prefix[0] = 0;
+    if (each == 1) {
+        if (first < end) prefix[first + 1] = before + mine;
+    } else {
+#pragma unroll 4
+        for (int row = first; row < end; ++row) {
+            before += count(row);
+            prefix[row + 1] = before;
+        }
+    }
+    __syncthreads();
 }
 
 // The row whose share holds `item`: prefix[row] <= item < prefix[row + 1].
