@@ -1236,10 +1236,10 @@ psx_status check_cache_8bit(const psx_cache_8bit* c, psx::Cache8bitView* view) {
         return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: cache sizes must be positive");
     }
     if ((c->block != 16 && c->block != 32 && c->block != 64) || c->head_dim % 16 != 0 || c->head_dim > 256 || c->batch > psx::kMostPrefixRows ||
-        c->kv_heads > 65536 || c->max_len > ((int64_t)1 << 36) || std::max<int64_t>(c->batch, 1) * c->kv_heads > 0x7fffffff / (c->max_len / 16 + 1)) {
+        c->kv_heads > 65536 || c->max_len > (1 << 30) || std::max<int64_t>(c->batch, 1) * c->kv_heads > 0x7fffffff / (c->max_len / 16 + 1)) {
         return fail(PSX_ERR_UNSUPPORTED,
                     "psx_b200: a cache in 8 bits has blocks of 16, 32 or 64 positions, a head dimension that is a multiple of 16 up to 256, "
-                    "at most 4096 rows and 2^31 blocks of 16 positions");
+                    "at most 4096 rows, 2^30 positions and 2^31 blocks of 16 positions altogether");
     }
     if (c->batch > 0 && (!c->key_codes || !c->key_scales || !c->value_codes || !c->value_scales)) {
         return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");

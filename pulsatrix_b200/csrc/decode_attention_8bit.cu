@@ -15,7 +15,7 @@
 // The cached positions of all (row, kv head) pairs lie on one axis, in tiles of 32, and every block takes an equal share of it:
 // lengths that differ from row to row leave no SM idle, and one long row is spread over all of them.  A pair that several
 // blocks share leaves a piece per block; the last block to arrive joins them, in order.  Inside a block each of four warps
-// takes every fourth tile, with its own three stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no
+// takes every fourth tile, with its own two stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no
 // warp waits for another until the end of a pair.  Bound by HBM: 2 bytes per position, head dimension and kv head.
 #include "decode_attention_8bit.cuh"
 
@@ -33,7 +33,7 @@ constexpr int kLeastShare = 2 * kWarps;  // tiles: shorter pieces cost more in j
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
-__host__ __device__ constexpr int stages_of(int dims) { return dims > 128 ? 2 : 3; }
+__host__ __device__ constexpr int stages_of(int) { return 2; }
 __host__ __device__ constexpr int stage_bytes(int dims) { return 2 * kTile * dims + 16; }  // keys, values, two scales each
 __host__ __device__ constexpr size_t shared_of(int dims) { return (size_t)kWarps * stages_of(dims) * stage_bytes(dims); }
 
@@ -41,6 +41,9 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
@@ -84,22 +87,21 @@ __device__ __forceinline__ int placed(int row, int chunk) {
 
 // Bounds of what query rows see, in positions.
 struct Sight {
-    int64_t length, first_own;  // the position of the first new one
-    int64_t window;
-    bool causal;
-    __device__ __forceinline__ int64_t last(int i) const { return causal ? first_own + i : length - 1; }
-    __device__ __forceinline__ int64_t first(int i) const { return causal && window > 0 ? first_own + i - window + 1 : 0; }
-    __device__ __forceinline__ int64_t first_tile() const { return max(first(0), (int64_t)0) / kTile; }
-    __device__ __forceinline__ int64_t end_tile() const { return max(length + kTile - 1, (int64_t)0) / kTile; }
+    int length, first_own;  // the position of the first new one
+    int window;             // 0: none
+    __device__ __forceinline__ int last(int i, bool causal) const { return causal ? first_own + i : length - 1; }
+    __device__ __forceinline__ int first(int i) const { return window > 0 ? first_own + i - window + 1 : 0; }
+    __device__ __forceinline__ int first_tile() const { return max(first(0), 0) / kTile; }
+    __device__ __forceinline__ int end_tile() const { return (length + kTile - 1) / kTile; }
 };
 
-__device__ __forceinline__ Sight sight_of(const Attention8bitParams& p, int64_t row) {
-    const int64_t length = min(max(p.lengths[row], (int64_t)0), p.cache.max_len);
-    return {length, length - p.q_len, p.window, p.causal != 0};
+__device__ __forceinline__ Sight sight_of(const Attention8bitParams& p, int row) {
+    const int length = (int)min(max(p.lengths[row], (int64_t)0), p.cache.max_len);
+    return {length, length - p.q_len, p.causal ? (int)p.window : 0};
 }
 
 template <class T, int dims, int tiles_of_rows>
-__global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const __grid_constant__ Attention8bitParams p) {
+__global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2 && dims == 128 ? 2 : dims == 128 ? 3 : 4) decode_attention_8bit_kernel(const __grid_constant__ Attention8bitParams p) {
     constexpr bool precise = sizeof(T) == 4;
     constexpr int kStages = stages_of(dims), kStageBytes = stage_bytes(dims), kSegments = dims / 64, kBlocks = dims / 16;
     constexpr int kRows = 8 * tiles_of_rows;
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
 
     sum_of_rows(batch, prefix, carry, [&](int row) {
         const Sight s = sight_of(p, row);
-        return (int)max(s.end_tile() - s.first_tile(), (int64_t)0) * c.kv_heads;
+        return max(s.end_tile() - s.first_tile(), 0) * c.kv_heads;
     });
     const int all = prefix[batch];
     const int share = max((int)(((int64_t)all + gridDim.x - 1) / gridDim.x), kLeastShare);
@@ -136,29 +138,42 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
         const int tiles = (prefix[row + 1] - prefix[row]) / c.kv_heads;
         const int head = (int)(at - prefix[row]) / tiles, from_tile = (int)(at - prefix[row]) % tiles;
         const int to_tile = (int)min((int64_t)tiles, from_tile + (stop - at));
-        const int64_t pair = (int64_t)row * c.kv_heads + head, tile0 = sight.first_tile();
+        const int64_t pair = (int64_t)row * c.kv_heads + head;
+        const int tile0 = sight.first_tile();
         const uint8_t* keys = c.key_codes + pair * c.max_len * head_dim;
         const uint8_t* values = c.value_codes + pair * c.max_len * head_dim;
         const float* key_scales = c.key_scales + pair * c.blocks;
         const float* value_scales = c.value_scales + pair * c.blocks;
 
-        const int64_t seen = max(sight.first(0), (int64_t)0);  // no row sees a position before this one
+        const int seen = max(sight.first(0), 0);  // no row sees a position before this one
         const auto fetch = [&](int tile, int stage) {  // positions that no row sees arrive as zeros, whatever the cache holds there
-            const int64_t position = (tile0 + tile) * kTile;
+            const int position = (tile0 + tile) * kTile;
             const uint32_t to = stages_at + stage * kStageBytes;
+            if (head_dim == dims && position >= seen && position + kTile <= sight.length) {  // 32 whole rows, one run of memory
+                const uint8_t* from = keys + (int64_t)position * dims + lane * 16;
+                const int64_t apart = values - keys;
 #pragma unroll
-            for (int i = 0; i < kBlocks; ++i) {
-                const int index = i * 32 + lane, r = index / kBlocks, chunk = index % kBlocks;
-                if (chunk < chunks) {
-                    const bool there = position + r < sight.length && position + r >= seen;
-                    const int64_t offset = there ? (position + r) * head_dim + chunk * 16 : 0;
-                    const uint32_t place = r * dims + placed<dims>(r, chunk) * 16;
-                    copy16(to + place, keys + offset, there);
-                    copy16(to + kTile * dims + place, values + offset, there);
+                for (int i = 0; i < kBlocks; ++i) {
+                    const int r = (i * 32 + lane) / kBlocks, chunk = lane % kBlocks;
+                    const uint32_t place = to + r * dims + placed<dims>(r, chunk) * 16;
+                    copy16(place, from + i * 512);
+                    copy16(place + kTile * dims, from + apart + i * 512);
+                }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < kBlocks; ++i) {
+                    const int index = i * 32 + lane, r = index / kBlocks, chunk = index % kBlocks;
+                    if (chunk < chunks) {
+                        const bool there = position + r < sight.length && position + r >= seen;
+                        const int64_t offset = there ? (int64_t)(position + r) * head_dim + chunk * 16 : 0;
+                        const uint32_t place = to + r * dims + placed<dims>(r, chunk) * 16;
+                        copy16(place, keys + offset, there);
+                        copy16(place + kTile * dims, values + offset, there);
+                    }
                 }
             }
             if (lane < 4) {  // the scales of the tile's two halves, keys' then values'
-                const int64_t first = position + lane % 2 * 16;
+                const int first = position + lane % 2 * 16;
                 const bool there = first < sight.length;
                 copy4(to + 2 * kTile * dims + lane * 4, (lane < 2 ? key_scales : value_scales) + (there ? first >> shift : 0), there);
             }
@@ -222,7 +237,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
             for (int m = 0; m < kBlocks; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
         }
         // Positions that every row sees need no mask.
-        const int64_t all_from = sight.first(p.q_len - 1), all_to = sight.last(0);
+        const int all_from = sight.first(p.q_len - 1), all_to = sight.last(0, p.causal != 0);
 
         int stage = 0;
         for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
@@ -236,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
             }
             const uint8_t* k_stage = stages + stage * kStageBytes;
             const float* scales = reinterpret_cast<const float*>(k_stage + 2 * kTile * dims);
-            const int64_t position = (tile0 + tile) * kTile;
+            const int position = (tile0 + tile) * kTile;
             float score[tiles_of_rows][2][4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -254,8 +269,9 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
                     const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const uint32_t a0 = codes_to_halves(aw[w]), a1 = codes_to_halves(bw[w]);
-                        const uint32_t a2 = codes_to_halves(aw[w] >> 16), a3 = codes_to_halves(bw[w] >> 16);
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_halves(aw[w], a0, a2);
+                        codes_to_halves(bw[w], a1, a3);
 #pragma unroll
                         for (int n = 0; n < tiles_of_rows; ++n) {
                             if constexpr (precise) multiply(score[n][half], a0, a1, a2, a3, ql[n][s][w][0], ql[n][s][w][1]);
@@ -283,12 +299,12 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int own = (n * 8 + 2 * tig + i) % p.q_len;
-                        const int64_t first = sight.first(own), last = sight.last(own);
+                        const int first = sight.first(own), last = sight.last(own, p.causal != 0);
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
 #pragma unroll
                             for (int o = 0; o < 2; ++o) {
-                                const int64_t j = position + half * 16 + o * 8 + gid;
+                                const int j = position + half * 16 + o * 8 + gid;
                                 if (j < first || j > last) score[n][half][2 * o + i] = kNone;
                             }
                         }
@@ -356,8 +372,9 @@ __global__ void __launch_bounds__(kThreads) decode_attention_8bit_kernel(const _
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const uint32_t low = __byte_perm(x[2 * i], 0, 0x3120), high = __byte_perm(x[2 * i + 1], 0, 0x3120);
-                            const uint32_t a0 = codes_to_halves(low), a1 = codes_to_halves(low >> 16);
-                            const uint32_t a2 = codes_to_halves(high), a3 = codes_to_halves(high >> 16);
+                            uint32_t a0, a1, a2, a3;
+                            codes_to_halves(low, a0, a1);
+                            codes_to_halves(high, a2, a3);
 #pragma unroll
                             for (int n = 0; n < tiles_of_rows; ++n) {
                                 if constexpr (precise) multiply(out[n][m + i], a0, a1, a2, a3, wl[n][half][0], wl[n][half][1]);
@@ -512,7 +529,7 @@ int padded_dims(const Attention8bitParams& p) { return p.cache.head_dim > 128 ? 
 int attention_8bit_grid(const Attention8bitParams& p, int sm_count) {
     // As many blocks as the GPU holds at once (shared memory: 227 KB of an SM), no more than there are least shares.
     const int dims = padded_dims(p);
-    const int resident = dims == 256 ? 1 : dims == 128 ? 2 : 4;
+    const int resident = dims == 256 ? 1 : dims == 64 ? 4 : p.rows > 8 ? 2 : 3;
     const int64_t tiles = p.cache.batch * p.cache.kv_heads * ((p.cache.max_len + kTile - 1) / kTile);
     return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count * resident, (tiles + kLeastShare - 1) / kLeastShare));
 }

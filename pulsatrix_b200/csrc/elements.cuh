@@ -47,6 +47,12 @@ __device__ __forceinline__ uint32_t codes_to_halves(uint32_t two) {
     return r;
 }
 
+// Four codes as two pairs of halves.
+__device__ __forceinline__ void codes_to_halves(uint32_t four, uint32_t& low, uint32_t& high) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(low), "=r"(high) : "r"(four));
+}
+
 // Two floats, each rounded to the nearest code (ties to even), beyond the largest code to that; NaN stays NaN.
 __device__ __forceinline__ uint32_t floats_to_codes(float low, float high) {
     unsigned short r;
