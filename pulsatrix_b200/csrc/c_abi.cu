@@ -1307,7 +1307,7 @@ psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const 
     const OnDevice device(ctx->device);
     PSX_CUDA(device.error);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    p.grid = psx::attention_8bit_grid(p, ctx->sm_count);
+    psx::plan_attention_8bit(p, ctx->sm_count);
     bool grown;
     const size_t counters = (size_t)(cache->batch * cache->kv_heads) * sizeof(int32_t);
     if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;

@@ -77,6 +77,13 @@ __device__ __forceinline__ uint32_t halves_left(float low, float high, uint32_t 
     return halves(low - t.x, high - t.y);
 }
 
+template <class T>
+__device__ __forceinline__ void store_four(T* to, float4 x, float factor) {
+    alignas(16) const T four[4] = {from_float<T>(x.x * factor), from_float<T>(x.y * factor), from_float<T>(x.z * factor), from_float<T>(x.w * factor)};
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(four);
+    else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(four);
+}
+
 // Chunk (16 codes) `chunk` of row `row` of a stage lies at this chunk of the row: eight rows' chunks of one column lie in
 // different banks, and so do four neighbouring chunks of two neighbouring rows.
 template <int dims>
@@ -122,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         return max(s.end_tile() - s.first_tile(), 0) * c.kv_heads;
     });
     const int all = prefix[batch];
-    const int share = max((int)(((int64_t)all + gridDim.x - 1) / gridDim.x), kLeastShare);
+    const int share = max((int)(((int64_t)all + gridDim.x - 1) / gridDim.x), p.least_share);
     // Rows that see nothing have no tiles, hence no block: their context is zero.
     for (int64_t row = blockIdx.x; row < batch; row += gridDim.x) {
         if (prefix[row + 1] != prefix[row]) continue;
@@ -417,80 +424,93 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         __syncthreads();
         const bool whole = from_tile == 0 && to_tile == tiles;
         T* context = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
-        const int piece_floats = kRows * (dims + 4);
+        const int piece_floats = kRows * (dims + 4);  // (a row's context, its maximum and sum, two unused)
+        const int fours = head_dim / 4;
         float* piece = p.partial + ((int64_t)blockIdx.x * 2 + (at == (int64_t)blockIdx.x * share ? 0 : 1)) * piece_floats;
-        for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) {
-            const int r = i / head_dim, d = i % head_dim;
-            float high = kNone, sum = 0.0f, value = 0.0f;
+        for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
+            const int r = i / fours, d = i % fours * 4;
+            float high = kNone, sum = 0.0f;
+            float4 value = make_float4(0, 0, 0, 0);
+#pragma unroll
             for (int w = 0; w < kWarps; ++w) high = fmaxf(high, tops[w][r]);
+#pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 if (totals[w][r] == 0.0f) continue;  // (a warp without a position that the row sees)
                 const float less = exp2_approx(tops[w][r] - high);
+                const float4 part = *reinterpret_cast<const float4*>(meet + (w * kRows + r) * dims + d);
                 sum += totals[w][r] * less;
-                value += meet[(w * kRows + r) * dims + d] * less;
+                value.x += part.x * less, value.y += part.y * less, value.z += part.z * less, value.w += part.w * less;
             }
             if (whole) {
-                context[i] = from_float<T>(sum == 0.0f ? 0.0f : value / sum);
+                store_four(context + r * head_dim + d, value, sum == 0.0f ? 0.0f : 1.0f / sum);
             } else {
-                __stcg(piece + r * (dims + 4) + d, value);
-                if (d == 0) {
-                    __stcg(piece + r * (dims + 4) + dims, high);
-                    __stcg(piece + r * (dims + 4) + dims + 1, sum);
-                }
+                __stcg(reinterpret_cast<float4*>(piece + r * (dims + 4) + d), value);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(piece + r * (dims + 4) + dims), make_float2(high, sum));
             }
         }
         if (!whole) {
-            const int64_t begin = prefix[row] + (int64_t)head * tiles, end = begin + tiles;
-            const int64_t first = begin / share, last = (end - 1) / share;
-            __threadfence();
+            const int begin = prefix[row] + head * tiles, end = begin + tiles;
+            const int first = begin / share, last = (end - 1) / share;
             __syncthreads();
-            if (threadIdx.x == 0) {
-                is_last = atomicAdd(p.arrived + pair, 1) == (int)(last - first);
+            if (threadIdx.x == 0) {  // (release: the block's pieces, ordered before by the barrier; acquire: the other blocks')
+                int before;
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + pair) : "memory");
+                is_last = before == last - first;
                 if (is_last) p.arrived[pair] = 0;
-                __threadfence();
             }
             __syncthreads();
             if (is_last) {
-                const int pieces = (int)(last - first) + 1;
-                const float* base = p.partial + first * 2 * piece_floats;  // (the first piece is its block's second one unless it starts it)
+                const int pieces = last - first + 1;
+                const float* base = p.partial + (int64_t)first * 2 * piece_floats;  // (the first piece is its block's second one unless it starts it)
                 const int skip = begin != first * share ? piece_floats : 0;
-                float* less = reinterpret_cast<float*>(shared);  // (piece, row): what a piece's sums count for
+                const auto piece_of = [&](int b) { return base + (b == 0 ? skip : (int64_t)b * 2 * piece_floats); };
+                // A thread's part of the first pieces' contexts is asked for along with their maxima and sums.
+                constexpr int kAhead = 8;
+                const int mine_row = threadIdx.x / fours, mine_d = threadIdx.x % fours * 4;
+                const bool mine_real = mine_row < p.rows;
+                float4 ahead[kAhead];
+#pragma unroll
+                for (int b = 0; b < kAhead; ++b) {
+                    ahead[b] = make_float4(0, 0, 0, 0);
+                    if (b < pieces && mine_real) ahead[b] = __ldcg(reinterpret_cast<const float4*>(piece_of(b) + mine_row * (dims + 4) + mine_d));
+                }
+                float2* less = reinterpret_cast<float2*>(shared);  // (piece, row): maximum and sum, then what the piece counts for
                 for (int i = threadIdx.x; i < pieces * p.rows; i += kThreads) {
-                    const int b = i / p.rows, r = i % p.rows;
-                    less[i] = __ldcg(base + (b == 0 ? skip : (int64_t)b * 2 * piece_floats) + r * (dims + 4) + dims);
+                    less[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(i / p.rows) + i % p.rows * (dims + 4) + dims));
                 }
                 __syncthreads();
                 for (int r = warp; r < p.rows; r += kWarps) {
                     float high = kNone, sum = 0.0f;
-                    for (int b = lane; b < pieces; b += 32) high = fmaxf(high, less[b * p.rows + r]);
+                    for (int b = lane; b < pieces; b += 32) high = fmaxf(high, less[b * p.rows + r].x);
 #pragma unroll
                     for (int step = 16; step > 0; step /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, step));
                     for (int b = lane; b < pieces; b += 32) {
-                        const float mine = less[b * p.rows + r];
-                        const float factor = mine > kNone ? exp2_approx(mine - high) : 0.0f;
-                        less[b * p.rows + r] = factor;
-                        sum += factor * __ldcg(base + (b == 0 ? skip : (int64_t)b * 2 * piece_floats) + r * (dims + 4) + dims + 1);
+                        const float2 mine = less[b * p.rows + r];
+                        const float factor = mine.x > kNone ? exp2_approx(mine.x - high) : 0.0f;
+                        less[b * p.rows + r].x = factor;
+                        sum += factor * mine.y;
                     }
 #pragma unroll
                     for (int step = 16; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
                     if (lane == 0) totals[0][r] = sum;
                 }
                 __syncthreads();
-                const int fours = head_dim / 4;
                 for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
                     const int r = i / fours, d = i % fours * 4;
-                    const float* from = base + r * (dims + 4) + d;
                     float4 value = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-                    for (int b = 0; b < pieces; ++b) {
-                        const float4 part = __ldcg(reinterpret_cast<const float4*>(from + (b == 0 ? skip : (int64_t)b * 2 * piece_floats)));
-                        const float factor = less[b * p.rows + r];
+                    const auto add = [&](const float4& part, float factor) {
                         value.x += part.x * factor, value.y += part.y * factor, value.z += part.z * factor, value.w += part.w * factor;
+                    };
+                    int b = 0;
+                    if (i == threadIdx.x) {
+#pragma unroll
+                        for (; b < kAhead; ++b) {
+                            if (b < pieces) add(ahead[b], less[b * p.rows + r].x);
+                        }
                     }
-                    const float inverse = totals[0][r] == 0.0f ? 0.0f : 1.0f / totals[0][r];
-                    T* to = context + r * head_dim + d;
-                    to[0] = from_float<T>(value.x * inverse), to[1] = from_float<T>(value.y * inverse);
-                    to[2] = from_float<T>(value.z * inverse), to[3] = from_float<T>(value.w * inverse);
+#pragma unroll 8
+                    for (; b < pieces; ++b) add(__ldcg(reinterpret_cast<const float4*>(piece_of(b) + r * (dims + 4) + d)), less[b * p.rows + r].x);
+                    store_four(context + r * head_dim + d, value, totals[0][r] == 0.0f ? 0.0f : 1.0f / totals[0][r]);
                 }
             }
         }
@@ -526,12 +546,16 @@ int padded_dims(const Attention8bitParams& p) { return p.cache.head_dim > 128 ? 
 
 }  // namespace
 
-int attention_8bit_grid(const Attention8bitParams& p, int sm_count) {
-    // As many blocks as the GPU holds at once (shared memory: 227 KB of an SM), no more than there are least shares.
+void plan_attention_8bit(Attention8bitParams& p, int sm_count) {
     const int dims = padded_dims(p);
+    const int64_t tiles = (p.cache.max_len + kTile - 1) / kTile;
+    // The pieces of a pair, one more at each end than whole shares, have their maxima and sums in shared memory when they are joined.
+    const int64_t most_pieces = (int64_t)(shared_of(dims) / (p.rows * sizeof(float2))) - 2;
+    p.least_share = (int)std::max<int64_t>(kLeastShare, (tiles + most_pieces - 1) / most_pieces);
+    // As many blocks as the GPU holds at once (by registers and shared memory), no more than there are least shares.
     const int resident = dims == 256 ? 1 : dims == 64 ? 4 : p.rows > 8 ? 2 : 3;
-    const int64_t tiles = p.cache.batch * p.cache.kv_heads * ((p.cache.max_len + kTile - 1) / kTile);
-    return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count * resident, (tiles + kLeastShare - 1) / kLeastShare));
+    const int64_t shares = (p.cache.batch * p.cache.kv_heads * tiles + p.least_share - 1) / p.least_share;
+    p.grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count * resident, shares));
 }
 
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p) {

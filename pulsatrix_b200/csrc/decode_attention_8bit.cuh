@@ -20,10 +20,11 @@ struct Attention8bitParams {
     int32_t heads, group, q_len, rows;  // rows = group * q_len
     int32_t type, causal;
     int32_t grid;            // blocks
+    int32_t least_share;     // tiles of 32 positions that a block takes at least
     float scale;
 };
 
-int attention_8bit_grid(const Attention8bitParams& p, int sm_count);
+void plan_attention_8bit(Attention8bitParams& p, int sm_count);  // grid and least_share
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p);
 // cudaErrorInvalidValue: see psx_b200_decode_attention_8bit for the shapes that are taken.
 cudaError_t launch_decode_attention_8bit(const Attention8bitParams& p, cudaStream_t stream);

@@ -14,15 +14,17 @@
 // the products about alike.
 //
 // fp32 operands: every number is split into three bf16 parts that add up to it (8 bits of the fraction each), and a product is the
-// six products of parts that reach fp32's precision, the small ones first; a split kernel writes the parts ahead of time.
-// One tile, blocks of 64 keys; the scores have two places and the weights' parts one of their own, so that the next block's
-// scores are formed while this block's weights are.  Six bf16 products are still several times faster than the FP32 pipes.
+// six products of parts that reach fp32's precision, the small ones first.  The keys' and values' parts are written by a kernel ahead,
+// the queries' go into tensor memory once, the weights' as they are made.  One tile, blocks of 64 keys; the scores have two places,
+// so that the next block's scores are formed while this block's weights are; contexts are added up in registers.  Six bf16 products are still
+// several times faster than the FP32 pipes.
 //
 // Rows behind a sequence's last key in a block belong to other sequences: their scores are masked, and their values are set to zero in
 // shared memory, so that a NaN there is not seen here.
 #include "prompt_attention.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "elements.cuh"
 #include "once_per_device.hpp"
@@ -42,18 +44,19 @@ struct Shape {
     static constexpr int dims = dims_, parts = parts_;  // the head dimension, rounded up to 64 or 128
     static constexpr int tiles = parts == 1 ? 2 : 1;
     static constexpr int block = parts == 1 ? 128 : 64;
-    static constexpr int stages = parts == 1 ? (dims == 64 ? 4 : 2) : (dims == 64 ? 2 : 1);
-    static constexpr int threads = tiles * 128 + 64;  // the warpgroups, the copying warp, the issuing warp
+    static constexpr int stages = dims == 64 ? 4 : 2;
+    static constexpr int threads = tiles * 128 + (parts == 1 ? 128 : 64);  // the warpgroups; the copying warp, the issuing warp
     static constexpr int slabs = dims / 64;            // a tile lies in slabs of 64 columns, rows of 128 bytes
-    static constexpr int q_part = kTileRows * dims * 2, q_bytes = parts * q_part;
+    static constexpr int q_bytes = parts == 1 ? kTileRows * dims * 2 : 0;  // of a tile (fp32: in tensor memory)
     static constexpr int k_part = block * dims * 2, k_bytes = parts * k_part;  // (of the values too)
     static constexpr int shared = tiles * q_bytes + 2 * stages * k_bytes;
-    // Tensor memory: scores (two places for each tile, or one that the weights share), weights' parts, contexts.
-    static constexpr int score_at = 0;
-    static constexpr int weight_at = parts == 1 ? 0 : 2 * block;
-    static constexpr int weight_part = block / 2;
-    static constexpr int context_at = parts == 1 ? tiles * block : 256;
-    static_assert(weight_at + parts * weight_part <= 256 && context_at + tiles * dims <= 512);
+    // Columns of tensor memory: scores, whose places the weights take; what has no room there of fp32 weights; contexts; fp32 queries.
+    static constexpr int score_places = parts == 1 ? tiles : 2;
+    static constexpr int third_at = score_places * block, context_at = parts == 1 ? third_at : third_at + block / 2;
+    static constexpr int query_at = context_at + tiles * dims, query_part = dims / 2;
+    static_assert(query_at + (parts == 1 ? 0 : parts * query_part) <= 512);
+    // Column of a part of the weights that take the scores' place.
+    static __host__ __device__ constexpr int weight_at(int place, int part) { return part == 2 ? third_at : place * block + part * (block / 2); }
 };
 
 struct alignas(64) PromptLaunch {
@@ -83,12 +86,75 @@ __device__ __forceinline__ uint32_t pack(float low, float high, __half) {
     return r;
 }
 
+// Two floats as three bf16 pairs that add up to them, the largest part first.  What is left of a number after a part is exact; of
+// one that is not finite it is 0, and the largest floats' first part is rounded down instead of to infinity.
+__device__ __forceinline__ void split_pair(float low, float high, uint32_t& first, uint32_t& second, uint32_t& third) {
+    const float largest = 3.3895313892515355e38f;  // of bf16
+    const auto bounded = [&](float x) { return fabsf(x) < -kNone ? fminf(fmaxf(x, -largest), largest) : x; };
+    first = pack(bounded(low), bounded(high), __nv_bfloat16{});
+    const auto left = [](float x, uint32_t taken) { return fabsf(x) < -kNone ? x - __uint_as_float(taken) : 0.0f; };
+    low = left(low, first << 16), high = left(high, first & 0xffff0000u);
+    second = pack(low, high, __nv_bfloat16{});
+    low -= __uint_as_float(second << 16), high -= __uint_as_float(second & 0xffff0000u);
+    third = pack(low, high, __nv_bfloat16{});
+}
+
+// {a, b} * {x, y} + {u, v}, each rounded as alone.
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 x, float2 u) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, x, u;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tmov.b64 u, {%6, %7};\n\tfma.rn.f32x2 a, a, x, u;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(x.x), "f"(x.y), "f"(u.x), "f"(u.y));
+    return r;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 x) {
+    float2 r;
+    asm("{\n\t.reg .b64 a, x;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tadd.rn.f32x2 a, a, x;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(x.x), "f"(x.y));
+    return r;
+}
+__device__ __forceinline__ float higher(float a, float b) {  // (a NaN stays one)
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float lower(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 2^x for x <= 2^6 on the FMA pipes, for a share of the weights that the special-function unit is relieved of: x = n + f with
+// |f| <= 1/2, the polynomial of least relative error for 2^f (of degree 3, off by 2^-13.7, for weights that are rounded to 8 bits; of
+// degree 4, off by 2^-18.6, for 11 bits; computed by exchange of the extrema), n added to the exponent.  Below 2^-126: that.
+template <class Elem>
+__device__ __forceinline__ float2 exp2_pair(float2 x) {
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: its sum with x is rounded to a whole number
+    x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+    const float2 n = add_pair(x, both(kRound));
+    const float2 f = fma_pair(add_pair(n, both(-kRound)), both(-1.0f), x);
+    float2 y;
+    if constexpr (__is_same(Elem, __nv_bfloat16)) {
+        y = fma_pair(f, both(0.0551716685295105f), both(0.2426111251115799f));
+        y = fma_pair(y, f, both(0.6932609677314758f));
+        y = fma_pair(y, f, both(0.9999280571937561f));
+    } else {
+        y = fma_pair(f, both(0.009570102207362652f), both(0.05591785907745361f));
+        y = fma_pair(y, f, both(0.240247443318367f));
+        y = fma_pair(y, f, both(0.6931217908859253f));
+        y = fma_pair(y, f, both(0.9999992847442627f));
+    }
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
+}
+constexpr int kPolynomialPairs = 4;  // of 16
+
 // Elem: the type of the products' operands (bf16 for the parts of fp32); Out: the type of the context.
 template <class Elem, class Out, class S>
 __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const __grid_constant__ PromptLaunch launch) {
     extern __shared__ uint8_t raw_shared[];
     __shared__ uint64_t q_full, k_full[S::stages], k_empty[S::stages], v_full[S::stages], v_empty[S::stages];
-    __shared__ uint64_t score_full[2], weight_full[2], context_full[2], drained;
+    __shared__ uint64_t score_full[2], weight_full[2][2], context_full[2], drained;
     __shared__ uint32_t tensor_at;
     __shared__ uint32_t give_up;
     __shared__ int carry[32];
@@ -122,7 +188,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     }
 
     if (threadIdx.x == 0) {
-        barrier_init(&q_full, 1);
+        barrier_init(&q_full, S::parts == 1 ? 1 : 128);
         for (int s = 0; s < S::stages; ++s) {
             barrier_init(&k_full[s], 1);
             barrier_init(&k_empty[s], 1);
@@ -131,7 +197,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         }
         for (int t = 0; t < 2; ++t) {
             barrier_init(&score_full[t], 1);
-            barrier_init(&weight_full[t], 128);
+            barrier_init(&weight_full[t][0], 128);
+            barrier_init(&weight_full[t][1], 128);
             barrier_init(&context_full[t], 1);
         }
         barrier_init(&drained, 1);
@@ -153,7 +220,16 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     };
     const uint32_t q_at = smem_address(shared), k_at = q_at + S::tiles * S::q_bytes, v_at = k_at + S::stages * S::k_bytes;
 
+    // Of the registers that the CTA was launched with (168 a thread) the warpgroups with a row per thread get more: 2 * 224 + 56 = 3 * 168.
+    const auto few_registers = [] {
+        if constexpr (S::parts == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    };
+    const auto many_registers = [] {
+        if constexpr (S::parts == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    };
+
     if (warp == kCopyWarp) {
+        few_registers();
         if (lane == 0 && most > 0) {
             const int kv_head = head / (p.heads / p.kv_heads);
             const auto fetch = [&](uint32_t to, int rows, const CUtensorMap* map, int y, int64_t z, int64_t total, uint64_t* bar) {
@@ -165,11 +241,13 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                 }
             };
             const uint32_t filled = (uint32_t)min(S::slabs, (p.head_dim + 63) / 64) * 128 * S::parts;  // bytes per row that arrive
-            uint32_t q_bytes = 0;
-            for (int t = 0; t < S::tiles; ++t) q_bytes += counts[t] > 0 ? kTileRows * filled : 0;
-            barrier_expect_bytes(&q_full, q_bytes);
-            for (int t = 0; t < S::tiles; ++t) {
-                if (counts[t] > 0) fetch(q_at + t * S::q_bytes, kTileRows, &launch.q_map, head, q_begin + row0 + t * kTileRows, p.total_q, &q_full);
+            if constexpr (S::parts == 1) {
+                uint32_t q_bytes = 0;
+                for (int t = 0; t < S::tiles; ++t) q_bytes += counts[t] > 0 ? kTileRows * filled : 0;
+                barrier_expect_bytes(&q_full, q_bytes);
+                for (int t = 0; t < S::tiles; ++t) {
+                    if (counts[t] > 0) fetch(q_at + t * S::q_bytes, kTileRows, &launch.q_map, head, q_begin + row0 + t * kTileRows, p.total_q, &q_full);
+                }
             }
             int asked = 0;
             bool fine = true;
@@ -188,7 +266,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             }
             // Nothing is on its way into shared memory when the CTA ends.  (Without a failure every copy has been waited for.)
             if (*(volatile uint32_t*)&give_up || !fine) {
-                barrier_wait_bounded(&q_full, 0, p.wait_limit_ns);
+                if constexpr (S::parts == 1) barrier_wait_bounded(&q_full, 0, p.wait_limit_ns);
                 for (int i = max(asked - S::stages, 0); i < asked; ++i) {
                     barrier_wait_bounded(&k_full[i % S::stages], (i / S::stages) & 1, p.wait_limit_ns);
                     barrier_wait_bounded(&v_full[i % S::stages], (i / S::stages) & 1, p.wait_limit_ns);
@@ -196,30 +274,40 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             }
         }
     } else if (warp == kIssueWarp) {
+        few_registers();
         constexpr bool bfloat = __is_same(Elem, __nv_bfloat16);
         const uint32_t score_kind = product_descriptor(bfloat, false, kTileRows, S::block);
         const uint32_t context_kind = product_descriptor(bfloat, true, kTileRows, launch.dims16);
+        // A descriptor's start address counts in 16 bytes, in its lowest bits.
+        const uint64_t q_rows = operand_descriptor(q_at, 16, 1024), k_rows = operand_descriptor(k_at, 16, 1024);
+        const uint64_t v_rows = operand_descriptor(v_at, S::block * 128, 1024);
         const auto score = [&](int t, int s, int place) {  // S = Q K^T of a tile and a stage of keys
             bool add = false;
             for (int sum = S::parts - 1; sum >= 0; --sum) {  // (the smallest products first)
                 for (int part = 0; part <= sum; ++part) {
-                    for (int step = 0; step < launch.steps; ++step) {
-                        const uint32_t inside = step % 4 * 32;
-                        const uint32_t a = q_at + t * S::q_bytes + part * S::q_part + step / 4 * (kTileRows * 128) + inside;
-                        const uint32_t c = k_at + s * S::k_bytes + (sum - part) * S::k_part + step / 4 * (S::block * 128) + inside;
-                        product_of_shared(tensor + place, operand_descriptor(a, 16, 1024), operand_descriptor(c, 16, 1024), score_kind, add);
+                    const uint64_t k = k_rows + ((s * S::k_bytes + (sum - part) * S::k_part) >> 4);
+#pragma unroll
+                    for (int step = 0; step < S::dims / 16; ++step) {
+                        if (step >= launch.steps) break;
+                        const uint64_t c = k + ((step / 4 * (S::block * 128) + step % 4 * 32) >> 4);
+                        if constexpr (S::parts == 1) {
+                            product_of_shared(tensor + place, q_rows + ((t * S::q_bytes + step / 4 * (kTileRows * 128) + step % 4 * 32) >> 4), c, score_kind, add);
+                        } else {
+                            product_of_tensor(tensor + place, tensor + S::query_at + part * S::query_part + step * 8, c, score_kind, add);
+                        }
                         add = true;
                     }
                 }
             }
         };
-        const auto weigh = [&](int t, int s, bool add) {  // O += P V
+        const auto weigh = [&](int t, int place, int s, int from, int to, bool add) {  // O += P V, of the block's keys 16 from .. 16 to
             for (int sum = S::parts - 1; sum >= 0; --sum) {
                 for (int part = 0; part <= sum; ++part) {
-                    for (int step = 0; step < S::block / 16; ++step) {
-                        const uint32_t a = tensor + S::weight_at + t * S::block + part * S::weight_part + step * 8;
-                        const uint32_t c = v_at + s * S::k_bytes + (sum - part) * S::k_part + step * (16 * 128);
-                        product_of_tensor(tensor + S::context_at + t * S::dims, a, operand_descriptor(c, S::block * 128, 1024), context_kind, add);
+                    const uint64_t v = v_rows + ((s * S::k_bytes + (sum - part) * S::k_part) >> 4);
+#pragma unroll
+                    for (int step = from; step < to; ++step) {
+                        product_of_tensor(tensor + S::context_at + t * S::dims, tensor + S::weight_at(place, part) + step * 8, v + (step * (16 * 128) >> 4),
+                                          context_kind, add);
                         add = true;
                     }
                 }
@@ -247,7 +335,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             if constexpr (S::tiles == 2) {
                 for (int t = 0; t < 2; ++t) {
                     if (counts[t] == 0) continue;
-                    if (lane == 0) score(t, 0, S::score_at + t * S::block);
+                    if (lane == 0) score(t, 0, t * S::block);
                     arrive(&score_full[t]);
                 }
                 arrive(&k_empty[0]);
@@ -258,41 +346,47 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                     bool next = false;  // the next block's keys are there
                     for (int t = 0; t < 2 && fine; ++t) {
                         if (c >= counts[t]) continue;
-                        fine = wait(&weight_full[t], c & 1);
+                        for (int half = 0; half < 2 && fine; ++half) {  // (the second half's weights are still on their way)
+                            fine = wait(&weight_full[t][half], c & 1);
+                            if (!fine) break;
+                            tensor_fence_after();
+                            if (lane == 0) {
+                                if (half == 0) weigh(t, t, c % S::stages, 0, S::block / 32, c > 0);
+                                else weigh(t, t, c % S::stages, S::block / 32, S::block / 16, true);
+                            }
+                        }
                         if (!fine) break;
-                        tensor_fence_after();
-                        if (lane == 0) weigh(t, c % S::stages, c > 0);
                         if (c + 1 == counts[t]) {
                             arrive(&context_full[t]);
                             continue;
                         }
                         if (!next) fine = next = stage_wait(k_full, c + 1);
                         if (!fine) break;
-                        if (lane == 0) score(t, (c + 1) % S::stages, S::score_at + t * S::block);
+                        if (lane == 0) score(t, (c + 1) % S::stages, t * S::block);
                         arrive(&score_full[t]);
                     }
                     arrive(&v_empty[c % S::stages]);
                     if (next) arrive(&k_empty[(c + 1) % S::stages]);
                 }
             } else {
-                if (lane == 0) score(0, 0, S::score_at);
+                if (lane == 0) score(0, 0, 0);
                 arrive(&score_full[0]);
                 arrive(&k_empty[0]);
                 for (int c = 0; c < most && fine; ++c) {
-                    if (c + 1 < most) {  // (the place of block c - 1's scores: its weights are complete, hence read)
+                    if (c + 1 < most) {  // (in the place of block c - 1's weights, which the products before this one read)
                         fine = stage_wait(k_full, c + 1);
                         if (!fine) break;
-                        if (lane == 0) score(0, (c + 1) % S::stages, S::score_at + ((c + 1) & 1) * S::block);
+                        if (lane == 0) score(0, (c + 1) % S::stages, ((c + 1) & 1) * S::block);
                         arrive(&score_full[(c + 1) & 1]);
                         arrive(&k_empty[(c + 1) % S::stages]);
                     }
                     fine = stage_wait(v_full, c);
                     if (!fine) break;
                     clear_tail(c, c % S::stages);
-                    fine = wait(&weight_full[0], c & 1);
+                    fine = wait(&weight_full[0][0], c & 1);
                     if (!fine) break;
                     tensor_fence_after();
-                    if (lane == 0) weigh(0, c % S::stages, c > 0);
+                    if (lane == 0) weigh(0, c & 1, c % S::stages, 0, S::block / 16, false);
                     arrive(&context_full[0]);
                     arrive(&v_empty[c % S::stages]);
                 }
@@ -301,7 +395,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         // Every product has ended before tensor memory is given back.
         arrive(&drained);
         barrier_wait_bounded(&drained, 0, p.wait_limit_ns);
-    } else {
+    } else if (warp < S::tiles * 4) {
+        many_registers();
         const int t = warp / 4;
         const int64_t row = row0 + t * kTileRows + (warp % 4) * 32 + lane;  // this thread's query
         const uint32_t lanes = tensor + ((uint32_t)(warp % 4) << 21);        // (32 lanes further: bits 16 up)
@@ -316,6 +411,46 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         const float masked = turned ? -kNone : kNone;
         float top = masked, total = 0.0f;   // of the scores before the factor
         bool fine = true;
+        // fp32: the context is summed up here, a block's at a time: the tensor core's sums are cut off, not rounded, and over
+        // thousands of keys that adds up.
+        constexpr int kSums = S::parts == 1 ? 1 : S::dims;
+        float context[kSums];
+        const auto add_block = [&]() {
+            if constexpr (S::parts == 3) {
+#pragma unroll
+                for (int i = 0; i < S::dims; i += 32) {
+                    if (i >= launch.dims16) break;
+                    float o[32];
+                    tensor_load32(context_at + i, o);
+                    tensor_loads_done();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) context[i + k] += o[k];
+                }
+            }
+        };
+        if constexpr (S::parts == 3) {  // the query's parts into tensor memory
+#pragma unroll
+            for (int i = 0; i < kSums; ++i) context[i] = 0.0f;
+            if (count > 0) {
+                const float* q = static_cast<const float*>(p.q) + (q_begin + row) * p.q_stride + (int64_t)head * p.head_dim;
+#pragma unroll 1
+                for (int i = 0; i < launch.dims16; i += 32) {
+                    uint32_t packed[3][16];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (row < queries && i + k < p.head_dim) x = __ldg(reinterpret_cast<const float4*>(q + i + k));
+                        split_pair(x.x, x.y, packed[0][k / 2], packed[1][k / 2], packed[2][k / 2]);
+                        split_pair(x.z, x.w, packed[0][k / 2 + 1], packed[1][k / 2 + 1], packed[2][k / 2 + 1]);
+                    }
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) tensor_store16(lanes + S::query_at + part * S::query_part + i / 2, packed[part]);
+                }
+                tensor_stores_done();
+                tensor_fence_before();
+                barrier_arrive(&q_full);
+            }
+        }
         for (int c = 0; c < count; ++c) {
             const int place = S::tiles == 2 ? t : c & 1;
             fine = wait(&score_full[place], S::tiles == 2 ? c & 1 : (c / 2) & 1);
@@ -323,10 +458,11 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             tensor_fence_after();
             float x[S::block];
 #pragma unroll
-            for (int i = 0; i < S::block; i += 32) tensor_load32(lanes + S::score_at + place * S::block + i, x + i);
+            for (int i = 0; i < S::block; i += 32) tensor_load32(lanes + place * S::block + i, x + i);
             tensor_loads_done();
             const int64_t key = (begin + c) * S::block;
-            if (key < all_first || key + S::block > all_end) {
+            const bool all_seen = key >= all_first && key + S::block <= all_end;
+            if (!all_seen) {
                 const int low = (int)min(max(first - key, (int64_t)0), (int64_t)S::block), high = (int)min(max(end - key, (int64_t)0), (int64_t)S::block);
 #pragma unroll
                 for (int i = 0; i < S::block; ++i) x[i] = i >= low && i < high ? x[i] : masked;
@@ -334,16 +470,17 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             float best = x[0];
             if (turned) {
 #pragma unroll
-                for (int i = 1; i < S::block; ++i) best = fminf(best, x[i]);
+                for (int i = 1; i < S::block; ++i) best = lower(best, x[i]);
             } else {
                 float m[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
                 for (int i = 4; i < S::block; i += 4) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], x[i + k]);
+                    for (int k = 0; k < 4; ++k) m[k] = higher(m[k], x[i + k]);
                 }
-                best = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                best = higher(higher(m[0], m[1]), higher(m[2], m[3]));
             }
+            if (best != masked) total += best - best;  // (a NaN or an infinity makes the row NaN, whichever way its weight is computed)
             // The reference point moves only where the weights would grow beyond 2^8.
             const float grown = top == masked ? (best == masked ? 0.0f : -kNone) : (best - top) * factor;
             const bool moves = grown > kMostGrowth;
@@ -353,14 +490,19 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                 top = best;
                 total *= less;
             }
-            if constexpr (S::tiles == 1) {  // the products that read this tile's weights and write its context have ended
-                if (c > 0) {
+            if constexpr (S::parts == 3) {
+                if (c > 0) {  // the last block's context, relative to the old reference point
                     fine = wait(&context_full[0], (c - 1) & 1);
                     if (!fine) break;
                     tensor_fence_after();
+                    add_block();
                 }
-            }
-            if (c > 0 && __any_sync(0xffffffffu, moves)) {
+                if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+                    for (int i = 0; i < kSums; ++i) context[i] *= less;
+                }
+            } else if (c > 0 && __any_sync(0xffffffffu, moves)) {
+#pragma unroll 1
                 for (int i = 0; i < launch.dims16; i += 32) {
                     float o[32];
                     tensor_load32(context_at + i, o);
@@ -371,45 +513,56 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                 }
             }
             const float offset = top == masked ? 0.0f : -top * factor;
-            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float2 sums[2] = {both(0.0f), both(0.0f)};
+            const auto weights = [&](auto mixed) {  // mixed: some of them by the polynomial
 #pragma unroll
-            for (int i = 0; i < S::block; i += 32) {
-                uint32_t packed[S::parts][16];
+                for (int i = 0; i < S::block; i += 32) {
+                    uint32_t packed[S::parts][16];
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    float w0 = exp2_approx(fmaf(x[i + k], factor, offset)), w1 = exp2_approx(fmaf(x[i + k + 1], factor, offset));
-                    sums[k & 2] += w0;
-                    sums[(k & 2) + 1] += w1;
+                    for (int k = 0; k < 32; k += 2) {
+                        float2 w = fma_pair(make_float2(x[i + k], x[i + k + 1]), both(factor), both(offset));
+                        if (decltype(mixed)::value && k / 2 % (16 / kPolynomialPairs) == 1) w = exp2_pair<Elem>(w);
+                        else w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
+                        sums[k / 2 % 2] = add_pair(sums[k / 2 % 2], w);
+                        if constexpr (S::parts == 1) packed[0][k / 2] = pack(w.x, w.y, Elem{});
+                        else split_pair(w.x, w.y, packed[0][k / 2], packed[1][k / 2], packed[2][k / 2]);
+                    }
 #pragma unroll
-                    for (int part = 0; part < S::parts; ++part) {
-                        const uint32_t two = pack(w0, w1, Elem{});
-                        packed[part][k / 2] = two;
-                        if (part + 1 < S::parts) {  // (bf16: what is left is exact)
-                            w0 -= __uint_as_float(two << 16);
-                            w1 -= __uint_as_float(two & 0xffff0000u);
-                        }
+                    for (int part = 0; part < S::parts; ++part) tensor_store16(lanes + S::weight_at(place, part) + i / 2, packed[part]);
+                    if (S::parts == 1 && i + 32 == S::block / 2) {
+                        tensor_stores_done();
+                        tensor_fence_before();
+                        barrier_arrive(&weight_full[t][0]);
                     }
                 }
-#pragma unroll
-                for (int part = 0; part < S::parts; ++part) {
-                    tensor_store16(lanes + S::weight_at + t * S::block + part * S::weight_part + i / 2, packed[part]);
-                }
+            };
+            if constexpr (S::parts == 1) {
+                if (all_seen) weights(std::true_type{});
+                else weights(std::false_type{});
+            } else {
+                weights(std::false_type{});
             }
-            total += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            total += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
             tensor_stores_done();
             tensor_fence_before();
-            barrier_arrive(&weight_full[t]);
+            barrier_arrive(&weight_full[t][S::parts == 1 ? 1 : 0]);
         }
         if (count > 0 && fine) {
-            fine = wait(&context_full[t], S::tiles == 2 ? 0 : (count - 1) & 1);
+            fine = wait(&context_full[t], S::parts == 1 ? 0 : (count - 1) & 1);
             tensor_fence_after();
         }
         if (fine) {
+            if (count > 0) add_block();
             const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
             Out* out = static_cast<Out*>(p.out) + ((q_begin + row) * p.heads + head) * p.head_dim;
-            for (int i = 0; i < p.head_dim; i += 32) {
+#pragma unroll
+            for (int i = 0; i < S::dims; i += 32) {
+                if (i >= p.head_dim) break;
                 float o[32];
-                if (count > 0) {
+                if constexpr (S::parts == 3) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = context[i + k];
+                } else if (count > 0) {
                     tensor_load32(context_at + i, o);
                     tensor_loads_done();
                 }
@@ -434,6 +587,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             }
         }
         tensor_fence_before();
+    } else {
+        few_registers();
     }
     __syncthreads();
     if (warp == kIssueWarp) {
@@ -443,25 +598,17 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     if (threadIdx.x == 0 && give_up && p.status) atomicOr(p.status, 1);
 }
 
-// Each fp32 number as three bf16 numbers that add up to it, (part, position, head, dimension).
+// Keys or values as three bf16 numbers each, (part, position, head, dimension).
 __global__ void split_kernel(const float* from, __nv_bfloat16* to, int64_t positions, int64_t stride, int width) {
     const int64_t fours = positions * (width / 4), all = positions * width;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < fours; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t position = i / (width / 4), at = i % (width / 4) * 4;
-        const float4 four = *reinterpret_cast<const float4*>(from + position * stride + at);
-        float x[4] = {four.x, four.y, four.z, four.w};
+        const float4 x = __ldg(reinterpret_cast<const float4*>(from + position * stride + at));
+        uint2 parts[3];
+        split_pair(x.x, x.y, parts[0].x, parts[1].x, parts[2].x);
+        split_pair(x.z, x.w, parts[0].y, parts[1].y, parts[2].y);
 #pragma unroll
-        for (int part = 0; part < 3; ++part) {
-            __nv_bfloat16 h[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool finite = fabsf(x[k]) < -kNone;
-                h[k] = __float2bfloat16_rn(x[k]);
-                if (finite && !(fabsf(__bfloat162float(h[k])) < -kNone)) h[k] = __float2bfloat16_rz(x[k]);  // (the largest floats)
-                x[k] = finite ? x[k] - __bfloat162float(h[k]) : 0.0f;
-            }
-            *reinterpret_cast<uint2*>(to + part * all + position * width + at) = *reinterpret_cast<const uint2*>(h);
-        }
+        for (int part = 0; part < 3; ++part) *reinterpret_cast<uint2*>(to + part * all + position * width + at) = parts[part];
     }
 }
 
@@ -499,7 +646,7 @@ cudaError_t launch(const PromptAttentionParams& p, cudaStream_t stream, int* lau
     const auto kernel = prompt_attention_kernel<Elem, Out, S>;
     // 1024 bytes to start on a boundary of that.  More than half of an SM's, so that a CTA has the tensor memory for itself.
     const size_t shared = S::shared + 1024 + (size_t)(p.batch + 1) * sizeof(int);
-    static_assert(S::shared > 114 << 10);
+    static_assert(S::shared + 1024 > 114 << 10 && S::shared + 1024 + (kMostPrefixRows + 1) * sizeof(int) <= 227 << 10);
     int device = 0;
     if (const cudaError_t e = cudaGetDevice(&device)) return e;
     const cudaError_t e = raised.run(device, [&] {
@@ -510,8 +657,8 @@ cudaError_t launch(const PromptAttentionParams& p, cudaStream_t stream, int* lau
     l.p = p;
     l.steps = (p.head_dim + 15) / 16;
     l.dims16 = l.steps * 16;
-    const void *q = p.q, *k = p.k, *v = p.v;
-    int64_t q_rows = p.total_q, k_rows = p.total_k, q_stride = p.q_stride, k_stride = p.k_stride, v_stride = p.v_stride;
+    const void *k = p.k, *v = p.v;
+    int64_t k_rows = p.total_k, k_stride = p.k_stride, v_stride = p.v_stride;
     if constexpr (S::parts == 3) {
         auto* to = static_cast<__nv_bfloat16*>(p.split);
         const auto split = [&](const void* from, int64_t positions, int64_t stride, int heads) {
@@ -525,15 +672,13 @@ cudaError_t launch(const PromptAttentionParams& p, cudaStream_t stream, int* lau
             }
             return parts;
         };
-        q = split(p.q, p.total_q, p.q_stride, p.heads);
         k = split(p.k, p.total_k, p.k_stride, p.kv_heads);
         v = split(p.v, p.total_k, p.v_stride, p.kv_heads);
-        q_rows *= 3, k_rows *= 3;
-        q_stride = (int64_t)p.heads * p.head_dim;
+        k_rows *= 3;
         k_stride = v_stride = (int64_t)p.kv_heads * p.head_dim;
     }
-    if (p.total_k == 0) k = v = q, k_stride = v_stride = (int64_t)p.kv_heads * p.head_dim;  // (never read)
-    if (!encode(&l.q_map, bfloat, q, q_rows, q_stride, p.heads, p.head_dim, kTileRows) ||
+    if (p.total_k == 0) k = v = p.q, k_stride = v_stride = (int64_t)p.kv_heads * p.head_dim;  // (never read)
+    if ((S::parts == 1 && !encode(&l.q_map, bfloat, p.q, p.total_q, p.q_stride, p.heads, p.head_dim, kTileRows)) ||
         !encode(&l.k_map, bfloat, k, k_rows, k_stride, p.kv_heads, p.head_dim, S::block) ||
         !encode(&l.v_map, bfloat, v, k_rows, v_stride, p.kv_heads, p.head_dim, S::block)) {
         return cudaErrorInvalidValue;
@@ -554,7 +699,7 @@ cudaError_t launch_dims(const PromptAttentionParams& p, cudaStream_t stream, int
 
 size_t prompt_split_bytes(const PromptAttentionParams& p) {
     if (p.type != kFloat32) return 0;
-    return (size_t)6 * p.head_dim * (p.total_q * p.heads + 2 * p.total_k * p.kv_heads);
+    return (size_t)12 * p.head_dim * p.total_k * p.kv_heads;
 }
 
 cudaError_t launch_prompt_attention(const PromptAttentionParams& p, cudaStream_t stream, int* launches) {

@@ -242,6 +242,7 @@ def test_few_rows_share_the_gpu_and_many_rows_fill_it():
     _check("bfloat16", 1, 8, 8, 1, 128, 30000, [29999], seed=1, block=64)        # pieces of one row over all blocks
     _check("bfloat16", 40, 16, 8, 1, 64, 700, list(np.random.RandomState(0).randint(0, 701, 40)), seed=2)
     _check("float32", 3, 2, 2, 1, 64, 5000, [5000, 3, 4000], seed=3)
+    _check("float16", 1, 16, 1, 1, 64, 160000, [160000], seed=4)                         # as many pieces as a pair can have
 
 
 def test_scores_and_scales_of_every_size():

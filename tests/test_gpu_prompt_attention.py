@@ -149,6 +149,21 @@ def test_a_nan_stays_in_its_sequence():
         assert (got[:100] == want[:100]).all() and (got[200:] == want[200:]).all() and got[150:200].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_a_key_that_is_not_finite_reaches_every_query_that_sees_it(dtype):
+    import torch
+    rng = np.random.RandomState(12)
+    q, k, v = (_tensor(rng.rand(400, 1, 64) + 0.1, dtype) for _ in range(3))
+    at = torch.tensor([0, 400], device="cuda")
+    want, _ = gh.ctx().prompt_attention(q, k, v, at)
+    for j in range(0, 400, 7):
+        for what in (float("nan"), float("inf")):
+            bad = k.clone()
+            bad[j] = what
+            got, _ = gh.ctx().prompt_attention(q, bad, v, at)
+            assert got[j:].isnan().all() and (got[:j] == want[:j]).all(), (j, what)
+
+
 def test_the_same_call_gives_the_same_bits_and_graphs_replay():
     import torch
     rng = np.random.RandomState(11)
