@@ -45,7 +45,7 @@ struct Shape {
     static constexpr int tiles = parts == 1 ? 2 : 1;
     static constexpr int block = parts == 1 ? 128 : 64;
     static constexpr int stages = dims == 64 ? 4 : 2;
-    static constexpr int threads = tiles * 128 + (parts == 1 ? 128 : 64);  // the warpgroups; the copying warp, the issuing warp
+    static constexpr int threads = tiles * 128 + (parts == 1 ? 128 : 96);  // the warpgroups; copying, issuing, clearing (and an idle) warp
     static constexpr int slabs = dims / 64;            // a tile lies in slabs of 64 columns, rows of 128 bytes
     static constexpr int q_bytes = parts == 1 ? kTileRows * dims * 2 : 0;  // of a tile (fp32: in tensor memory)
     static constexpr int k_part = block * dims * 2, k_bytes = parts * k_part;  // (of the values too)
@@ -154,7 +154,7 @@ template <class Elem, class Out, class S>
 __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const __grid_constant__ PromptLaunch launch) {
     extern __shared__ uint8_t raw_shared[];
     __shared__ uint64_t q_full, k_full[S::stages], k_empty[S::stages], v_full[S::stages], v_empty[S::stages];
-    __shared__ uint64_t score_full[2], weight_full[2][2], context_full[2], drained;
+    __shared__ uint64_t score_full[2], weight_full[2][2], context_full[2], ragged_there, cleared, drained;
     __shared__ uint32_t tensor_at;
     __shared__ uint32_t give_up;
     __shared__ int carry[32];
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     uint8_t* shared = raw_shared + ((1024 - (smem_address(raw_shared) & 1023)) & 1023);
     int* prefix = reinterpret_cast<int*>(shared + S::shared);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    constexpr int kCopyWarp = S::tiles * 4, kIssueWarp = S::tiles * 4 + 1;
+    constexpr int kCopyWarp = S::tiles * 4, kIssueWarp = kCopyWarp + 1, kTailWarp = kCopyWarp + 2;
     constexpr int kRows = S::tiles * kTileRows;
 
     const auto queries_of = [&](int b) { return max(min(p.q_offsets[b + 1], p.total_q) - max(p.q_offsets[b], (int64_t)0), (int64_t)0); };
@@ -187,6 +187,9 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         most = max(most, counts[t]);
     }
 
+    // The block that ends behind the sequence's last key, if there is one.
+    const int ragged = most > 0 && (begin + most) * S::block > keys ? most - 1 : -1;
+
     if (threadIdx.x == 0) {
         barrier_init(&q_full, S::parts == 1 ? 1 : 128);
         for (int s = 0; s < S::stages; ++s) {
@@ -201,6 +204,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             barrier_init(&weight_full[t][1], 128);
             barrier_init(&context_full[t], 1);
         }
+        barrier_init(&ragged_there, 1);
+        barrier_init(&cleared, 1);
         barrier_init(&drained, 1);
         barrier_init_fence();
         give_up = 0;
@@ -275,6 +280,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         }
     } else if (warp == kIssueWarp) {
         few_registers();
+        // The warp waits as a whole, and meets after one thread has issued: lanes that went ahead to the next wait would hold it up.
         constexpr bool bfloat = __is_same(Elem, __nv_bfloat16);
         const uint32_t score_kind = product_descriptor(bfloat, false, kTileRows, S::block);
         const uint32_t context_kind = product_descriptor(bfloat, true, kTileRows, launch.dims16);
@@ -313,36 +319,33 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                 }
             }
         };
-        // Values behind the sequence's last key become zeros, by the whole warp, when their block has arrived.
-        const auto clear_tail = [&](int c, int s) {
-            const int64_t real = keys - (begin + c) * S::block;
-            if (real >= S::block) return;
-            const int rows = S::block - (int)real;
-            for (int slab = 0; slab < S::parts * S::slabs; ++slab) {
-                uint4* row = reinterpret_cast<uint4*>(shared + (v_at - q_at) + s * S::k_bytes + slab * (S::block * 128) + real * 128);
-                for (int i = lane; i < rows * 8; i += 32) row[i] = make_uint4(0, 0, 0, 0);
-            }
-            shared_writes_before_async();
+        const auto issue = [&](auto what) {
+            if (elected()) what();
             __syncwarp();
         };
-        const auto arrive = [&](uint64_t* bar) {
-            if (lane == 0) products_arrive(bar);
-        };
         const auto stage_wait = [&](uint64_t* full, int c) { return wait(&full[c % S::stages], (c / S::stages) & 1); };
+        // The values of block c: the last one's when another warp has cleared what lies behind the sequence.
+        const auto values_wait = [&](int c) {
+            if (!stage_wait(v_full, c)) return false;
+            if (c != ragged) return true;
+            if (lane == 0) barrier_arrive(&ragged_there);
+            return wait(&cleared, 0);
+        };
         bool fine = most == 0 || (wait(&q_full, 0) && stage_wait(k_full, 0));
         if (most > 0 && fine) {
             tensor_fence_after();
             if constexpr (S::tiles == 2) {
                 for (int t = 0; t < 2; ++t) {
                     if (counts[t] == 0) continue;
-                    if (lane == 0) score(t, 0, t * S::block);
-                    arrive(&score_full[t]);
+                    issue([&] {
+                        score(t, 0, t * S::block);
+                        products_arrive(&score_full[t]);
+                    });
                 }
-                arrive(&k_empty[0]);
+                issue([&] { products_arrive(&k_empty[0]); });
                 for (int c = 0; c < most && fine; ++c) {
-                    fine = stage_wait(v_full, c);
+                    fine = values_wait(c);
                     if (!fine) break;
-                    clear_tail(c, c % S::stages);
                     bool next = false;  // the next block's keys are there
                     for (int t = 0; t < 2 && fine; ++t) {
                         if (c >= counts[t]) continue;
@@ -350,51 +353,77 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                             fine = wait(&weight_full[t][half], c & 1);
                             if (!fine) break;
                             tensor_fence_after();
-                            if (lane == 0) {
+                            issue([&] {
                                 if (half == 0) weigh(t, t, c % S::stages, 0, S::block / 32, c > 0);
                                 else weigh(t, t, c % S::stages, S::block / 32, S::block / 16, true);
-                            }
+                            });
                         }
                         if (!fine) break;
                         if (c + 1 == counts[t]) {
-                            arrive(&context_full[t]);
+                            issue([&] { products_arrive(&context_full[t]); });
                             continue;
                         }
                         if (!next) fine = next = stage_wait(k_full, c + 1);
                         if (!fine) break;
-                        if (lane == 0) score(t, (c + 1) % S::stages, t * S::block);
-                        arrive(&score_full[t]);
+                        issue([&] {
+                            score(t, (c + 1) % S::stages, t * S::block);
+                            products_arrive(&score_full[t]);
+                        });
                     }
-                    arrive(&v_empty[c % S::stages]);
-                    if (next) arrive(&k_empty[(c + 1) % S::stages]);
+                    issue([&] {
+                        products_arrive(&v_empty[c % S::stages]);
+                        if (next) products_arrive(&k_empty[(c + 1) % S::stages]);
+                    });
                 }
             } else {
-                if (lane == 0) score(0, 0, 0);
-                arrive(&score_full[0]);
-                arrive(&k_empty[0]);
+                issue([&] {
+                    score(0, 0, 0);
+                    products_arrive(&score_full[0]);
+                    products_arrive(&k_empty[0]);
+                });
                 for (int c = 0; c < most && fine; ++c) {
                     if (c + 1 < most) {  // (in the place of block c - 1's weights, which the products before this one read)
                         fine = stage_wait(k_full, c + 1);
                         if (!fine) break;
-                        if (lane == 0) score(0, (c + 1) % S::stages, ((c + 1) & 1) * S::block);
-                        arrive(&score_full[(c + 1) & 1]);
-                        arrive(&k_empty[(c + 1) % S::stages]);
+                        issue([&] {
+                            score(0, (c + 1) % S::stages, ((c + 1) & 1) * S::block);
+                            products_arrive(&score_full[(c + 1) & 1]);
+                            products_arrive(&k_empty[(c + 1) % S::stages]);
+                        });
                     }
-                    fine = stage_wait(v_full, c);
+                    fine = values_wait(c);
                     if (!fine) break;
-                    clear_tail(c, c % S::stages);
                     fine = wait(&weight_full[0][0], c & 1);
                     if (!fine) break;
                     tensor_fence_after();
-                    if (lane == 0) weigh(0, c & 1, c % S::stages, 0, S::block / 16, false);
-                    arrive(&context_full[0]);
-                    arrive(&v_empty[c % S::stages]);
+                    issue([&] {
+                        weigh(0, c & 1, c % S::stages, 0, S::block / 16, false);
+                        products_arrive(&context_full[0]);
+                        products_arrive(&v_empty[c % S::stages]);
+                    });
                 }
             }
         }
         // Every product has ended before tensor memory is given back.
-        arrive(&drained);
+        issue([&] { products_arrive(&drained); });
         barrier_wait_bounded(&drained, 0, p.wait_limit_ns);
+    } else if (warp == kTailWarp) {
+        few_registers();
+        // Values behind the sequence's last key become zeros when their block has arrived.  (The issuing thread says when: it is the
+        // one that follows the barriers' phases.)
+        if (ragged >= 0) {
+            const int s = ragged % S::stages;
+            if (wait(&ragged_there, 0)) {
+                const int real = (int)(keys - (begin + ragged) * S::block), rows = S::block - real;
+                for (int slab = 0; slab < S::parts * S::slabs; ++slab) {
+                    uint4* row = reinterpret_cast<uint4*>(shared + (v_at - q_at) + s * S::k_bytes + slab * (S::block * 128) + real * 128);
+                    for (int i = lane; i < rows * 8; i += 32) row[i] = make_uint4(0, 0, 0, 0);
+                }
+                shared_writes_before_async();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(&cleared);
+            }
+        }
     } else if (warp < S::tiles * 4) {
         many_registers();
         const int t = warp / 4;

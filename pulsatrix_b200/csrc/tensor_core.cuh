@@ -36,6 +36,13 @@ __device__ __forceinline__ void products_arrive(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(bar)) : "memory");
 }
 
+// One thread of a warp whose threads are all here.
+__device__ __forceinline__ bool elected() {
+    uint32_t mine;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(mine));
+    return mine != 0;
+}
+
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
