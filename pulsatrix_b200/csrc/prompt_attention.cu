@@ -99,6 +99,15 @@ __device__ __forceinline__ void split_pair(float low, float high, uint32_t& firs
     third = pack(low, high, __nv_bfloat16{});
 }
 
+// The same for numbers that are neither large nor infinite.
+__device__ __forceinline__ void split_weights(float2 w, uint32_t& first, uint32_t& second, uint32_t& third) {
+    first = pack(w.x, w.y, __nv_bfloat16{});
+    w.x -= __uint_as_float(first << 16), w.y -= __uint_as_float(first & 0xffff0000u);
+    second = pack(w.x, w.y, __nv_bfloat16{});
+    w.x -= __uint_as_float(second << 16), w.y -= __uint_as_float(second & 0xffff0000u);
+    third = pack(w.x, w.y, __nv_bfloat16{});
+}
+
 // {a, b} * {x, y} + {u, v}, each rounded as alone.
 __device__ __forceinline__ float2 fma_pair(float2 a, float2 x, float2 u) {
     float2 r;
@@ -153,7 +162,7 @@ constexpr int kPolynomialPairs = 4;  // of 16
 template <class Elem, class Out, class S>
 __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const __grid_constant__ PromptLaunch launch) {
     extern __shared__ uint8_t raw_shared[];
-    __shared__ uint64_t q_full, k_full[S::stages], k_empty[S::stages], v_full[S::stages], v_empty[S::stages];
+    __shared__ uint64_t q_full, k_full[S::stages], v_full[S::stages], k_empty[S::stages], v_empty[S::stages];
     __shared__ uint64_t score_full[2], weight_full[2][2], context_full[2], ragged_there, cleared, drained;
     __shared__ uint32_t tensor_at;
     __shared__ uint32_t give_up;
@@ -194,8 +203,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         barrier_init(&q_full, S::parts == 1 ? 1 : 128);
         for (int s = 0; s < S::stages; ++s) {
             barrier_init(&k_full[s], 1);
-            barrier_init(&k_empty[s], 1);
             barrier_init(&v_full[s], 1);
+            barrier_init(&k_empty[s], 1);
             barrier_init(&v_empty[s], 1);
         }
         for (int t = 0; t < 2; ++t) {
@@ -221,6 +230,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         return false;
     };
     const auto wait = [&](uint64_t* bar, uint32_t parity) {  // (a warp goes on as a whole or not at all)
+        if (__all_sync(0xffffffffu, barrier_passed(bar, parity))) return true;
         return __all_sync(0xffffffffu, wait_alone(bar, parity)) != 0;
     };
     const uint32_t q_at = smem_address(shared), k_at = q_at + S::tiles * S::q_bytes, v_at = k_at + S::stages * S::k_bytes;
@@ -256,7 +266,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             }
             int asked = 0;
             bool fine = true;
-            for (; asked < most && fine; ++asked) {
+            for (; asked < most; ++asked) {
                 const int s = asked % S::stages, round = asked / S::stages;
                 const int64_t z = k_begin + (begin + asked) * S::block;
                 if (round > 0 && !(fine = wait_alone(&k_empty[s], (round - 1) & 1))) break;
@@ -331,6 +341,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             if (lane == 0) barrier_arrive(&ragged_there);
             return wait(&cleared, 0);
         };
+        const auto last_tile = [&](int c) { return S::tiles == 2 && counts[S::tiles - 1] > c ? 1 : 0; };  // that works on block c
         bool fine = most == 0 || (wait(&q_full, 0) && stage_wait(k_full, 0));
         if (most > 0 && fine) {
             tensor_fence_after();
@@ -340,12 +351,11 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                     issue([&] {
                         score(t, 0, t * S::block);
                         products_arrive(&score_full[t]);
+                        if (t == last_tile(0)) products_arrive(&k_empty[0]);
                     });
                 }
-                issue([&] { products_arrive(&k_empty[0]); });
+                fine = values_wait(0);
                 for (int c = 0; c < most && fine; ++c) {
-                    fine = values_wait(c);
-                    if (!fine) break;
                     bool next = false;  // the next block's keys are there
                     for (int t = 0; t < 2 && fine; ++t) {
                         if (c >= counts[t]) continue;
@@ -360,20 +370,22 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                         }
                         if (!fine) break;
                         if (c + 1 == counts[t]) {
-                            issue([&] { products_arrive(&context_full[t]); });
+                            issue([&] {
+                                products_arrive(&context_full[t]);
+                                if (t == last_tile(c)) products_arrive(&v_empty[c % S::stages]);
+                            });
                             continue;
                         }
                         if (!next) fine = next = stage_wait(k_full, c + 1);
                         if (!fine) break;
                         issue([&] {
+                            if (t == last_tile(c)) products_arrive(&v_empty[c % S::stages]);
                             score(t, (c + 1) % S::stages, t * S::block);
                             products_arrive(&score_full[t]);
+                            if (t == last_tile(c + 1)) products_arrive(&k_empty[(c + 1) % S::stages]);
                         });
                     }
-                    issue([&] {
-                        products_arrive(&v_empty[c % S::stages]);
-                        if (next) products_arrive(&k_empty[(c + 1) % S::stages]);
-                    });
+                    if (c + 1 < most) fine = fine && values_wait(c + 1);  // (while the last products run)
                 }
             } else {
                 issue([&] {
@@ -391,9 +403,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                             products_arrive(&k_empty[(c + 1) % S::stages]);
                         });
                     }
-                    fine = values_wait(c);
-                    if (!fine) break;
-                    fine = wait(&weight_full[0][0], c & 1);
+                    fine = values_wait(c) && wait(&weight_full[0][0], c & 1);
                     if (!fine) break;
                     tensor_fence_after();
                     issue([&] {
@@ -447,13 +457,17 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         const auto add_block = [&]() {
             if constexpr (S::parts == 3) {
 #pragma unroll
-                for (int i = 0; i < S::dims; i += 32) {
+                for (int i = 0; i < S::dims; i += 64) {
                     if (i >= launch.dims16) break;
-                    float o[32];
+                    float o[64];
                     tensor_load32(context_at + i, o);
+                    tensor_load32(context_at + i + 32, o + 32);
                     tensor_loads_done();
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) context[i + k] += o[k];
+                    for (int k = 0; k < 64; k += 2) {
+                        const float2 sum = add_pair(make_float2(context[i + k], context[i + k + 1]), make_float2(o[k], o[k + 1]));
+                        context[i + k] = sum.x, context[i + k + 1] = sum.y;
+                    }
                 }
             }
         };
@@ -554,7 +568,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                         else w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
                         sums[k / 2 % 2] = add_pair(sums[k / 2 % 2], w);
                         if constexpr (S::parts == 1) packed[0][k / 2] = pack(w.x, w.y, Elem{});
-                        else split_pair(w.x, w.y, packed[0][k / 2], packed[1][k / 2], packed[2][k / 2]);
+                        else split_weights(w, packed[0][k / 2], packed[1][k / 2], packed[2][k / 2]);
                     }
 #pragma unroll
                     for (int part = 0; part < S::parts; ++part) tensor_store16(lanes + S::weight_at(place, part) + i / 2, packed[part]);

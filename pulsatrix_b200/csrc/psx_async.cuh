@@ -40,6 +40,19 @@ __device__ __forceinline__ unsigned long long global_nanoseconds() {
     return t;
 }
 
+// Whether the phase of parity `parity` has completed, after a short wait in the hardware at most.
+__device__ __forceinline__ bool barrier_passed(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_address(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // Waits for the phase of parity `parity` to complete, but not for ever: a try blocks in the
 // hardware for a short, implementation-defined time only; every 32 failed tries the global timer is
 // read, and `limit_ns` nanoseconds after its first reading the wait gives up and returns false.
@@ -47,18 +60,9 @@ __device__ __forceinline__ unsigned long long global_nanoseconds() {
 // this wait gives up at once as well.
 __device__ __forceinline__ bool barrier_wait_bounded(uint64_t* bar, uint32_t parity, unsigned long long limit_ns,
                                                      const volatile uint32_t* give_up = nullptr) {
-    const uint32_t addr = smem_address(bar);
     unsigned long long started = 0;
     for (uint32_t tries = 1;; ++tries) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (done) return true;
+        if (barrier_passed(bar, parity)) return true;
         if ((tries & 31u) == 0) {
             if (give_up && *give_up) return false;
             const unsigned long long now = global_nanoseconds();
