@@ -24,7 +24,6 @@
 #include "prompt_attention.cuh"
 
 #include <algorithm>
-#include <type_traits>
 
 #include "elements.cuh"
 #include "once_per_device.hpp"
@@ -121,42 +120,7 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 x) {
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(x.x), "f"(x.y));
     return r;
 }
-__device__ __forceinline__ float higher(float a, float b) {  // (a NaN stays one)
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float lower(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-
-// 2^x for x <= 2^6 on the FMA pipes, for a share of the weights that the special-function unit is relieved of: x = n + f with
-// |f| <= 1/2, the polynomial of least relative error for 2^f (of degree 3, off by 2^-13.7, for weights that are rounded to 8 bits; of
-// degree 4, off by 2^-18.6, for 11 bits; computed by exchange of the extrema), n added to the exponent.  Below 2^-126: that.
-template <class Elem>
-__device__ __forceinline__ float2 exp2_pair(float2 x) {
-    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: its sum with x is rounded to a whole number
-    x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
-    const float2 n = add_pair(x, both(kRound));
-    const float2 f = fma_pair(add_pair(n, both(-kRound)), both(-1.0f), x);
-    float2 y;
-    if constexpr (__is_same(Elem, __nv_bfloat16)) {
-        y = fma_pair(f, both(0.0551716685295105f), both(0.2426111251115799f));
-        y = fma_pair(y, f, both(0.6932609677314758f));
-        y = fma_pair(y, f, both(0.9999280571937561f));
-    } else {
-        y = fma_pair(f, both(0.009570102207362652f), both(0.05591785907745361f));
-        y = fma_pair(y, f, both(0.240247443318367f));
-        y = fma_pair(y, f, both(0.6931217908859253f));
-        y = fma_pair(y, f, both(0.9999992847442627f));
-    }
-    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
-                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
-}
-constexpr int kPolynomialPairs = 4;  // of 16
 
 // Elem: the type of the products' operands (bf16 for the parts of fp32); Out: the type of the context.
 template <class Elem, class Out, class S>
@@ -354,38 +318,30 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                         if (t == last_tile(0)) products_arrive(&k_empty[0]);
                     });
                 }
-                fine = values_wait(0);
                 for (int c = 0; c < most && fine; ++c) {
-                    bool next = false;  // the next block's keys are there
+                    // What can be waited for while the weights are being made comes first.
+                    fine = values_wait(c) && (c + 1 == most || stage_wait(k_full, c + 1));
                     for (int t = 0; t < 2 && fine; ++t) {
                         if (c >= counts[t]) continue;
-                        for (int half = 0; half < 2 && fine; ++half) {  // (the second half's weights are still on their way)
-                            fine = wait(&weight_full[t][half], c & 1);
-                            if (!fine) break;
-                            tensor_fence_after();
-                            issue([&] {
-                                if (half == 0) weigh(t, t, c % S::stages, 0, S::block / 32, c > 0);
-                                else weigh(t, t, c % S::stages, S::block / 32, S::block / 16, true);
-                            });
-                        }
+                        fine = wait(&weight_full[t][0], c & 1);
                         if (!fine) break;
-                        if (c + 1 == counts[t]) {
-                            issue([&] {
-                                products_arrive(&context_full[t]);
-                                if (t == last_tile(c)) products_arrive(&v_empty[c % S::stages]);
-                            });
-                            continue;
-                        }
-                        if (!next) fine = next = stage_wait(k_full, c + 1);
+                        tensor_fence_after();
+                        issue([&] { weigh(t, t, c % S::stages, 0, S::block / 32, c > 0); });
+                        fine = wait(&weight_full[t][1], c & 1);  // (the second half's weights are still on their way)
                         if (!fine) break;
+                        tensor_fence_after();
                         issue([&] {
+                            weigh(t, t, c % S::stages, S::block / 32, S::block / 16, true);
+                            if (c + 1 < counts[t]) {
+                                score(t, (c + 1) % S::stages, t * S::block);
+                                products_arrive(&score_full[t]);
+                                if (t == last_tile(c + 1)) products_arrive(&k_empty[(c + 1) % S::stages]);
+                            } else {
+                                products_arrive(&context_full[t]);
+                            }
                             if (t == last_tile(c)) products_arrive(&v_empty[c % S::stages]);
-                            score(t, (c + 1) % S::stages, t * S::block);
-                            products_arrive(&score_full[t]);
-                            if (t == last_tile(c + 1)) products_arrive(&k_empty[(c + 1) % S::stages]);
                         });
                     }
-                    if (c + 1 < most) fine = fine && values_wait(c + 1);  // (while the last products run)
                 }
             } else {
                 issue([&] {
@@ -504,8 +460,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             for (int i = 0; i < S::block; i += 32) tensor_load32(lanes + place * S::block + i, x + i);
             tensor_loads_done();
             const int64_t key = (begin + c) * S::block;
-            const bool all_seen = key >= all_first && key + S::block <= all_end;
-            if (!all_seen) {
+            if (key < all_first || key + S::block > all_end) {
                 const int low = (int)min(max(first - key, (int64_t)0), (int64_t)S::block), high = (int)min(max(end - key, (int64_t)0), (int64_t)S::block);
 #pragma unroll
                 for (int i = 0; i < S::block; ++i) x[i] = i >= low && i < high ? x[i] : masked;
@@ -513,17 +468,16 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             float best = x[0];
             if (turned) {
 #pragma unroll
-                for (int i = 1; i < S::block; ++i) best = lower(best, x[i]);
+                for (int i = 1; i < S::block; ++i) best = fminf(best, x[i]);
             } else {
                 float m[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
                 for (int i = 4; i < S::block; i += 4) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) m[k] = higher(m[k], x[i + k]);
+                    for (int k = 0; k < 4; ++k) m[k] = fmaxf(m[k], x[i + k]);
                 }
-                best = higher(higher(m[0], m[1]), higher(m[2], m[3]));
+                best = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
             }
-            if (best != masked) total += best - best;  // (a NaN or an infinity makes the row NaN, whichever way its weight is computed)
             // The reference point moves only where the weights would grow beyond 2^8.
             const float grown = top == masked ? (best == masked ? 0.0f : -kNone) : (best - top) * factor;
             const bool moves = grown > kMostGrowth;
@@ -557,33 +511,24 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             }
             const float offset = top == masked ? 0.0f : -top * factor;
             float2 sums[2] = {both(0.0f), both(0.0f)};
-            const auto weights = [&](auto mixed) {  // mixed: some of them by the polynomial
 #pragma unroll
-                for (int i = 0; i < S::block; i += 32) {
-                    uint32_t packed[S::parts][16];
+            for (int i = 0; i < S::block; i += 32) {
+                uint32_t packed[S::parts][16];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        float2 w = fma_pair(make_float2(x[i + k], x[i + k + 1]), both(factor), both(offset));
-                        if (decltype(mixed)::value && k / 2 % (16 / kPolynomialPairs) == 1) w = exp2_pair<Elem>(w);
-                        else w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
-                        sums[k / 2 % 2] = add_pair(sums[k / 2 % 2], w);
-                        if constexpr (S::parts == 1) packed[0][k / 2] = pack(w.x, w.y, Elem{});
-                        else split_weights(w, packed[0][k / 2], packed[1][k / 2], packed[2][k / 2]);
-                    }
-#pragma unroll
-                    for (int part = 0; part < S::parts; ++part) tensor_store16(lanes + S::weight_at(place, part) + i / 2, packed[part]);
-                    if (S::parts == 1 && i + 32 == S::block / 2) {
-                        tensor_stores_done();
-                        tensor_fence_before();
-                        barrier_arrive(&weight_full[t][0]);
-                    }
+                for (int k = 0; k < 32; k += 2) {
+                    float2 w = fma_pair(make_float2(x[i + k], x[i + k + 1]), both(factor), both(offset));
+                    w = make_float2(exp2_approx(w.x), exp2_approx(w.y));
+                    sums[k / 2 % 2] = add_pair(sums[k / 2 % 2], w);
+                    if constexpr (S::parts == 1) packed[0][k / 2] = pack(w.x, w.y, Elem{});
+                    else split_weights(w, packed[0][k / 2], packed[1][k / 2], packed[2][k / 2]);
                 }
-            };
-            if constexpr (S::parts == 1) {
-                if (all_seen) weights(std::true_type{});
-                else weights(std::false_type{});
-            } else {
-                weights(std::false_type{});
+#pragma unroll
+                for (int part = 0; part < S::parts; ++part) tensor_store16(lanes + S::weight_at(place, part) + i / 2, packed[part]);
+                if (S::parts == 1 && i + 32 == S::block / 2) {
+                    tensor_stores_done();
+                    tensor_fence_before();
+                    barrier_arrive(&weight_full[t][0]);
+                }
             }
             total += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
             tensor_stores_done();
