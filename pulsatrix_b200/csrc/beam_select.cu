@@ -2,7 +2,7 @@
 //
 //     value(b, v) = (score_b - log sum_w exp(l_bw)) + l_bv        (double precision; ties: the lowest b, then the lowest v)
 //
-// First kernel, a block per part of a row: the logits are read once, in chunks of 16 per thread (4 where that would leave SMs
+// A block takes a part of a row: the logits are read once, in chunks of 16 per thread (4 where that would leave SMs
 // idle) with the next chunk on its way, a running maximum and sum per thread; the part leaves its maximum, its sum of
 // exponentials and its `keep` best logits in order.  Within a row the order by value is the order by logit, so nothing else of
 // the part can be among the group's best.  The `keep` best are found without sorting the part: every warp gives the n-th
@@ -11,8 +11,8 @@
 // (some more than `keep`); an entry's place is the number of keys above its own.  A list that overflows (thousands of equal
 // logits) is replaced by `keep` sweeps over those chunks.  Bound by HBM: 4 bytes per logit.
 //
-// Second kernel, a block per group: the rows' normalisers from the parts' sums, then the same selection over the parts' lists.
-// It is launched early and waits for the first kernel's end.
+// The block of a group that ends last goes on with the group: the rows' normalisers from the parts' sums, then the same selection over
+// the parts' lists.  (A second kernel for that cost one call of 4 beams 3 us on the GPU and as much on the host.)
 //
 // The exponentials are summed in float over a thread's logits, relative to its maximum so far, and in double from there on, in
 // an order that depends on columns alone: equal rows have equal normalisers, so that their candidates tie.
@@ -28,7 +28,7 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMostChunks = 8;  // of a part
 constexpr int kPartList = 1024, kGroupList = 1024;
-constexpr int kHeldEntries = 8;  // per thread of the second kernel
+constexpr int kHeldEntries = 8;  // per thread, of the parts' lists
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -80,13 +80,16 @@ __device__ __forceinline__ float2 mul_pair(float2 a, float2 x) {
     return r;
 }
 
+struct PartShared {
+    uint64_t list[kPartList], best_of[kWarps];
+    uint32_t bounds[kWarps], tops[kWarps];
+    double sums[kWarps];
+    int listed;
+};
+
 template <int values, bool aligned>
-__global__ void __launch_bounds__(kThreads, 4) beam_parts_kernel(const __grid_constant__ BeamSelectParams p) {
+__device__ __forceinline__ void part_of_row(const BeamSelectParams& p, PartShared& s) {
     constexpr int kChunk = kThreads * values;
-    __shared__ uint64_t list[kPartList], best_of[kWarps];
-    __shared__ uint32_t bounds[kWarps], tops[kWarps];
-    __shared__ double sums[kWarps];
-    __shared__ int listed;
     const int64_t part_row = blockIdx.x;
     const int64_t row = part_row / p.parts;
     const int part = (int)(part_row % p.parts), keep = p.keep, begin = part * p.chunks * kChunk, end = min(begin + p.chunks * kChunk, p.vocab);
@@ -100,10 +103,9 @@ __global__ void __launch_bounds__(kThreads, 4) beam_parts_kernel(const __grid_co
             entries[i] = {offers ? 0.0f : kNone, offers ? (int)p.finished_token : -1};
         }
         if (threadIdx.x == 0) p.part_stats[part_row] = {0.0, kNone, 0};
-        asm volatile("griddepcontrol.launch_dependents;");
         return;
     }
-    if (threadIdx.x == 0) listed = 0;
+    if (threadIdx.x == 0) s.listed = 0;
 
     const float* from = p.logits + row * p.row_stride;
     // Column of a thread's j-th logit of a chunk: fours of neighbours where the rows are aligned, neighbours on neighbouring lanes else.
@@ -161,14 +163,14 @@ __global__ void __launch_bounds__(kThreads, 4) beam_parts_kernel(const __grid_co
 #pragma unroll
     for (int step = 16; step > 0; step /= 2) total += __shfl_xor_sync(0xffffffffu, total, step);
     if (lane == 0) {
-        bounds[warp] = mine;
-        tops[warp] = warp_top_key;
-        sums[warp] = total;
+        s.bounds[warp] = mine;
+        s.tops[warp] = warp_top_key;
+        s.sums[warp] = total;
     }
     __syncthreads();
-    uint32_t bound_key = bounds[0];
+    uint32_t bound_key = s.bounds[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) bound_key = min(bound_key, bounds[w]);
+    for (int w = 1; w < kWarps; ++w) bound_key = min(bound_key, s.bounds[w]);
     const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
     uint32_t hits = 0;  // the chunks that reach the bound; they are read again, out of L2
 #pragma unroll
@@ -179,28 +181,28 @@ __global__ void __launch_bounds__(kThreads, 4) beam_parts_kernel(const __grid_co
 #pragma unroll
         for (int j = 0; j < values; ++j) {
             if (v[0][j] >= bound && v[0][j] > kNone) {
-                const int at = atomicAdd(&listed, 1);
-                if (at < kPartList) list[at] = entry_key(v[0][j], column(c, j));
+                const int at = atomicAdd(&s.listed, 1);
+                if (at < kPartList) s.list[at] = entry_key(v[0][j], column(c, j));
             }
         }
     }
     __syncthreads();
-    const int count = listed;
+    const int count = s.listed;
     if (warp == kWarps - 1) {  // the part's record
-        const float warp_top = lane < kWarps ? from_ordered(tops[lane]) : kNone;
+        const float warp_top = lane < kWarps ? from_ordered(s.tops[lane]) : kNone;
         float part_top = warp_top;
         for (int step = 16; step > 0; step /= 2) part_top = fmaxf(part_top, __shfl_xor_sync(0xffffffffu, part_top, step));
         const float level = part_top > kNone ? part_top : 0.0f;
-        double part_sum = lane < kWarps ? sums[lane] * exp((double)warp_top - (double)level) : 0.0;
+        double part_sum = lane < kWarps ? s.sums[lane] * exp((double)warp_top - (double)level) : 0.0;
         for (int step = 16; step > 0; step /= 2) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, step);
         if (lane == 0) p.part_stats[part_row] = {part_sum, part_top, part_sum != part_sum};
     }
     int placed = min(count, keep);
     if (count <= kPartList) {
         for (int e = threadIdx.x; e < count; e += kThreads) {
-            const uint64_t key = list[e];
+            const uint64_t key = s.list[e];
             int place = 0;
-            for (int k = 0; k < count; ++k) place += list[k] > key;
+            for (int k = 0; k < count; ++k) place += s.list[k] > key;
             if (place < keep) entries[place] = {from_ordered((uint32_t)(key >> 32)), (int)~(uint32_t)key};
         }
     } else {
@@ -216,14 +218,13 @@ __global__ void __launch_bounds__(kThreads, 4) beam_parts_kernel(const __grid_co
                     if (key < last) best = max(best, key);
                 }
             }
-            best = block_max(best, best_of);
+            best = block_max(best, s.best_of);
             if (best == 0) break;
             if (threadIdx.x == 0) entries[placed] = {from_ordered((uint32_t)(best >> 32)), (int)~(uint32_t)best};
             last = best;
         }
     }
     for (int i = placed + threadIdx.x; i < keep; i += kThreads) entries[i] = {kNone, -1};
-    asm volatile("griddepcontrol.launch_dependents;");
 }
 
 struct Candidate {
@@ -238,15 +239,26 @@ __device__ __forceinline__ bool ahead(const Candidate& a, const Candidate& b) {
 // The value as a float, in an order that rounding keeps; what is below the lowest float counts as that, so that it stays a candidate.
 __device__ __forceinline__ float as_float(double value) { return value > (double)kNone ? fmaxf((float)value, -3.402823466e38f) : kNone; }
 
-__global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_constant__ BeamSelectParams p) {
-    __shared__ double base[kMostSelectBeams];  // score - normaliser; -inf: the beam offers nothing
-    __shared__ Candidate list[kGroupList], best_of[kWarps];
-    __shared__ uint32_t bounds[kWarps];
-    __shared__ int listed, not_finite;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t group = blockIdx.x;
+// What other blocks have written: out of L2.
+__device__ __forceinline__ BeamEntry load_entry(const BeamEntry* at) {
+    const float2 two = __ldcg(reinterpret_cast<const float2*>(at));
+    return {two.x, __float_as_int(two.y)};
+}
+__device__ __forceinline__ BeamPart load_part(const BeamPart* at) {
+    const double2 two = __ldcg(reinterpret_cast<const double2*>(at));
+    return {two.x, __int_as_float(__double2loint(two.y)), __double2hiint(two.y)};
+}
+
+struct GroupShared {
+    double base[kMostSelectBeams];  // score - normaliser; -inf: the beam offers nothing
+    Candidate list[kGroupList], best_of[kWarps];
+    uint32_t bounds[kWarps];
+    int listed, not_finite;
+};
+
+__device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupShared& s, int64_t group) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, keep = p.keep;
-    if (threadIdx.x == 0) listed = 0, not_finite = 0;
+    if (threadIdx.x == 0) s.listed = 0, s.not_finite = 0;
     // The lists' first entries, the best of all lists, then the second ones and so on, are asked for ahead of the normalisers and
     // kept.  Every eight neighbours go to the eight warps in an order that changes: the bound is good where each warp has its
     // share of the best, and one beam's lists are neighbours.
@@ -262,7 +274,7 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
 #pragma unroll
     for (int i = 0; i < kHeldEntries; ++i) {
         const int x = place_of(i);
-        held[i] = x < all_held ? entries[x % lists * keep + x / lists] : BeamEntry{kNone, -1};
+        held[i] = x < all_held ? load_entry(entries + x % lists * keep + x / lists) : BeamEntry{kNone, -1};
     }
     __syncthreads();
     for (int b = warp; b < p.beams; b += kWarps) {
@@ -273,27 +285,27 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
         float top = kNone;
         int wrong = !(score < -kNone);
         for (int i = lane; i < p.parts; i += 32) {
-            const BeamPart part = parts[i];
+            const BeamPart part = load_part(parts + i);
             top = fmaxf(top, part.top);
             wrong |= part.not_finite;
         }
         for (int step = 16; step > 0; step /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
         double sum = 0.0;
         for (int i = lane; i < p.parts; i += 32) {
-            const BeamPart part = parts[i];
+            const BeamPart part = load_part(parts + i);
             if (part.top > kNone) sum += part.sum * exp((double)part.top - (double)top);
         }
         for (int step = 16; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
         wrong = __any_sync(0xffffffffu, wrong);
         if (lane == 0) {
-            if (wrong) not_finite = 1;
-            base[b] = ended ? (double)score : sum > 0.0 ? (double)score - ((double)top + log(sum)) : (double)kNone;
+            if (wrong) s.not_finite = 1;
+            s.base[b] = ended ? (double)score : sum > 0.0 ? (double)score - ((double)top + log(sum)) : (double)kNone;
         }
     }
     __syncthreads();
     const auto candidate_of = [&](int of_list, BeamEntry entry) {
         const int b = of_list / p.parts;
-        return Candidate{base[b] + (double)entry.logit, (uint64_t)b << 32 | (uint32_t)entry.token};
+        return Candidate{s.base[b] + (double)entry.logit, (uint64_t)b << 32 | (uint32_t)entry.token};
     };
     float largest = kNone;
 #pragma unroll
@@ -302,16 +314,16 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
         if (x < all_held) largest = fmaxf(largest, as_float(candidate_of(x % lists, held[i]).value));
     }
     const uint32_t mine = warp_bound(largest, keep, nullptr);
-    if (lane == 0) bounds[warp] = mine;
+    if (lane == 0) s.bounds[warp] = mine;
     __syncthreads();
-    uint32_t bound_key = bounds[0];
-    for (int w = 1; w < kWarps; ++w) bound_key = min(bound_key, bounds[w]);
+    uint32_t bound_key = s.bounds[0];
+    for (int w = 1; w < kWarps; ++w) bound_key = min(bound_key, s.bounds[w]);
     const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
     // (rounding to float keeps the order: what is at or above the bound in double is so in float)
     const auto offer = [&](const Candidate& c) {
         if (!(c.value > (double)kNone && as_float(c.value) >= bound)) return false;
-        const int at = atomicAdd(&listed, 1);
-        if (at < kGroupList) list[at] = c;
+        const int at = atomicAdd(&s.listed, 1);
+        if (at < kGroupList) s.list[at] = c;
         return true;
     };
     if (largest >= bound && largest > kNone) {
@@ -323,13 +335,13 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
     }
     if (all_held < lists * keep) {  // lists are in order: each from where it is not held on, as far as it reaches the bound
         for (int q = threadIdx.x; q < lists; q += kThreads) {
-            for (int slot = max(kHeld - q + lists - 1, 0) / lists; slot < keep && offer(candidate_of(q, entries[q * keep + slot])); ++slot) {
+            for (int slot = max(kHeld - q + lists - 1, 0) / lists; slot < keep && offer(candidate_of(q, load_entry(entries + q * keep + slot))); ++slot) {
             }
         }
     }
     __syncthreads();
-    const int count = listed;
-    const bool wrong = not_finite != 0;
+    const int count = s.listed;
+    const bool wrong = s.not_finite != 0;
     int placed = wrong ? 0 : min(count, keep);
     const auto put = [&](int place, const Candidate& c) {
         const int64_t at = group * keep + place;
@@ -340,9 +352,9 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
     if (wrong) {
     } else if (count <= kGroupList) {
         for (int e = threadIdx.x; e < count; e += kThreads) {
-            const Candidate c = list[e];
+            const Candidate c = s.list[e];
             int place = 0;
-            for (int k = 0; k < count; ++k) place += ahead(list[k], c);
+            for (int k = 0; k < count; ++k) place += ahead(s.list[k], c);
             if (place < keep) put(place, c);
         }
     } else {  // more that tie at the bound than the list holds: sweep after sweep, the best that is behind the last one
@@ -350,17 +362,17 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
         for (placed = 0; placed < keep; ++placed) {
             Candidate best{(double)kNone, ~0ull};
             for (int e = threadIdx.x; e < lists * keep; e += kThreads) {
-                const Candidate c = candidate_of(e / keep, entries[e]);
+                const Candidate c = candidate_of(e / keep, load_entry(entries + e));
                 if (ahead(last, c) && ahead(c, best)) best = c;
             }
             for (int step = 16; step > 0; step /= 2) {
                 const Candidate other{__shfl_xor_sync(0xffffffffu, best.value, step), __shfl_xor_sync(0xffffffffu, best.place, step)};
                 if (ahead(other, best)) best = other;
             }
-            if (lane == 0) best_of[warp] = best;
+            if (lane == 0) s.best_of[warp] = best;
             __syncthreads();
             for (int w = 0; w < kWarps; ++w) {
-                if (ahead(best_of[w], best)) best = best_of[w];
+                if (ahead(s.best_of[w], best)) best = s.best_of[w];
             }
             __syncthreads();
             if (best.value == (double)kNone) break;
@@ -374,6 +386,27 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(const __grid_cons
         p.tokens[group * keep + i] = -1;
     }
     if (threadIdx.x == 0 && p.group_status) p.group_status[group] = wrong ? 4 : placed == 0 ? 5 : 0;  // (psx_row_status)
+}
+
+template <int values, bool aligned>
+__global__ void __launch_bounds__(kThreads, values == 16 ? 4 : 2) beam_select_kernel(const __grid_constant__ BeamSelectParams p) {
+    __shared__ union Shared {
+        PartShared part;
+        GroupShared group;
+        __device__ Shared() {}
+    } shared;
+    __shared__ int is_last;
+    part_of_row<values, aligned>(p, shared.part);
+    const int64_t group = blockIdx.x / (unsigned)(p.beams * p.parts);
+    __syncthreads();
+    if (threadIdx.x == 0) {  // (release: the block's part, ordered before by the barrier; acquire: the others')
+        int before;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + group) : "memory");
+        is_last = before == p.beams * p.parts - 1;
+        if (is_last) p.arrived[group] = 0;
+    }
+    __syncthreads();
+    if (is_last) best_of_group(p, shared.group, group);
 }
 
 }  // namespace
@@ -395,23 +428,13 @@ void plan_beam_select(BeamSelectParams& p, int sm_count) {
 cudaError_t launch_beam_select(const BeamSelectParams& p, cudaStream_t stream) {
     const unsigned blocks = (unsigned)(p.groups * p.beams * p.parts);
     if (p.values == 4) {
-        if (p.aligned) beam_parts_kernel<4, true><<<blocks, kThreads, 0, stream>>>(p);
-        else beam_parts_kernel<4, false><<<blocks, kThreads, 0, stream>>>(p);
+        if (p.aligned) beam_select_kernel<4, true><<<blocks, kThreads, 0, stream>>>(p);
+        else beam_select_kernel<4, false><<<blocks, kThreads, 0, stream>>>(p);
     } else {
-        if (p.aligned) beam_parts_kernel<16, true><<<blocks, kThreads, 0, stream>>>(p);
-        else beam_parts_kernel<16, false><<<blocks, kThreads, 0, stream>>>(p);
+        if (p.aligned) beam_select_kernel<16, true><<<blocks, kThreads, 0, stream>>>(p);
+        else beam_select_kernel<16, false><<<blocks, kThreads, 0, stream>>>(p);
     }
-    if (const cudaError_t e = cudaGetLastError()) return e;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)p.groups);
-    config.blockDim = dim3(kThreads);
-    config.stream = stream;
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, beam_groups_kernel, p);
+    return cudaGetLastError();
 }
 
 }  // namespace psx

@@ -10,7 +10,7 @@ namespace psx {
 constexpr int kMostKept = 128;         // candidates per group
 constexpr int kMostSelectBeams = 64;
 
-struct BeamPart {        // what the first kernel leaves of a part of a row
+struct BeamPart {        // what is left of a part of a row
     double sum;          // of exp(logit - top) over the part
     float top;           // the part's largest logit; -inf: none
     int32_t not_finite;  // it holds a NaN or +inf
@@ -35,6 +35,7 @@ struct BeamSelectParams {
     int32_t values;           // logits per thread of a chunk: 4 or 16
     int32_t chunks;           // of a part, 1 to 8
     int32_t aligned;          // every row starts on a 16-byte boundary and is a multiple of four long
+    int32_t* arrived;         // scratch: (groups), zero between calls
     BeamPart* part_stats;     // (groups * beams, parts)
     BeamEntry* entries;       // (groups * beams, parts, keep), best first
 };

@@ -91,7 +91,7 @@ struct psx_ctx {
     // staging of the sharded path
     Buffer shard_uniform_scratch;
     // Scratch that captured graphs may hold: what it outgrows stays allocated until the context goes (see reserve_kept).
-    Buffer beam_scratch, attention_8bit_pieces, attention_8bit_arrived, prompt_parts;
+    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts;
     std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
     bool timing = false;
@@ -131,6 +131,17 @@ psx_status reserve_kept(psx_ctx* ctx, cudaStream_t stream, Buffer& b, size_t byt
     b.ptr = ptr;
     b.bytes = want;
     if (grown) *grown = true;
+    return PSX_OK;
+}
+
+// Counters that are zero between calls: every call leaves them so.
+psx_status reserve_counters(psx_ctx* ctx, cudaStream_t stream, Buffer& b, size_t count) {
+    bool grown;
+    if (psx_status s = reserve_kept(ctx, stream, b, count * sizeof(int32_t), &grown)) return s;
+    if (!grown) return PSX_OK;
+    const cudaError_t e = cudaMemsetAsync(b.ptr, 0, b.bytes, stream);
+    if (e != cudaSuccess) b.bytes = 0;  // (what is not zero is not used)
+    PSX_CUDA(e);
     return PSX_OK;
 }
 
@@ -423,7 +434,7 @@ void psx_b200_ctx_destroy(psx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Buffer* b : {&ctx->stats[0], &ctx->stats[1], &ctx->part_counts[0], &ctx->part_counts[1], &ctx->candidates[0], &ctx->candidates[1], &ctx->banned, &ctx->sort_keys, &ctx->head_logits, &ctx->attention_partial, &ctx->surv_cols, &ctx->surv_vals,
                       &ctx->surv_counts, &ctx->pl_tokens, &ctx->pl_log_probs, &ctx->pl_status, &ctx->h_logits, &ctx->h_inputs,
-                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts}) {
+                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts}) {
         if (b->ptr) cudaFree(b->ptr);
     }
     for (void* p : ctx->outgrown) cudaFree(p);
@@ -1173,8 +1184,10 @@ psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream_ptr, const float* log
     if (psx_status s = reserve_kept(ctx, stream, ctx->beam_scratch, stats_bytes + (size_t)(lists * keep) * sizeof(psx::BeamEntry))) return s;
     p.part_stats = static_cast<psx::BeamPart*>(ctx->beam_scratch.ptr);
     p.entries = reinterpret_cast<psx::BeamEntry*>(static_cast<char*>(ctx->beam_scratch.ptr) + stats_bytes);
+    if (psx_status s = reserve_counters(ctx, stream, ctx->beam_arrived, (size_t)groups)) return s;
+    p.arrived = static_cast<int32_t*>(ctx->beam_arrived.ptr);
     PSX_CUDA(psx::launch_beam_select(p, stream));
-    ctx->launches += 2;
+    ctx->launches += 1;
     return PSX_OK;
 }
 
@@ -1188,6 +1201,7 @@ psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream_ptr, const psx_bea
     if (groups > 0x7fffffff / beams) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
     // The bytes that the call touches, none of them twice.
     std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+    ranges.reserve((size_t)count + 2);
     for (int64_t i = 0; i < count; ++i) {
         const psx_beam_state& s = states[i];
         if (s.heads < 0 || s.positions < 0 || s.position_bytes <= 0 || s.tokens_per_position <= 0) {
@@ -1211,7 +1225,8 @@ psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream_ptr, const psx_bea
     }
     const OnDevice device(ctx->device);
     PSX_CUDA(device.error);
-    psx::ReorderParams p{};
+    psx::ReorderParams p;
+    p.count = 0;
     p.beams = (int32_t)beams; p.groups = groups; p.parents = parents; p.lengths = lengths;
     for (int64_t i = 0; i < count; ++i) {
         const psx_beam_state& s = states[i];
@@ -1308,15 +1323,8 @@ psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const 
     PSX_CUDA(device.error);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     psx::plan_attention_8bit(p, ctx->sm_count);
-    bool grown;
-    const size_t counters = (size_t)(cache->batch * cache->kv_heads) * sizeof(int32_t);
     if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;
-    if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_arrived, counters, &grown)) return s;
-    if (grown) {
-        const cudaError_t e = cudaMemsetAsync(ctx->attention_8bit_arrived.ptr, 0, ctx->attention_8bit_arrived.bytes, stream);
-        if (e != cudaSuccess) ctx->attention_8bit_arrived.bytes = 0;  // (counters that are not zero are not used)
-        PSX_CUDA(e);
-    }
+    if (psx_status s = reserve_counters(ctx, stream, ctx->attention_8bit_arrived, (size_t)(cache->batch * cache->kv_heads))) return s;
     p.partial = static_cast<float*>(ctx->attention_8bit_pieces.ptr);
     p.arrived = static_cast<int32_t*>(ctx->attention_8bit_arrived.ptr);
     PSX_CUDA(psx::launch_decode_attention_8bit(p, stream));

@@ -12,9 +12,11 @@
 // rounded to halves (2^-11, below the rounding of a bf16 or fp16 context; for fp32 contexts again two halves).  Maxima, sums
 // and contexts are floats.
 //
-// The cached positions of all (row, kv head) pairs lie on one axis, in tiles of 32, and every block takes an equal share of it:
-// lengths that differ from row to row leave no SM idle, and one long row is spread over all of them.  A pair that several
-// blocks share leaves a piece per block; the last block to arrive joins them, in order.  Inside a block each of four warps
+// A (row, kv head) pair's cached positions are cut into tiles of 32.  With many pairs the tiles of all lie on one axis and every
+// block takes an equal share of it: lengths that differ from row to row leave no SM idle.  With few (four blocks for each, at least, fit
+// on the GPU) every pair has as many blocks as fit, which saves a block the sums over the rows' lengths and the end of one pair
+// before the start of the next (one request of 777 positions: 12.2 us with shares of the axis, PIECES_US with blocks of its own).
+// A pair that several blocks share leaves a piece per block; the last block to arrive joins them, in order.  Inside a block each of four warps
 // takes every fourth tile, with its own two stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no
 // warp waits for another until the end of a pair.  Bound by HBM: 2 bytes per position, head dimension and kv head.
 #include "decode_attention_8bit.cuh"
@@ -124,27 +126,52 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
     const uint32_t stages_at = shared_address(stages);
     const int shift = 31 - __clz(c.block);
 
-    sum_of_rows(batch, prefix, carry, [&](int row) {
-        const Sight s = sight_of(p, row);
-        return max(s.end_tile() - s.first_tile(), 0) * c.kv_heads;
-    });
-    const int all = prefix[batch];
-    const int share = max((int)(((int64_t)all + gridDim.x - 1) / gridDim.x), p.least_share);
-    // Rows that see nothing have no tiles, hence no block: their context is zero.
-    for (int64_t row = blockIdx.x; row < batch; row += gridDim.x) {
-        if (prefix[row + 1] != prefix[row]) continue;
-        T* out = static_cast<T*>(p.context) + row * p.heads * p.q_len * head_dim;
-        for (int i = threadIdx.x; i < p.heads * p.q_len * head_dim; i += kThreads) out[i] = from_float<T>(0.0f);
+    // Which tiles of which pairs: see the two ways above.
+    const int pieces_each = p.pieces;
+    int share = p.least_share, row = 0;
+    int64_t at = 0, stop = 1;
+    if (pieces_each > 0) {
+        row = (int)(blockIdx.x / (unsigned)(c.kv_heads * pieces_each));
+    } else {
+        sum_of_rows(batch, prefix, carry, [&](int row) {
+            const Sight s = sight_of(p, row);
+            return max(s.end_tile() - s.first_tile(), 0) * c.kv_heads;
+        });
+        const int all = prefix[batch];
+        share = max((int)(((int64_t)all + gridDim.x - 1) / gridDim.x), p.least_share);
+        // Rows that see nothing have no tiles, hence no block: their context is zero.
+        for (int64_t row = blockIdx.x; row < batch; row += gridDim.x) {
+            if (prefix[row + 1] != prefix[row]) continue;
+            T* out = static_cast<T*>(p.context) + row * p.heads * p.q_len * head_dim;
+            for (int i = threadIdx.x; i < p.heads * p.q_len * head_dim; i += kThreads) out[i] = from_float<T>(0.0f);
+        }
+        at = (int64_t)blockIdx.x * share;
+        stop = min(at + share, (int64_t)all);
+        if (at < stop) row = row_of_item(prefix, batch, (int)at);
     }
-    int64_t at = (int64_t)blockIdx.x * share;
-    const int64_t stop = min(at + share, (int64_t)all);
-    int row = at < stop ? row_of_item(prefix, batch, (int)at) : 0;
     while (at < stop) {
-        while (prefix[row + 1] <= at) ++row;
+        int tiles, head, from_tile, to_tile;
+        if (pieces_each > 0) {
+            const Sight sight = sight_of(p, row);
+            tiles = max(sight.end_tile() - sight.first_tile(), 0);
+            share = max((tiles + pieces_each - 1) / pieces_each, p.least_share);
+            head = (int)(blockIdx.x / (unsigned)pieces_each) % c.kv_heads;
+            from_tile = (int)(blockIdx.x % (unsigned)pieces_each) * share;
+            to_tile = min(tiles, from_tile + share);
+            if (from_tile >= to_tile) {
+                if (tiles == 0 && from_tile == 0) {
+                    T* out = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+                    for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) out[i] = from_float<T>(0.0f);
+                }
+                return;
+            }
+        } else {
+            while (prefix[row + 1] <= at) ++row;
+            tiles = (prefix[row + 1] - prefix[row]) / c.kv_heads;
+            head = (int)(at - prefix[row]) / tiles, from_tile = (int)(at - prefix[row]) % tiles;
+            to_tile = (int)min((int64_t)tiles, from_tile + (stop - at));
+        }
         const Sight sight = sight_of(p, row);
-        const int tiles = (prefix[row + 1] - prefix[row]) / c.kv_heads;
-        const int head = (int)(at - prefix[row]) / tiles, from_tile = (int)(at - prefix[row]) % tiles;
-        const int to_tile = (int)min((int64_t)tiles, from_tile + (stop - at));
         const int64_t pair = (int64_t)row * c.kv_heads + head;
         const int tile0 = sight.first_tile();
         const uint8_t* keys = c.key_codes + pair * c.max_len * head_dim;
@@ -426,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         T* context = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
         const int piece_floats = kRows * (dims + 4);  // (a row's context, its maximum and sum, two unused)
         const int fours = head_dim / 4;
-        float* piece = p.partial + ((int64_t)blockIdx.x * 2 + (at == (int64_t)blockIdx.x * share ? 0 : 1)) * piece_floats;
+        const int64_t slot = pieces_each > 0 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 2 + (at == (int64_t)blockIdx.x * share ? 0 : 1);
+        float* piece = p.partial + slot * piece_floats;
         for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
             const int r = i / fours, d = i % fours * 4;
             float high = kNone, sum = 0.0f;
@@ -449,21 +477,28 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
             }
         }
         if (!whole) {
-            const int begin = prefix[row] + head * tiles, end = begin + tiles;
-            const int first = begin / share, last = (end - 1) / share;
+            // Where the pair's pieces are: the first one's slot, and the step to the next ones'.
+            int pieces, step, skip = 0;
+            int64_t first_slot;
+            if (pieces_each > 0) {
+                pieces = (tiles + share - 1) / share, step = 1;
+                first_slot = pair * pieces_each;
+            } else {
+                const int begin = prefix[row] + head * tiles, first = begin / share;
+                pieces = (begin + tiles - 1) / share - first + 1, step = 2;
+                first_slot = (int64_t)first * 2;
+                skip = begin != first * share ? 1 : 0;  // (it is its block's second one unless it starts it)
+            }
             __syncthreads();
             if (threadIdx.x == 0) {  // (release: the block's pieces, ordered before by the barrier; acquire: the other blocks')
                 int before;
                 asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + pair) : "memory");
-                is_last = before == last - first;
+                is_last = before == pieces - 1;
                 if (is_last) p.arrived[pair] = 0;
             }
             __syncthreads();
             if (is_last) {
-                const int pieces = last - first + 1;
-                const float* base = p.partial + (int64_t)first * 2 * piece_floats;  // (the first piece is its block's second one unless it starts it)
-                const int skip = begin != first * share ? piece_floats : 0;
-                const auto piece_of = [&](int b) { return base + (b == 0 ? skip : (int64_t)b * 2 * piece_floats); };
+                const auto piece_of = [&](int b) { return p.partial + (first_slot + (b == 0 ? skip : b * step)) * piece_floats; };
                 // A thread's part of the first pieces' contexts is asked for along with their maxima and sums.
                 constexpr int kAhead = 8;
                 const int mine_row = threadIdx.x / fours, mine_d = threadIdx.x % fours * 4;
@@ -514,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
                 }
             }
         }
-        at += to_tile - from_tile;
+        at += pieces_each > 0 ? 1 : to_tile - from_tile;
         __syncthreads();  // (shared memory is free for the next pair)
     }
 }
@@ -551,11 +586,18 @@ void plan_attention_8bit(Attention8bitParams& p, int sm_count) {
     const int64_t tiles = (p.cache.max_len + kTile - 1) / kTile;
     // The pieces of a pair, one more at each end than whole shares, have their maxima and sums in shared memory when they are joined.
     const int64_t most_pieces = (int64_t)(shared_of(dims) / (p.rows * sizeof(float2))) - 2;
-    p.least_share = (int)std::max<int64_t>(kLeastShare, (tiles + most_pieces - 1) / most_pieces);
     // As many blocks as the GPU holds at once (by registers and shared memory), no more than there are least shares.
     const int resident = dims == 256 ? 1 : dims == 64 ? 4 : p.rows > 8 ? 2 : 3;
-    const int64_t shares = (p.cache.batch * p.cache.kv_heads * tiles + p.least_share - 1) / p.least_share;
-    p.grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sm_count * resident, shares));
+    const int64_t pairs = p.cache.batch * p.cache.kv_heads, blocks = (int64_t)sm_count * resident;
+    if (pairs * 4 <= blocks) {
+        p.least_share = kWarps;
+        p.pieces = (int)std::max<int64_t>(1, std::min({blocks / pairs, (tiles + kWarps - 1) / kWarps, most_pieces}));
+        p.grid = (int)(pairs * p.pieces);
+        return;
+    }
+    p.pieces = 0;
+    p.least_share = (int)std::max<int64_t>(kLeastShare, (tiles + most_pieces - 1) / most_pieces);
+    p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(blocks, (pairs * tiles + p.least_share - 1) / p.least_share));
 }
 
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p) {

@@ -21,10 +21,11 @@ struct Attention8bitParams {
     int32_t type, causal;
     int32_t grid;            // blocks
     int32_t least_share;     // tiles of 32 positions that a block takes at least
+    int32_t pieces;          // blocks of every (row, kv head); 0: every block takes an equal share of all tiles
     float scale;
 };
 
-void plan_attention_8bit(Attention8bitParams& p, int sm_count);  // grid and least_share
+void plan_attention_8bit(Attention8bitParams& p, int sm_count);  // grid, least_share and pieces
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p);
 // cudaErrorInvalidValue: see psx_b200_decode_attention_8bit for the shapes that are taken.
 cudaError_t launch_decode_attention_8bit(const Attention8bitParams& p, cudaStream_t stream);

@@ -11,11 +11,13 @@
 #include "reorder_states.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace psx {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kFewStates = 8;  // a layer's or two layers' caches
 
 struct Move {
     int64_t to, from, end;  // byte offsets of the two rows; bytes of a head that are taken over
@@ -37,8 +39,8 @@ __device__ __forceinline__ void move_columns(char* base, int64_t begin, int64_t 
     }
 }
 
-template <int beams>
-__global__ void __launch_bounds__(kThreads) reorder_states_kernel(const __grid_constant__ ReorderParams p) {
+template <int beams, int most>
+__global__ void __launch_bounds__(kThreads) reorder_states_kernel(const __grid_constant__ ReorderParamsOf<most> p) {
     __shared__ Move moves[beams];
     __shared__ int count;
     __shared__ int64_t longest;
@@ -112,11 +114,22 @@ cudaError_t launch_reorder_states(ReorderParams& p, int sm_count, cudaStream_t s
         if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
     }
     if (blocks == 0) return cudaSuccess;
-    if (p.beams <= 4) reorder_states_kernel<4><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    else if (p.beams <= 8) reorder_states_kernel<8><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    else if (p.beams <= 16) reorder_states_kernel<16><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    else if (p.beams <= 32) reorder_states_kernel<32><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    else reorder_states_kernel<64><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
+    const auto launch = [&](const auto& params, auto few) {
+        constexpr int most = decltype(few)::value;
+        if (p.beams <= 4) reorder_states_kernel<4, most><<<(unsigned)blocks, kThreads, 0, stream>>>(params);
+        else if (p.beams <= 8) reorder_states_kernel<8, most><<<(unsigned)blocks, kThreads, 0, stream>>>(params);
+        else if (p.beams <= 16) reorder_states_kernel<16, most><<<(unsigned)blocks, kThreads, 0, stream>>>(params);
+        else if (p.beams <= 32) reorder_states_kernel<32, most><<<(unsigned)blocks, kThreads, 0, stream>>>(params);
+        else reorder_states_kernel<64, most><<<(unsigned)blocks, kThreads, 0, stream>>>(params);
+    };
+    if (p.count <= kFewStates) {  // (a launch copies its parameters: half a kilobyte instead of four)
+        ReorderParamsOf<kFewStates> few;
+        std::copy(p.states, p.states + p.count, few.states);
+        few.count = p.count, few.beams = p.beams, few.groups = p.groups, few.parents = p.parents, few.lengths = p.lengths;
+        launch(few, std::integral_constant<int, kFewStates>{});
+    } else {
+        launch(p, std::integral_constant<int, kStatesPerLaunch>{});
+    }
     return cudaGetLastError();
 }
 

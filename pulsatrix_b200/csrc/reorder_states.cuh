@@ -18,13 +18,15 @@ struct BeamState {
     int32_t width;                // bytes that a thread moves at a time
 };
 
-struct ReorderParams {
-    BeamState states[kStatesPerLaunch];
+template <int most>
+struct ReorderParamsOf {
+    BeamState states[most];
     int32_t count, beams;
     int64_t groups;
     const int64_t* parents;  // (groups, beams): row of the same group, else the row stays as it is
     const int64_t* lengths;  // (groups * beams): tokens that a row holds; null: all positions
 };
+using ReorderParams = ReorderParamsOf<kStatesPerLaunch>;
 
 // Fills in splits, first_block and width of p.states[0 .. p.count) and launches.  cudaErrorInvalidValue: more than
 // kMostBeams beams or too many blocks.
