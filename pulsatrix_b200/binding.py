@@ -316,6 +316,7 @@ class Context:
         _check(self._lib.psx_b200_ctx_create(C.c_int(device), C.byref(self._ctx)))
         self._handle = self._ctx.value  # (what the native calls take)
         self.device = device
+        self._made = {}  # (shape, dtype) of small outputs -> a tensor like them
 
     def close(self):
         if self._ctx:
@@ -552,6 +553,18 @@ class Context:
         return context, status
 
     # ---- beams, states that follow them, the cache in 8 bits, prompts -------------------------------------
+    def _empty(self, shape, dtype):
+        """torch.empty on the context's device.  Small outputs of one shape come call after call, and like a tensor that is there they are
+        made in half the time."""
+        like = self._made.get((shape, dtype))
+        if like is None:
+            if math.prod(shape) > 65536:
+                return _torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+            if len(self._made) >= 64:
+                self._made.clear()
+            like = self._made[shape, dtype] = _torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        return _torch.empty_like(like)
+
     def _elsewhere(self, tensor):
         return ValueError(f"tensors on cuda:{self.device} are expected, got one on {tensor.device}")
 
@@ -583,9 +596,9 @@ class Context:
             self._here(finished)
         groups = rows // beams
         stream = _stream_of(logits) if stream is None else stream
-        shape, device = (groups, max(keep, 0)), logits.device
-        out_scores, parents = torch.empty(shape, device=device, dtype=torch.float32), torch.empty(shape, dtype=torch.int64, device=device)
-        tokens, status = torch.empty_like(parents), torch.empty(groups, dtype=torch.int32, device=device)
+        shape = (groups, max(keep, 0))
+        out_scores, parents = self._empty(shape, torch.float32), self._empty(shape, torch.int64)
+        tokens, status = torch.empty_like(parents), self._empty((groups,), torch.int32)
         code = _native.beam_select(self._handle, stream, logits.data_ptr(), groups, beams, vocab, row_stride, scores.data_ptr(),
                                    None if finished is None else finished.data_ptr(), finished_token, keep, out_scores.data_ptr(),
                                    parents.data_ptr(), tokens.data_ptr(), status.data_ptr())
@@ -642,7 +655,7 @@ class Context:
         here = self.device
         if not (cache.device == here == keys.get_device() == values.get_device() == offsets.get_device() == cached.get_device()):
             self._here(cache.key_codes, keys, values, offsets, cached)
-        status = torch.empty(batch, dtype=torch.int32, device=offsets.device)
+        status = self._empty((batch,), torch.int32)
         width = kv_heads * head_dim
         code = _native.store_cache_8bit(self._handle, _stream_of(keys) if stream is None else stream, cache._address, keys.data_ptr(), values.data_ptr(),
                                         _dtype_code(keys), total, key_stride[0] if total > 1 else width, value_stride[0] if total > 1 else width,
@@ -702,7 +715,7 @@ class Context:
             self._here(q, k, v, out, q_offsets, k_offsets)
         if scale is None:
             scale = head_dim ** -0.5
-        status = torch.empty(1, dtype=torch.int32, device=q.device)
+        status = self._empty((1,), torch.int32)
         code = _native.prompt_attention(self._handle, _stream_of(q) if stream is None else stream, _dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                         out.data_ptr(), total_q, total_k, q_stride[0] if total_q > 1 else heads * head_dim,
                                         k_stride[0] if total_k > 1 else kv_heads * head_dim, v_stride[0] if total_k > 1 else kv_heads * head_dim,

@@ -193,7 +193,7 @@ __device__ __forceinline__ void part_of_row(const BeamSelectParams& p, PartShare
         float part_top = warp_top;
         for (int step = 16; step > 0; step /= 2) part_top = fmaxf(part_top, __shfl_xor_sync(0xffffffffu, part_top, step));
         const float level = part_top > kNone ? part_top : 0.0f;
-        double part_sum = lane < kWarps ? s.sums[lane] * exp((double)warp_top - (double)level) : 0.0;
+        double part_sum = lane < kWarps ? s.sums[lane] * exp2_approx((warp_top - level) * kLog2e) : 0.0;
         for (int step = 16; step > 0; step /= 2) part_sum += __shfl_xor_sync(0xffffffffu, part_sum, step);
         if (lane == 0) p.part_stats[part_row] = {part_sum, part_top, part_sum != part_sum};
     }
@@ -202,6 +202,7 @@ __device__ __forceinline__ void part_of_row(const BeamSelectParams& p, PartShare
         for (int e = threadIdx.x; e < count; e += kThreads) {
             const uint64_t key = s.list[e];
             int place = 0;
+#pragma unroll 4
             for (int k = 0; k < count; ++k) place += s.list[k] > key;
             if (place < keep) entries[place] = {from_ordered((uint32_t)(key >> 32)), (int)~(uint32_t)key};
         }
@@ -227,13 +228,28 @@ __device__ __forceinline__ void part_of_row(const BeamSelectParams& p, PartShare
     for (int i = placed + threadIdx.x; i < keep; i += kThreads) entries[i] = {kNone, -1};
 }
 
+// A value in double precision as an integer of the same order (comparing integers is quicker), and where it is.
 struct Candidate {
-    double value;
+    uint64_t key;
     uint64_t place;  // beam << 32 | token
+    __device__ __forceinline__ double value() const { return __longlong_as_double((long long)((key >> 63) ? key & 0x7fffffffffffffffull : ~key)); }
 };
+constexpr uint64_t kNoKey = 0x000fffffffffffffull;  // of -inf
+
+__device__ __forceinline__ Candidate candidate_at(double value, uint64_t place) {
+    const uint64_t bits = (uint64_t)__double_as_longlong(value + 0.0);  // (-0 as +0)
+    return {(bits >> 63) ? ~bits : bits | 0x8000000000000000ull, place};
+}
 
 __device__ __forceinline__ bool ahead(const Candidate& a, const Candidate& b) {
-    return a.value > b.value || (a.value == b.value && a.place < b.place);
+    return a.key > b.key || (a.key == b.key && a.place < b.place);
+}
+
+// The logarithm of a sum of at least one half or so: the exponent's in double, the fraction's in float.
+__device__ __forceinline__ double log_of(double x) {
+    const int high = __double2hiint(x), exponent = (high >> 20) - 1023;
+    const double fraction = __hiloint2double((high & 0xfffff) | 0x3ff00000, __double2loint(x));
+    return exponent * 0.6931471805599453 + (double)logf((float)fraction);
 }
 
 // The value as a float, in an order that rounding keeps; what is below the lowest float counts as that, so that it stays a candidate.
@@ -266,15 +282,14 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
     const int lists = p.beams * p.parts;
     constexpr int kHeld = kHeldEntries * kThreads;
     const int all_held = min(lists * keep, kHeld);
-    const auto place_of = [&](int i) {
-        const uint32_t y = i * 32 + lane;
-        return (int)(y * 8 + ((warp + (y * 2654435761u >> 29)) & 7));
-    };
     BeamEntry held[kHeldEntries];
+    int held_list[kHeldEntries];
 #pragma unroll
     for (int i = 0; i < kHeldEntries; ++i) {
-        const int x = place_of(i);
-        held[i] = x < all_held ? load_entry(entries + x % lists * keep + x / lists) : BeamEntry{kNone, -1};
+        const uint32_t y = i * 32 + lane;
+        const int x = (int)(y * 8 + ((warp + (y * 2654435761u >> 29)) & 7)), slot = (int)p.by_lists.quotient(x);
+        held_list[i] = x - slot * lists;
+        held[i] = x < all_held ? load_entry(entries + held_list[i] * keep + slot) : BeamEntry{kNone, -1};
     }
     __syncthreads();
     for (int b = warp; b < p.beams; b += kWarps) {
@@ -283,35 +298,40 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
         const float score = p.scores[row];
         const bool ended = p.finished && p.finished[row];
         float top = kNone;
-        int wrong = !(score < -kNone);
-        for (int i = lane; i < p.parts; i += 32) {
-            const BeamPart part = load_part(parts + i);
-            top = fmaxf(top, part.top);
-            wrong |= part.not_finite;
-        }
-        for (int step = 16; step > 0; step /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
         double sum = 0.0;
-        for (int i = lane; i < p.parts; i += 32) {
-            const BeamPart part = load_part(parts + i);
-            if (part.top > kNone) sum += part.sum * exp((double)part.top - (double)top);
+        int wrong = !(score < -kNone);
+        for (int first = 0; first < p.parts; first += 64) {  // (two a lane: one trip to memory where the parts are few)
+            BeamPart part[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = first + i * 32 + lane;
+                part[i] = at < p.parts ? load_part(parts + at) : BeamPart{0.0, kNone, 0};
+                wrong |= part[i].not_finite;
+            }
+            float next = fmaxf(top, fmaxf(part[0].top, part[1].top));
+            for (int step = 16; step > 0; step /= 2) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, step));
+            const float level = next > kNone ? next : 0.0f;
+            sum *= exp2_approx((top - level) * kLog2e);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sum += part[i].sum * exp2_approx((part[i].top - level) * kLog2e);
+            top = next;
         }
         for (int step = 16; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
         wrong = __any_sync(0xffffffffu, wrong);
         if (lane == 0) {
             if (wrong) s.not_finite = 1;
-            s.base[b] = ended ? (double)score : sum > 0.0 ? (double)score - ((double)top + log(sum)) : (double)kNone;
+            s.base[b] = ended ? (double)score : sum > 0.0 ? (double)score - ((double)top + log_of(sum)) : (double)kNone;
         }
     }
     __syncthreads();
     const auto candidate_of = [&](int of_list, BeamEntry entry) {
-        const int b = of_list / p.parts;
-        return Candidate{s.base[b] + (double)entry.logit, (uint64_t)b << 32 | (uint32_t)entry.token};
+        const int b = (int)p.by_parts.quotient(of_list);
+        return candidate_at(s.base[b] + (double)entry.logit, (uint64_t)b << 32 | (uint32_t)entry.token);
     };
     float largest = kNone;
 #pragma unroll
     for (int i = 0; i < kHeldEntries; ++i) {
-        const int x = place_of(i);
-        if (x < all_held) largest = fmaxf(largest, as_float(candidate_of(x % lists, held[i]).value));
+        largest = fmaxf(largest, as_float(candidate_of(held_list[i], held[i]).value()));
     }
     const uint32_t mine = warp_bound(largest, keep, nullptr);
     if (lane == 0) s.bounds[warp] = mine;
@@ -321,7 +341,7 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
     const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
     // (rounding to float keeps the order: what is at or above the bound in double is so in float)
     const auto offer = [&](const Candidate& c) {
-        if (!(c.value > (double)kNone && as_float(c.value) >= bound)) return false;
+        if (!(c.key > kNoKey && as_float(c.value()) >= bound)) return false;
         const int at = atomicAdd(&s.listed, 1);
         if (at < kGroupList) s.list[at] = c;
         return true;
@@ -329,8 +349,7 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
     if (largest >= bound && largest > kNone) {
 #pragma unroll
         for (int i = 0; i < kHeldEntries; ++i) {
-            const int x = place_of(i);
-            if (x < all_held) offer(candidate_of(x % lists, held[i]));
+            offer(candidate_of(held_list[i], held[i]));
         }
     }
     if (all_held < lists * keep) {  // lists are in order: each from where it is not held on, as far as it reaches the bound
@@ -345,7 +364,7 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
     int placed = wrong ? 0 : min(count, keep);
     const auto put = [&](int place, const Candidate& c) {
         const int64_t at = group * keep + place;
-        p.out_scores[at] = as_float(c.value);
+        p.out_scores[at] = as_float(c.value());
         p.parents[at] = (int64_t)(c.place >> 32);
         p.tokens[at] = (int64_t)(uint32_t)c.place;
     };
@@ -354,19 +373,20 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
         for (int e = threadIdx.x; e < count; e += kThreads) {
             const Candidate c = s.list[e];
             int place = 0;
+#pragma unroll 4
             for (int k = 0; k < count; ++k) place += ahead(s.list[k], c);
             if (place < keep) put(place, c);
         }
     } else {  // more that tie at the bound than the list holds: sweep after sweep, the best that is behind the last one
-        Candidate last{(double)-kNone, 0};
+        Candidate last{~0ull, 0};
         for (placed = 0; placed < keep; ++placed) {
-            Candidate best{(double)kNone, ~0ull};
+            Candidate best{kNoKey, ~0ull};
             for (int e = threadIdx.x; e < lists * keep; e += kThreads) {
                 const Candidate c = candidate_of(e / keep, load_entry(entries + e));
                 if (ahead(last, c) && ahead(c, best)) best = c;
             }
             for (int step = 16; step > 0; step /= 2) {
-                const Candidate other{__shfl_xor_sync(0xffffffffu, best.value, step), __shfl_xor_sync(0xffffffffu, best.place, step)};
+                const Candidate other{__shfl_xor_sync(0xffffffffu, best.key, step), __shfl_xor_sync(0xffffffffu, best.place, step)};
                 if (ahead(other, best)) best = other;
             }
             if (lane == 0) s.best_of[warp] = best;
@@ -375,7 +395,7 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
                 if (ahead(s.best_of[w], best)) best = s.best_of[w];
             }
             __syncthreads();
-            if (best.value == (double)kNone) break;
+            if (best.key == kNoKey) break;
             if (threadIdx.x == 0) put(placed, best);
             last = best;
         }
@@ -411,6 +431,8 @@ __global__ void __launch_bounds__(kThreads, values == 16 ? 4 : 2) beam_select_ke
 
 }  // namespace
 
+Quotients::Quotients(uint32_t by) : one(by == 1), magic((uint32_t)(((uint64_t(1) << 32) + by - 1) / by)) {}
+
 void plan_beam_select(BeamSelectParams& p, int sm_count) {
     const int64_t rows = p.groups * p.beams;
     // Long parts cost least per logit (what a part costs besides is shared by up to eight chunks of 4096); where they would be
@@ -422,6 +444,8 @@ void plan_beam_select(BeamSelectParams& p, int sm_count) {
     while (p.chunks > 1 && rows * ((all + p.chunks - 1) / p.chunks) < 2 * sm_count) --p.chunks;
     p.parts = (all + p.chunks - 1) / p.chunks;
     p.chunks = (all + p.parts - 1) / p.parts;  // (no part much shorter than the others)
+    p.by_parts = Quotients((uint32_t)p.parts);
+    p.by_lists = Quotients((uint32_t)(p.beams * p.parts));
     p.aligned = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.row_stride % 4 == 0 && p.vocab % 4 == 0;
 }
 

@@ -21,6 +21,16 @@ struct BeamEntry {
     int32_t token;
 };
 
+// x / by for x * by < 2^32, by a multiplication: the magic number is 2^32 / by rounded up, off by less than `by` 2^-32 of it.
+struct Quotients {
+    uint32_t one = 1, magic = 0;
+    Quotients() = default;
+    explicit Quotients(uint32_t by);
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t quotient(uint32_t x) const { return one ? x : __umulhi(x, magic); }
+#endif
+};
+
 struct BeamSelectParams {
     const float* logits;      // (groups * beams, vocab), row r at logits + r * row_stride
     const float* scores;      // (groups * beams): the beams' scores so far
@@ -34,6 +44,7 @@ struct BeamSelectParams {
     int32_t parts;            // of a row
     int32_t values;           // logits per thread of a chunk: 4 or 16
     int32_t chunks;           // of a part, 1 to 8
+    Quotients by_parts, by_lists;  // the parts of a row, those of a group's rows together
     int32_t aligned;          // every row starts on a 16-byte boundary and is a multiple of four long
     int32_t* arrived;         // scratch: (groups), zero between calls
     BeamPart* part_stats;     // (groups * beams, parts)

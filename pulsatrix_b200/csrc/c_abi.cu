@@ -1176,7 +1176,7 @@ psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream_ptr, const float* log
     p.beams = (int32_t)beams; p.vocab = (int32_t)vocab; p.keep = (int32_t)keep;
     psx::plan_beam_select(p, ctx->sm_count);
     const int64_t lists = groups * beams * p.parts;
-    if (lists > 0x7fffffff || beams * p.parts * keep > 0x7fffffff) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
+    if (lists > 0x7fffffff || beams * p.parts * keep > 0x7fffffff || beams * p.parts > (1 << 21)) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
     const OnDevice device(ctx->device);
     PSX_CUDA(device.error);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
