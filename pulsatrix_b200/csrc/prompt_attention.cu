@@ -1,23 +1,32 @@
 // Attention of whole prompts, packed one behind the other: per sequence and head softmax(scale q k^T, masked) v, on the
 // fifth-generation tensor cores, without the scores in memory.
 //
-// A CTA takes `tiles` tiles of 128 queries of one (sequence, head) and goes through the keys that they see in blocks.  One thread
-// asks for copies (tiled, 128-byte swizzle), one thread issues the products, and a warpgroup per tile turns scores into weights, a
+// A CTA takes one or two tiles of 128 queries of one (sequence, head) and goes through the keys that they see in blocks.  One thread
+// asks for copies (tiled, 128-byte swizzle), one issues the products, and a warpgroup per tile turns scores into weights, a
 // thread per query: it loads its row of scores from tensor memory, keeps the running maximum and sum in registers (no
-// exchange between threads), and writes the weights back to tensor memory, from where they are the left operand of the second
-// product.  The context stays in tensor memory; it is rescaled only where a row's maximum has grown by more than 2^8 since
-// the last time (weights are then up to 2^8 instead of 1, which costs no precision).
+// exchange between threads), and writes the weights back to tensor memory, in the place of the scores, from where they are the left
+// operand of the second product.  The reference point of a row's weights moves only where its maximum has grown by more than 2^8
+// (weights are then up to 2^8 instead of 1, which costs no precision).
 //
-// 16-bit operands: two tiles, blocks of 128 keys, two stages of keys and of values; while the tensor core works for one tile the
-// other tile's warpgroup works on its scores; a tile's weights take its scores' place.  Weights are rounded to the operands'
-// type, the error of which is of the size of the context's own rounding.  Bound by the exponentials (16 a clock and SM) and
-// the products about alike.
+// 16-bit operands: two tiles, blocks of 128 keys, two stages of keys and of values (four up to 64 dimensions).  The first half of a block's
+// weights is handed on while the second is made.  The context stays in tensor memory and is rescaled there when the reference point
+// moves.  While the tensor core works for one tile the other tile's warpgroup works on its scores: the one issuing warp goes from
+// tile to tile, which keeps the two half a turn apart (with an issuing warp for each, both tiles ask for the same unit at a time: 773 us
+// instead of 662 for two prompts of up to 8192 positions, 32 heads of 128 in bf16, causal).  Weights are rounded to the operands'
+// type, an error of the size of the context's own rounding.
+// Bound by a tile's turn: some 1700 clocks from scores to weights (570 for the maximum, 1024 of exponentials at four a clock and
+// scheduler), 1024 of products, and the way between the two; 1.05 PFLOP/s at those sizes.  Tried and taken back: a share of the
+// exponentials by a polynomial (no gain, 662 and 668 us), two threads for a query (771 us).
 //
 // fp32 operands: every number is split into three bf16 parts that add up to it (8 bits of the fraction each), and a product is the
 // six products of parts that reach fp32's precision, the small ones first.  The keys' and values' parts are written by a kernel ahead,
 // the queries' go into tensor memory once, the weights' as they are made.  One tile, blocks of 64 keys; the scores have two places,
-// so that the next block's scores are formed while this block's weights are; contexts are added up in registers.  Six bf16 products are still
-// several times faster than the FP32 pipes.
+// so that the next block's scores are formed while this block's weights are.  The tensor core cuts its sums off instead of rounding them, which
+// adds up over thousands of keys; so a block's context is formed from zero and added up in registers (error of the context against
+// 64 bits 2e-7, summed by the tensor core 5e-6).  Six bf16 products are still several times faster than the FP32 pipes.
+// Bound by the products: 48 of 128 x 64 x 16 for the scores of a block and 128 dimensions (59 clocks each, the queries out of tensor
+// memory), 24 of 128 x 128 x 16 for its context (64 clocks).  Blocks of 128 keys with the queries in shared memory need fewer clocks of the
+// tensor core but all of shared memory's: 226 us instead of 221 for five prompts of up to 1501 positions with a prefix, 16 heads of 96.
 //
 // Rows behind a sequence's last key in a block belong to other sequences: their scores are masked, and their values are set to zero in
 // shared memory, so that a NaN there is not seen here.
@@ -406,8 +415,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         const float masked = turned ? -kNone : kNone;
         float top = masked, total = 0.0f;   // of the scores before the factor
         bool fine = true;
-        // fp32: the context is summed up here, a block's at a time: the tensor core's sums are cut off, not rounded, and over
-        // thousands of keys that adds up.
+        // fp32: the context is summed up here, a block's at a time.
         constexpr int kSums = S::parts == 1 ? 1 : S::dims;
         float context[kSums];
         const auto add_block = [&]() {
