@@ -11,7 +11,10 @@
  *     compute call fails with PSX_ERR_CUDA.
  *   - A psx_ctx belongs to one device and one host thread at a time (like the reference's
  *     DeviceBackend, include/pulsatrix/cuda_backend.hpp:159-166).  It owns scratch memory that
- *     grows on demand; growing synchronises the device, steady-state calls do not allocate.
+ *     grows on demand; growing synchronises the device, steady-state calls do not allocate.  Scratch of
+ *     beam_select, decode_attention_8bit and prompt_attention that a larger call outgrows stays allocated
+ *     until the context goes, because a captured graph may hold it.  Calls of one context that use scratch
+ *     must not run at the same time, replays of graphs among them.
  *   - Device entry points are asynchronous on `stream` (a cudaStream_t; NULL is CUDA's default
  *     stream, as everywhere in CUDA); outputs are valid once that stream has been synchronised.
  *     Host entry points run on the context's own stream and synchronise before returning.
@@ -379,7 +382,8 @@ PSX_API psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream, const psx
 
 /* A cache of keys and values in 8 bits: codes in e4m3 (1 sign, 4 exponent and 3 fraction bits, largest 448, no infinities),
  * (batch, kv_heads, max_len, head_dim), and a scale for every `block` positions of a (row, kv head): (batch, kv_heads,
- * ceil(max_len / block)) fp32.  An element's value is its code times its block's scale.  A quarter of the bytes of the fp32
+ * ceil(max_len / block)) fp32.  An element's value is its code times its block's scale, which is not
+ * negative.  A quarter of the bytes of the fp32
  * cache.  All device pointers, codes 16-byte aligned; block is 16, 32 or 64, head_dim a multiple of 16 up to 256, batch <= 4096
  * (else PSX_ERR_UNSUPPORTED). */
 typedef struct psx_cache_8bit {
@@ -390,7 +394,7 @@ typedef struct psx_cache_8bit {
     int64_t batch, kv_heads, max_len, head_dim, block;
 } psx_cache_8bit;
 
-/* Appends new positions to such a cache (KVCache::append, src/kv_cache.cpp, in 8 bits): prompts, or the one position of a
+/* Appends new positions to such a cache (what src/kv_cache.cpp does for the fp32 cache): prompts, or the one position of a
  * decoding step.  keys, values: device, `dtype`, (total, kv_heads, head_dim) with the positions of all rows one row behind the
  * other, a position at keys + i * key_stride elements (a slice of a wider projection will do; positions start on
  * 16-byte boundaries).  Row b's are offsets[b] .. offsets[b + 1] (device int64, batch + 1) and become
@@ -417,13 +421,14 @@ PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, co
                                                   int32_t causal, int64_t window);
 
 /* Attention of whole prompts, for sequences of different lengths packed one behind the other: what psx_b200_decode_attention does
- * for a few new positions and declines for many (src/multihead_attention_module.cpp:443-480, forward(), without padding).  q:
+ * for a few new positions and declines for many (the core of src/multihead_attention_module.cpp:562-586, without padding).  q:
  * device, `dtype`, (total_q, heads, head_dim), a position at q + i * q_stride elements, its heads contiguous; k, v: (total_k,
  * kv_heads, head_dim), likewise (slices of one projection will do); query head h reads kv head h / (heads / kv_heads).  Sequence
  * b has queries q_offsets[b] .. q_offsets[b + 1] and keys k_offsets[b] .. k_offsets[b + 1] (device int64, batch + 1, ascending); with
  * more keys than queries the queries are the last positions (a prompt that continues a cached prefix).  Query i of n, with m
  * keys, is position p = m - n + i: with `causal` it sees no key j > p and, with window > 0, no key j + window <= p.  A query that
- * sees nothing gets 0.  out: (total_q, heads, head_dim), contiguous; rows that belong to no sequence are left as they were.
+ * sees nothing gets 0.  out: (total_q, heads, head_dim), contiguous, apart from the operands; rows that belong to no sequence are left
+ * as they were.
  * Products run on the tensor cores with float accumulators.  bf16 and fp16: weights are rounded to that type; fp32: every
  * factor as three bf16 parts, so that products are exact to about 2^-24 (an infinity counts as NaN).  Keys and values of other
  * sequences, finite or not, have no influence; a NaN among a sequence's own values reaches the queries of the 128 positions

@@ -1323,10 +1323,12 @@ psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const 
     PSX_CUDA(device.error);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     psx::plan_attention_8bit(p, ctx->sm_count);
-    if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;
-    if (psx_status s = reserve_counters(ctx, stream, ctx->attention_8bit_arrived, (size_t)(cache->batch * cache->kv_heads))) return s;
-    p.partial = static_cast<float*>(ctx->attention_8bit_pieces.ptr);
-    p.arrived = static_cast<int32_t*>(ctx->attention_8bit_arrived.ptr);
+    if (p.pieces > 1) {
+        if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;
+        if (psx_status s = reserve_counters(ctx, stream, ctx->attention_8bit_arrived, (size_t)(cache->batch * cache->kv_heads))) return s;
+        p.partial = static_cast<float*>(ctx->attention_8bit_pieces.ptr);
+        p.arrived = static_cast<int32_t*>(ctx->attention_8bit_arrived.ptr);
+    }
     PSX_CUDA(psx::launch_decode_attention_8bit(p, stream));
     ctx->launches += 1;
     return PSX_OK;

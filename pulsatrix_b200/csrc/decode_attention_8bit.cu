@@ -12,26 +12,27 @@
 // rounded to halves (2^-11, below the rounding of a bf16 or fp16 context; for fp32 contexts again two halves).  Maxima, sums
 // and contexts are floats.
 //
-// A (row, kv head) pair's cached positions are cut into tiles of 32.  With many pairs the tiles of all lie on one axis and every
-// block takes an equal share of it: lengths that differ from row to row leave no SM idle.  With few (four blocks for each, at least, fit
-// on the GPU) every pair has as many blocks as fit, which saves a block the sums over the rows' lengths and the end of one pair
-// before the start of the next (one request of 777 positions: 12.2 us with shares of the axis, PIECES_US with blocks of its own).
-// A pair that several blocks share leaves a piece per block; the last block to arrive joins them, in order.  Inside a block each of four warps
-// takes every fourth tile, with its own two stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no
-// warp waits for another until the end of a pair.  Bound by HBM: 2 bytes per position, head dimension and kv head.
+// A (row, kv head) pair's cached positions are cut into tiles of 32, and the tiles into pieces, a block each: as many as fill the GPU
+// once, or as pieces of 64 tiles make where that is more, which evens out rows of different lengths (64 rows x 8 kv heads of up to 8191
+// positions: 167 us as one piece each, 138 as four; the same of 1000 positions: 24.7 as one, 31 as two).  The last block of a pair to
+// end joins its pieces, in order.  (Equal shares of all pairs' tiles laid on one axis: 137 and 42 us; 24 rows x 8 of up to 4096: 52 instead of 33:
+// most blocks then have the end of one pair and the start of another.)  Inside a block each of four warps takes every fourth tile, with
+// its own two stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no warp waits for another until the end.
+// Bound by HBM for long caches (2 bytes per position, head dimension and kv head), by the chain of a tile for short ones: some 2100
+// clocks from a tile's arrival to its weights' products, most of them conversions of codes (64 instructions for 32 positions x 64
+// dimensions, two clocks each).
 #include "decode_attention_8bit.cuh"
 
 #include <algorithm>
 
 #include "elements.cuh"
 #include "once_per_device.hpp"
-#include "row_prefix.cuh"
 
 namespace psx {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4, kTile = 32;
-constexpr int kLeastShare = 2 * kWarps;  // tiles: shorter pieces cost more in joining than they gain (see the launch)
+constexpr int kMostShare = 64;  // tiles that a block takes where shorter pieces only balance
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -115,442 +116,391 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
     constexpr int kStages = stages_of(dims), kStageBytes = stage_bytes(dims), kSegments = dims / 64, kBlocks = dims / 16;
     constexpr int kRows = 8 * tiles_of_rows;
     extern __shared__ __align__(16) uint8_t shared[];
-    int* prefix = reinterpret_cast<int*>(shared + shared_of(dims));
-    __shared__ int carry[kWarps];
     __shared__ float tops[kWarps][kRows], totals[kWarps][kRows];
     __shared__ int is_last;
     const Cache8bitView& c = p.cache;
-    const int batch = (int)c.batch, head_dim = c.head_dim, chunks = head_dim / 16;
+    const int head_dim = c.head_dim, chunks = head_dim / 16;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, gid = lane / 4, tig = lane % 4;
     uint8_t* stages = shared + warp * kStages * kStageBytes;
     const uint32_t stages_at = shared_address(stages);
     const int shift = 31 - __clz(c.block);
 
-    // Which tiles of which pairs: see the two ways above.
-    const int pieces_each = p.pieces;
-    int share = p.least_share, row = 0;
-    int64_t at = 0, stop = 1;
-    if (pieces_each > 0) {
-        row = (int)(blockIdx.x / (unsigned)(c.kv_heads * pieces_each));
-    } else {
-        sum_of_rows(batch, prefix, carry, [&](int row) {
-            const Sight s = sight_of(p, row);
-            return max(s.end_tile() - s.first_tile(), 0) * c.kv_heads;
-        });
-        const int all = prefix[batch];
-        share = max((int)(((int64_t)all + gridDim.x - 1) / gridDim.x), p.least_share);
-        // Rows that see nothing have no tiles, hence no block: their context is zero.
-        for (int64_t row = blockIdx.x; row < batch; row += gridDim.x) {
-            if (prefix[row + 1] != prefix[row]) continue;
-            T* out = static_cast<T*>(p.context) + row * p.heads * p.q_len * head_dim;
-            for (int i = threadIdx.x; i < p.heads * p.q_len * head_dim; i += kThreads) out[i] = from_float<T>(0.0f);
+    // This block's pair, and its tiles of the pair's.
+    const int64_t pair = blockIdx.x / (unsigned)p.pieces;
+    const int number = (int)(blockIdx.x % (unsigned)p.pieces), row = (int)(pair / c.kv_heads), head = (int)(pair % c.kv_heads);
+    const Sight sight = sight_of(p, row);
+    const int tiles = max(sight.end_tile() - sight.first_tile(), 0);
+    const int share = max(max(kWarps, (tiles + p.pieces - 1) / p.pieces), min((tiles + p.spread - 1) / p.spread, kMostShare));
+    const int from_tile = number * share, to_tile = min(tiles, from_tile + share);
+    T* context = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+    if (from_tile >= to_tile) {
+        if (tiles == 0 && number == 0) {  // a row that sees nothing
+            for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) context[i] = from_float<T>(0.0f);
         }
-        at = (int64_t)blockIdx.x * share;
-        stop = min(at + share, (int64_t)all);
-        if (at < stop) row = row_of_item(prefix, batch, (int)at);
+        return;
     }
-    while (at < stop) {
-        int tiles, head, from_tile, to_tile;
-        if (pieces_each > 0) {
-            const Sight sight = sight_of(p, row);
-            tiles = max(sight.end_tile() - sight.first_tile(), 0);
-            share = max((tiles + pieces_each - 1) / pieces_each, p.least_share);
-            head = (int)(blockIdx.x / (unsigned)pieces_each) % c.kv_heads;
-            from_tile = (int)(blockIdx.x % (unsigned)pieces_each) * share;
-            to_tile = min(tiles, from_tile + share);
-            if (from_tile >= to_tile) {
-                if (tiles == 0 && from_tile == 0) {
-                    T* out = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
-                    for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) out[i] = from_float<T>(0.0f);
-                }
-                return;
+    const int tile0 = sight.first_tile();
+    const uint8_t* keys = c.key_codes + pair * c.max_len * head_dim;
+    const uint8_t* values = c.value_codes + pair * c.max_len * head_dim;
+    const float* key_scales = c.key_scales + pair * c.blocks;
+    const float* value_scales = c.value_scales + pair * c.blocks;
+
+    const int seen = max(sight.first(0), 0);  // no row sees a position before this one
+    const auto fetch = [&](int tile, int stage) {  // positions that no row sees arrive as zeros, whatever the cache holds there
+        const int position = (tile0 + tile) * kTile;
+        const uint32_t to = stages_at + stage * kStageBytes;
+        if (head_dim == dims && position >= seen && position + kTile <= sight.length) {  // 32 whole rows, one run of memory
+            const uint8_t* from = keys + (int64_t)position * dims + lane * 16;
+            const int64_t apart = values - keys;
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) {
+                const int r = (i * 32 + lane) / kBlocks, chunk = lane % kBlocks;
+                const uint32_t place = to + r * dims + placed<dims>(r, chunk) * 16;
+                copy16(place, from + i * 512);
+                copy16(place + kTile * dims, from + apart + i * 512);
             }
         } else {
-            while (prefix[row + 1] <= at) ++row;
-            tiles = (prefix[row + 1] - prefix[row]) / c.kv_heads;
-            head = (int)(at - prefix[row]) / tiles, from_tile = (int)(at - prefix[row]) % tiles;
-            to_tile = (int)min((int64_t)tiles, from_tile + (stop - at));
-        }
-        const Sight sight = sight_of(p, row);
-        const int64_t pair = (int64_t)row * c.kv_heads + head;
-        const int tile0 = sight.first_tile();
-        const uint8_t* keys = c.key_codes + pair * c.max_len * head_dim;
-        const uint8_t* values = c.value_codes + pair * c.max_len * head_dim;
-        const float* key_scales = c.key_scales + pair * c.blocks;
-        const float* value_scales = c.value_scales + pair * c.blocks;
-
-        const int seen = max(sight.first(0), 0);  // no row sees a position before this one
-        const auto fetch = [&](int tile, int stage) {  // positions that no row sees arrive as zeros, whatever the cache holds there
-            const int position = (tile0 + tile) * kTile;
-            const uint32_t to = stages_at + stage * kStageBytes;
-            if (head_dim == dims && position >= seen && position + kTile <= sight.length) {  // 32 whole rows, one run of memory
-                const uint8_t* from = keys + (int64_t)position * dims + lane * 16;
-                const int64_t apart = values - keys;
-#pragma unroll
-                for (int i = 0; i < kBlocks; ++i) {
-                    const int r = (i * 32 + lane) / kBlocks, chunk = lane % kBlocks;
-                    const uint32_t place = to + r * dims + placed<dims>(r, chunk) * 16;
-                    copy16(place, from + i * 512);
-                    copy16(place + kTile * dims, from + apart + i * 512);
-                }
-            } else {
 #pragma unroll 1
-                for (int i = 0; i < kBlocks; ++i) {
-                    const int index = i * 32 + lane, r = index / kBlocks, chunk = index % kBlocks;
-                    if (chunk < chunks) {
-                        const bool there = position + r < sight.length && position + r >= seen;
-                        const int64_t offset = there ? (int64_t)(position + r) * head_dim + chunk * 16 : 0;
-                        const uint32_t place = to + r * dims + placed<dims>(r, chunk) * 16;
-                        copy16(place, keys + offset, there);
-                        copy16(place + kTile * dims, values + offset, there);
-                    }
+            for (int i = 0; i < kBlocks; ++i) {
+                const int index = i * 32 + lane, r = index / kBlocks, chunk = index % kBlocks;
+                if (chunk < chunks) {
+                    const bool there = position + r < sight.length && position + r >= seen;
+                    const int64_t offset = there ? (int64_t)(position + r) * head_dim + chunk * 16 : 0;
+                    const uint32_t place = to + r * dims + placed<dims>(r, chunk) * 16;
+                    copy16(place, keys + offset, there);
+                    copy16(place + kTile * dims, values + offset, there);
                 }
             }
-            if (lane < 4) {  // the scales of the tile's two halves, keys' then values'
-                const int first = position + lane % 2 * 16;
-                const bool there = first < sight.length;
-                copy4(to + 2 * kTile * dims + lane * 4, (lane < 2 ? key_scales : value_scales) + (there ? first >> shift : 0), there);
-            }
-        };
-        int fetched = from_tile + warp;
+        }
+        if (lane < 4) {  // the scales of the tile's two halves, keys' then values'
+            const int first = position + lane % 2 * 16;
+            const bool there = first < sight.length;
+            copy4(to + 2 * kTile * dims + lane * 4, (lane < 2 ? key_scales : value_scales) + (there ? first >> shift : 0), there);
+        }
+    };
+    int fetched = from_tile + warp;
 #pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) {
-            if (fetched < to_tile) fetch(fetched, s);
+    for (int s = 0; s < kStages - 1; ++s) {
+        if (fetched < to_tile) fetch(fetched, s);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        fetched += kWarps;
+    }
+
+    // The query rows as the right-hand operand: lane (gid, tig) holds row gid's dimensions 16 tig .. 16 tig + 15 of every 64.
+    uint32_t qh[tiles_of_rows][kSegments][4][2], ql[precise ? tiles_of_rows : 1][precise ? kSegments : 1][4][2];
+    float row_scale[tiles_of_rows][2];  // of the score rows that this lane holds: rows 2 tig and 2 tig + 1
+    const T* q = static_cast<const T*>(p.q) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+#pragma unroll
+    for (int n = 0; n < tiles_of_rows; ++n) {
+        const int r = n * 8 + gid;
+        float x[kSegments][16];
+        float largest = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSegments; ++s) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = s * 64 + tig * 16 + i;
+                float4 four = make_float4(0, 0, 0, 0);
+                if (r < p.rows && d < head_dim) four = load_four(q + (int64_t)r * head_dim + d);
+                x[s][i] = four.x, x[s][i + 1] = four.y, x[s][i + 2] = four.z, x[s][i + 3] = four.w;
+                largest = fmaxf(largest, fmaxf(fmaxf(fabsf(four.x), fabsf(four.y)), fmaxf(fabsf(four.z), fabsf(four.w))));
+            }
+        }
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        // 2^-e with largest = m 2^e, 1 <= m < 2 (kept where it and its inverse are normal numbers)
+        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int s = 0; s < kSegments; ++s) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float low = x[s][4 * w + 2 * h] * down, high = x[s][4 * w + 2 * h + 1] * down;
+                    qh[n][s][w][h] = halves(low, high);
+                    if constexpr (precise) ql[n][s][w][h] = halves_left(low, high, qh[n][s][w][h]);
+                }
+            }
+        }
+        const float factor = up * (p.scale * kLog2e);
+        row_scale[n][0] = __shfl_sync(0xffffffffu, factor, 8 * tig);      // (row 2 tig is lanes 8 tig .. 8 tig + 3)
+        row_scale[n][1] = __shfl_sync(0xffffffffu, factor, 8 * tig + 4);
+    }
+
+    float out[tiles_of_rows][kBlocks][4], top[tiles_of_rows][2], total[tiles_of_rows][2];
+#pragma unroll
+    for (int n = 0; n < tiles_of_rows; ++n) {
+        top[n][0] = top[n][1] = kNone;
+        total[n][0] = total[n][1] = 0.0f;
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
+    }
+    // Positions that every row sees need no mask.
+    const int all_from = sight.first(p.q_len - 1), all_to = sight.last(0, p.causal != 0);
+
+    int stage = 0;
+    for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
+        copies_done<kStages - 2>();
+        __syncwarp();
+        {
+            const int next = stage == 0 ? kStages - 1 : stage - 1;  // the stage that the tile before this one used
+            if (fetched < to_tile) fetch(fetched, next);
             asm volatile("cp.async.commit_group;" ::: "memory");
             fetched += kWarps;
         }
-
-        // The query rows as the right-hand operand: lane (gid, tig) holds row gid's dimensions 16 tig .. 16 tig + 15 of every 64.
-        uint32_t qh[tiles_of_rows][kSegments][4][2], ql[precise ? tiles_of_rows : 1][precise ? kSegments : 1][4][2];
-        float row_scale[tiles_of_rows][2];  // of the score rows that this lane holds: rows 2 tig and 2 tig + 1
-        const T* q = static_cast<const T*>(p.q) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+        const uint8_t* k_stage = stages + stage * kStageBytes;
+        const float* scales = reinterpret_cast<const float*>(k_stage + 2 * kTile * dims);
+        const int position = (tile0 + tile) * kTile;
+        float score[tiles_of_rows][2][4];
 #pragma unroll
-        for (int n = 0; n < tiles_of_rows; ++n) {
-            const int r = n * 8 + gid;
-            float x[kSegments][16];
-            float largest = 0.0f;
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int n = 0; n < tiles_of_rows; ++n) score[n][half][0] = score[n][half][1] = score[n][half][2] = score[n][half][3] = 0.0f;
+            const int r0 = half * 16 + gid, r1 = r0 + 8;
 #pragma unroll
             for (int s = 0; s < kSegments; ++s) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int d = s * 64 + tig * 16 + i;
-                    float4 four = make_float4(0, 0, 0, 0);
-                    if (r < p.rows && d < head_dim) four = load_four(q + (int64_t)r * head_dim + d);
-                    x[s][i] = four.x, x[s][i + 1] = four.y, x[s][i + 2] = four.z, x[s][i + 3] = four.w;
-                    largest = fmaxf(largest, fmaxf(fmaxf(fabsf(four.x), fabsf(four.y)), fmaxf(fabsf(four.z), fabsf(four.w))));
+                const int chunk = s * 4 + tig;
+                uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                if (chunk < chunks) {
+                    a = *reinterpret_cast<const uint4*>(k_stage + r0 * dims + placed<dims>(r0, chunk) * 16);
+                    b = *reinterpret_cast<const uint4*>(k_stage + r1 * dims + placed<dims>(r1, chunk) * 16);
                 }
-            }
-            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-            // 2^-e with largest = m 2^e, 1 <= m < 2 (kept where it and its inverse are normal numbers)
-            const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-            for (int s = 0; s < kSegments; ++s) {
+                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_halves(aw[w], a0, a2);
+                    codes_to_halves(bw[w], a1, a3);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float low = x[s][4 * w + 2 * h] * down, high = x[s][4 * w + 2 * h + 1] * down;
-                        qh[n][s][w][h] = halves(low, high);
-                        if constexpr (precise) ql[n][s][w][h] = halves_left(low, high, qh[n][s][w][h]);
+                    for (int n = 0; n < tiles_of_rows; ++n) {
+                        if constexpr (precise) multiply(score[n][half], a0, a1, a2, a3, ql[n][s][w][0], ql[n][s][w][1]);
+                        multiply(score[n][half], a0, a1, a2, a3, qh[n][s][w][0], qh[n][s][w][1]);
                     }
                 }
             }
-            const float factor = up * (p.scale * kLog2e);
-            row_scale[n][0] = __shfl_sync(0xffffffffu, factor, 8 * tig);      // (row 2 tig is lanes 8 tig .. 8 tig + 3)
-            row_scale[n][1] = __shfl_sync(0xffffffffu, factor, 8 * tig + 4);
         }
-
-        float out[tiles_of_rows][kBlocks][4], top[tiles_of_rows][2], total[tiles_of_rows][2];
+        // score[n][half][2 o + i]: position half * 16 + 8 o + gid, query row 8 n + 2 tig + i
+        float value_scale[2], value_log[2];
 #pragma unroll
-        for (int n = 0; n < tiles_of_rows; ++n) {
-            top[n][0] = top[n][1] = kNone;
-            total[n][0] = total[n][1] = 0.0f;
-#pragma unroll
-            for (int m = 0; m < kBlocks; ++m) out[n][m][0] = out[n][m][1] = out[n][m][2] = out[n][m][3] = 0.0f;
-        }
-        // Positions that every row sees need no mask.
-        const int all_from = sight.first(p.q_len - 1), all_to = sight.last(0, p.causal != 0);
-
-        int stage = 0;
-        for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
-            copies_done<kStages - 2>();
-            __syncwarp();
-            {
-                const int next = stage == 0 ? kStages - 1 : stage - 1;  // the stage that the tile before this one used
-                if (fetched < to_tile) fetch(fetched, next);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                fetched += kWarps;
-            }
-            const uint8_t* k_stage = stages + stage * kStageBytes;
-            const float* scales = reinterpret_cast<const float*>(k_stage + 2 * kTile * dims);
-            const int position = (tile0 + tile) * kTile;
-            float score[tiles_of_rows][2][4];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                for (int n = 0; n < tiles_of_rows; ++n) score[n][half][0] = score[n][half][1] = score[n][half][2] = score[n][half][3] = 0.0f;
-                const int r0 = half * 16 + gid, r1 = r0 + 8;
-#pragma unroll
-                for (int s = 0; s < kSegments; ++s) {
-                    const int chunk = s * 4 + tig;
-                    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                    if (chunk < chunks) {
-                        a = *reinterpret_cast<const uint4*>(k_stage + r0 * dims + placed<dims>(r0, chunk) * 16);
-                        b = *reinterpret_cast<const uint4*>(k_stage + r1 * dims + placed<dims>(r1, chunk) * 16);
-                    }
-                    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t a0, a1, a2, a3;
-                        codes_to_halves(aw[w], a0, a2);
-                        codes_to_halves(bw[w], a1, a3);
-#pragma unroll
-                        for (int n = 0; n < tiles_of_rows; ++n) {
-                            if constexpr (precise) multiply(score[n][half], a0, a1, a2, a3, ql[n][s][w][0], ql[n][s][w][1]);
-                            multiply(score[n][half], a0, a1, a2, a3, qh[n][s][w][0], qh[n][s][w][1]);
-                        }
-                    }
-                }
-            }
-            // score[n][half][2 o + i]: position half * 16 + 8 o + gid, query row 8 n + 2 tig + i
-            float value_scale[2], value_log[2];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const float key_scale = scales[half];
-                value_scale[half] = scales[2 + half];
-                value_log[half] = __log2f(fmaxf(value_scale[half], 0x1p-100f));
-#pragma unroll
-                for (int n = 0; n < tiles_of_rows; ++n) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) score[n][half][i] *= key_scale * row_scale[n][i & 1];
-                }
-            }
-            if (position < all_from || position + kTile - 1 > all_to) {
-#pragma unroll
-                for (int n = 0; n < tiles_of_rows; ++n) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int own = (n * 8 + 2 * tig + i) % p.q_len;
-                        const int first = sight.first(own), last = sight.last(own, p.causal != 0);
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                            for (int o = 0; o < 2; ++o) {
-                                const int j = position + half * 16 + o * 8 + gid;
-                                if (j < first || j > last) score[n][half][2 * o + i] = kNone;
-                            }
-                        }
-                    }
-                }
-            }
+        for (int half = 0; half < 2; ++half) {
+            const float key_scale = scales[half];
+            value_scale[half] = scales[2 + half];
+            value_log[half] = __log2f(fmaxf(value_scale[half], 0x1p-100f));
 #pragma unroll
             for (int n = 0; n < tiles_of_rows; ++n) {
-                float high[2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) score[n][half][i] *= key_scale * row_scale[n][i & 1];
+            }
+        }
+        if (position < all_from || position + kTile - 1 > all_to) {
+#pragma unroll
+            for (int n = 0; n < tiles_of_rows; ++n) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    high[i] = fmaxf(fmaxf(score[n][0][i], score[n][0][2 + i]) + value_log[0], fmaxf(score[n][1][i], score[n][1][2 + i]) + value_log[1]);
+                    const int own = (n * 8 + 2 * tig + i) % p.q_len;
+                    const int first = sight.first(own), last = sight.last(own, p.causal != 0);
 #pragma unroll
-                    for (int step = 4; step < 32; step *= 2) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], step));
-                }
-                if (__any_sync(0xffffffffu, high[0] > top[n][0] || high[1] > top[n][1])) {
-                    float less[2];
+                    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float next = fmaxf(top[n][i], high[i]);
-                        less[i] = next > kNone ? exp2_approx(top[n][i] - next) : 1.0f;
-                        top[n][i] = next;
-                        total[n][i] *= less[i];
-                    }
-#pragma unroll
-                    for (int m = 0; m < kBlocks; ++m) {
-                        out[n][m][0] *= less[0], out[n][m][1] *= less[1];
-                        out[n][m][2] *= less[0], out[n][m][3] *= less[1];
-                    }
-                }
-            }
-            // Weights, rounded to halves and turned round: lane (gid, tig) then holds query row gid's weights of positions 2 tig, 2 tig + 1.
-            uint32_t wh[tiles_of_rows][2][2], wl[precise ? tiles_of_rows : 1][2][2];
-#pragma unroll
-            for (int n = 0; n < tiles_of_rows; ++n) {
-                const float t0 = top[n][0] > kNone ? top[n][0] : 0.0f, t1 = top[n][1] > kNone ? top[n][1] : 0.0f;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                    for (int o = 0; o < 2; ++o) {
-                        const float e0 = exp2_approx(score[n][half][2 * o] - t0), e1 = exp2_approx(score[n][half][2 * o + 1] - t1);
-                        total[n][0] += e0;
-                        total[n][1] += e1;
-                        const float w0 = e0 * value_scale[half], w1 = e1 * value_scale[half];
-                        const uint32_t taken = halves(w0, w1);
-                        wh[n][half][o] = transposed(taken);
-                        if constexpr (precise) wl[n][half][o] = transposed(halves_left(w0, w1, taken));
-                    }
-                }
-            }
-            // The values come as 8 x 8 matrices of code pairs, turned round: lane (gid, tig) gets dimensions 2 gid, 2 gid + 1 of
-            // positions 2 tig and 2 tig + 1; dimension 2 gid is row gid of the left-hand operand, 2 gid + 1 row gid + 8.
-            const uint32_t v_at = stages_at + stage * kStageBytes + kTile * dims;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = half * 16 + lane % 16;
-#pragma unroll
-                for (int m = 0; m < kBlocks; m += 2) {
-                    if (m < chunks) {
-                        uint32_t x[4];
-                        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                            : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                            : "r"(v_at + r * dims + placed<dims>(r, m + lane / 16) * 16)
-                            : "memory");
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t low = __byte_perm(x[2 * i], 0, 0x3120), high = __byte_perm(x[2 * i + 1], 0, 0x3120);
-                            uint32_t a0, a1, a2, a3;
-                            codes_to_halves(low, a0, a1);
-                            codes_to_halves(high, a2, a3);
-#pragma unroll
-                            for (int n = 0; n < tiles_of_rows; ++n) {
-                                if constexpr (precise) multiply(out[n][m + i], a0, a1, a2, a3, wl[n][half][0], wl[n][half][1]);
-                                multiply(out[n][m + i], a0, a1, a2, a3, wh[n][half][0], wh[n][half][1]);
-                            }
+                        for (int o = 0; o < 2; ++o) {
+                            const int j = position + half * 16 + o * 8 + gid;
+                            if (j < first || j > last) score[n][half][2 * o + i] = kNone;
                         }
                     }
                 }
             }
-            stage = stage + 1 == kStages ? 0 : stage + 1;
         }
-        copies_done<0>();
-
-        // The four warps' results meet in shared memory.  (The stages are free: every warp has read its own.)
 #pragma unroll
         for (int n = 0; n < tiles_of_rows; ++n) {
+            float high[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+                high[i] = fmaxf(fmaxf(score[n][0][i], score[n][0][2 + i]) + value_log[0], fmaxf(score[n][1][i], score[n][1][2 + i]) + value_log[1]);
 #pragma unroll
-                for (int step = 4; step < 32; step *= 2) total[n][i] += __shfl_xor_sync(0xffffffffu, total[n][i], step);
-                if (gid == 0) {
-                    tops[warp][n * 8 + 2 * tig + i] = top[n][i];
-                    totals[warp][n * 8 + 2 * tig + i] = total[n][i];
+                for (int step = 4; step < 32; step *= 2) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], step));
+            }
+            if (__any_sync(0xffffffffu, high[0] > top[n][0] || high[1] > top[n][1])) {
+                float less[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float next = fmaxf(top[n][i], high[i]);
+                    less[i] = next > kNone ? exp2_approx(top[n][i] - next) : 1.0f;
+                    top[n][i] = next;
+                    total[n][i] *= less[i];
+                }
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    out[n][m][0] *= less[0], out[n][m][1] *= less[1];
+                    out[n][m][2] *= less[0], out[n][m][3] *= less[1];
                 }
             }
         }
-        __syncthreads();
-        float* meet = reinterpret_cast<float*>(shared);  // (warp, row, dimension)
+        // Weights, rounded to halves and turned round: lane (gid, tig) then holds query row gid's weights of positions 2 tig, 2 tig + 1.
+        uint32_t wh[tiles_of_rows][2][2], wl[precise ? tiles_of_rows : 1][2][2];
 #pragma unroll
         for (int n = 0; n < tiles_of_rows; ++n) {
+            const float t0 = top[n][0] > kNone ? top[n][0] : 0.0f, t1 = top[n][1] > kNone ? top[n][1] : 0.0f;
 #pragma unroll
-            for (int m = 0; m < kBlocks; ++m) {
+            for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = n * 8 + 2 * tig + (i & 1), d = m * 16 + 2 * gid + (i >> 1);
-                    meet[(warp * kRows + r) * dims + d] = out[n][m][i];
+                for (int o = 0; o < 2; ++o) {
+                    const float e0 = exp2_approx(score[n][half][2 * o] - t0), e1 = exp2_approx(score[n][half][2 * o + 1] - t1);
+                    total[n][0] += e0;
+                    total[n][1] += e1;
+                    const float w0 = e0 * value_scale[half], w1 = e1 * value_scale[half];
+                    const uint32_t taken = halves(w0, w1);
+                    wh[n][half][o] = transposed(taken);
+                    if constexpr (precise) wl[n][half][o] = transposed(halves_left(w0, w1, taken));
                 }
             }
         }
-        __syncthreads();
-        const bool whole = from_tile == 0 && to_tile == tiles;
-        T* context = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
-        const int piece_floats = kRows * (dims + 4);  // (a row's context, its maximum and sum, two unused)
-        const int fours = head_dim / 4;
-        const int64_t slot = pieces_each > 0 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 2 + (at == (int64_t)blockIdx.x * share ? 0 : 1);
-        float* piece = p.partial + slot * piece_floats;
-        for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
-            const int r = i / fours, d = i % fours * 4;
-            float high = kNone, sum = 0.0f;
-            float4 value = make_float4(0, 0, 0, 0);
+        // The values come as 8 x 8 matrices of code pairs, turned round: lane (gid, tig) gets dimensions 2 gid, 2 gid + 1 of
+        // positions 2 tig and 2 tig + 1; dimension 2 gid is row gid of the left-hand operand, 2 gid + 1 row gid + 8.
+        const uint32_t v_at = stages_at + stage * kStageBytes + kTile * dims;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) high = fmaxf(high, tops[w][r]);
+        for (int half = 0; half < 2; ++half) {
+            const int r = half * 16 + lane % 16;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                if (totals[w][r] == 0.0f) continue;  // (a warp without a position that the row sees)
-                const float less = exp2_approx(tops[w][r] - high);
-                const float4 part = *reinterpret_cast<const float4*>(meet + (w * kRows + r) * dims + d);
-                sum += totals[w][r] * less;
-                value.x += part.x * less, value.y += part.y * less, value.z += part.z * less, value.w += part.w * less;
-            }
-            if (whole) {
-                store_four(context + r * head_dim + d, value, sum == 0.0f ? 0.0f : 1.0f / sum);
-            } else {
-                __stcg(reinterpret_cast<float4*>(piece + r * (dims + 4) + d), value);
-                if (d == 0) __stcg(reinterpret_cast<float2*>(piece + r * (dims + 4) + dims), make_float2(high, sum));
-            }
-        }
-        if (!whole) {
-            // Where the pair's pieces are: the first one's slot, and the step to the next ones'.
-            int pieces, step, skip = 0;
-            int64_t first_slot;
-            if (pieces_each > 0) {
-                pieces = (tiles + share - 1) / share, step = 1;
-                first_slot = pair * pieces_each;
-            } else {
-                const int begin = prefix[row] + head * tiles, first = begin / share;
-                pieces = (begin + tiles - 1) / share - first + 1, step = 2;
-                first_slot = (int64_t)first * 2;
-                skip = begin != first * share ? 1 : 0;  // (it is its block's second one unless it starts it)
-            }
-            __syncthreads();
-            if (threadIdx.x == 0) {  // (release: the block's pieces, ordered before by the barrier; acquire: the other blocks')
-                int before;
-                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + pair) : "memory");
-                is_last = before == pieces - 1;
-                if (is_last) p.arrived[pair] = 0;
-            }
-            __syncthreads();
-            if (is_last) {
-                const auto piece_of = [&](int b) { return p.partial + (first_slot + (b == 0 ? skip : b * step)) * piece_floats; };
-                // A thread's part of the first pieces' contexts is asked for along with their maxima and sums.
-                constexpr int kAhead = 8;
-                const int mine_row = threadIdx.x / fours, mine_d = threadIdx.x % fours * 4;
-                const bool mine_real = mine_row < p.rows;
-                float4 ahead[kAhead];
+            for (int m = 0; m < kBlocks; m += 2) {
+                if (m < chunks) {
+                    uint32_t x[4];
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                        : "r"(v_at + r * dims + placed<dims>(r, m + lane / 16) * 16)
+                        : "memory");
 #pragma unroll
-                for (int b = 0; b < kAhead; ++b) {
-                    ahead[b] = make_float4(0, 0, 0, 0);
-                    if (b < pieces && mine_real) ahead[b] = __ldcg(reinterpret_cast<const float4*>(piece_of(b) + mine_row * (dims + 4) + mine_d));
-                }
-                float2* less = reinterpret_cast<float2*>(shared);  // (piece, row): maximum and sum, then what the piece counts for
-                for (int i = threadIdx.x; i < pieces * p.rows; i += kThreads) {
-                    less[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(i / p.rows) + i % p.rows * (dims + 4) + dims));
-                }
-                __syncthreads();
-                for (int r = warp; r < p.rows; r += kWarps) {
-                    float high = kNone, sum = 0.0f;
-                    for (int b = lane; b < pieces; b += 32) high = fmaxf(high, less[b * p.rows + r].x);
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t low = __byte_perm(x[2 * i], 0, 0x3120), high = __byte_perm(x[2 * i + 1], 0, 0x3120);
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_halves(low, a0, a1);
+                        codes_to_halves(high, a2, a3);
 #pragma unroll
-                    for (int step = 16; step > 0; step /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, step));
-                    for (int b = lane; b < pieces; b += 32) {
-                        const float2 mine = less[b * p.rows + r];
-                        const float factor = mine.x > kNone ? exp2_approx(mine.x - high) : 0.0f;
-                        less[b * p.rows + r].x = factor;
-                        sum += factor * mine.y;
-                    }
-#pragma unroll
-                    for (int step = 16; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
-                    if (lane == 0) totals[0][r] = sum;
-                }
-                __syncthreads();
-                for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
-                    const int r = i / fours, d = i % fours * 4;
-                    float4 value = make_float4(0, 0, 0, 0);
-                    const auto add = [&](const float4& part, float factor) {
-                        value.x += part.x * factor, value.y += part.y * factor, value.z += part.z * factor, value.w += part.w * factor;
-                    };
-                    int b = 0;
-                    if (i == threadIdx.x) {
-#pragma unroll
-                        for (; b < kAhead; ++b) {
-                            if (b < pieces) add(ahead[b], less[b * p.rows + r].x);
+                        for (int n = 0; n < tiles_of_rows; ++n) {
+                            if constexpr (precise) multiply(out[n][m + i], a0, a1, a2, a3, wl[n][half][0], wl[n][half][1]);
+                            multiply(out[n][m + i], a0, a1, a2, a3, wh[n][half][0], wh[n][half][1]);
                         }
                     }
-#pragma unroll 8
-                    for (; b < pieces; ++b) add(__ldcg(reinterpret_cast<const float4*>(piece_of(b) + r * (dims + 4) + d)), less[b * p.rows + r].x);
-                    store_four(context + r * head_dim + d, value, totals[0][r] == 0.0f ? 0.0f : 1.0f / totals[0][r]);
                 }
             }
         }
-        at += pieces_each > 0 ? 1 : to_tile - from_tile;
-        __syncthreads();  // (shared memory is free for the next pair)
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    copies_done<0>();
+
+    // The four warps' results meet in shared memory.  (The stages are free: every warp has read its own.)
+#pragma unroll
+    for (int n = 0; n < tiles_of_rows; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int step = 4; step < 32; step *= 2) total[n][i] += __shfl_xor_sync(0xffffffffu, total[n][i], step);
+            if (gid == 0) {
+                tops[warp][n * 8 + 2 * tig + i] = top[n][i];
+                totals[warp][n * 8 + 2 * tig + i] = total[n][i];
+            }
+        }
+    }
+    __syncthreads();
+    float* meet = reinterpret_cast<float*>(shared);  // (warp, row, dimension)
+#pragma unroll
+    for (int n = 0; n < tiles_of_rows; ++n) {
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = n * 8 + 2 * tig + (i & 1), d = m * 16 + 2 * gid + (i >> 1);
+                meet[(warp * kRows + r) * dims + d] = out[n][m][i];
+            }
+        }
+    }
+    __syncthreads();
+    const bool whole = from_tile == 0 && to_tile == tiles;
+    const int piece_floats = kRows * (dims + 4);  // (a row's context, its maximum and sum, two unused)
+    const int fours = head_dim / 4;
+    float* piece = p.partial + (int64_t)blockIdx.x * piece_floats;
+    for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
+        const int r = i / fours, d = i % fours * 4;
+        float high = kNone, sum = 0.0f;
+        float4 value = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) high = fmaxf(high, tops[w][r]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (totals[w][r] == 0.0f) continue;  // (a warp without a position that the row sees)
+            const float less = exp2_approx(tops[w][r] - high);
+            const float4 part = *reinterpret_cast<const float4*>(meet + (w * kRows + r) * dims + d);
+            sum += totals[w][r] * less;
+            value.x += part.x * less, value.y += part.y * less, value.z += part.z * less, value.w += part.w * less;
+        }
+        if (whole) {
+            store_four(context + r * head_dim + d, value, sum == 0.0f ? 0.0f : 1.0f / sum);
+        } else {
+            __stcg(reinterpret_cast<float4*>(piece + r * (dims + 4) + d), value);
+            if (d == 0) __stcg(reinterpret_cast<float2*>(piece + r * (dims + 4) + dims), make_float2(high, sum));
+        }
+    }
+    if (!whole) {
+        const int pieces = (tiles + share - 1) / share;
+        __syncthreads();
+        if (threadIdx.x == 0) {  // (release: the block's pieces, ordered before by the barrier; acquire: the other blocks')
+            int before;
+            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + pair) : "memory");
+            is_last = before == pieces - 1;
+            if (is_last) p.arrived[pair] = 0;
+        }
+        __syncthreads();
+        if (is_last) {
+            const auto piece_of = [&](int b) { return p.partial + (pair * p.pieces + b) * piece_floats; };
+            // A thread's part of the first pieces' contexts is asked for along with their maxima and sums.
+            constexpr int kAhead = 8;
+            const int mine_row = threadIdx.x / fours, mine_d = threadIdx.x % fours * 4;
+            const bool mine_real = mine_row < p.rows;
+            float4 ahead[kAhead];
+#pragma unroll
+            for (int b = 0; b < kAhead; ++b) {
+                ahead[b] = make_float4(0, 0, 0, 0);
+                if (b < pieces && mine_real) ahead[b] = __ldcg(reinterpret_cast<const float4*>(piece_of(b) + mine_row * (dims + 4) + mine_d));
+            }
+            float2* less = reinterpret_cast<float2*>(shared);  // (piece, row): maximum and sum, then what the piece counts for
+            for (int i = threadIdx.x; i < pieces * p.rows; i += kThreads) {
+                less[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(i / p.rows) + i % p.rows * (dims + 4) + dims));
+            }
+            __syncthreads();
+            for (int r = warp; r < p.rows; r += kWarps) {
+                float high = kNone, sum = 0.0f;
+                for (int b = lane; b < pieces; b += 32) high = fmaxf(high, less[b * p.rows + r].x);
+#pragma unroll
+                for (int step = 16; step > 0; step /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, step));
+                for (int b = lane; b < pieces; b += 32) {
+                    const float2 mine = less[b * p.rows + r];
+                    const float factor = mine.x > kNone ? exp2_approx(mine.x - high) : 0.0f;
+                    less[b * p.rows + r].x = factor;
+                    sum += factor * mine.y;
+                }
+#pragma unroll
+                for (int step = 16; step > 0; step /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+                if (lane == 0) totals[0][r] = sum;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
+                const int r = i / fours, d = i % fours * 4;
+                float4 value = make_float4(0, 0, 0, 0);
+                const auto add = [&](const float4& part, float factor) {
+                    value.x += part.x * factor, value.y += part.y * factor, value.z += part.z * factor, value.w += part.w * factor;
+                };
+                int b = 0;
+                if (i == threadIdx.x) {
+#pragma unroll
+                    for (; b < kAhead; ++b) {
+                        if (b < pieces) add(ahead[b], less[b * p.rows + r].x);
+                    }
+                }
+#pragma unroll 8
+                for (; b < pieces; ++b) add(__ldcg(reinterpret_cast<const float4*>(piece_of(b) + r * (dims + 4) + d)), less[b * p.rows + r].x);
+                store_four(context + r * head_dim + d, value, totals[0][r] == 0.0f ? 0.0f : 1.0f / totals[0][r]);
+            }
+        }
     }
 }
 
@@ -561,11 +511,10 @@ cudaError_t launch(const Attention8bitParams& p, cudaStream_t stream) {
     int device = 0;
     if (const cudaError_t e = cudaGetDevice(&device)) return e;
     const cudaError_t e = raised.run(device, [&] {
-        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(shared_of(dims) + (kMostPrefixRows + 1) * sizeof(int)));
+        return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_of(dims));
     });
     if (e != cudaSuccess) return e;
-    const size_t shared = shared_of(dims) + (size_t)(p.cache.batch + 1) * sizeof(int);
-    kernel<<<(unsigned)p.grid, kThreads, shared, stream>>>(p);
+    kernel<<<(unsigned)(p.cache.batch * p.cache.kv_heads * p.pieces), kThreads, shared_of(dims), stream>>>(p);
     return cudaGetLastError();
 }
 
@@ -583,26 +532,20 @@ int padded_dims(const Attention8bitParams& p) { return p.cache.head_dim > 128 ? 
 
 void plan_attention_8bit(Attention8bitParams& p, int sm_count) {
     const int dims = padded_dims(p);
-    const int64_t tiles = (p.cache.max_len + kTile - 1) / kTile;
-    // The pieces of a pair, one more at each end than whole shares, have their maxima and sums in shared memory when they are joined.
-    const int64_t most_pieces = (int64_t)(shared_of(dims) / (p.rows * sizeof(float2))) - 2;
-    // As many blocks as the GPU holds at once (by registers and shared memory), no more than there are least shares.
-    const int resident = dims == 256 ? 1 : dims == 64 ? 4 : p.rows > 8 ? 2 : 3;
-    const int64_t pairs = p.cache.batch * p.cache.kv_heads, blocks = (int64_t)sm_count * resident;
-    if (pairs * 4 <= blocks) {
-        p.least_share = kWarps;
-        p.pieces = (int)std::max<int64_t>(1, std::min({blocks / pairs, (tiles + kWarps - 1) / kWarps, most_pieces}));
-        p.grid = (int)(pairs * p.pieces);
-        return;
-    }
-    p.pieces = 0;
-    p.least_share = (int)std::max<int64_t>(kLeastShare, (tiles + most_pieces - 1) / most_pieces);
-    p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(blocks, (pairs * tiles + p.least_share - 1) / p.least_share));
+    const int64_t tiles = (p.cache.max_len + kTile - 1) / kTile, pairs = p.cache.batch * p.cache.kv_heads;
+    // Blocks that the GPU holds at once, by registers and shared memory.
+    const int64_t blocks = (int64_t)sm_count * (dims == 256 ? 1 : dims == 64 ? 4 : p.rows > 8 ? 2 : 3);
+    // The pieces of a pair have their maxima and sums in shared memory when they are joined.
+    const int64_t most = std::min<int64_t>((tiles + kWarps - 1) / kWarps, shared_of(dims) / (p.rows * sizeof(float2)));
+    const int64_t spread = std::max<int64_t>(1, blocks / pairs);
+    const int64_t balanced = std::min((tiles + kMostShare - 1) / kMostShare, 8 * blocks / pairs);  // (blocks that find nothing to do cost time too)
+    p.spread = (int)std::min(spread, most);
+    p.pieces = (int)std::min(std::max(spread, balanced), most);
 }
 
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p) {
     const int rows = p.rows <= 8 ? 8 : 16;
-    return (size_t)p.grid * 2 * rows * (padded_dims(p) + 4) * sizeof(float);
+    return (size_t)(p.cache.batch * p.cache.kv_heads * p.pieces) * rows * (padded_dims(p) + 4) * sizeof(float);
 }
 
 cudaError_t launch_decode_attention_8bit(const Attention8bitParams& p, cudaStream_t stream) {

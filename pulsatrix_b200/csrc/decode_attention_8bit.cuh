@@ -14,18 +14,17 @@ struct Attention8bitParams {
     const void* q;           // (batch, heads, q_len, head_dim)
     void* context;           // likewise
     const int64_t* lengths;  // (batch): positions of the cache that row b sees, the new ones among them
-    float* partial;          // scratch: two pieces per block of the launch
+    float* partial;          // scratch: a piece per block of the launch
     int32_t* arrived;        // scratch: (batch, kv_heads), zero between calls
     int64_t window;          // sliding window of a causal mask; 0: none
     int32_t heads, group, q_len, rows;  // rows = group * q_len
     int32_t type, causal;
-    int32_t grid;            // blocks
-    int32_t least_share;     // tiles of 32 positions that a block takes at least
-    int32_t pieces;          // blocks of every (row, kv head); 0: every block takes an equal share of all tiles
+    int32_t pieces;          // blocks of every (row, kv head)
+    int32_t spread;          // pieces that fill the GPU
     float scale;
 };
 
-void plan_attention_8bit(Attention8bitParams& p, int sm_count);  // grid, least_share and pieces
+void plan_attention_8bit(Attention8bitParams& p, int sm_count);  // pieces and spread
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p);
 // cudaErrorInvalidValue: see psx_b200_decode_attention_8bit for the shapes that are taken.
 cudaError_t launch_decode_attention_8bit(const Attention8bitParams& p, cudaStream_t stream);

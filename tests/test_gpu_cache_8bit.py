@@ -290,6 +290,28 @@ def test_the_same_call_gives_the_same_bits_and_graphs_replay():
     assert (out == psx.Context(0).decode_attention_8bit(q, cache, lengths)).all()
 
 
+def test_as_many_rows_as_there_may_be():
+    import torch
+    batch = 4096
+    rng = np.random.RandomState(13)
+    cache = psx.Cache8bit.empty(batch, 1, 48, 16, 16)
+    counts = rng.randint(0, 9, batch)
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int64)
+    new = [_tensor(rng.randn(int(offsets[-1]), 1, 16), "float16") for _ in range(2)]
+    cached = np.zeros(batch, dtype=np.int64)
+    status = gh.ctx().store_cache_8bit(cache, *new, torch.from_numpy(offsets).cuda(), torch.from_numpy(cached).cuda())
+    assert (status == 0).all()
+    codes, scales = _parts(cache)
+    for i in range(2):
+        want = _store(np.zeros((batch, 1, 48, 16)), np.zeros((batch, 1, 3)), new[i].double().cpu().numpy(), offsets, cached, 16)
+        assert (codes[i] == want[0]).all() and (scales[i] == want[1]).all()
+    q = _tensor(rng.randn(batch, 2, 1, 16), "float16")
+    got = gh.ctx().decode_attention_8bit(q, cache, torch.from_numpy(counts.astype(np.int64)).cuda()).double().cpu().numpy()
+    want, most, value = _attention(q.double().cpu().numpy(), cache, counts, 0.25, True, 0)
+    slack, step = _tolerance("float16", most, value, 16, 9)
+    assert (np.abs(got - want) <= slack + step * np.abs(want)).all()
+
+
 def test_refusals():
     import torch
     ctx = gh.ctx()

@@ -124,6 +124,12 @@ def test_many_short_sequences():
     _check("float32", lens[:300], lens[:300], 2, 2, 64)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_as_many_sequences_as_there_may_be(dtype):
+    lens = np.random.RandomState(14).randint(0, 4, 4096).tolist()
+    _check(dtype, lens, lens, 1, 1, 128)
+
+
 def test_slices_of_one_projection():
     import torch
     rng = np.random.RandomState(9)
