@@ -13,10 +13,12 @@
 // and contexts are floats.
 //
 // A (row, kv head) pair's cached positions are cut into tiles of 32, and the tiles into pieces, a block each: as many as fill the GPU
-// once, or as pieces of 64 tiles make where that is more, which evens out rows of different lengths (64 rows x 8 kv heads of up to 8191
-// positions: 167 us as one piece each, 138 as four; the same of 1000 positions: 24.7 as one, 31 as two).  The last block of a pair to
-// end joins its pieces, in order.  (Equal shares of all pairs' tiles laid on one axis: 137 and 42 us; 24 rows x 8 of up to 4096: 52 instead of 33:
-// most blocks then have the end of one pair and the start of another.)  Inside a block each of four warps takes every fourth tile, with
+// once, or as pieces of 128 tiles make where that is more, which evens out rows of different lengths (64 rows x 8 kv heads of up to 8191
+// positions: 167 us as one piece each, 141 as two; pieces of 64 tiles: 138, but 96 rows x 1 of up to 16,000: 70 instead of 61).  The last
+// block of a pair to end joins its pieces, in order.  (Equal shares of all pairs' tiles laid on one axis: 139 us there,
+// with a cold L2 143 instead of 155; but 64 x 8 of 1000: 41 instead of 25, 24 x 8 of up to 4096: 52 instead of 33, since most blocks then have
+// the end of one pair
+// and the start of another.)  Inside a block each of four warps takes every fourth tile, with
 // its own two stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no warp waits for another until the end.
 // Bound by HBM for long caches (2 bytes per position, head dimension and kv head), by the chain of a tile for short ones: some 2100
 // clocks from a tile's arrival to its weights' products, most of them conversions of codes (64 instructions for 32 positions x 64
@@ -32,7 +34,7 @@ namespace psx {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4, kTile = 32;
-constexpr int kMostShare = 64;  // tiles that a block takes where shorter pieces only balance
+constexpr int kMostShare = 128;  // tiles that a block takes where shorter pieces only balance
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
