@@ -356,7 +356,7 @@ PSX_API psx_status psx_b200_decode_attention(psx_ctx* ctx, void* stream, const f
  *                that is alive and not finished, or among the scores (all places are -inf, -1, -1); PSX_ROW_ALL_REMOVED: nothing
  *                is left at all
  * keep may be larger than beams (twice as many leave enough when finished ones are set aside).  Limits: beams <= 64,
- * keep <= 128, vocab <= 2^30 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; the outputs must not overlap the inputs.
+ * keep <= 128, vocab <= 2^30, beams * vocab <= 2^31 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; the outputs must not overlap the inputs.
  * The context's scratch grows to groups * beams * (vocab / 1024) * (keep * 8 + 16) bytes at most; inside a stream capture it
  * cannot grow (PSX_ERR_UNSUPPORTED): make a call of that size before. */
 PSX_API psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream, const float* logits, int64_t groups, int64_t beams, int64_t vocab,

@@ -1167,8 +1167,11 @@ psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream_ptr, const float* log
     }
     if (groups == 0) return PSX_OK;
     if (!logits || !scores || !out_scores || !parents || !tokens) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
-    if (beams > psx::kMostSelectBeams || keep > psx::kMostKept || vocab > (int64_t(1) << 30) || groups > 0x7fffffff / beams) {
-        return fail(PSX_ERR_UNSUPPORTED, "psx_b200: beam selection takes at most 64 beams, 128 candidates per group and 2^30 tokens");
+    // (2^31 candidates of a group: its rows' parts then number less than 2^17, and times the parts of a row less than 2^32, as Quotients want)
+    if (beams > psx::kMostSelectBeams || keep > psx::kMostKept || vocab > (int64_t(1) << 30) || beams * vocab > (int64_t(1) << 31) ||
+        groups > 0x7fffffff / beams) {
+        return fail(PSX_ERR_UNSUPPORTED,
+                    "psx_b200: beam selection takes at most 64 beams, 128 candidates per group, 2^30 tokens and 2^31 (beam, token) pairs of a group");
     }
     psx::BeamSelectParams p{};
     p.logits = logits; p.scores = scores; p.finished = finished; p.out_scores = out_scores; p.parents = parents; p.tokens = tokens;
@@ -1176,7 +1179,7 @@ psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream_ptr, const float* log
     p.beams = (int32_t)beams; p.vocab = (int32_t)vocab; p.keep = (int32_t)keep;
     psx::plan_beam_select(p, ctx->sm_count);
     const int64_t lists = groups * beams * p.parts;
-    if (lists > 0x7fffffff || beams * p.parts * keep > 0x7fffffff || beams * p.parts > (1 << 21)) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
+    if (lists > 0x7fffffff) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
     const OnDevice device(ctx->device);
     PSX_CUDA(device.error);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);

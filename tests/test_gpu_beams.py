@@ -189,6 +189,14 @@ def test_refusals_of_the_selection():
     assert ctx.beam_select(x[:0], s[:0], 2, 2)["tokens"].shape == (0, 2)
 
 
+def test_more_pairs_of_a_group_than_there_may_be_are_refused():
+    import torch
+    ctx, x = gh.ctx(), torch.zeros(64, device="cuda")  # (refused ahead of any launch: the logits do not exist)
+    for beams, vocab in ((64, 2 ** 25 + 1), (3, 2 ** 30), (1, 2 ** 30 + 1)):
+        assert ctx._lib.psx_b200_beam_select(ctx._ctx, None, x.data_ptr(), 1, beams, vocab, vocab, x.data_ptr(), None, 0, 4, x.data_ptr(),
+                                             x.data_ptr(), x.data_ptr(), None) == psx.ERR_UNSUPPORTED
+
+
 # ---- states ---------------------------------------------------------------------------------------------------------------
 def _moved(x, parents, lengths, per):
     groups, beams = parents.shape
