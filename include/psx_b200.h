@@ -376,7 +376,8 @@ typedef struct psx_beam_state {
  * 0 .. beams - 1 stays as it is.  lengths: device int64 (groups * beams), tokens that each row holds before the call; the first
  * ceil(lengths[parent] / tokens_per_position) positions are taken over and what lies behind them in the row is left as it was;
  * NULL: all positions.  `states` is a host array, read during the call.  The states must overlap neither each other nor
- * parents or lengths (PSX_ERR_BAD_ARGUMENT).  Limit: beams <= 64 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`. */
+ * parents or lengths (PSX_ERR_BAD_ARGUMENT).  Limits: beams <= 64, count <= 65,536, groups times all states' heads < 2^31 (else
+ * PSX_ERR_UNSUPPORTED; nothing has moved then).  Asynchronous on `stream`. */
 PSX_API psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream, const psx_beam_state* states, int64_t count, int64_t groups,
                                            int64_t beams, const int64_t* parents, const int64_t* lengths);
 

@@ -1202,9 +1202,11 @@ psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream_ptr, const psx_bea
     if (!states || !parents) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
     if (beams > psx::kMostBeams) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: states follow at most 64 beams");
     if (groups > 0x7fffffff / beams) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many beams for one call");
+    if (count > 65536) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: at most 65,536 states follow their beams in a call");
     // The bytes that the call touches, none of them twice.
     std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
     ranges.reserve((size_t)count + 2);
+    int64_t heads = 0;
     for (int64_t i = 0; i < count; ++i) {
         const psx_beam_state& s = states[i];
         if (s.heads < 0 || s.positions < 0 || s.position_bytes <= 0 || s.tokens_per_position <= 0) {
@@ -1215,10 +1217,13 @@ psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream_ptr, const psx_bea
             return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a state is larger than any memory");
         }
         if (bytes == 0) continue;
+        heads += s.heads;
         if (!s.data) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
         const uintptr_t at = reinterpret_cast<uintptr_t>(s.data);
         ranges.emplace_back(at, at + (uintptr_t)bytes);
     }
+    // A block per group and head at least (more only while that fills the GPU); refused here, before any state has moved.
+    if (heads > 0x7fffffff / groups) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many heads of states for one call");
     const size_t rows_bytes = (size_t)(groups * beams) * sizeof(int64_t);
     ranges.emplace_back(reinterpret_cast<uintptr_t>(parents), reinterpret_cast<uintptr_t>(parents) + rows_bytes);
     if (lengths) ranges.emplace_back(reinterpret_cast<uintptr_t>(lengths), reinterpret_cast<uintptr_t>(lengths) + rows_bytes);
@@ -1237,9 +1242,7 @@ psx_status psx_b200_reorder_states(psx_ctx* ctx, void* stream_ptr, const psx_bea
             p.states[p.count++] = {static_cast<char*>(s.data), s.heads, s.positions, s.position_bytes, s.tokens_per_position, 0, 0, 0};
         }
         if (p.count == psx::kStatesPerLaunch || (i + 1 == count && p.count > 0)) {
-            const cudaError_t e = psx::launch_reorder_states(p, ctx->sm_count, static_cast<cudaStream_t>(stream_ptr));
-            if (e == cudaErrorInvalidValue) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many heads of states for one call");
-            PSX_CUDA(e);
+            PSX_CUDA(psx::launch_reorder_states(p, ctx->sm_count, static_cast<cudaStream_t>(stream_ptr)));
             ctx->launches += 1;
             p.count = 0;
         }

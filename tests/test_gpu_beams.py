@@ -287,3 +287,15 @@ def test_refusals_of_the_states():
     with pytest.raises(psx.PsxError) as e:
         ctx.reorder_states(torch.zeros((1, 65), dtype=torch.int64, device="cuda"), [torch.zeros(65, 1, 1, device="cuda")])
     assert e.value.status == psx.ERR_UNSUPPORTED
+
+
+def test_a_refused_call_moves_no_state():
+    import torch
+    ctx, parents = gh.ctx(), torch.tensor([[1, 0], [1, 0]], device="cuda")
+    states = [torch.arange(4.0, device="cuda").view(4, 1, 1) for _ in range(64)]
+    described = (psx.binding.BeamState * 65)(*[psx.binding.BeamState(s.data_ptr(), 1, 1, 4, 1) for s in states])
+    described[64] = psx.binding.BeamState(1 << 46, 1 << 30, 1, 1, 1)  # (does not exist; groups x heads of all is beyond 2^31)
+    call = lambda count: ctx._lib.psx_b200_reorder_states(ctx._ctx, None, described, count, 2, 2, parents.data_ptr(), None)
+    assert call(65) == psx.ERR_UNSUPPORTED and call(65537) == psx.ERR_UNSUPPORTED and call(2 ** 62) == psx.ERR_UNSUPPORTED
+    torch.cuda.synchronize()
+    assert all((s.flatten() == torch.arange(4.0, device="cuda")).all() for s in states)
