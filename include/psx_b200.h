@@ -435,7 +435,7 @@ PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, co
  * sequences, finite or not, have no influence; a NaN among a sequence's own values reaches the queries of the 128 positions
  * around it that do not see it, too.
  * All pointers 16-byte aligned, strides a multiple of 16 bytes.  Limits: head_dim a multiple of 8 up to 128, batch <= 4096, total_q
- * and total_k <= 2^29 (else PSX_ERR_UNSUPPORTED).  status (device, may be null): set to 0 by the call, to 1 if a
+ * and total_k <= 2^29, strides < 2^36 (else PSX_ERR_UNSUPPORTED).  status (device, may be null): set to 0 by the call, to 1 if a
  * bounded device-side wait ran out (psx_b200_ctx_set_wait_limit).  Asynchronous on `stream`; fp32 takes scratch of 1.5 times the
  * bytes of k and v (in a stream capture as psx_b200_beam_select). */
 PSX_API psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream, int32_t dtype, const void* q, const void* k, const void* v, void* out,

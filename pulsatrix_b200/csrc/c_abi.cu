@@ -1359,6 +1359,9 @@ psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dty
     if (q_stride < heads * head_dim || k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim) {
         return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a position's stride is at least its heads times head_dim");
     }
+    if (std::max({q_stride, k_stride, v_stride}) >= int64_t(1) << 36) {  // (a tensor map's are below 2^40 bytes)
+        return fail(PSX_ERR_UNSUPPORTED, "psx_b200: attention of prompts takes strides below 2^36 elements");
+    }
     if (batch == 0 || total_q == 0) {
         if (status) {
             const OnDevice device(ctx->device);

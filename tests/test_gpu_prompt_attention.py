@@ -254,3 +254,11 @@ def test_refusals():
     x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda")
     out, _ = ctx.prompt_attention(x, q, q, torch.tensor([0, 3], device="cuda"), torch.tensor([0, 0], device="cuda"))  # no keys at all
     assert (out == 0).all()
+
+
+def test_a_stride_that_no_tensor_map_has_is_refused():
+    import torch
+    ctx, x, at = gh.ctx(), torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda"), torch.tensor([0, 1], device="cuda")
+    for strides in ((2 ** 40, 64, 64), (64, 2 ** 36, 64), (64, 64, 2 ** 62)):
+        assert ctx._lib.psx_b200_prompt_attention(ctx._ctx, None, 1, x.data_ptr(), x.data_ptr(), x.data_ptr(), x.data_ptr(), 1, 1, *strides, at.data_ptr(),
+                                                  at.data_ptr(), 1, 1, 1, 64, 1.0, 1, 0, None) == psx.ERR_UNSUPPORTED
