@@ -1389,7 +1389,7 @@ psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dty
     }
     if (status) PSX_CUDA(cudaMemsetAsync(status, 0, sizeof(int32_t), stream));
     int launches = 0;
-    const cudaError_t e = psx::launch_prompt_attention(p, stream, &launches);
+    const cudaError_t e = psx::launch_prompt_attention(p, ctx->sm_count, stream, &launches);
     ctx->launches += launches;
     if (e == cudaErrorNotSupported) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: the driver has no tensor maps");
     PSX_CUDA(e);

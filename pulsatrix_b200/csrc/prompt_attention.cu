@@ -45,6 +45,8 @@ namespace {
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileRows = 128;
+constexpr int kMostPieces = 8;         // of a group of rows' keys, where there are few groups: the CTAs of a cluster
+constexpr int kLeastShared = 5;        // blocks of keys that are shared out
 constexpr float kMostGrowth = 8.0f;  // of a row's maximum, in powers of two, before its context is rescaled
 
 template <int dims_, int parts_>
@@ -63,6 +65,9 @@ struct Shape {
     static constexpr int third_at = score_places * block, context_at = parts == 1 ? third_at : third_at + block / 2;
     static constexpr int query_at = context_at + tiles * dims, query_part = dims / 2;
     static_assert(query_at + (parts == 1 ? 0 : parts * query_part) <= 512);
+    // A piece's result in shared memory, in floats: per tile (four dimensions, row) fours of the context, then a row's reference point and sum.
+    static constexpr int tile_floats = kTileRows * (dims + 2);
+    static_assert(tiles * tile_floats * 4 <= shared);
     // Column of a part of the weights that take the scores' place.
     static __host__ __device__ constexpr int weight_at(int place, int part) { return part == 2 ? third_at : place * block + part * (block / 2); }
 };
@@ -71,6 +76,7 @@ struct alignas(64) PromptLaunch {
     CUtensorMap q_map, k_map, v_map;
     PromptAttentionParams p;
     int32_t steps;  // of 16 dimensions
+    int32_t pieces;  // CTAs of a cluster
     int32_t dims16;  // the head dimension, rounded up to 16
 };
 
@@ -92,6 +98,22 @@ __device__ __forceinline__ uint32_t pack(float low, float high, __half) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(high), "f"(low));
     return r;
+}
+
+// All threads of the cluster's CTAs meet, each by itself.
+__device__ __forceinline__ void cluster_meets() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// From the shared memory of the cluster's CTA `rank`, where this CTA has `address`.
+template <class T>
+__device__ __forceinline__ T load_of_peer(uint32_t address, int rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(address), "r"(rank));
+    T x;
+    if constexpr (sizeof(T) == 16) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+    else asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+    return x;
 }
 
 // Two floats as three bf16 pairs that add up to them, the largest part first.  What is left of a number after a part is exact; of
@@ -131,8 +153,9 @@ __device__ __forceinline__ float2 add_pair(float2 a, float2 x) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// Elem: the type of the products' operands (bf16 for the parts of fp32); Out: the type of the context.
-template <class Elem, class Out, class S>
+// Elem: the type of the products' operands (bf16 for the parts of fp32); Out: the type of the context; pieced: the CTAs of a cluster
+// share a group of rows' keys.
+template <class Elem, class Out, class S, bool pieced>
 __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const __grid_constant__ PromptLaunch launch) {
     extern __shared__ uint8_t raw_shared[];
     __shared__ uint64_t q_full, k_full[S::stages], v_full[S::stages], k_empty[S::stages], v_empty[S::stages];
@@ -149,7 +172,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
 
     const auto queries_of = [&](int b) { return max(min(p.q_offsets[b + 1], p.total_q) - max(p.q_offsets[b], (int64_t)0), (int64_t)0); };
     sum_of_rows(p.batch, prefix, carry, [&](int b) { return (int)((queries_of(b) + kRows - 1) / kRows); });
-    const int group_of_rows = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+    const int item = pieced ? blockIdx.x / launch.pieces : blockIdx.x, number = pieced ? blockIdx.x % launch.pieces : 0;
+    const int group_of_rows = item / p.heads, head = item % p.heads;
     if (group_of_rows >= prefix[p.batch]) return;
     const int b = row_of_item(prefix, p.batch, group_of_rows);
     const int64_t queries = queries_of(b), q_begin = max(p.q_offsets[b], (int64_t)0), k_begin = max(p.k_offsets[b], (int64_t)0);
@@ -167,6 +191,19 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         ends[t] = last_row < first_row ? 0 : max(sight.end(last_row), (int64_t)0);
         counts[t] = (int)max((ends[t] + S::block - 1) / S::block - begin, (int64_t)0);
         most = max(most, counts[t]);
+    }
+    int pieces = 1;
+    if constexpr (pieced) {  // this CTA's piece of the blocks
+        const int share = most < kLeastShared ? max(most, 1) : (most + launch.pieces - 1) / launch.pieces, before = number * share;
+        pieces = max((most + share - 1) / share, 1);
+        if (number >= pieces) {
+            if (pieces > 1) cluster_meets(), cluster_meets();
+            return;
+        }
+        begin += before;
+        most = min(most - before, share);
+#pragma unroll
+        for (int t = 0; t < S::tiles; ++t) counts[t] = min(max(counts[t] - before, 0), share);
     }
 
     // The block that ends behind the sequence's last key, if there is one.
@@ -547,10 +584,27 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             fine = wait(&context_full[t], S::parts == 1 ? 0 : (count - 1) & 1);
             tensor_fence_after();
         }
+        // Eight dimensions of a row's context, times what makes its weights add up to one.
+        const auto put = [&](int64_t to, int d, const float* o, float sum) {
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+            Out* out = static_cast<Out*>(p.out) + ((q_begin + to) * p.heads + head) * p.head_dim + d;
+            if constexpr (sizeof(Out) == 4) {
+                float4 a = make_float4(o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse);
+                float4 c = make_float4(o[4] * inverse, o[5] * inverse, o[6] * inverse, o[7] * inverse);
+                if (sum == 0.0f) a = c = make_float4(0, 0, 0, 0);
+                reinterpret_cast<float4*>(out)[0] = a;
+                reinterpret_cast<float4*>(out)[1] = c;
+            } else {
+                uint4 a = make_uint4(pack(o[0] * inverse, o[1] * inverse, Elem{}), pack(o[2] * inverse, o[3] * inverse, Elem{}),
+                                     pack(o[4] * inverse, o[5] * inverse, Elem{}), pack(o[6] * inverse, o[7] * inverse, Elem{}));
+                if (sum == 0.0f) a = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(out) = a;
+            }
+        };
+        if (pieced && pieces > 1 && S::tiles == 2 && fine && counts[1 - t] > 0) fine = wait(&context_full[1 - t], 0);  // (shared memory is free then)
         if (fine) {
+            float4* fours = reinterpret_cast<float4*>(shared) + t * (S::tile_floats / 4) + (warp % 4) * 32 + lane;
             if (count > 0) add_block();
-            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-            Out* out = static_cast<Out*>(p.out) + ((q_begin + row) * p.heads + head) * p.head_dim;
 #pragma unroll
             for (int i = 0; i < S::dims; i += 32) {
                 if (i >= p.head_dim) break;
@@ -562,29 +616,65 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                     tensor_load32(context_at + i, o);
                     tensor_loads_done();
                 }
-                if (row < queries) {
+                if (!pieced || pieces == 1) {
+                    if (row < queries) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        if (i + k >= p.head_dim) break;
-                        if constexpr (sizeof(Out) == 4) {
-                            float4 a = make_float4(o[k] * inverse, o[k + 1] * inverse, o[k + 2] * inverse, o[k + 3] * inverse);
-                            float4 c = make_float4(o[k + 4] * inverse, o[k + 5] * inverse, o[k + 6] * inverse, o[k + 7] * inverse);
-                            if (total == 0.0f) a = c = make_float4(0, 0, 0, 0);
-                            reinterpret_cast<float4*>(out + i + k)[0] = a;
-                            reinterpret_cast<float4*>(out + i + k)[1] = c;
-                        } else {
-                            uint4 a = make_uint4(pack(o[k] * inverse, o[k + 1] * inverse, Elem{}), pack(o[k + 2] * inverse, o[k + 3] * inverse, Elem{}),
-                                                 pack(o[k + 4] * inverse, o[k + 5] * inverse, Elem{}), pack(o[k + 6] * inverse, o[k + 7] * inverse, Elem{}));
-                            if (total == 0.0f) a = make_uint4(0, 0, 0, 0);
-                            *reinterpret_cast<uint4*>(out + i + k) = a;
+                        for (int k = 0; k < 32; k += 8) {
+                            if (i + k >= p.head_dim) break;
+                            put(row, i + k, o + k, total);
                         }
                     }
+                } else if (count > 0) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) fours[(i + k) / 4 * kTileRows] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+            }
+            if (pieced && pieces > 1) {
+                reinterpret_cast<float2*>(shared)[(t * S::tile_floats + kTileRows * S::dims) / 2 + (warp % 4) * 32 + lane] = make_float2(top, total);
+            }
+        }
+        if (pieced && pieces > 1) {
+            // Every CTA joins its share of the rows, out of all pieces' shared memory.  (Every warp comes here, whatever its waits have come to.)
+            cluster_meets();
+            const int rows = (kRows + pieces - 1) / pieces, parts = (S::tiles * 128) / rows, mine = threadIdx.x % rows, joined = number * rows + mine;
+            if (joined < kRows && row0 + joined < queries && (int)threadIdx.x / rows < parts) {
+                const int tile = joined / kTileRows, of_tile = joined % kTileRows;
+                float less[kMostPieces], sum = 0.0f, high = masked;  // what a piece counts for; negative: it has nothing
+                float2 ends_at[kMostPieces];
+#pragma unroll
+                for (int b = 0; b < kMostPieces; ++b) {
+                    ends_at[b] = make_float2(masked, 0.0f);
+                    if (b < pieces) ends_at[b] = load_of_peer<float2>(q_at + (tile * S::tile_floats + kTileRows * S::dims + 2 * of_tile) * 4, b);
+                    high = turned ? fminf(high, ends_at[b].x) : fmaxf(high, ends_at[b].x);
+                }
+#pragma unroll
+                for (int b = 0; b < kMostPieces; ++b) {
+                    // (a sum that is NaN counts, so that it is seen)
+                    const bool nothing = ends_at[b].x == masked && ends_at[b].y == 0.0f;
+                    less[b] = nothing ? -1.0f : ends_at[b].x == high ? 1.0f : exp2_approx((ends_at[b].x - high) * factor);
+                    sum += nothing ? 0.0f : less[b] * ends_at[b].y;
+                }
+                for (int d = (int)threadIdx.x / rows * 8; d < p.head_dim; d += parts * 8) {
+                    float o[8] = {};
+#pragma unroll
+                    for (int b = 0; b < kMostPieces; ++b) {
+                        if (less[b] == -1.0f) continue;
+                        const uint32_t from = q_at + (tile * S::tile_floats + (d / 4 * kTileRows + of_tile) * 4) * 4;
+                        const float4 x = load_of_peer<float4>(from, b), y = load_of_peer<float4>(from + kTileRows * 16, b);
+                        o[0] += x.x * less[b], o[1] += x.y * less[b], o[2] += x.z * less[b], o[3] += x.w * less[b];
+                        o[4] += y.x * less[b], o[5] += y.y * less[b], o[6] += y.z * less[b], o[7] += y.w * less[b];
+                    }
+                    put(row0 + joined, d, o, sum);
                 }
             }
         }
         tensor_fence_before();
     } else {
         few_registers();
+    }
+    if (pieced && pieces > 1) {
+        if (warp >= S::tiles * 4) cluster_meets();
+        cluster_meets();  // (its shared memory is read by others until then)
     }
     __syncthreads();
     if (warp == kIssueWarp) {
@@ -636,16 +726,20 @@ bool encode(CUtensorMap* map, bool bfloat, const void* at, int64_t positions, in
 }
 
 template <class Elem, class Out, class S>
-cudaError_t launch(const PromptAttentionParams& p, cudaStream_t stream, int* launches) {
+cudaError_t launch(const PromptAttentionParams& p, int sm_count, cudaStream_t stream, int* launches) {
     constexpr bool bfloat = __is_same(Elem, __nv_bfloat16);
-    static OncePerDevice raised;
-    const auto kernel = prompt_attention_kernel<Elem, Out, S>;
+    // Where the groups of rows leave half of the SMs idle, clusters share the keys of each (lengths are not known here: a CTA that finds
+    // nothing to do ends early).
+    const int64_t blocks = (p.total_q / (S::tiles * kTileRows) + p.batch) * p.heads;  // no more than these groups of rows
+    const int pieces = (int)std::max<int64_t>(1, std::min({sm_count / blocks, p.total_k / S::block + 1, (int64_t)kMostPieces}));
+    static OncePerDevice raised[2];
+    const auto kernel = pieces > 1 ? prompt_attention_kernel<Elem, Out, S, true> : prompt_attention_kernel<Elem, Out, S, false>;
     // 1024 bytes to start on a boundary of that.  More than half of an SM's, so that a CTA has the tensor memory for itself.
     const size_t shared = S::shared + 1024 + (size_t)(p.batch + 1) * sizeof(int);
     static_assert(S::shared + 1024 > 114 << 10 && S::shared + 1024 + (kMostPrefixRows + 1) * sizeof(int) <= 227 << 10);
     int device = 0;
     if (const cudaError_t e = cudaGetDevice(&device)) return e;
-    const cudaError_t e = raised.run(device, [&] {
+    const cudaError_t e = raised[pieces > 1].run(device, [&] {
         return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(S::shared + 1024 + (kMostPrefixRows + 1) * sizeof(int)));
     });
     if (e != cudaSuccess) return e;
@@ -653,6 +747,7 @@ cudaError_t launch(const PromptAttentionParams& p, cudaStream_t stream, int* lau
     l.p = p;
     l.steps = (p.head_dim + 15) / 16;
     l.dims16 = l.steps * 16;
+    l.pieces = pieces;
     const void *k = p.k, *v = p.v;
     int64_t k_rows = p.total_k, k_stride = p.k_stride, v_stride = p.v_stride;
     if constexpr (S::parts == 3) {
@@ -679,16 +774,29 @@ cudaError_t launch(const PromptAttentionParams& p, cudaStream_t stream, int* lau
         !encode(&l.v_map, bfloat, v, k_rows, v_stride, p.kv_heads, p.head_dim, S::block)) {
         return cudaErrorInvalidValue;
     }
-    const int64_t row_groups = p.total_q / (S::tiles * kTileRows) + p.batch;  // no more than these
-    kernel<<<(unsigned)(row_groups * p.heads), S::threads, shared, stream>>>(l);
+    if (pieces > 1) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3((unsigned)(blocks * pieces));
+        config.blockDim = dim3(S::threads);
+        config.dynamicSmemBytes = shared;
+        config.stream = stream;
+        cudaLaunchAttribute cluster;
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = (unsigned)pieces, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+        config.attrs = &cluster;
+        config.numAttrs = 1;
+        if (const cudaError_t failed = cudaLaunchKernelEx(&config, kernel, l)) return failed;
+    } else {
+        kernel<<<(unsigned)blocks, S::threads, shared, stream>>>(l);
+    }
     ++*launches;
     return cudaGetLastError();
 }
 
 template <class Elem, class Out, int parts>
-cudaError_t launch_dims(const PromptAttentionParams& p, cudaStream_t stream, int* launches) {
-    if (p.head_dim <= 64) return launch<Elem, Out, Shape<64, parts>>(p, stream, launches);
-    return launch<Elem, Out, Shape<128, parts>>(p, stream, launches);
+cudaError_t launch_dims(const PromptAttentionParams& p, int sm_count, cudaStream_t stream, int* launches) {
+    if (p.head_dim <= 64) return launch<Elem, Out, Shape<64, parts>>(p, sm_count, stream, launches);
+    return launch<Elem, Out, Shape<128, parts>>(p, sm_count, stream, launches);
 }
 
 }  // namespace
@@ -698,12 +806,12 @@ size_t prompt_split_bytes(const PromptAttentionParams& p) {
     return (size_t)12 * p.head_dim * p.total_k * p.kv_heads;
 }
 
-cudaError_t launch_prompt_attention(const PromptAttentionParams& p, cudaStream_t stream, int* launches) {
+cudaError_t launch_prompt_attention(const PromptAttentionParams& p, int sm_count, cudaStream_t stream, int* launches) {
     *launches = 0;
     if (!encoder()) return cudaErrorNotSupported;
-    if (p.type == kFloat32) return launch_dims<__nv_bfloat16, float, 3>(p, stream, launches);
-    if (p.type == kBfloat16) return launch_dims<__nv_bfloat16, __nv_bfloat16, 1>(p, stream, launches);
-    return launch_dims<__half, __half, 1>(p, stream, launches);
+    if (p.type == kFloat32) return launch_dims<__nv_bfloat16, float, 3>(p, sm_count, stream, launches);
+    if (p.type == kBfloat16) return launch_dims<__nv_bfloat16, __nv_bfloat16, 1>(p, sm_count, stream, launches);
+    return launch_dims<__half, __half, 1>(p, sm_count, stream, launches);
 }
 
 }  // namespace psx

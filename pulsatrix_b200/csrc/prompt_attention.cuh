@@ -25,6 +25,6 @@ struct PromptAttentionParams {
 
 size_t prompt_split_bytes(const PromptAttentionParams& p);
 // *launches: kernels launched.  cudaErrorNotSupported: the driver does not know tensor maps.
-cudaError_t launch_prompt_attention(const PromptAttentionParams& p, cudaStream_t stream, int* launches);
+cudaError_t launch_prompt_attention(const PromptAttentionParams& p, int sm_count, cudaStream_t stream, int* launches);
 
 }  // namespace psx
