@@ -18,6 +18,13 @@
 // scheduler), 1024 of products, and the way between the two; 1.05 PFLOP/s at those sizes.  Tried and taken back: a share of the
 // exponentials by a polynomial (no gain, 662 and 668 us), two threads for a query (771 us).
 //
+// Few groups of rows: where they would leave half of the SMs idle, the CTAs of a cluster, up to eight, take a piece of a group's keys each,
+// leave their contexts, reference points and sums in their own shared memory and join them there, each its share of the rows, out of
+// all of the others' (one head of 4096 positions of 128: 25 us instead of 61; fp32 50 instead of 134; 16 queries of 8 heads behind 16,000
+// keys: 35 instead of 189).  The same through memory, the last CTA to end joining all: 33, 55 and 47 us.  Clusters of two where the GPU
+// is between half full and twice full cost more than they gain (16 heads of 4096: 108 us instead of 70): most of them would be the
+// short rows', and a CTA that finds nothing to do still takes its turn.
+//
 // fp32 operands: every number is split into three bf16 parts that add up to it (8 bits of the fraction each), and a product is the
 // six products of parts that reach fp32's precision, the small ones first.  The keys' and values' parts are written by a kernel ahead,
 // the queries' go into tensor memory once, the weights' as they are made.  One tile, blocks of 64 keys; the scores have two places,
@@ -234,14 +241,16 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     __syncthreads();
     tensor_fence_after();
     const uint32_t tensor = tensor_at;
-    const auto wait_alone = [&](uint64_t* bar, uint32_t parity) {
-        if (barrier_wait_bounded(bar, parity, p.wait_limit_ns, &give_up)) return true;
+    // The limit is that of a block's step; `blocks`: how many of them may lie between.
+    const auto wait_alone = [&](uint64_t* bar, uint32_t parity, uint32_t blocks = 1) {
+        const uint64_t limit = p.wait_limit_ns < ~0ull >> 32 ? p.wait_limit_ns * blocks : p.wait_limit_ns;
+        if (barrier_wait_bounded(bar, parity, limit, &give_up)) return true;
         *(volatile uint32_t*)&give_up = 1;
         return false;
     };
-    const auto wait = [&](uint64_t* bar, uint32_t parity) {  // (a warp goes on as a whole or not at all)
+    const auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t blocks = 1) {  // (a warp goes on as a whole or not at all)
         if (__all_sync(0xffffffffu, barrier_passed(bar, parity))) return true;
-        return __all_sync(0xffffffffu, wait_alone(bar, parity)) != 0;
+        return __all_sync(0xffffffffu, wait_alone(bar, parity, blocks)) != 0;
     };
     const uint32_t q_at = smem_address(shared), k_at = q_at + S::tiles * S::q_bytes, v_at = k_at + S::stages * S::k_bytes;
 
@@ -425,7 +434,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         // one that follows the barriers' phases.)
         if (ragged >= 0) {
             const int s = ragged % S::stages;
-            if (wait(&ragged_there, 0)) {
+            if (wait(&ragged_there, 0, most + 1)) {
                 const int real = (int)(keys - (begin + ragged) * S::block), rows = S::block - real;
                 for (int slab = 0; slab < S::parts * S::slabs; ++slab) {
                     uint4* row = reinterpret_cast<uint4*>(shared + (v_at - q_at) + s * S::k_bytes + slab * (S::block * 128) + real * 128);
@@ -601,7 +610,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                 *reinterpret_cast<uint4*>(out) = a;
             }
         };
-        if (pieced && pieces > 1 && S::tiles == 2 && fine && counts[1 - t] > 0) fine = wait(&context_full[1 - t], 0);  // (shared memory is free then)
+        if (pieced && pieces > 1 && S::tiles == 2 && fine && counts[1 - t] > 0) fine = wait(&context_full[1 - t], 0, most + 1);  // (shared memory is free then)
         if (fine) {
             float4* fours = reinterpret_cast<float4*>(shared) + t * (S::tile_floats / 4) + (warp % 4) * 32 + lane;
             if (count > 0) add_block();

@@ -262,3 +262,73 @@ def test_a_stride_that_no_tensor_map_has_is_refused():
     for strides in ((2 ** 40, 64, 64), (64, 2 ** 36, 64), (64, 64, 2 ** 62)):
         assert ctx._lib.psx_b200_prompt_attention(ctx._ctx, None, 1, x.data_ptr(), x.data_ptr(), x.data_ptr(), x.data_ptr(), 1, 1, *strides, at.data_ptr(),
                                                   at.data_ptr(), 1, 1, 1, 64, 1.0, 1, 0, None) == psx.ERR_UNSUPPORTED
+
+
+# Few groups of rows: clusters of CTAs share their keys.  (A piece's factor is one more exponential, 2^-22, and its sums one more rounding:
+# within the 2^-21 and the eight roundings of the slack.)
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,head_dim", [([16], [16000], 4, 2, 64), ([1], [5000], 1, 1, 128), ([300, 7], [4000, 900], 3, 1, 96),
+                                                                   ([1], [640], 1, 1, 8), ([1], [641], 2, 1, 128), ([2000], [500], 1, 1, 64)])
+def test_keys_shared_out(dtype, q_lens, k_lens, heads, kv_heads, head_dim):
+    _check(dtype, q_lens, k_lens, heads, kv_heads, head_dim, lead=2, behind=90)
+    _check(dtype, q_lens, k_lens, heads, kv_heads, head_dim, causal=False, scale=-0.2)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("heads", [18, 21, 24, 29, 37, 49, 74, 75])
+def test_every_number_of_pieces(dtype, heads):
+    _check(dtype, [40], [1500], heads, 1, 64)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("window", [1, 64, 700, 1300])
+def test_windows_of_keys_shared_out(dtype, window):
+    _check(dtype, [600, 130], [3000, 1700], 2, 1, 64, window=window)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_prompts_whose_keys_are_not_shared_out(dtype):
+    _check(dtype, [1500, 700], [1500, 1100], 16, 4, 128)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_nan_among_keys_shared_out(dtype):
+    import torch
+    q, k = (torch.randn(n, 2, 64, device="cuda").to(getattr(torch, dtype)) for n in (300, 2000))
+    q_at, k_at = torch.tensor([0, 300], device="cuda"), torch.tensor([0, 2000], device="cuda")
+    want = gh.ctx().prompt_attention(q, k, k, q_at, k_at)[0]
+    bad = k.clone()
+    bad[1850] = float("nan")   # query 150 and those behind it see the key
+    got, status = gh.ctx().prompt_attention(q, bad, k, q_at, k_at)
+    assert int(status) == 0 and got[150:].isnan().all() and (got[:150] == want[:150]).all()
+
+
+def test_a_captured_call_whose_keys_are_shared_out():
+    import torch
+    ctx = psx.Context(0)
+    q, k = (torch.randn(n, 2, 128, device="cuda").bfloat16() for n in (200, 4000))
+    q_at, k_at = torch.tensor([0, 200], device="cuda"), torch.tensor([0, 4000], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):   # (no scratch: nothing has to be called before)
+        got, status = ctx.prompt_attention(q, k, k, q_at, k_at)
+    for lens in ((200, 4000), (200, 700), (130, 130), (0, 0)):
+        q_at[1], k_at[1] = lens
+        q.normal_()
+        graph.replay()
+        want = ctx.prompt_attention(q, k, k, q_at, k_at)[0]
+        torch.cuda.synchronize()
+        assert int(status) == 0 and (got[:lens[0]] == want[:lens[0]]).all() and not want[:lens[0]].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_the_limit_of_a_wait_is_that_of_a_block(dtype):
+    import torch
+    ctx = psx.Context(0)
+    q, k = (torch.randn(n, 1, 64, device="cuda").to(getattr(torch, dtype)) for n in (1, 400_001))
+    at = torch.tensor([0, 1], device="cuda"), torch.tensor([0, 400_001], device="cuda")
+    want = ctx.prompt_attention(q, k, k, *at)[0]
+    torch.cuda.synchronize()
+    ctx.set_wait_limit(150_000)   # the keys' last block comes some 400 microseconds after the first
+    got, status = ctx.prompt_attention(q, k, k, *at)
+    assert int(status) == 0 and (got == want).all()
