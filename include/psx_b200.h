@@ -415,7 +415,7 @@ PSX_API psx_status psx_b200_store_cache_8bit(psx_ctx* ctx, void* stream, const p
  * p = lengths[b] - q_len + i: with `causal` it sees no key j > p and, with window > 0, no key j + window <= p.  A query that sees
  * nothing has the context 0.  Positions that no query of a row sees are not read.  Softmax statistics and sums are floats; codes
  * are exact in the products, queries and weights carry 11 bits (bf16, fp16) or 22 (fp32).
- * Limits: (heads / kv_heads) * q_len <= 16, <= 8 where head_dim > 128 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; scratch
+ * Limit: (heads / kv_heads) * q_len <= 16 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; scratch
  * in a stream capture as psx_b200_beam_select. */
 PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, const void* q, int32_t dtype, const psx_cache_8bit* cache,
                                                   const int64_t* lengths, void* context, int64_t heads, int64_t q_len, float scale,

@@ -1311,11 +1311,10 @@ psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const 
     if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
     if (heads <= 0 || q_len <= 0 || window < 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: attention sizes must be positive");
     if (heads % cache->kv_heads != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: heads must be a multiple of kv_heads");
-    const int64_t group = heads / cache->kv_heads, most = cache->head_dim > 128 ? 8 : 16;
-    if (group > most || q_len > most || group * q_len > most) {
+    const int64_t group = heads / cache->kv_heads;
+    if (group > 16 || q_len > 16 || group * q_len > 16) {
         return fail(PSX_ERR_UNSUPPORTED,
-                    "psx_b200: attention over the cache in 8 bits takes at most 16 query rows per kv head (group x new positions), 8 beyond a "
-                    "head dimension of 128");
+                    "psx_b200: attention over the cache in 8 bits takes at most 16 query rows per kv head (group x new positions)");
     }
     if (p.cache.batch == 0) return PSX_OK;
     if (!q || !lengths || !context) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
@@ -1331,7 +1330,7 @@ psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const 
     psx::plan_attention_8bit(p, ctx->sm_count);
     if (p.pieces > 1) {
         if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;
-        if (psx_status s = reserve_counters(ctx, stream, ctx->attention_8bit_arrived, (size_t)(cache->batch * cache->kv_heads))) return s;
+        if (psx_status s = reserve_counters(ctx, stream, ctx->attention_8bit_arrived, (size_t)psx::attention_8bit_counters(p))) return s;
         p.partial = static_cast<float*>(ctx->attention_8bit_pieces.ptr);
         p.arrived = static_cast<int32_t*>(ctx->attention_8bit_arrived.ptr);
     }

@@ -127,17 +127,19 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
     const uint32_t stages_at = shared_address(stages);
     const int shift = 31 - __clz(c.block);
 
-    // This block's pair, and its tiles of the pair's.
-    const int64_t pair = blockIdx.x / (unsigned)p.pieces;
+    // This block's pair (its query rows from first_row on, eight at a time beyond 128 dimensions), and its tiles of the pair's.
+    const int64_t unit = blockIdx.x / (unsigned)p.pieces, pair = dims == 256 ? unit / p.row_groups : unit;
+    const int first_row = dims == 256 ? (int)(unit % p.row_groups) * kRows : 0, rows = dims == 256 ? min(p.rows - first_row, kRows) : p.rows;
     const int number = (int)(blockIdx.x % (unsigned)p.pieces), row = (int)(pair / c.kv_heads), head = (int)(pair % c.kv_heads);
     const Sight sight = sight_of(p, row);
     const int tiles = max(sight.end_tile() - sight.first_tile(), 0);
     const int share = max(max(kWarps, (tiles + p.pieces - 1) / p.pieces), min((tiles + p.spread - 1) / p.spread, kMostShare));
     const int from_tile = number * share, to_tile = min(tiles, from_tile + share);
-    T* context = static_cast<T*>(p.context) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+    const int64_t first_element = (((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len + first_row) * head_dim;
+    T* context = static_cast<T*>(p.context) + first_element;
     if (from_tile >= to_tile) {
         if (tiles == 0 && number == 0) {  // a row that sees nothing
-            for (int i = threadIdx.x; i < p.rows * head_dim; i += kThreads) context[i] = from_float<T>(0.0f);
+            for (int i = threadIdx.x; i < rows * head_dim; i += kThreads) context[i] = from_float<T>(0.0f);
         }
         return;
     }
@@ -191,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
     // The query rows as the right-hand operand: lane (gid, tig) holds row gid's dimensions 16 tig .. 16 tig + 15 of every 64.
     uint32_t qh[tiles_of_rows][kSegments][4][2], ql[precise ? tiles_of_rows : 1][precise ? kSegments : 1][4][2];
     float row_scale[tiles_of_rows][2];  // of the score rows that this lane holds: rows 2 tig and 2 tig + 1
-    const T* q = static_cast<const T*>(p.q) + ((int64_t)row * p.heads + (int64_t)head * p.group) * p.q_len * head_dim;
+    const T* q = static_cast<const T*>(p.q) + first_element;
 #pragma unroll
     for (int n = 0; n < tiles_of_rows; ++n) {
         const int r = n * 8 + gid;
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
             for (int i = 0; i < 16; i += 4) {
                 const int d = s * 64 + tig * 16 + i;
                 float4 four = make_float4(0, 0, 0, 0);
-                if (r < p.rows && d < head_dim) four = load_four(q + (int64_t)r * head_dim + d);
+                if (r < rows && d < head_dim) four = load_four(q + (int64_t)r * head_dim + d);
                 x[s][i] = four.x, x[s][i + 1] = four.y, x[s][i + 2] = four.z, x[s][i + 3] = four.w;
                 largest = fmaxf(largest, fmaxf(fmaxf(fabsf(four.x), fabsf(four.y)), fmaxf(fabsf(four.z), fabsf(four.w))));
             }
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
             for (int n = 0; n < tiles_of_rows; ++n) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int own = (n * 8 + 2 * tig + i) % p.q_len;
+                    const int own = (first_row + n * 8 + 2 * tig + i) % p.q_len;
                     const int first = sight.first(own), last = sight.last(own, p.causal != 0);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
     const int piece_floats = kRows * (dims + 4);  // (a row's context, its maximum and sum, two unused)
     const int fours = head_dim / 4;
     float* piece = p.partial + (int64_t)blockIdx.x * piece_floats;
-    for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
+    for (int i = threadIdx.x; i < rows * fours; i += kThreads) {
         const int r = i / fours, d = i % fours * 4;
         float high = kNone, sum = 0.0f;
         float4 value = make_float4(0, 0, 0, 0);
@@ -447,17 +449,17 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         __syncthreads();
         if (threadIdx.x == 0) {  // (release: the block's pieces, ordered before by the barrier; acquire: the other blocks')
             int before;
-            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + pair) : "memory");
+            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + unit) : "memory");
             is_last = before == pieces - 1;
-            if (is_last) p.arrived[pair] = 0;
+            if (is_last) p.arrived[unit] = 0;
         }
         __syncthreads();
         if (is_last) {
-            const auto piece_of = [&](int b) { return p.partial + (pair * p.pieces + b) * piece_floats; };
+            const auto piece_of = [&](int b) { return p.partial + (unit * p.pieces + b) * piece_floats; };
             // A thread's part of the first pieces' contexts is asked for along with their maxima and sums.
             constexpr int kAhead = 8;
             const int mine_row = threadIdx.x / fours, mine_d = threadIdx.x % fours * 4;
-            const bool mine_real = mine_row < p.rows;
+            const bool mine_real = mine_row < rows;
             float4 ahead[kAhead];
 #pragma unroll
             for (int b = 0; b < kAhead; ++b) {
@@ -465,19 +467,19 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
                 if (b < pieces && mine_real) ahead[b] = __ldcg(reinterpret_cast<const float4*>(piece_of(b) + mine_row * (dims + 4) + mine_d));
             }
             float2* less = reinterpret_cast<float2*>(shared);  // (piece, row): maximum and sum, then what the piece counts for
-            for (int i = threadIdx.x; i < pieces * p.rows; i += kThreads) {
-                less[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(i / p.rows) + i % p.rows * (dims + 4) + dims));
+            for (int i = threadIdx.x; i < pieces * rows; i += kThreads) {
+                less[i] = __ldcg(reinterpret_cast<const float2*>(piece_of(i / rows) + i % rows * (dims + 4) + dims));
             }
             __syncthreads();
-            for (int r = warp; r < p.rows; r += kWarps) {
+            for (int r = warp; r < rows; r += kWarps) {
                 float high = kNone, sum = 0.0f;
-                for (int b = lane; b < pieces; b += 32) high = fmaxf(high, less[b * p.rows + r].x);
+                for (int b = lane; b < pieces; b += 32) high = fmaxf(high, less[b * rows + r].x);
 #pragma unroll
                 for (int step = 16; step > 0; step /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, step));
                 for (int b = lane; b < pieces; b += 32) {
-                    const float2 mine = less[b * p.rows + r];
+                    const float2 mine = less[b * rows + r];
                     const float factor = mine.x > kNone ? exp2_approx(mine.x - high) : 0.0f;
-                    less[b * p.rows + r].x = factor;
+                    less[b * rows + r].x = factor;
                     sum += factor * mine.y;
                 }
 #pragma unroll
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
                 if (lane == 0) totals[0][r] = sum;
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < p.rows * fours; i += kThreads) {
+            for (int i = threadIdx.x; i < rows * fours; i += kThreads) {
                 const int r = i / fours, d = i % fours * 4;
                 float4 value = make_float4(0, 0, 0, 0);
                 const auto add = [&](const float4& part, float factor) {
@@ -495,11 +497,11 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
                 if (i == threadIdx.x) {
 #pragma unroll
                     for (; b < kAhead; ++b) {
-                        if (b < pieces) add(ahead[b], less[b * p.rows + r].x);
+                        if (b < pieces) add(ahead[b], less[b * rows + r].x);
                     }
                 }
 #pragma unroll 8
-                for (; b < pieces; ++b) add(__ldcg(reinterpret_cast<const float4*>(piece_of(b) + r * (dims + 4) + d)), less[b * p.rows + r].x);
+                for (; b < pieces; ++b) add(__ldcg(reinterpret_cast<const float4*>(piece_of(b) + r * (dims + 4) + d)), less[b * rows + r].x);
                 store_four(context + r * head_dim + d, value, totals[0][r] == 0.0f ? 0.0f : 1.0f / totals[0][r]);
             }
         }
@@ -516,7 +518,7 @@ cudaError_t launch(const Attention8bitParams& p, cudaStream_t stream) {
         return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_of(dims));
     });
     if (e != cudaSuccess) return e;
-    kernel<<<(unsigned)(p.cache.batch * p.cache.kv_heads * p.pieces), kThreads, shared_of(dims), stream>>>(p);
+    kernel<<<(unsigned)(p.cache.batch * p.cache.kv_heads * p.row_groups * p.pieces), kThreads, shared_of(dims), stream>>>(p);
     return cudaGetLastError();
 }
 
@@ -530,28 +532,33 @@ cudaError_t launch_type(const Attention8bitParams& p, cudaStream_t stream) {
 
 int padded_dims(const Attention8bitParams& p) { return p.cache.head_dim > 128 ? 256 : p.cache.head_dim > 64 ? 128 : 64; }
 
+// Query rows of a block's kernel.
+int rows_of_block(const Attention8bitParams& p) { return p.rows <= 8 || padded_dims(p) == 256 ? 8 : 16; }
+
 }  // namespace
 
 void plan_attention_8bit(Attention8bitParams& p, int sm_count) {
     const int dims = padded_dims(p);
-    const int64_t tiles = (p.cache.max_len + kTile - 1) / kTile, pairs = p.cache.batch * p.cache.kv_heads;
+    p.row_groups = dims == 256 ? (p.rows + 7) / 8 : 1;  // (more rows' contexts do not fit the registers; the cache comes out of L2 the second time)
+    const int64_t tiles = (p.cache.max_len + kTile - 1) / kTile, units = p.cache.batch * p.cache.kv_heads * p.row_groups;
     // Blocks that the GPU holds at once, by registers and shared memory.
     const int64_t blocks = (int64_t)sm_count * (dims == 256 ? 1 : dims == 64 ? 4 : p.rows > 8 ? 2 : 3);
     // The pieces of a pair have their maxima and sums in shared memory when they are joined.
-    const int64_t most = std::min<int64_t>((tiles + kWarps - 1) / kWarps, shared_of(dims) / (p.rows * sizeof(float2)));
-    const int64_t spread = std::max<int64_t>(1, blocks / pairs);
-    const int64_t balanced = std::min((tiles + kMostShare - 1) / kMostShare, 8 * blocks / pairs);  // (blocks that find nothing to do cost time too)
+    const int64_t most = std::min<int64_t>((tiles + kWarps - 1) / kWarps, shared_of(dims) / (rows_of_block(p) * sizeof(float2)));
+    const int64_t spread = std::max<int64_t>(1, blocks / units);
+    const int64_t balanced = std::min((tiles + kMostShare - 1) / kMostShare, 8 * blocks / units);  // (blocks that find nothing to do cost time too)
     p.spread = (int)std::min(spread, most);
     p.pieces = (int)std::min(std::max(spread, balanced), most);
 }
 
+int64_t attention_8bit_counters(const Attention8bitParams& p) { return p.cache.batch * p.cache.kv_heads * p.row_groups; }
+
 size_t attention_8bit_partial_bytes(const Attention8bitParams& p) {
-    const int rows = p.rows <= 8 ? 8 : 16;
-    return (size_t)(p.cache.batch * p.cache.kv_heads * p.pieces) * rows * (padded_dims(p) + 4) * sizeof(float);
+    return (size_t)(attention_8bit_counters(p) * p.pieces) * rows_of_block(p) * (padded_dims(p) + 4) * sizeof(float);
 }
 
 cudaError_t launch_decode_attention_8bit(const Attention8bitParams& p, cudaStream_t stream) {
-    if (p.rows > 16 || p.cache.head_dim > 256 || (p.cache.head_dim > 128 && p.rows > 8)) return cudaErrorInvalidValue;
+    if (p.rows > 16 || p.cache.head_dim > 256) return cudaErrorInvalidValue;
     if (p.type == kFloat32) return launch_type<float>(p, stream);
     if (p.type == kBfloat16) return launch_type<__nv_bfloat16>(p, stream);
     return launch_type<__half>(p, stream);

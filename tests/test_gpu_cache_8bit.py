@@ -322,7 +322,7 @@ def test_refusals():
         return ctx.decode_attention_8bit(_tensor(np.zeros((2, heads, q_len, cache.head_dim)), dtype), cache, lengths, **kw)
 
     for status, call in ((psx.ERR_BAD_ARGUMENT, lambda: decode(3, 1)), (psx.ERR_UNSUPPORTED, lambda: decode(34, 1)), (psx.ERR_UNSUPPORTED, lambda: decode(4, 9)),
-                         (psx.ERR_BAD_ARGUMENT, lambda: decode(4, 1, window=-1)), (psx.ERR_UNSUPPORTED, lambda: decode(18, 1, psx.Cache8bit.empty(2, 2, 64, 144, 32))),
+                         (psx.ERR_BAD_ARGUMENT, lambda: decode(4, 1, window=-1)), (psx.ERR_UNSUPPORTED, lambda: decode(34, 1, psx.Cache8bit.empty(2, 2, 64, 144, 32))),
                          (psx.ERR_UNSUPPORTED, lambda: decode(2, 1, psx.Cache8bit.empty(2, 2, 64, 40, 32))), (psx.ERR_UNSUPPORTED, lambda: decode(2, 1, psx.Cache8bit.empty(2, 2, 64, 64, 8))),
                          (psx.ERR_UNSUPPORTED, lambda: decode(2, 1, psx.Cache8bit.empty(2, 2, 64, 272, 32)))):
         with pytest.raises(psx.PsxError) as e:
@@ -347,3 +347,11 @@ def test_refusals():
     with pytest.raises(psx.PsxError) as e:
         ctx.decode_attention_8bit(torch.zeros(4097, 1, 1, 16, device="cuda"), too_many, torch.ones(4097, dtype=torch.int64, device="cuda"))
     assert e.value.status == psx.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("heads,kv_heads,q_len,head_dim", [(16, 2, 2, 256), (9, 1, 1, 144), (16, 1, 1, 256), (2, 2, 11, 208), (6, 2, 5, 176)])
+def test_more_than_eight_query_rows_beyond_128_dimensions(dtype, heads, kv_heads, q_len, head_dim):
+    _check(dtype, 7, heads, kv_heads, q_len, head_dim, 1500, [1500, 1, 16, 33, 0, 640, 5], block=32)
+    _check(dtype, 2, heads, kv_heads, q_len, head_dim, 90, [90, 70], block=16, window=9, causal=True)
+    _check(dtype, 100, heads, kv_heads, q_len, head_dim, 40, [40 - i % 37 for i in range(100)], block=64, causal=False)
