@@ -1351,7 +1351,7 @@ psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dty
     if (heads % kv_heads != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: heads must be a multiple of kv_heads");
     if (!std::isfinite(scale)) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the score scale must be finite");
     if (head_dim % 8 != 0 || head_dim > 128 || batch > psx::kMostPrefixRows || total_q > (1 << 29) || total_k > (1 << 29) || heads > 65536 ||
-        (total_q / 128 + batch) * heads > 0x7fffffff) {
+        (total_q / 64 + batch) * heads > 0x7fffffff) {
         return fail(PSX_ERR_UNSUPPORTED,
                     "psx_b200: attention of prompts takes a head dimension that is a multiple of 8 up to 128, at most 4096 sequences and 2^29 positions");
     }

@@ -1,7 +1,7 @@
 // Attention of whole prompts, packed one behind the other: per sequence and head softmax(scale q k^T, masked) v, on the
 // fifth-generation tensor cores, without the scores in memory.
 //
-// A CTA takes one or two tiles of 128 queries of one (sequence, head) and goes through the keys that they see in blocks.  One thread
+// A CTA takes one or two tiles of 128 rows, queries of a sequence and of the heads that share a kv head, and goes through the keys that they see in blocks.  One thread
 // asks for copies (tiled, 128-byte swizzle), one issues the products, and a warpgroup per tile turns scores into weights, a
 // thread per query: it loads its row of scores from tensor memory, keeps the running maximum and sum in registers (no
 // exchange between threads), and writes the weights back to tensor memory, in the place of the scores, from where they are the left
@@ -84,6 +84,7 @@ struct alignas(64) PromptLaunch {
     PromptAttentionParams p;
     int32_t steps;  // of 16 dimensions
     int32_t pieces;  // CTAs of a cluster
+    int32_t packed, positions;  // heads, and positions, of a tile's rows
     int32_t dims16;  // the head dimension, rounded up to 16
 };
 
@@ -176,25 +177,26 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     constexpr int kCopyWarp = S::tiles * 4, kIssueWarp = kCopyWarp + 1, kTailWarp = kCopyWarp + 2;
     constexpr int kRows = S::tiles * kTileRows;
+    const int positions = S::tiles * launch.positions;  // of a CTA
 
     const auto queries_of = [&](int b) { return max(min(p.q_offsets[b + 1], p.total_q) - max(p.q_offsets[b], (int64_t)0), (int64_t)0); };
-    sum_of_rows(p.batch, prefix, carry, [&](int b) { return (int)((queries_of(b) + kRows - 1) / kRows); });
+    sum_of_rows(p.batch, prefix, carry, [&](int b) { return (int)((queries_of(b) + positions - 1) / positions); });
     const int item = pieced ? blockIdx.x / launch.pieces : blockIdx.x, number = pieced ? blockIdx.x % launch.pieces : 0;
-    const int group_of_rows = item / p.heads, head = item % p.heads;
+    const int units = p.heads / launch.packed, group_of_rows = item / units, head0 = item % units * launch.packed;
     if (group_of_rows >= prefix[p.batch]) return;
     const int b = row_of_item(prefix, p.batch, group_of_rows);
     const int64_t queries = queries_of(b), q_begin = max(p.q_offsets[b], (int64_t)0), k_begin = max(p.k_offsets[b], (int64_t)0);
     const int64_t keys = max(min(p.k_offsets[b + 1], p.total_k) - k_begin, (int64_t)0);
     const Sight sight{keys, keys - queries, p.window, p.causal != 0};
     // The last queries see the most keys: they come first, so that the short work is left for the end.
-    const int64_t row0 = (int64_t)(prefix[b + 1] - 1 - group_of_rows) * kRows;
+    const int64_t row0 = (int64_t)(prefix[b + 1] - 1 - group_of_rows) * positions;  // (in positions)
     if (row0 < 0 || row0 >= queries) return;  // (offsets that make no sense)
     int64_t ends[S::tiles];
     int64_t begin = sight.first(row0) / S::block;  // blocks of keys, for all tiles
     int counts[S::tiles], most = 0;
 #pragma unroll
     for (int t = 0; t < S::tiles; ++t) {
-        const int64_t first_row = row0 + t * kTileRows, last_row = min(first_row + kTileRows, queries) - 1;
+        const int64_t first_row = row0 + t * launch.positions, last_row = min(first_row + launch.positions, queries) - 1;
         ends[t] = last_row < first_row ? 0 : max(sight.end(last_row), (int64_t)0);
         counts[t] = (int)max((ends[t] + S::block - 1) / S::block - begin, (int64_t)0);
         most = max(most, counts[t]);
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     if (warp == kCopyWarp) {
         few_registers();
         if (lane == 0 && most > 0) {
-            const int kv_head = head / (p.heads / p.kv_heads);
+            const int kv_head = head0 / (p.heads / p.kv_heads);
             const auto fetch = [&](uint32_t to, int rows, const CUtensorMap* map, int y, int64_t z, int64_t total, uint64_t* bar) {
                 for (int part = 0; part < S::parts; ++part) {
                     for (int slab = 0; slab < S::slabs; ++slab) {
@@ -277,10 +279,10 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             const uint32_t filled = (uint32_t)min(S::slabs, (p.head_dim + 63) / 64) * 128 * S::parts;  // bytes per row that arrive
             if constexpr (S::parts == 1) {
                 uint32_t q_bytes = 0;
-                for (int t = 0; t < S::tiles; ++t) q_bytes += counts[t] > 0 ? kTileRows * filled : 0;
+                for (int t = 0; t < S::tiles; ++t) q_bytes += counts[t] > 0 ? launch.positions * launch.packed * filled : 0;
                 barrier_expect_bytes(&q_full, q_bytes);
                 for (int t = 0; t < S::tiles; ++t) {
-                    if (counts[t] > 0) fetch(q_at + t * S::q_bytes, kTileRows, &launch.q_map, head, q_begin + row0 + t * kTileRows, p.total_q, &q_full);
+                    if (counts[t] > 0) fetch(q_at + t * S::q_bytes, kTileRows, &launch.q_map, head0, q_begin + row0 + t * launch.positions, p.total_q, &q_full);
                 }
             }
             int asked = 0;
@@ -448,12 +450,18 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
     } else if (warp < S::tiles * 4) {
         many_registers();
         const int t = warp / 4;
-        const int64_t row = row0 + t * kTileRows + (warp % 4) * 32 + lane;  // this thread's query
+        // A tile's rows: positions, and of each the packed heads.  This thread's query; whether there is one.
+        const int tile_row = (warp % 4) * 32 + lane;
+        const auto row_of = [&](int tile, int r) { return row0 + tile * launch.positions + r / launch.packed; };
+        const auto is_row = [&](int r, int64_t its) { return r < launch.positions * launch.packed && its < queries; };
+        const int64_t row = row_of(t, tile_row);
+        const int head = head0 + tile_row % launch.packed;
+        const bool real = is_row(tile_row, row);
         const uint32_t lanes = tensor + ((uint32_t)(warp % 4) << 21);        // (32 lanes further: bits 16 up)
         const uint32_t context_at = lanes + S::context_at + t * S::dims;
         const int64_t end = sight.end(row), first = sight.first(row);
         // What all queries of the warp see needs no mask.
-        const int64_t warp_row = row - lane, all_end = sight.end(warp_row), all_first = sight.first(min(warp_row + 31, max(queries - 1, (int64_t)0)));
+        const int64_t all_end = sight.end(row_of(t, tile_row - lane)), all_first = sight.first(min(row_of(t, tile_row - lane + 31), max(queries - 1, (int64_t)0)));
         const int count = counts[t];
         const float scale = p.scale * kLog2e;
         const float factor = fabsf(scale) < 1e-37f ? copysignf(1e-37f, scale) : scale;  // (masked scores times it stay infinite)
@@ -492,7 +500,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
                         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (row < queries && i + k < p.head_dim) x = __ldg(reinterpret_cast<const float4*>(q + i + k));
+                        if (real && i + k < p.head_dim) x = __ldg(reinterpret_cast<const float4*>(q + i + k));
                         split_pair(x.x, x.y, packed[0][k / 2], packed[1][k / 2], packed[2][k / 2]);
                         split_pair(x.z, x.w, packed[0][k / 2 + 1], packed[1][k / 2 + 1], packed[2][k / 2 + 1]);
                     }
@@ -594,9 +602,9 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             tensor_fence_after();
         }
         // Eight dimensions of a row's context, times what makes its weights add up to one.
-        const auto put = [&](int64_t to, int d, const float* o, float sum) {
+        const auto put = [&](int64_t to, int of_head, int d, const float* o, float sum) {
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-            Out* out = static_cast<Out*>(p.out) + ((q_begin + to) * p.heads + head) * p.head_dim + d;
+            Out* out = static_cast<Out*>(p.out) + ((q_begin + to) * p.heads + of_head) * p.head_dim + d;
             if constexpr (sizeof(Out) == 4) {
                 float4 a = make_float4(o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse);
                 float4 c = make_float4(o[4] * inverse, o[5] * inverse, o[6] * inverse, o[7] * inverse);
@@ -626,11 +634,11 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                     tensor_loads_done();
                 }
                 if (!pieced || pieces == 1) {
-                    if (row < queries) {
+                    if (real) {
 #pragma unroll
                         for (int k = 0; k < 32; k += 8) {
                             if (i + k >= p.head_dim) break;
-                            put(row, i + k, o + k, total);
+                            put(row, head, i + k, o + k, total);
                         }
                     }
                 } else if (count > 0) {
@@ -646,8 +654,9 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             // Every CTA joins its share of the rows, out of all pieces' shared memory.  (Every warp comes here, whatever its waits have come to.)
             cluster_meets();
             const int rows = (kRows + pieces - 1) / pieces, parts = (S::tiles * 128) / rows, mine = threadIdx.x % rows, joined = number * rows + mine;
-            if (joined < kRows && row0 + joined < queries && (int)threadIdx.x / rows < parts) {
-                const int tile = joined / kTileRows, of_tile = joined % kTileRows;
+            const int tile = joined / kTileRows, of_tile = joined % kTileRows;
+            const int64_t to = row_of(tile, of_tile);
+            if (joined < kRows && is_row(of_tile, to) && (int)threadIdx.x / rows < parts) {
                 float less[kMostPieces], sum = 0.0f, high = masked;  // what a piece counts for; negative: it has nothing
                 float2 ends_at[kMostPieces];
 #pragma unroll
@@ -673,7 +682,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                         o[0] += x.x * less[b], o[1] += x.y * less[b], o[2] += x.z * less[b], o[3] += x.w * less[b];
                         o[4] += y.x * less[b], o[5] += y.y * less[b], o[6] += y.z * less[b], o[7] += y.w * less[b];
                     }
-                    put(row0 + joined, d, o, sum);
+                    put(to, head0 + of_tile % launch.packed, d, o, sum);
                 }
             }
         }
@@ -724,14 +733,36 @@ EncodeTiled encoder() {
     return found;
 }
 
-// (dimension, head, position): boxes of 64 dimensions of one head and `rows` positions.
-bool encode(CUtensorMap* map, bool bfloat, const void* at, int64_t positions, int64_t stride, int heads, int head_dim, int rows) {
+// (dimension, head, position): boxes of 64 dimensions of `packed` heads and `rows` positions.
+bool encode(CUtensorMap* map, bool bfloat, const void* at, int64_t positions, int64_t stride, int heads, int head_dim, int rows, int packed = 1) {
     const cuuint64_t sizes[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)std::max<int64_t>(positions, 1)};
     const cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)stride * 2};
-    const cuuint32_t box[3] = {64, 1, (cuuint32_t)rows}, steps[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {64, (cuuint32_t)packed, (cuuint32_t)rows}, steps[3] = {1, 1, 1};
     return encoder()(map, bfloat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(at), sizes, strides, box, steps,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Groups of rows where a tile has `packed` heads: no more than these.
+template <class S>
+int64_t groups_of_rows(const PromptAttentionParams& p, int packed) {
+    return (p.total_q / (S::tiles * (kTileRows / packed)) + p.batch) * (p.heads / packed);
+}
+
+// Heads of one kv head that a tile takes together, a divisor of them up to 16: as few as keep the CTAs to one for an SM (they are quicker with
+// few rows: one prompt of 100 positions with 8 heads on 2 takes 10.3 us by one head, 12.3 by four), else as many as there are: short
+// sequences fill the tiles then (20 of up to 28 positions behind 416, 64 heads on 8, fp32: 78 us instead of 211; five of up to 1501
+// with 16 on 4: 214 instead of 230).
+template <class S>
+int heads_packed(const PromptAttentionParams& p, int sm_count) {
+    const int group = p.heads / p.kv_heads;
+    int packed = 1;
+    for (int d = 1; d <= std::min(group, 16); ++d) {
+        if (group % d != 0) continue;
+        packed = d;
+        if (groups_of_rows<S>(p, d) <= sm_count) break;
+    }
+    return packed;
 }
 
 template <class Elem, class Out, class S>
@@ -739,7 +770,8 @@ cudaError_t launch(const PromptAttentionParams& p, int sm_count, cudaStream_t st
     constexpr bool bfloat = __is_same(Elem, __nv_bfloat16);
     // Where the groups of rows leave half of the SMs idle, clusters share the keys of each (lengths are not known here: a CTA that finds
     // nothing to do ends early).
-    const int64_t blocks = (p.total_q / (S::tiles * kTileRows) + p.batch) * p.heads;  // no more than these groups of rows
+    const int packed = heads_packed<S>(p, sm_count), positions = kTileRows / packed;
+    const int64_t blocks = groups_of_rows<S>(p, packed);
     const int pieces = (int)std::max<int64_t>(1, std::min({sm_count / blocks, p.total_k / S::block + 1, (int64_t)kMostPieces}));
     static OncePerDevice raised[2];
     const auto kernel = pieces > 1 ? prompt_attention_kernel<Elem, Out, S, true> : prompt_attention_kernel<Elem, Out, S, false>;
@@ -756,7 +788,7 @@ cudaError_t launch(const PromptAttentionParams& p, int sm_count, cudaStream_t st
     l.p = p;
     l.steps = (p.head_dim + 15) / 16;
     l.dims16 = l.steps * 16;
-    l.pieces = pieces;
+    l.pieces = pieces, l.packed = packed, l.positions = positions;
     const void *k = p.k, *v = p.v;
     int64_t k_rows = p.total_k, k_stride = p.k_stride, v_stride = p.v_stride;
     if constexpr (S::parts == 3) {
@@ -778,7 +810,7 @@ cudaError_t launch(const PromptAttentionParams& p, int sm_count, cudaStream_t st
         k_stride = v_stride = (int64_t)p.kv_heads * p.head_dim;
     }
     if (p.total_k == 0) k = v = p.q, k_stride = v_stride = (int64_t)p.kv_heads * p.head_dim;  // (never read)
-    if ((S::parts == 1 && !encode(&l.q_map, bfloat, p.q, p.total_q, p.q_stride, p.heads, p.head_dim, kTileRows)) ||
+    if ((S::parts == 1 && !encode(&l.q_map, bfloat, p.q, p.total_q, p.q_stride, p.heads, p.head_dim, positions, packed)) ||
         !encode(&l.k_map, bfloat, k, k_rows, k_stride, p.kv_heads, p.head_dim, S::block) ||
         !encode(&l.v_map, bfloat, v, k_rows, v_stride, p.kv_heads, p.head_dim, S::block)) {
         return cudaErrorInvalidValue;

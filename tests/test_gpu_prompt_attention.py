@@ -332,3 +332,14 @@ def test_the_limit_of_a_wait_is_that_of_a_block(dtype):
     ctx.set_wait_limit(150_000)   # the keys' last block comes some 400 microseconds after the first
     got, status = ctx.prompt_attention(q, k, k, *at)
     assert int(status) == 0 and (got == want).all()
+
+
+# Many groups of rows: a tile takes the heads that share a kv head together, a divisor of them up to 16.
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("heads,kv_heads", [(16, 4), (24, 8), (10, 2), (14, 2), (64, 2), (34, 2), (48, 2), (16, 1)])
+def test_heads_of_a_tile(dtype, heads, kv_heads):
+    lens = [1, 130, 33, 0, 7, 64, 65, 16, 12, 129] * 3
+    longer = [n + (37 * i) % 200 for i, n in enumerate(lens)]
+    _check(dtype, lens, lens, heads, kv_heads, 64, lead=1, behind=30)
+    _check(dtype, lens, longer, heads, kv_heads, 72, window=50)
+    _check(dtype, lens, longer[::-1], heads, kv_heads, 128, causal=False, behind=5)
