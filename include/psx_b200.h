@@ -432,8 +432,8 @@ PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, co
  * as they were.
  * Products run on the tensor cores with float accumulators.  bf16 and fp16: weights are rounded to that type; fp32: every
  * factor as three bf16 parts, so that products are exact to about 2^-24 (an infinity counts as NaN).  Keys and values of other
- * sequences, finite or not, have no influence; a NaN among a sequence's own values reaches the queries of the 128 positions
- * around it that do not see it, too.
+ * sequences, finite or not, have no influence; a NaN or infinity among a sequence's own values may reach queries of the sequence that
+ * do not see it, too, up to 384 positions from those that do.
  * All pointers 16-byte aligned, strides a multiple of 16 bytes.  Limits: head_dim a multiple of 8 up to 128, batch <= 4096, total_q
  * and total_k <= 2^29, strides < 2^36 (else PSX_ERR_UNSUPPORTED).  status (device, may be null): set to 0 by the call, to 1 if a
  * bounded device-side wait ran out (psx_b200_ctx_set_wait_limit).  Asynchronous on `stream`; fp32 takes scratch of 1.5 times the
