@@ -176,9 +176,9 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
                 }
             }
         }
-        if (lane < 4) {  // the scales of the tile's two halves, keys' then values'
+        if (lane < 4) {  // the scales of the tile's two halves, keys' then values' (of a half that no row sees, 0 too: a NaN times 0 is one)
             const int first = position + lane % 2 * 16;
-            const bool there = first < sight.length;
+            const bool there = first < sight.length && first + 16 > seen;
             copy4(to + 2 * kTile * dims + lane * 4, (lane < 2 ? key_scales : value_scales) + (there ? first >> shift : 0), there);
         }
     };

@@ -355,3 +355,26 @@ def test_more_than_eight_query_rows_beyond_128_dimensions(dtype, heads, kv_heads
     _check(dtype, 7, heads, kv_heads, q_len, head_dim, 1500, [1500, 1, 16, 33, 0, 640, 5], block=32)
     _check(dtype, 2, heads, kv_heads, q_len, head_dim, 90, [90, 70], block=16, window=9, causal=True)
     _check(dtype, 100, heads, kv_heads, q_len, head_dim, 40, [40 - i % 37 for i in range(100)], block=64, causal=False)
+
+
+# Positions that no query of a row sees are not read: neither their codes nor their scales, ahead of a window or behind the length.
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("block", [16, 32, 64])
+@pytest.mark.parametrize("head_dim,heads,q_len,window", [(64, 2, 1, 7), (128, 4, 2, 40), (96, 2, 1, 1), (256, 2, 3, 17)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_scales_and_codes_that_no_query_sees_are_not_read(dtype, block, head_dim, heads, q_len, window, what):
+    import torch
+    rng = np.random.RandomState(block + head_dim)
+    lengths = [130, 113, 200, 48, 3, 161, 0]
+    cache = _cache(rng, len(lengths), 2, 210, head_dim, block, lengths)
+    q, seen_to = _tensor(rng.randn(len(lengths), heads, q_len, head_dim), dtype), torch.tensor(lengths, device="cuda")
+    want = gh.ctx().decode_attention_8bit(q, cache, seen_to, window=window)
+    assert want.isfinite().all()
+    for row, n in enumerate(lengths):
+        seen = max(n - q_len - window + 1, 0)  # the first position that a query sees
+        for codes, scales in ((cache.key_codes, cache.key_scales), (cache.value_codes, cache.value_scales)):
+            codes[row, :, :seen].copy_(torch.full_like(codes[row, :, :seen].float(), float("nan")).to(codes.dtype))
+            scales[row, :, :seen // block] = what
+            scales[row, :, -(-n // block):] = what
+    got = gh.ctx().decode_attention_8bit(q, cache, seen_to, window=window)
+    assert (got == want).all()
