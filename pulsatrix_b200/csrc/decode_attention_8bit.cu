@@ -8,9 +8,11 @@
 // new positions, up to 16) are the narrow side, which wastes nothing at 8 rows; the codes are converted once for all of them.
 // A query row is brought to a power of two near 1 and rounded to halves (bf16 and fp16 queries lose nothing but bits below 2^-24 of
 // their largest element); an fp32 row is a half and the half that is left, two instructions each, some 22 bits.  Weights:
-// the running maximum M is taken over s_j + log2(b_j), so that w_j = exp(s_j - M) b_j is at most 1 whatever the scales; it is
-// rounded to halves (2^-11, below the rounding of a bf16 or fp16 context; for fp32 contexts again two halves).  Maxima, sums
-// and contexts are floats.
+// the running maximum M is taken over s_j + log2(b_j) - 15, so that w_j = exp(s_j - M) b_j is at most 2^15 whatever the scales; it is
+// rounded to halves (2^-11, below the rounding of a bf16 or fp16 context; for fp32 contexts again two halves).  Halves reach from
+// 65,504 down to 2^-14 with all their bits and end at 2^-24, so a weight has its 11 bits down to 2^-29 of the largest, and the 22 of two down
+// to 2^-18 (brought to 1 instead, weights below 2^-25 of the largest were lost: many of them behind one that leads by 18 nats
+// are all of a context whose first value is 0).  Maxima, sums and contexts are floats.
 //
 // A (row, kv head) pair's cached positions are cut into tiles of 32, and the tiles into pieces, a block each: as many as fill the GPU
 // once, or as pieces of 128 tiles make where that is more, which evens out rows of different lengths (64 rows x 8 kv heads of up to 8191
@@ -37,6 +39,10 @@ constexpr int kThreads = 128, kWarps = 4, kTile = 32;
 constexpr int kMostShare = 128;  // tiles that a block takes where shorter pieces only balance
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kWeightLift = 15.0f;  // the largest weight is 2^15
+// The least value scale for which that holds; below it weights are smaller, by its ratio to this.  A weight without its scale is 2^97 at most
+// then, and 2^30 of them (the longest cache) add up to a float.
+constexpr float kLeastScale = 0x1p-82f;
 
 __host__ __device__ constexpr int stages_of(int) { return 2; }
 __host__ __device__ constexpr int stage_bytes(int dims) { return 2 * kTile * dims + 16; }  // keys, values, two scales each
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         for (int half = 0; half < 2; ++half) {
             const float key_scale = scales[half];
             value_scale[half] = scales[2 + half];
-            value_log[half] = __log2f(fmaxf(value_scale[half], 0x1p-100f));
+            value_log[half] = __log2f(fmaxf(value_scale[half], kLeastScale)) - kWeightLift;
 #pragma unroll
             for (int n = 0; n < tiles_of_rows; ++n) {
 #pragma unroll

@@ -378,3 +378,56 @@ def test_scales_and_codes_that_no_query_sees_are_not_read(dtype, block, head_dim
             scales[row, :, -(-n // block):] = what
     got = gh.ctx().decode_attention_8bit(q, cache, seen_to, window=window)
     assert (got == want).all()
+
+
+def _check_by_size(got, q, cache, lengths, scale, dtype):
+    """Relative to what a context's terms add up to without their signs, not to the largest value."""
+    want, most, _ = _attention(q.double().cpu().numpy(), cache, lengths, scale, True, 0)
+    bare = psx.Cache8bit(cache.key_codes, cache.key_scales, cache.value_codes.float().abs().to(cache.value_codes.dtype), cache.value_scales, block=cache.block)
+    size, _, _ = _attention(q.double().cpu().numpy(), bare, lengths, scale, True, 0)
+    slack, step = _tolerance(dtype, most, 1.0, cache.head_dim, max(lengths))
+    error = np.abs(got.double().cpu().numpy() - want)
+    assert (error <= slack * size + step * np.abs(want)).all(), (error / size).max()
+
+
+# A first position far above the rest whose value is 0: what the rest weigh, 2^-26 each, is all that there is.  Weights are halves of at
+# most 2^15 with 11 bits down to 2^-14, 2^-29 of the largest.
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows,length,every", [(1, 8192, 8192), (1, 4000, 32), (40, 1000, 32), (300, 500, 500)])
+def test_weights_far_below_the_largest_count(dtype, rows, length, every):
+    import torch
+    rng = np.random.RandomState(length)
+    keys, values = np.zeros((rows, 1, length, 64)), _codes(rng.uniform(-300, 300, (rows, 1, length, 64)))
+    keys[:, :, :, 1] = _codes(rng.randn(rows, 1, length) * 0.5)
+    keys[:, :, ::every, 0] = 18.0                      # 18 nats above the others
+    values[:, :, ::every] = 0.0
+    blocks = -(-length // 32)
+    parts = [t for x in (keys, values) for t in (torch.from_numpy(x.astype(np.float32)).cuda().to(torch.float8_e4m3fn), torch.ones(rows, 1, blocks, device="cuda"))]
+    cache = psx.Cache8bit(*parts, block=32)
+    q = torch.zeros(rows, 2, 1, 64, device="cuda", dtype=getattr(torch, dtype))
+    q[..., :2] = 1.0
+    got = gh.ctx().decode_attention_8bit(q, cache, torch.full((rows,), length, device="cuda"), scale=1.0)
+    _check_by_size(got, q, cache, [length] * rows, 1.0, dtype)
+
+
+def test_values_of_zero_and_of_every_scale():
+    import torch
+    # blocks of zeros have the scale 2^-100, whose weights are the largest floats; blocks of 1e36 the smallest
+    rng = np.random.RandomState(2)
+    cache = _cache(rng, 2, 1, 40000, 16, 16, [40000, 40000])
+    cache.key_scales.fill_(2.0 ** -8)
+    cache.value_scales.fill_(2.0 ** -100)
+    cache.value_codes[0].copy_(torch.zeros_like(cache.value_codes[0].float()).to(cache.value_codes.dtype))
+    q = _tensor(rng.randn(2, 1, 1, 16), "float32")
+    n = torch.tensor([40000, 40000], device="cuda")
+    got = gh.ctx().decode_attention_8bit(q, cache, n)
+    assert (got[0] == 0).all()
+    # (the context has some 2^-95: values of a scale below 2^-82 have weights below 2^15, by 2^18 here, so 2^-3 at most and halves of 2^-25)
+    want, most, _ = _attention(q.double().cpu().numpy(), cache, [40000, 40000], 0.25, True, 0)
+    slack, step = _tolerance("float32", most, 448 * 2.0 ** -100, 16, 40000)
+    assert (np.abs(got[1].double().cpu().numpy() - want[1]) <= slack + 448 * 2.0 ** -122 + step * np.abs(want[1])).all()
+    cache.value_scales.fill_(2.0 ** 110)
+    got = gh.ctx().decode_attention_8bit(q, cache, n)
+    want, most, value = _attention(q.double().cpu().numpy(), cache, [40000, 40000], 0.25, True, 0)
+    slack, step = _tolerance("float32", most, value, 16, 40000)
+    assert (np.abs(got.double().cpu().numpy() - want) <= slack + step * np.abs(want)).all()
