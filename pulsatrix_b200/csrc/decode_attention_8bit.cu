@@ -6,8 +6,9 @@
 // Codes become halves exactly, so both products run as half matrix instructions (m16n8k16, float accumulators) in the
 // transposed form: 16 positions by 8 query rows, then 16 dimensions by 8 query rows.  The query rows of a kv head (group x
 // new positions, up to 16) are the narrow side, which wastes nothing at 8 rows; the codes are converted once for all of them.
-// A query row is brought to a power of two near 1 and rounded to halves (bf16 and fp16 queries lose nothing but bits below 2^-24 of
-// their largest element); an fp32 row is a half and the half that is left, two instructions each, some 22 bits.  Weights:
+// A query row is brought to between 2^14 and 2^15 and rounded to halves (bf16 and fp16 queries lose nothing but bits below 2^-38 of
+// their largest element); an fp32 row is a half and the half that is left, two instructions each: 22 bits for elements down to 2^-17 of
+// the largest, for those below 2^-39 of that.  Weights:
 // the running maximum M is taken over s_j + log2(b_j) - 15, so that w_j = exp(s_j - M) b_j is at most 2^15 whatever the scales; it is
 // rounded to halves (2^-11, below the rounding of a bf16 or fp16 context; for fp32 contexts again two halves).  Halves reach from
 // 65,504 down to 2^-14 with all their bits and end at 2^-24, so a weight has its 11 bits down to 2^-29 of the largest, and the 22 of two down
@@ -39,6 +40,7 @@ constexpr int kThreads = 128, kWarps = 4, kTile = 32;
 constexpr int kMostShare = 128;  // tiles that a block takes where shorter pieces only balance
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kQueryLift = 14;        // a query row's largest element has the exponent 14: halves end at 65,504
 constexpr float kWeightLift = 15.0f;  // the largest weight is 2^15
 // The least value scale for which that holds; below it weights are smaller, by its ratio to this.  A weight without its scale is 2^97 at most
 // then, and 2^30 of them (the longest cache) add up to a float.
@@ -218,8 +220,8 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         }
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        // 2^-e with largest = m 2^e, 1 <= m < 2 (kept where it and its inverse are normal numbers)
-        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
+        // 2^-e with largest = m 2^(14 + e), 1 <= m < 2 (kept where it and its inverse are normal numbers)
+        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100) - kQueryLift;
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
         for (int s = 0; s < kSegments; ++s) {

@@ -431,3 +431,30 @@ def test_values_of_zero_and_of_every_scale():
     want, most, value = _attention(q.double().cpu().numpy(), cache, [40000, 40000], 0.25, True, 0)
     slack, step = _tolerance("float32", most, value, 16, 40000)
     assert (np.abs(got.double().cpu().numpy() - want) <= slack + step * np.abs(want)).all()
+
+
+# Elements of a query far below its largest: the keys are 0 where that is.  Queries are brought to 2^14, so that what is left of an
+# element of 2^-17 of the largest has 22 bits in two halves, and one of 2^-28 has 11 in one.
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("ratio", [2.0 ** 10, 2.0 ** 14, 2.0 ** 17])
+@pytest.mark.parametrize("head_dim", [64, 256])
+def test_elements_of_a_query_far_below_its_largest_count(dtype, ratio, head_dim):
+    import torch
+    rng = np.random.RandomState(head_dim)
+    cache = _cache(rng, 2, 1, 300, head_dim, 32, [300, 299])
+    cache.key_scales.fill_(1.0 / 64)
+    cache.key_codes.view(torch.uint8)[..., 5] = 0
+    x = np.where(rng.rand(2, 2, 1, head_dim) < 0.5, -1.0, 1.0) * rng.uniform(1, 2, (2, 2, 1, head_dim))
+    x[..., 5] = ratio
+    q, n = _tensor(x, dtype), torch.tensor([300, 299], device="cuda")
+    got = gh.ctx().decode_attention_8bit(q, cache, n, scale=1.0)
+    plain = q.clone()
+    plain[..., 5] = 0
+    cache.value_codes.copy_(cache.value_codes.float().nan_to_num(0.0).to(cache.value_codes.dtype))
+    cache.key_codes.copy_(cache.key_codes.float().nan_to_num(0.0).to(cache.key_codes.dtype))
+    want, _, value = _attention(plain.double().cpu().numpy(), cache, [300, 299], 1.0, True, 0)
+    codes, scales = _parts(cache)
+    most = max((np.abs(codes[0][b, 0]) / 64 @ np.abs(plain.double().cpu().numpy()[b].reshape(2, -1).T)).max() for b in range(2))
+    slack, step = _tolerance(dtype, most, value, head_dim, 300)
+    error = np.abs(got.double().cpu().numpy() - want)
+    assert (error <= slack + step * np.abs(want)).all(), (error.max(), slack)
