@@ -220,8 +220,8 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         }
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        // 2^-e with largest = m 2^(14 + e), 1 <= m < 2 (kept where it and its inverse are normal numbers)
-        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100) - kQueryLift;
+        // 2^-e with largest = m 2^(14 + e), 1 <= m < 2, for every finite row (of tiny ones no more than 2^114: both powers are normal numbers)
+        const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 127) - kQueryLift;
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
         for (int s = 0; s < kSegments; ++s) {

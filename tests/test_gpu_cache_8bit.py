@@ -458,3 +458,17 @@ def test_elements_of_a_query_far_below_its_largest_count(dtype, ratio, head_dim)
     slack, step = _tolerance(dtype, most, value, head_dim, 300)
     error = np.abs(got.double().cpu().numpy() - want)
     assert (error <= slack + step * np.abs(want)).all(), (error.max(), slack)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("exponent", [100, 115, 119, 125])
+def test_large_queries_over_small_keys(dtype, exponent):
+    import torch
+    rng = np.random.RandomState(exponent)
+    cache = _cache(rng, 2, 1, 200, 64, 32, [200, 200])
+    cache.key_scales.fill_(2.0 ** -100)
+    q, scale = _tensor(np.clip(rng.randn(2, 2, 1, 64), -3.9, 3.9) * 2.0 ** exponent, dtype), 2.0 ** (92 - exponent)
+    got = gh.ctx().decode_attention_8bit(q, cache, torch.tensor([200, 200], device="cuda"), scale=scale)
+    want, most, value = _attention(q.double().cpu().numpy(), cache, [200, 200], scale, True, 0)
+    slack, step = _tolerance(dtype, most, value, 64, 200)
+    assert (np.abs(got.double().cpu().numpy() - want) <= slack + step * np.abs(want)).all()
