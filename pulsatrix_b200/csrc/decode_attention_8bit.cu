@@ -427,6 +427,12 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
         }
     }
     __syncthreads();
+    // What makes a row's weights add up to one.  A sum of 0: the row sees nothing, or (as in any softmax, NaN) scores of -inf alone.
+    const auto inverse_of = [&](int r, float sum) {
+        if (sum != 0.0f) return 1.0f / sum;
+        const int own = (first_row + r) % p.q_len;
+        return sight.last(own, p.causal != 0) < max(sight.first(own), 0) ? 0.0f : __int_as_float(0x7fffffff);
+    };
     const bool whole = from_tile == 0 && to_tile == tiles;
     const int piece_floats = kRows * (dims + 4);  // (a row's context, its maximum and sum, two unused)
     const int fours = head_dim / 4;
@@ -446,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
             value.x += part.x * less, value.y += part.y * less, value.z += part.z * less, value.w += part.w * less;
         }
         if (whole) {
-            store_four(context + r * head_dim + d, value, sum == 0.0f ? 0.0f : 1.0f / sum);
+            store_four(context + r * head_dim + d, value, inverse_of(r, sum));
         } else {
             __stcg(reinterpret_cast<float4*>(piece + r * (dims + 4) + d), value);
             if (d == 0) __stcg(reinterpret_cast<float2*>(piece + r * (dims + 4) + dims), make_float2(high, sum));
@@ -510,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
                 }
 #pragma unroll 8
                 for (; b < pieces; ++b) add(__ldcg(reinterpret_cast<const float4*>(piece_of(b) + r * (dims + 4) + d)), less[b * rows + r].x);
-                store_four(context + r * head_dim + d, value, totals[0][r] == 0.0f ? 0.0f : 1.0f / totals[0][r]);
+                store_four(context + r * head_dim + d, value, inverse_of(r, totals[0][r]));
             }
         }
     }

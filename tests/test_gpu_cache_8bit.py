@@ -472,3 +472,17 @@ def test_large_queries_over_small_keys(dtype, exponent):
     want, most, value = _attention(q.double().cpu().numpy(), cache, [200, 200], scale, True, 0)
     slack, step = _tolerance(dtype, most, value, 64, 200)
     assert (np.abs(got.double().cpu().numpy() - want) <= slack + step * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("length", [1, 40, 3000])
+def test_scores_that_are_all_minus_infinity_are_not_an_empty_row(length):
+    import torch
+    # an infinite query against keys of the other sign: softmax of nothing but -inf is NaN; a query that sees nothing has the context 0
+    rng = np.random.RandomState(length)
+    cache = _cache(rng, 3, 1, length, 64, 16, [length] * 3)
+    cache.key_codes[..., 3] = cache.key_codes[..., 3].float().abs().clamp(min=1.0).neg().to(cache.key_codes.dtype)
+    q = torch.zeros(3, 1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    q[1, 0, 1, 3] = float("inf")
+    got = gh.ctx().decode_attention_8bit(q, cache, torch.tensor([length, length, 0], device="cuda"))
+    assert got[1, 0, 1].isnan().all() and got[0].isfinite().all() and (got[2] == 0).all()
+    assert got[1, 0, 0].isfinite().all() and (length > 1 or (got[1, 0, 0] == 0).all())
