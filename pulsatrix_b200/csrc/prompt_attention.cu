@@ -6,7 +6,9 @@
 // thread per query: it loads its row of scores from tensor memory, keeps the running maximum and sum in registers (no
 // exchange between threads), and writes the weights back to tensor memory, in the place of the scores, from where they are the left
 // operand of the second product.  The reference point of a row's weights moves only where its maximum has grown by more than 2^8
-// (weights are then up to 2^8 instead of 1, which costs no precision).
+// (weights are then up to 2^8 times the first ones, which costs no precision).  fp16 weights start at 2^7, so that they use the type's range from
+// 65,504 down: they have their 11 bits down to 2^-21 of the reference point's, and end at 2^-31 of it (from 1 on, those below 2^-25 were lost, and with
+// them all of a context whose leading key has the value 0).
 //
 // 16-bit operands: two tiles, blocks of 128 keys, two stages of keys and of values (four up to 64 dimensions).  The first half of a block's
 // weights is handed on while the second is made.  The context stays in tensor memory and is rescaled there when the reference point
@@ -55,6 +57,7 @@ constexpr int kTileRows = 128;
 constexpr int kMostPieces = 8;         // of a group of rows' keys, where there are few groups: the CTAs of a cluster
 constexpr int kLeastShared = 5;        // blocks of keys that are shared out
 constexpr float kMostGrowth = 8.0f;  // of a row's maximum, in powers of two, before its context is rescaled
+constexpr float kHalfLift = 7.0f;    // fp16 weights are 2^7 at the reference point, 2^15 at most
 
 template <int dims_, int parts_>
 struct Shape {
@@ -571,7 +574,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                     tensor_store32(context_at + i, reinterpret_cast<const uint32_t*>(o));
                 }
             }
-            const float offset = top == masked ? 0.0f : -top * factor;
+            constexpr float lift = __is_same(Elem, __half) ? kHalfLift : 0.0f;
+            const float offset = top == masked ? 0.0f : fmaf(-top, factor, lift);
             float2 sums[2] = {both(0.0f), both(0.0f)};
 #pragma unroll
             for (int i = 0; i < S::block; i += 32) {

@@ -343,3 +343,25 @@ def test_heads_of_a_tile(dtype, heads, kv_heads):
     _check(dtype, lens, lens, heads, kv_heads, 64, lead=1, behind=30)
     _check(dtype, lens, longer, heads, kv_heads, 72, window=50)
     _check(dtype, lens, longer[::-1], heads, kv_heads, 128, causal=False, behind=5)
+
+
+# Keys 18 nats above the rest whose values are 0: what the rest weigh, 2^-26 each, is all that there is.  fp16 weights are 2^7 at the row's reference
+# point: those of e^-18.5 of it are multiples of 2^-24, off by 2^-25, which is 0.026 of them (as 1 at the reference point they would be 0).
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("queries,keys,every,heads", [(3, 8192, 8192, 1), (300, 3000, 60, 1), (200, 1000, 1000, 40)])
+def test_weights_far_below_the_largest_count(dtype, queries, keys, every, heads):
+    import torch
+    rng = np.random.RandomState(keys)
+    q, k, v = np.zeros((queries, heads, 64)), np.zeros((keys, 1, 64)), rng.uniform(0.5, 2.0, (keys, 1, 64))
+    q[:, :, :2] = 1.0
+    k[:, 0, 1] = rng.randint(-4, 5, keys) / 8
+    k[::every, 0, 0], v[::every] = 18.0, 0.0
+    q, k, v = (_tensor(x, dtype) for x in (q, k, v))
+    at, to = torch.tensor([0, queries], device="cuda"), torch.tensor([0, keys], device="cuda")
+    got, status = gh.ctx().prompt_attention(q, k, v, at, to, scale=1.0, causal=False)
+    want, most, _ = _attention(*(x.double().cpu().numpy() for x in (q, k, v)), at.tolist(), to.tolist(), 1.0, False, 0)
+    # (relative to the context, whose terms all have one sign)
+    slack = _slack(dtype, most, 1.0, 64, keys) + (2.0 ** -25 / (2.0 ** 7 * np.exp(-18.5)) if dtype == "float16" else 0.0)
+    context = got.double().cpu().numpy()
+    step = np.maximum(HALF_STEP[dtype] * want, 2.0 ** -25 if dtype == "float16" else 0.0)  # (fp16 below 2^-14: multiples of 2^-24)
+    assert int(status) == 0 and (np.abs(context - want) <= slack * want + step).all(), (np.abs(context - want) / want).max()
