@@ -605,6 +605,8 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
             fine = wait(&context_full[t], S::parts == 1 ? 0 : (count - 1) & 1);
             tensor_fence_after();
         }
+        // A sum of 0: the row sees nothing, or (as in any softmax, NaN) scores of -inf alone.
+        const auto sum_of = [&](float sum, bool sees) { return sum == 0.0f && sees ? __int_as_float(0x7fffffff) : sum; };
         // Eight dimensions of a row's context, times what makes its weights add up to one.
         const auto put = [&](int64_t to, int of_head, int d, const float* o, float sum) {
             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -626,6 +628,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
         if (fine) {
             float4* fours = reinterpret_cast<float4*>(shared) + t * (S::tile_floats / 4) + (warp % 4) * 32 + lane;
             if (count > 0) add_block();
+            const float sum = sum_of(total, end > first);
 #pragma unroll
             for (int i = 0; i < S::dims; i += 32) {
                 if (i >= p.head_dim) break;
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
 #pragma unroll
                         for (int k = 0; k < 32; k += 8) {
                             if (i + k >= p.head_dim) break;
-                            put(row, head, i + k, o + k, total);
+                            put(row, head, i + k, o + k, sum);
                         }
                     }
                 } else if (count > 0) {
@@ -676,6 +679,7 @@ __global__ void __launch_bounds__(S::threads, 1) prompt_attention_kernel(const _
                     less[b] = nothing ? -1.0f : ends_at[b].x == high ? 1.0f : exp2_approx((ends_at[b].x - high) * factor);
                     sum += nothing ? 0.0f : less[b] * ends_at[b].y;
                 }
+                sum = sum_of(sum, sight.end(to) > sight.first(to));
                 for (int d = (int)threadIdx.x / rows * 8; d < p.head_dim; d += parts * 8) {
                     float o[8] = {};
 #pragma unroll

@@ -365,3 +365,30 @@ def test_weights_far_below_the_largest_count(dtype, queries, keys, every, heads)
     context = got.double().cpu().numpy()
     step = np.maximum(HALF_STEP[dtype] * want, 2.0 ** -25 if dtype == "float16" else 0.0)  # (fp16 below 2^-14: multiples of 2^-24)
     assert int(status) == 0 and (np.abs(context - want) <= slack * want + step).all(), (np.abs(context - want) / want).max()
+
+
+# Visible scores of -inf.  A softmax over nothing else is NaN, beside finite ones they weigh nothing; a query that sees no key has the context 0.
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("scale", [0.125, -0.125])
+@pytest.mark.parametrize("heads,kv_heads,sequences,keys", [(1, 1, 1, 60), (2, 1, 1, 3000), (4, 1, 200, 60)])
+def test_scores_of_minus_infinity(dtype, scale, heads, kv_heads, sequences, keys):
+    import torch
+    far = float("inf") if dtype == "float16" else 2.0 ** 100   # (2^100 has one bf16 part; times 2^100 it is beyond a float)
+    q, v = torch.zeros(4 * sequences, heads, 64, device="cuda"), torch.randn(keys * sequences, kv_heads, 64, device="cuda")
+    k = torch.zeros_like(v)
+    first = torch.arange(sequences, device="cuda") * keys
+    k[:, :, :3] = (-1.0 if scale > 0 else 1.0) * min(far, 1e4 if dtype == "float16" else far)
+    k[first, :, 1] = k[first + keys - 1, :, 2] = 0.0
+    q[1::4, :, 0] = far             # every key
+    if dtype != "float16":
+        q[2::4, :, 1] = q[3::4, :, 2] = far  # every key but the first, but the last
+    q, k, v = (x.to(getattr(torch, dtype)) for x in (q, k, v))
+    at, to = torch.arange(sequences + 1, device="cuda") * 4, torch.arange(sequences + 1, device="cuda") * keys
+    got, status = gh.ctx().prompt_attention(q, k, v, at, to, scale=scale, causal=False)
+    assert int(status) == 0 and got[1::4].isnan().all() and got[0::4].isfinite().all()
+    if dtype != "float16":
+        for i, of in ((2, first), (3, first + keys - 1)):
+            want = v[of].repeat_interleave(heads // kv_heads, 1)
+            assert ((got[i::4] - want).abs() <= 2.0 ** -20 * want.abs()).all()
+    got = gh.ctx().prompt_attention(q, k, v, at, torch.zeros_like(to), scale=scale, causal=False)[0]
+    assert (got == 0).all()
