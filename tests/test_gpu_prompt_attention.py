@@ -392,3 +392,49 @@ def test_scores_of_minus_infinity(dtype, scale, heads, kv_heads, sequences, keys
             assert ((got[i::4] - want).abs() <= 2.0 ** -20 * want.abs()).all()
     got = gh.ctx().prompt_attention(q, k, v, at, torch.zeros_like(to), scale=scale, causal=False)[0]
     assert (got == 0).all()
+
+
+def _plan(dtype, q_lens, heads, kv_heads, head_dim, total_k):
+    """(heads of a tile, pieces) by the kernel's rule: as few heads as keep the CTAs to one for an SM, clusters where half of the SMs were idle."""
+    import torch
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    tiles, block = (1, 64) if dtype == "float32" else (2, 128)
+    groups = lambda packed: (sum(q_lens) // (tiles * (128 // packed)) + len(q_lens)) * (heads // packed)  # noqa: E731
+    packed = 1
+    for d in range(1, min(heads // kv_heads, 16) + 1):
+        if heads // kv_heads % d == 0:
+            packed = d
+            if groups(d) <= sms:
+                break
+    return packed, max(1, min(sms // groups(packed), total_k // block + 1, 8))
+
+
+# Few groups of rows, each of several heads of a kv head: the CTAs of a cluster share their keys.
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,head_dim", [([1, 20, 7, 13, 3, 18], [3000, 2000, 70, 900, 128, 1], 28, 4, 128),
+                                                                   ([1, 20, 7, 13, 3, 18], [90, 20, 57, 13, 83, 18], 28, 4, 64),
+                                                                   ([1] * 16, [17 * i for i in range(16)], 10, 2, 72), ([2, 1] * 8, [700, 40] * 8, 20, 2, 64),
+                                                                   ([5] * 3 + [0, 130], [1000, 0, 65, 30, 640], 33, 3, 96), ([40, 3], [41, 1500], 91, 7, 128)])
+def test_heads_of_a_tile_whose_keys_are_shared_out(dtype, q_lens, k_lens, heads, kv_heads, head_dim):
+    import torch
+    packed, pieces = _plan(dtype, q_lens, heads, kv_heads, head_dim, sum(k_lens))
+    assert packed > 1 and pieces > 1
+    _check(dtype, q_lens, k_lens, heads, kv_heads, head_dim, lead=2, behind=9)
+    _check(dtype, q_lens, k_lens, heads, kv_heads, head_dim, causal=False, scale=-0.2, behind=80)
+    for window in (1, 60, 700):
+        _check(dtype, q_lens, k_lens, heads, kv_heads, head_dim, window=window)
+    # a key that is not finite reaches the queries of its sequence that see it and their heads, no other
+    rng = np.random.RandomState(len(q_lens))
+    q_at, k_at = (np.concatenate([[0], np.cumsum(n)]).astype(np.int64) for n in (q_lens, k_lens))
+    q, k, v = (_tensor(rng.rand(n[-1], h, head_dim) + 0.1, dtype) for n, h in ((q_at, heads), (k_at, kv_heads), (k_at, kv_heads)))
+    at, to = torch.from_numpy(q_at).cuda(), torch.from_numpy(k_at).cuda()
+    want = gh.ctx().prompt_attention(q, k, v, at, to)[0]
+    longest = int(np.argmax(k_lens))
+    for j in (0, k_lens[longest] // 2, k_lens[longest] - 1):
+        bad = k.clone()
+        bad[k_at[longest] + j, kv_heads - 1] = float("nan")
+        got, status = gh.ctx().prompt_attention(q, bad, v, at, to)
+        hit = torch.zeros(got.shape[:2], dtype=torch.bool, device="cuda")
+        sees = max(j - (k_lens[longest] - q_lens[longest]), 0)
+        hit[q_at[longest] + sees:q_at[longest + 1], heads - heads // kv_heads:] = True
+        assert int(status) == 0 and got[hit].isnan().all() and (got[~hit] == want[~hit]).all()
