@@ -807,7 +807,7 @@ cudaError_t launch(const PromptAttentionParams& p, int sm_count, cudaStream_t st
             to += 3 * positions * width;
             if (positions > 0) {
                 const int64_t blocks = (positions * (width / 4) + 255) / 256;
-                split_kernel<<<(unsigned)std::min<int64_t>(blocks, 148 * 8), 256, 0, stream>>>(static_cast<const float*>(from), parts, positions, stride, width);
+                split_kernel<<<(unsigned)std::min<int64_t>(blocks, (int64_t)sm_count * 8), 256, 0, stream>>>(static_cast<const float*>(from), parts, positions, stride, width);
                 ++*launches;
             }
             return parts;
