@@ -11,10 +11,11 @@
  *     compute call fails with PSX_ERR_CUDA.
  *   - A psx_ctx belongs to one device and one host thread at a time (like the reference's
  *     DeviceBackend, include/pulsatrix/cuda_backend.hpp:159-166).  It owns scratch memory that
- *     grows on demand; growing synchronises the device, steady-state calls do not allocate.  Scratch of
- *     beam_select, decode_attention_8bit and prompt_attention that a larger call outgrows stays allocated
- *     until the context goes, because a captured graph may hold it.  Calls of one context that use scratch
- *     must not run at the same time, replays of graphs among them.
+ *     grows on demand; growing synchronises the device, steady-state calls do not allocate.  It grows to what
+ *     a call needs and a quarter more where that is free.  Scratch of beam_select, decode_attention_8bit and
+ *     prompt_attention that a larger call outgrows is freed, or, if a stream capture has used it, stays
+ *     allocated until the context goes, because a captured graph may hold it.  Calls of one context that use
+ *     scratch must not run at the same time, replays of graphs among them.
  *   - Device entry points are asynchronous on `stream` (a cudaStream_t; NULL is CUDA's default
  *     stream, as everywhere in CUDA); outputs are valid once that stream has been synchronised.
  *     Host entry points run on the context's own stream and synchronise before returning.
@@ -357,8 +358,8 @@ PSX_API psx_status psx_b200_decode_attention(psx_ctx* ctx, void* stream, const f
  *                is left at all
  * keep may be larger than beams (twice as many leave enough when finished ones are set aside).  Limits: beams <= 64,
  * keep <= 128, vocab <= 2^30, beams * vocab <= 2^31 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; the outputs must not overlap the inputs.
- * The context's scratch grows to groups * beams * (vocab / 1024) * (keep * 8 + 16) bytes at most; inside a stream capture it
- * cannot grow (PSX_ERR_UNSUPPORTED): make a call of that size before. */
+ * Needs scratch of groups * beams * ceil(vocab / 1024) * (keep * 8 + 16) + 4 * groups bytes at most (far less where there are many
+ * rows); inside a stream capture the context's scratch cannot grow (PSX_ERR_UNSUPPORTED): make a call of that size before. */
 PSX_API psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream, const float* logits, int64_t groups, int64_t beams, int64_t vocab,
                                         int64_t row_stride, const float* scores, const uint8_t* finished, int64_t finished_token,
                                         int64_t keep, float* out_scores, int64_t* parents, int64_t* tokens, int32_t* group_status);
@@ -436,7 +437,7 @@ PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, co
  * do not see it, too, up to 384 positions from those that do.
  * All pointers 16-byte aligned, strides a multiple of 16 bytes.  Limits: head_dim a multiple of 8 up to 128, batch <= 4096, total_q
  * and total_k <= 2^29, strides < 2^36 (else PSX_ERR_UNSUPPORTED).  status (device, may be null): set to 0 by the call, to 1 if a
- * bounded device-side wait ran out (psx_b200_ctx_set_wait_limit).  Asynchronous on `stream`; fp32 takes scratch of 1.5 times the
+ * bounded device-side wait ran out (psx_b200_ctx_set_wait_limit).  Asynchronous on `stream`; fp32 needs scratch of 1.5 times the
  * bytes of k and v (in a stream capture as psx_b200_beam_select). */
 PSX_API psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream, int32_t dtype, const void* q, const void* k, const void* v, void* out,
                                              int64_t total_q, int64_t total_k, int64_t q_stride, int64_t k_stride, int64_t v_stride,

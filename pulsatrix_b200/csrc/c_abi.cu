@@ -53,6 +53,7 @@ psx_status fail(psx_status code, std::string message) {
 struct Buffer {
     void* ptr = nullptr;
     size_t bytes = 0;
+    bool captured = false;  // by a stream capture, since it was allocated (see reserve_kept)
 };
 
 // Page-locked staging for rows that lie in ordinary host memory: eight slots of 256 KB.
@@ -114,30 +115,45 @@ psx_status reserve(Buffer& b, size_t bytes) {
     return PSX_OK;
 }
 
-// The same for scratch whose address a captured graph may replay: what is outgrown is kept (each is a quarter larger than what
-// asked for it, at least), and inside a capture nothing is allocated.  `grown`: whether the memory is new.
-psx_status reserve_kept(psx_ctx* ctx, cudaStream_t stream, Buffer& b, size_t bytes, bool* grown = nullptr) {
-    if (grown) *grown = false;
-    if (bytes <= b.bytes) return PSX_OK;
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    PSX_CUDA(cudaStreamIsCapturing(stream, &capturing));
-    if (capturing != cudaStreamCaptureStatusNone) {
+psx_status is_capturing(cudaStream_t stream, bool* capturing) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    PSX_CUDA(cudaStreamIsCapturing(stream, &status));
+    *capturing = status != cudaStreamCaptureStatusNone;
+    return PSX_OK;
+}
+
+// The same for scratch whose address a captured graph may replay: what is outgrown is kept if a capture has used it, and inside a
+// capture (`capturing`) nothing is allocated.  Where a quarter more than the call needs is not free, it is what the call needs.
+// `grown`: whether the memory is new.
+psx_status reserve_kept(psx_ctx* ctx, bool capturing, Buffer& b, size_t bytes, bool* grown = nullptr) {
+    if (grown) *grown = bytes > b.bytes;
+    if (bytes <= b.bytes) {
+        b.captured |= capturing;
+        return PSX_OK;
+    }
+    if (capturing) {
         return fail(PSX_ERR_UNSUPPORTED, "psx_b200: the context's scratch cannot grow inside a stream capture: make a call of this size before");
     }
-    const size_t want = std::max(bytes + bytes / 4 + 256, 2 * b.bytes);
-    void* ptr = nullptr;
-    PSX_CUDA(cudaMalloc(&ptr, want));
-    if (b.ptr) ctx->outgrown.push_back(b.ptr);
-    b.ptr = ptr;
+    if (b.ptr && b.captured) ctx->outgrown.push_back(b.ptr);
+    else if (b.ptr) PSX_CUDA(cudaFree(b.ptr));
+    b = Buffer{};
+    size_t want = bytes + bytes / 4 + 256;
+    cudaError_t e = cudaMalloc(&b.ptr, want);
+    if (e == cudaErrorMemoryAllocation) {
+        cudaGetLastError();  // (the next launch's check is not to find it)
+        want = bytes;
+        e = cudaMalloc(&b.ptr, want);
+    }
+    if (e != cudaSuccess) b.ptr = nullptr;
+    PSX_CUDA(e);
     b.bytes = want;
-    if (grown) *grown = true;
     return PSX_OK;
 }
 
 // Counters that are zero between calls: every call leaves them so.
-psx_status reserve_counters(psx_ctx* ctx, cudaStream_t stream, Buffer& b, size_t count) {
+psx_status reserve_counters(psx_ctx* ctx, cudaStream_t stream, bool capturing, Buffer& b, size_t count) {
     bool grown;
-    if (psx_status s = reserve_kept(ctx, stream, b, count * sizeof(int32_t), &grown)) return s;
+    if (psx_status s = reserve_kept(ctx, capturing, b, count * sizeof(int32_t), &grown)) return s;
     if (!grown) return PSX_OK;
     const cudaError_t e = cudaMemsetAsync(b.ptr, 0, b.bytes, stream);
     if (e != cudaSuccess) b.bytes = 0;  // (what is not zero is not used)
@@ -1184,10 +1200,12 @@ psx_status psx_b200_beam_select(psx_ctx* ctx, void* stream_ptr, const float* log
     PSX_CUDA(device.error);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     const size_t stats_bytes = (size_t)lists * sizeof(psx::BeamPart);
-    if (psx_status s = reserve_kept(ctx, stream, ctx->beam_scratch, stats_bytes + (size_t)(lists * keep) * sizeof(psx::BeamEntry))) return s;
+    bool capturing;
+    if (psx_status s = is_capturing(stream, &capturing)) return s;
+    if (psx_status s = reserve_kept(ctx, capturing, ctx->beam_scratch, stats_bytes + (size_t)(lists * keep) * sizeof(psx::BeamEntry))) return s;
     p.part_stats = static_cast<psx::BeamPart*>(ctx->beam_scratch.ptr);
     p.entries = reinterpret_cast<psx::BeamEntry*>(static_cast<char*>(ctx->beam_scratch.ptr) + stats_bytes);
-    if (psx_status s = reserve_counters(ctx, stream, ctx->beam_arrived, (size_t)groups)) return s;
+    if (psx_status s = reserve_counters(ctx, stream, capturing, ctx->beam_arrived, (size_t)groups)) return s;
     p.arrived = static_cast<int32_t*>(ctx->beam_arrived.ptr);
     PSX_CUDA(psx::launch_beam_select(p, stream));
     ctx->launches += 1;
@@ -1329,8 +1347,10 @@ psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream_ptr, const 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     psx::plan_attention_8bit(p, ctx->sm_count);
     if (p.pieces > 1) {
-        if (psx_status s = reserve_kept(ctx, stream, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;
-        if (psx_status s = reserve_counters(ctx, stream, ctx->attention_8bit_arrived, (size_t)psx::attention_8bit_counters(p))) return s;
+        bool capturing;
+        if (psx_status s = is_capturing(stream, &capturing)) return s;
+        if (psx_status s = reserve_kept(ctx, capturing, ctx->attention_8bit_pieces, psx::attention_8bit_partial_bytes(p))) return s;
+        if (psx_status s = reserve_counters(ctx, stream, capturing, ctx->attention_8bit_arrived, (size_t)psx::attention_8bit_counters(p))) return s;
         p.partial = static_cast<float*>(ctx->attention_8bit_pieces.ptr);
         p.arrived = static_cast<int32_t*>(ctx->attention_8bit_arrived.ptr);
     }
@@ -1383,7 +1403,9 @@ psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dty
     PSX_CUDA(device.error);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     if (dtype == psx::kFloat32) {
-        if (psx_status s = reserve_kept(ctx, stream, ctx->prompt_parts, psx::prompt_split_bytes(p))) return s;
+        bool capturing;
+        if (psx_status s = is_capturing(stream, &capturing)) return s;
+        if (psx_status s = reserve_kept(ctx, capturing, ctx->prompt_parts, psx::prompt_split_bytes(p))) return s;
         p.split = ctx->prompt_parts.ptr;
     }
     if (status) PSX_CUDA(cudaMemsetAsync(status, 0, sizeof(int32_t), stream));

@@ -438,3 +438,52 @@ def test_heads_of_a_tile_whose_keys_are_shared_out(dtype, q_lens, k_lens, heads,
         sees = max(j - (k_lens[longest] - q_lens[longest]), 0)
         hit[q_at[longest] + sees:q_at[longest + 1], heads - heads // kv_heads:] = True
         assert int(status) == 0 and got[hit].isnan().all() and (got[~hit] == want[~hit]).all()
+
+
+def test_scratch_is_as_much_as_the_call_needs_where_more_is_not_free():
+    import torch
+    # fp32 keys and values take scratch of 1.5 times their bytes; the quarter on top gives way when the device is nearly full
+    ctx, positions = psx.Context(0), 400_000
+    q, k = torch.randn(2, 8, 128, device="cuda"), torch.randn(positions, 8, 128, device="cuda")
+    at, to = torch.tensor([0, 2], device="cuda"), torch.tensor([0, positions], device="cuda")
+    other = psx.Context(0)
+    want = other.prompt_attention(q, k, k, at, to)[0]
+    torch.cuda.synchronize()
+    other.close()
+    need = 12 * 128 * positions * 8
+    few = torch.tensor([0, 40], device="cuda")
+    ctx.prompt_attention(q, k[:40], k[:40], at, few)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    held = torch.empty(torch.cuda.mem_get_info()[0] - need - need // 8, dtype=torch.uint8, device="cuda")
+    got, status = ctx.prompt_attention(q, k, k, at, to)
+    assert int(status) == 0 and (got == want).all()
+    ctx.close()
+    del held
+    torch.cuda.empty_cache()
+    # not even that: the call says so, and the context stays usable
+    ctx = psx.Context(0)
+    ctx.prompt_attention(q, k[:40], k[:40], at, few)
+    held = torch.empty(torch.cuda.mem_get_info()[0] - need // 8, dtype=torch.uint8, device="cuda")
+    with pytest.raises(psx.PsxError) as e:
+        ctx.prompt_attention(q, k, k, at, to)
+    assert e.value.status == psx.ERR_CUDA
+    del held
+    torch.cuda.empty_cache()
+    got, status = ctx.prompt_attention(q, k, k, at, to)
+    assert int(status) == 0 and (got == want).all()
+
+
+def test_scratch_that_no_capture_has_used_goes_when_it_is_outgrown():
+    import torch
+    ctx, most = psx.Context(0), 120_000
+    q, k = torch.randn(2, 8, 128, device="cuda"), torch.randn(most, 8, 128, device="cuda")
+    at = torch.tensor([0, 2], device="cuda")
+    ctx.prompt_attention(q, k[:2], k[:2], at, at)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    free = torch.cuda.mem_get_info()[0]
+    for positions in range(20_000, most + 1, 10_000):   # a conversation that goes on
+        ctx.prompt_attention(q, k[:positions], k[:positions], at, at * (positions // 2))
+    torch.cuda.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] <= 1.25 * 12 * 128 * most * 8 + (64 << 20)   # (and what torch holds of its own)
