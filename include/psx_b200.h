@@ -343,14 +343,17 @@ PSX_API psx_status psx_b200_decode_attention(psx_ctx* ctx, void* stream, const f
 
 /* Beam search's step over a whole batch (no counterpart in the reference, whose Generate() has no beams): of all
  * (beam, token) pairs of a group of `beams` rows, the `keep` with the largest score + log-probability,
- *     value(b, v) = (scores[b] - log sum_w exp(logits[b][w])) + logits[b][v]     in double precision,
- * best first; of equal values the lowest beam's, then the lowest token's.  What offers nothing: logits of -inf (tokens that
+ *     value(b, v) = (scores[b] - log sum_w exp(logits[b][w])) + logits[b][v],
+ * best first; of equal values the lowest beam's, then the lowest token's.  The three terms are added in double precision.  The
+ * exponentials, and a thread's share of their sum, are floats: a row's logarithm is off by at most 5e-6, or 1e-6 + 5e-6 r where
+ * all other terms add r < 1 of the largest to it.  That moves all of a beam's candidates together, so of two beams' values that are
+ * nearer to each other than this either may come first; equal rows have equal logarithms. What offers nothing: logits of -inf (tokens that
  * psx_b200_process_logits removed), beams whose score is -inf (before the first step all but the first), and the other tokens
  * of a finished beam, which offers finished_token at its own score.  Places that no candidate is left for get -inf, -1, -1.
  *   logits       device fp32, row g * beams + b at logits + row * row_stride (row_stride >= vocab)
  *   scores       device fp32 (groups * beams): the beams' scores so far
  *   finished     device bytes (groups * beams), non-zero: the beam has ended; may be NULL
- *   out_scores   device fp32 (groups, keep), the values rounded once (below the lowest float: that)
+ *   out_scores   device fp32 (groups, keep), the values rounded once more (below the lowest float: that)
  *   parents      device int64 (groups, keep): the beam continued, 0 .. beams - 1, as psx_b200_reorder_states takes it
  *   tokens       device int64 (groups, keep)
  *   group_status device int32 (groups), may be NULL: PSX_ROW_OK; PSX_ROW_NON_FINITE: a NaN or +inf among the logits of a beam

@@ -299,3 +299,41 @@ def test_a_refused_call_moves_no_state():
     assert call(65) == psx.ERR_UNSUPPORTED and call(65537) == psx.ERR_UNSUPPORTED and call(2 ** 62) == psx.ERR_UNSUPPORTED
     torch.cuda.synchronize()
     assert all((s.flatten() == torch.arange(4.0, device="cuda")).all() for s in states)
+
+
+# Strongly peaked rows: the largest logit's term is 1 and what the others add, r, is small.  In units of 2^-24 of the sum: the terms of r are off by 80 r
+# as above; the thread that holds the 1 rounds what it adds to it, four times in that chunk and three in its joins, then once for each of eight chunks, a
+# unit each: 15.  Joins and the logarithm are in double precision.  Together 80 r + 16.
+@pytest.mark.parametrize("gap", [5.0, 12.0, 14.0, 17.0, 20.0, 40.0])
+@pytest.mark.parametrize("groups,vocab", [(1, 50257), (40, 8192), (3, 151936), (1, 1000)])
+def test_peaked_rows(gap, groups, vocab):
+    rng = np.random.RandomState(int(gap))
+    beams = 4
+    logits = (rng.randn(groups * beams, vocab) * 0.5).astype(np.float32)
+    logits[np.arange(groups * beams), rng.randint(0, vocab, groups * beams)] = np.float32(gap + 3)
+    out = _run(logits, np.zeros(groups * beams, dtype=np.float32), beams, beams)
+    value = _values(logits, np.zeros(groups * beams, dtype=np.float32), beams)
+    for g in range(groups):
+        best = value[g].max(1)
+        rest = np.expm1(-best)                       # r of each beam
+        slack = (80 * rest + 16) * 2.0 ** -24
+        at, tokens = out["parents"][g], out["tokens"][g]
+        assert (np.abs(out["scores"][g] - value[g, at, tokens]) <= slack[at] + 2.0 ** -24 * np.abs(value[g, at, tokens])).all()
+        if rest.max() < 0.3:                          # every beam's best is ahead of every other candidate
+            assert sorted(at.tolist()) == [0, 1, 2, 3] and (tokens == value[g].argmax(1)[at]).all()
+            assert (np.diff(best[at]) <= 2 * slack.max()).all()
+
+
+def test_a_token_that_is_nearly_certain_has_its_own_logarithm():
+    # beams whose best token leaves 2^-26 and less to the others: the values differ by less than a float's step at 1, and are in order
+    rest = -18.0 - np.arange(8) * 0.5
+    logits = np.full((8, 5000), -200.0, dtype=np.float32)
+    logits[:, 2500] = rest
+    logits[:, 10] = 0.0
+    scores = np.zeros(8, dtype=np.float32)
+    for rows in (np.arange(8), np.arange(8)[::-1], np.array([3, 7, 0, 5, 1, 6, 2, 4])):
+        out = _run(logits[rows], scores, 8, 8)
+        assert (out["tokens"] == 10).all()
+        assert (rows[out["parents"][0]] == np.arange(8)[::-1]).all()
+        want = -np.log1p(np.exp(np.float64(rest[::-1])))
+        assert (np.abs(out["scores"][0] - want) <= 100 * 2.0 ** -24 * np.abs(want)).all()
