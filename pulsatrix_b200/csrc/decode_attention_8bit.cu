@@ -37,6 +37,7 @@ namespace psx {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4, kTile = 32;
+constexpr int kStages = 2;       // of a warp: the tile in work and the one on its way
 constexpr int kMostShare = 128;  // tiles that a block takes where shorter pieces only balance
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
@@ -46,9 +47,8 @@ constexpr float kWeightLift = 15.0f;  // the largest weight is 2^15
 // then, and 2^30 of them (the longest cache) add up to a float.
 constexpr float kLeastScale = 0x1p-82f;
 
-__host__ __device__ constexpr int stages_of(int) { return 2; }
 __host__ __device__ constexpr int stage_bytes(int dims) { return 2 * kTile * dims + 16; }  // keys, values, two scales each
-__host__ __device__ constexpr size_t shared_of(int dims) { return (size_t)kWarps * stages_of(dims) * stage_bytes(dims); }
+__host__ __device__ constexpr size_t shared_of(int dims) { return (size_t)kWarps * kStages * stage_bytes(dims); }
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -61,8 +61,7 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
-template <int pending>
-__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" ::"n"(pending) : "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ void multiply(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -123,7 +122,7 @@ __device__ __forceinline__ Sight sight_of(const Attention8bitParams& p, int row)
 template <class T, int dims, int tiles_of_rows>
 __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2 && dims == 128 ? 2 : dims == 128 ? 3 : 4) decode_attention_8bit_kernel(const __grid_constant__ Attention8bitParams p) {
     constexpr bool precise = sizeof(T) == 4;
-    constexpr int kStages = stages_of(dims), kStageBytes = stage_bytes(dims), kSegments = dims / 64, kBlocks = dims / 16;
+    constexpr int kStageBytes = stage_bytes(dims), kSegments = dims / 64, kBlocks = dims / 16;
     constexpr int kRows = 8 * tiles_of_rows;
     extern __shared__ __align__(16) uint8_t shared[];
     __shared__ float tops[kWarps][kRows], totals[kWarps][kRows];
@@ -190,13 +189,7 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
             copy4(to + 2 * kTile * dims + lane * 4, (lane < 2 ? key_scales : value_scales) + (there ? first >> shift : 0), there);
         }
     };
-    int fetched = from_tile + warp;
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-        if (fetched < to_tile) fetch(fetched, s);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        fetched += kWarps;
-    }
+    if (from_tile + warp < to_tile) fetch(from_tile + warp, 0);
 
     // The query rows as the right-hand operand: lane (gid, tig) holds row gid's dimensions 16 tig .. 16 tig + 15 of every 64.
     uint32_t qh[tiles_of_rows][kSegments][4][2], ql[precise ? tiles_of_rows : 1][precise ? kSegments : 1][4][2];
@@ -253,14 +246,9 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
 
     int stage = 0;
     for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
-        copies_done<kStages - 2>();
+        copies_done();
         __syncwarp();
-        {
-            const int next = stage == 0 ? kStages - 1 : stage - 1;  // the stage that the tile before this one used
-            if (fetched < to_tile) fetch(fetched, next);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            fetched += kWarps;
-        }
+        if (tile + kWarps < to_tile) fetch(tile + kWarps, stage ^ 1);  // (where the tile before this one was)
         const uint8_t* k_stage = stages + stage * kStageBytes;
         const float* scales = reinterpret_cast<const float*>(k_stage + 2 * kTile * dims);
         const int position = (tile0 + tile) * kTile;
@@ -396,9 +384,8 @@ __global__ void __launch_bounds__(kThreads, dims == 256 ? 1 : tiles_of_rows == 2
                 }
             }
         }
-        stage = stage + 1 == kStages ? 0 : stage + 1;
+        stage ^= 1;
     }
-    copies_done<0>();
 
     // The four warps' results meet in shared memory.  (The stages are free: every warp has read its own.)
 #pragma unroll
