@@ -417,8 +417,12 @@ PSX_API psx_status psx_b200_store_cache_8bit(psx_ctx* ctx, void* stream, const p
  * q_len, head_dim), contiguous, 16-byte aligned; row b sees positions 0 .. lengths[b] - 1 (device int64; outside 0 .. max_len:
  * the nearer end), its q_len new positions being the last of them (already stored).  New position i is position
  * p = lengths[b] - q_len + i: with `causal` it sees no key j > p and, with window > 0, no key j + window <= p.  A query that sees
- * nothing has the context 0.  Positions that no query of a row sees are not read.  Softmax statistics and sums are floats; codes
- * are exact in the products, queries and weights carry 11 bits (bf16, fp16) or 22 (fp32).
+ * nothing has the context 0; one whose visible scores are all -inf, as in any softmax, NaN.  Positions that no query of a row sees are
+ * not read, nor the scales of blocks of them; a NaN in a position that one of a row's new positions sees may reach the others.  Softmax
+ * statistics and sums are floats; codes are exact in the products.  bf16 and fp16: a query's elements are exact to 2^-38 of its
+ * largest, weights carry 11 bits down to 2^-29 of the largest.  fp32: elements carry 22 bits down to 2^-17 of the largest, weights 22 bits
+ * down to 2^-18.  What is smaller has fewer bits and ends at 2^-39 and 2^-40.  (Value scales from 2^-82 to 2^100; outside that weights
+ * lose bits sooner.)
  * Limit: (heads / kv_heads) * q_len <= 16 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; scratch
  * in a stream capture as psx_b200_beam_select. */
 PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, const void* q, int32_t dtype, const psx_cache_8bit* cache,
@@ -432,9 +436,10 @@ PSX_API psx_status psx_b200_decode_attention_8bit(psx_ctx* ctx, void* stream, co
  * b has queries q_offsets[b] .. q_offsets[b + 1] and keys k_offsets[b] .. k_offsets[b + 1] (device int64, batch + 1, ascending); with
  * more keys than queries the queries are the last positions (a prompt that continues a cached prefix).  Query i of n, with m
  * keys, is position p = m - n + i: with `causal` it sees no key j > p and, with window > 0, no key j + window <= p.  A query that
- * sees nothing gets 0.  out: (total_q, heads, head_dim), contiguous, apart from the operands; rows that belong to no sequence are left
+ * sees nothing gets 0, one whose visible scores are all -inf, as in any softmax, NaN.  out: (total_q, heads, head_dim), contiguous, apart from the operands; rows that belong to no sequence are left
  * as they were.
- * Products run on the tensor cores with float accumulators.  bf16 and fp16: weights are rounded to that type; fp32: every
+ * Products run on the tensor cores with float accumulators.  bf16 and fp16: weights are rounded to that type (fp16: 11 bits
+ * down to 2^-21 of the first or largest, ending at 2^-32); fp32: every
  * factor as three bf16 parts, so that products are exact to about 2^-24 (an infinity counts as NaN).  Keys and values of other
  * sequences, finite or not, have no influence; a NaN or infinity among a sequence's own values may reach queries of the sequence that
  * do not see it, too, up to 384 positions from those that do.

@@ -17,11 +17,11 @@
 //
 // A (row, kv head) pair's cached positions are cut into tiles of 32, and the tiles into pieces, a block each: as many as fill the GPU
 // once, or as pieces of 128 tiles make where that is more, which evens out rows of different lengths (64 rows x 8 kv heads of up to 8191
-// positions: 167 us as one piece each, 141 as two; pieces of 64 tiles: 138, but 96 rows x 1 of up to 16,000: 70 instead of 61).  The last
-// block of a pair to end joins its pieces, in order.  (Equal shares of all pairs' tiles laid on one axis: 139 us there,
+// positions, in a graph: 167 us as one piece each, 141 to 145 as two from box to box; pieces of 64 tiles: 138, but 96 rows x 1 of up to
+// 16,000: 70 instead of 61.  A call among others, with a cold L2: 157).  The last block of a pair to end joins its pieces, in order.
+// (Equal shares of all pairs' tiles laid on one axis: 139 us there,
 // with a cold L2 143 instead of 155; but 64 x 8 of 1000: 41 instead of 25, 24 x 8 of up to 4096: 52 instead of 33, since most blocks then have
-// the end of one pair
-// and the start of another.)  Inside a block each of four warps takes every fourth tile, with
+// the end of one pair and the start of another.)  Inside a block each of four warps takes every fourth tile, with
 // its own two stages of 32 positions in shared memory (cp.async, 16 bytes a lane), so that no warp waits for another until the end.
 // Bound by HBM for long caches (2 bytes per position, head dimension and kv head), by the chain of a tile for short ones: some 2100
 // clocks from a tile's arrival to its weights' products, most of them conversions of codes (64 instructions for 32 positions x 64

@@ -14,10 +14,10 @@
 // weights is handed on while the second is made.  The context stays in tensor memory and is rescaled there when the reference point
 // moves.  While the tensor core works for one tile the other tile's warpgroup works on its scores: the one issuing warp goes from
 // tile to tile, which keeps the two half a turn apart (with an issuing warp for each, both tiles ask for the same unit at a time: 773 us
-// instead of 662 for two prompts of up to 8192 positions, 32 heads of 128 in bf16, causal).  Weights are rounded to the operands'
+// instead of 662 for two prompts of up to 8192 positions, 32 heads of 128 in bf16, causal; 640 to 676 from box to box since).  Weights are rounded to the operands'
 // type, an error of the size of the context's own rounding.
 // Bound by a tile's turn: some 1700 clocks from scores to weights (570 for the maximum, 1024 of exponentials at four a clock and
-// scheduler), 1024 of products, and the way between the two; 1.05 PFLOP/s at those sizes.  Tried and taken back: a share of the
+// scheduler), 1024 of products, and the way between the two; 1.02 to 1.08 PFLOP/s at those sizes.  Tried and taken back: a share of the
 // exponentials by a polynomial (no gain, 662 and 668 us), two threads for a query (771 us).
 //
 // Few groups of rows: where they would leave half of the SMs idle, the CTAs of a cluster, up to eight, take a piece of a group's keys each,
