@@ -91,7 +91,7 @@ struct psx_ctx {
     cudaEvent_t ring_done[kRingSlots] = {};  // the copy out of (or into) a slot has finished
     // staging of the sharded path
     Buffer shard_uniform_scratch;
-    // Scratch that captured graphs may hold: what it outgrows stays allocated until the context goes (see reserve_kept).
+    // Scratch that captured graphs may hold: what a capture has used stays allocated until the context goes (see reserve_kept).
     Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts;
     std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
