@@ -12,8 +12,8 @@
  *   - A psx_ctx belongs to one device and one host thread at a time (like the reference's
  *     DeviceBackend, include/pulsatrix/cuda_backend.hpp:159-166).  It owns scratch memory that
  *     grows on demand; growing synchronises the device, steady-state calls do not allocate.  It grows to what
- *     a call needs and a quarter more where that is free.  Scratch of beam_select, decode_attention_8bit and
- *     prompt_attention that a larger call outgrows is freed, or, if a stream capture has used it, stays
+ *     a call needs and a quarter more where that is free.  Scratch of beam_select, decode_attention_8bit,
+ *     prompt_attention and the calls on pages that a larger call outgrows is freed, or, if a stream capture has used it, stays
  *     allocated until the context goes, because a captured graph may hold it.  Calls of one context that use
  *     scratch must not run at the same time, replays of graphs among them.
  *   - Device entry points are asynchronous on `stream` (a cudaStream_t; NULL is CUDA's default
@@ -55,8 +55,9 @@ typedef enum psx_row_status {
                                 row is decided from the row itself */
     PSX_ROW_DEVICE_TIMEOUT = 32, /* a bounded device-side wait (a bulk copy of a piece of the row into
                                 shared memory) ran out; nothing was drawn for this row */
-    PSX_ROW_CACHE_FULL = 64,  /* psx_b200_store_cache_8bit: the row's new positions do not fit; none was stored */
-    PSX_ROW_BAD_OFFSETS = 65  /* psx_b200_store_cache_8bit: the row's offsets or its filled length make no sense; nothing was stored */
+    PSX_ROW_CACHE_FULL = 64,  /* psx_b200_store_cache_8bit, psx_b200_extend_pages: the row's new positions do not fit; none was stored, or
+                                 no room made */
+    PSX_ROW_BAD_OFFSETS = 65  /* the same: the row's offsets, its filled length or the number of its new positions make no sense */
 } psx_row_status;
 
 /* GenerationConfig (include/pulsatrix/generation.hpp:29-52) without the loop fields, plus the
@@ -451,6 +452,52 @@ PSX_API psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream, int32_t
                                              int64_t total_q, int64_t total_k, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                                              const int64_t* q_offsets, const int64_t* k_offsets, int64_t batch, int64_t heads,
                                              int64_t kv_heads, int64_t head_dim, float scale, int32_t causal, int64_t window, int32_t* status);
+
+/* A cache of keys and values in pages (no counterpart in the reference, whose cache is one piece per row): a pool of num_pages
+ * pages for the keys, one for the values, of every layer, each (num_pages, kv_heads, page_size, head_dim) and contiguous, and one
+ * table for all layers.  Row b of the table holds positions 0 .. lengths[b] - 1; position i lies in page pages[b][i / page_size], at place
+ * i % page_size of it.  The first ceil(lengths[b] / page_size) entries of a row are in use, the others are not looked at.  Several rows may name a
+ * page (beams, samples of one prompt): references counts the entries in use that do, and a page is free where it is 0.  An
+ * empty table has lengths and references 0; the four calls below keep the counts.  All device pointers.
+ * Limits: page_size is 16, 32, 64 or 128, rows <= 4096, num_pages <= 2^30, max_pages * page_size <= 2^30 (else PSX_ERR_UNSUPPORTED). */
+typedef struct psx_page_table {
+    int32_t* pages;      /* (rows, max_pages) */
+    int64_t* lengths;    /* (rows) */
+    int32_t* references; /* (num_pages) */
+    int64_t rows, max_pages, num_pages, page_size;
+} psx_page_table;
+
+/* A pool: (num_pages, heads, page_size) of position_bytes each, contiguous (keys: kv_heads and head_dim elements). */
+typedef struct psx_page_pool {
+    void* data;
+    int64_t heads, position_bytes;
+} psx_page_pool;
+
+/* Room for new positions: lengths[b] += added[b] (device int64, rows), with the pages that this takes.  Rows come in order, the
+ * lowest free page first.  A row that goes on in a last page which other rows hold too gets a page of its own for it, and what the row
+ * holds of it is copied in all `pools` (a host array, read during the call); where all who hold the page go on in it, the last of
+ * them keeps it.  What a page holds behind that is left as it was.  row_status (device int32, rows, may be NULL): PSX_ROW_OK;
+ * PSX_ROW_CACHE_FULL: the row would need more than max_pages, or this row or one before it asked for more pages than were free;
+ * PSX_ROW_BAD_OFFSETS: added[b] or lengths[b] is negative, the length beyond max_pages * page_size, or the last page not one of the pool.  Such
+ * rows are left alone, their positions from lengths[b] on have no room.  pool_count may be 0 where no page is shared.  The pools must
+ * overlap neither each other nor the table (PSX_ERR_BAD_ARGUMENT); page bytes of a pool <= 2^30 (else PSX_ERR_UNSUPPORTED).  Asynchronous on
+ * `stream`; needs scratch of 16 bytes per row (in a stream capture as psx_b200_beam_select). */
+PSX_API psx_status psx_b200_extend_pages(psx_ctx* ctx, void* stream, const psx_page_table* table, const int64_t* added,
+                                         const psx_page_pool* pools, int64_t pool_count, int32_t* row_status);
+/* Rows that follow their beams, as psx_b200_reorder_states does with whole states, by sharing pages: row j of every group of `beams`
+ * rows becomes what row parents[j] of the group was (device int64, (rows / beams, beams), in any order and with repetitions; a row whose parent lies
+ * outside 0 .. beams - 1 stays as it is).  No position is copied; psx_b200_extend_pages parts rows that go on in one page.
+ * rows must be a multiple of beams.  Limit: beams <= 64 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`. */
+PSX_API psx_status psx_b200_fork_pages(psx_ctx* ctx, void* stream, const psx_page_table* table, const int64_t* parents, int64_t beams);
+/* Positions given back: row b keeps its first keep[b] (device int64, rows; a row that holds no more than that stays as it is, a negative
+ * number counts as 0; NULL: no row keeps any), and pages that it no longer needs lose its reference.  Asynchronous on `stream`. */
+PSX_API psx_status psx_b200_release_pages(psx_ctx* ctx, void* stream, const psx_page_table* table, const int64_t* keep);
+/* Pools brought together: with `used` pages in use (device int64, 1 element, written by the call), those numbered `used` and up move
+ * into the free ones below, in ascending order, in all `pools` (as above), and the rows' entries with them; pages from `used` on are free then,
+ * and the pools may be cut there.  The caller has to name every pool of the table, or what it leaves out is lost.  Asynchronous on `stream`;
+ * needs scratch of 12 bytes per page (in a stream capture as psx_b200_beam_select). */
+PSX_API psx_status psx_b200_compact_pages(psx_ctx* ctx, void* stream, const psx_page_table* table, const psx_page_pool* pools,
+                                          int64_t pool_count, int64_t* used);
 
 /* Replace DeviceBackend::softmax_rows, logsumexp_rows and gather_rows
  * (include/pulsatrix/device_backend.hpp:456,465,596; CUDA implementations src/cuda_backend.cu with

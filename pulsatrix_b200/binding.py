@@ -23,6 +23,7 @@ EXPORTS = [
     "psx_b200_exchange_sample", "psx_b200_exchange_results", "psx_b200_exchange_test_wait",
     "psx_b200_top_k_rows", "psx_b200_lm_head_logits", "psx_b200_lm_head_sample_rows", "psx_b200_softmax_rows", "psx_b200_logsumexp_rows", "psx_b200_gather_rows", "psx_b200_decode_attention",
     "psx_b200_beam_select", "psx_b200_reorder_states", "psx_b200_store_cache_8bit", "psx_b200_decode_attention_8bit", "psx_b200_prompt_attention",
+    "psx_b200_extend_pages", "psx_b200_fork_pages", "psx_b200_release_pages", "psx_b200_compact_pages",
     "psx_uniforms_mt19937_64", "psx_uniforms_portable",
 ]
 
@@ -85,6 +86,13 @@ class Cache8bitLayout(C.Structure):
 
     _fields_ = [("key_codes", C.c_void_p), ("key_scales", C.c_void_p), ("value_codes", C.c_void_p), ("value_scales", C.c_void_p),
                 ("batch", C.c_int64), ("kv_heads", C.c_int64), ("max_len", C.c_int64), ("head_dim", C.c_int64), ("block", C.c_int64)]
+
+
+class PageTableLayout(C.Structure):
+    """psx_page_table."""
+
+    _fields_ = [("pages", C.c_void_p), ("lengths", C.c_void_p), ("references", C.c_void_p), ("rows", C.c_int64), ("max_pages", C.c_int64),
+                ("num_pages", C.c_int64), ("page_size", C.c_int64)]
 
 
 _lib = None
@@ -158,6 +166,10 @@ def library():
         lib.psx_b200_decode_attention_8bit.argtypes = [ptr, ptr, ptr, C.c_int32, ptr, ptr, ptr, i64, i64, C.c_float, C.c_int32, i64]
         lib.psx_b200_prompt_attention.argtypes = [ptr, ptr, C.c_int32, ptr, ptr, ptr, ptr, i64, i64, i64, i64, i64, ptr, ptr, i64, i64, i64, i64,
                                                   C.c_float, C.c_int32, i64, ptr]
+        lib.psx_b200_extend_pages.argtypes = [ptr, ptr, ptr, ptr, ptr, i64, ptr]
+        lib.psx_b200_fork_pages.argtypes = [ptr, ptr, ptr, ptr, i64]
+        lib.psx_b200_release_pages.argtypes = [ptr, ptr, ptr, ptr]
+        lib.psx_b200_compact_pages.argtypes = [ptr, ptr, ptr, ptr, i64, ptr]
         lib.psx_uniforms_mt19937_64.argtypes = [ptr, i64, ptr]
         lib.psx_uniforms_portable.argtypes = [ptr, i64, ptr]
         from . import _native as native
@@ -305,6 +317,35 @@ class Cache8bit:
     def states(self):
         """Its tensors as Context.reorder_states takes them."""
         return [(self.key_codes, 1), (self.key_scales, self.block), (self.value_codes, 1), (self.value_scales, self.block)]
+
+
+class PageTable:
+    """The table of a cache in pages (psx_page_table) over tensors of the caller's: pages int32 (rows, max_pages), lengths int64 (rows),
+    references int32 (num_pages), all contiguous."""
+
+    def __init__(self, pages, lengths, references, page_size=64):
+        torch = _torch or _torch_module()
+        shape = pages.shape
+        if len(shape) != 2 or pages.dtype is not torch.int32 or not pages.is_contiguous():
+            raise ValueError("pages are contiguous int32 (rows, max_pages)")
+        rows, max_pages = shape
+        if not (lengths.dtype is torch.int64 and lengths.numel() == rows and lengths.is_contiguous() and references.dtype is torch.int32 and
+                references.is_contiguous()):
+            raise ValueError("lengths are int64 (rows), references int32 (num_pages)")
+        self.device = device = pages.get_device()
+        if not device == lengths.get_device() == references.get_device():
+            raise ValueError("a page table lies on one device")
+        self.pages, self.lengths, self.references = pages, lengths, references
+        self.rows, self.max_pages, self.num_pages, self.page_size = rows, max_pages, references.numel(), page_size
+        self._layout = PageTableLayout(pages.data_ptr(), lengths.data_ptr(), references.data_ptr(), rows, max_pages, self.num_pages, page_size)
+        self._address = C.addressof(self._layout)
+
+    @classmethod
+    def empty(cls, rows, max_pages, num_pages, page_size=64, device="cuda"):
+        """One whose rows hold nothing and whose pages are free."""
+        import torch
+        return cls(torch.full((rows, max_pages), -1, dtype=torch.int32, device=device), torch.zeros(rows, dtype=torch.int64, device=device),
+                   torch.zeros(num_pages, dtype=torch.int32, device=device), page_size)
 
 
 class Context:
@@ -724,6 +765,72 @@ class Context:
         if code:
             _check(code)
         return out, status
+
+    # ---- a cache in pages ---------------------------------------------------------------------------------
+    def _pools(self, table, pools):
+        """The pools as psx_page_pool (three words each)."""
+        described, num_pages, page_size, here = [], table.num_pages, table.page_size, self.device
+        for pool in pools:
+            shape = pool.shape
+            if len(shape) < 3 or shape[0] != num_pages or shape[2] != page_size or not pool.is_contiguous():
+                raise ValueError("a pool is a contiguous (num_pages, heads, page_size, ...) tensor")
+            if pool.get_device() != here:
+                raise self._elsewhere(pool)
+            described += (pool.data_ptr(), shape[1], pool.element_size() * (shape[3] if len(shape) == 4 else math.prod(shape[3:])))
+        return array.array("q", described)
+
+    def extend_pages(self, table, added, pools=(), stream=None):
+        """Room for new positions (psx_b200_extend_pages): the rows of a PageTable hold added (int64, rows) more afterwards.  pools: the tensors
+        (num_pages, heads, page_size, ...) of the cache, in which shared last pages are copied.  Returns the rows' statuses, int32."""
+        torch = _torch or _torch_module()
+        rows = table.rows
+        if not (added.dtype is torch.int64 and added.numel() == rows and added.is_contiguous()):
+            raise ValueError("one int64 number of new positions per row")
+        if not table.device == self.device == added.get_device():
+            self._here(table.pages, added)
+        described = self._pools(table, pools)
+        status = self._empty((rows,), torch.int32)
+        code = _native.extend_pages(self._handle, _stream_of(added) if stream is None else stream, table._address, added.data_ptr(),
+                                    described.buffer_info()[0], len(pools), status.data_ptr())
+        if code:
+            _check(code)
+        return status
+
+    def fork_pages(self, table, parents, stream=None):
+        """Rows of a PageTable that follow their beams by sharing pages (psx_b200_fork_pages).  parents: int64 (groups, beams)."""
+        torch = _torch or _torch_module()
+        if not (parents.dim() == 2 and parents.dtype is torch.int64 and parents.is_contiguous() and parents.numel() == table.rows):
+            raise ValueError("parents are contiguous int64 (groups, beams), one per row")
+        if not table.device == self.device == parents.get_device():
+            self._here(table.pages, parents)
+        code = _native.fork_pages(self._handle, _stream_of(parents) if stream is None else stream, table._address, parents.data_ptr(), parents.shape[1])
+        if code:
+            _check(code)
+
+    def release_pages(self, table, keep=None, stream=None):
+        """Positions given back (psx_b200_release_pages): rows keep their first keep (int64, rows), or none."""
+        torch = _torch or _torch_module()
+        if keep is not None and not (keep.dtype is torch.int64 and keep.numel() == table.rows and keep.is_contiguous()):
+            raise ValueError("one int64 number of positions per row")
+        if not table.device == self.device == (self.device if keep is None else keep.get_device()):
+            self._here(table.pages, *(() if keep is None else (keep,)))
+        code = _native.release_pages(self._handle, _stream_of(table.pages) if stream is None else stream, table._address,
+                                     None if keep is None else keep.data_ptr())
+        if code:
+            _check(code)
+
+    def compact_pages(self, table, pools, stream=None):
+        """Brings the pages in use of all pools to their beginning (psx_b200_compact_pages).  Returns how many there are, int64 (1)."""
+        torch = _torch or _torch_module()
+        if table.device != self.device:
+            self._here(table.pages)
+        described = self._pools(table, pools)
+        used = self._empty((1,), torch.int64)
+        code = _native.compact_pages(self._handle, _stream_of(table.pages) if stream is None else stream, table._address, described.buffer_info()[0],
+                                     len(pools), used.data_ptr())
+        if code:
+            _check(code)
+        return used
 
     # ---- vocabulary-sharded -----------------------------------------------------------------------------
     def shard_record_bytes(self, config) -> int:

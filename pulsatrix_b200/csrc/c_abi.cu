@@ -16,6 +16,7 @@
 #include "elements.cuh"
 #include "lm_head.cuh"
 #include "merge_rows.cuh"
+#include "page_table.cuh"
 #include "peer_exchange.cuh"
 #include "decode_attention.cuh"
 #include "process_rows.cuh"
@@ -92,7 +93,7 @@ struct psx_ctx {
     // staging of the sharded path
     Buffer shard_uniform_scratch;
     // Scratch that captured graphs may hold: what a capture has used stays allocated until the context goes (see reserve_kept).
-    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts;
+    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts, page_copies, page_moves;
     std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
     bool timing = false;
@@ -450,7 +451,7 @@ void psx_b200_ctx_destroy(psx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Buffer* b : {&ctx->stats[0], &ctx->stats[1], &ctx->part_counts[0], &ctx->part_counts[1], &ctx->candidates[0], &ctx->candidates[1], &ctx->banned, &ctx->sort_keys, &ctx->head_logits, &ctx->attention_partial, &ctx->surv_cols, &ctx->surv_vals,
                       &ctx->surv_counts, &ctx->pl_tokens, &ctx->pl_log_probs, &ctx->pl_status, &ctx->h_logits, &ctx->h_inputs,
-                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts}) {
+                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts, &ctx->page_copies, &ctx->page_moves}) {
         if (b->ptr) cudaFree(b->ptr);
     }
     for (void* p : ctx->outgrown) cudaFree(p);
@@ -1414,6 +1415,156 @@ psx_status psx_b200_prompt_attention(psx_ctx* ctx, void* stream_ptr, int32_t dty
     ctx->launches += launches;
     if (e == cudaErrorNotSupported) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: the driver has no tensor maps");
     PSX_CUDA(e);
+    return PSX_OK;
+}
+
+// ---- a cache in pages -----------------------------------------------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+psx_status check_page_table(const psx_page_table* t, psx::PageTableView* view) {
+    if (!t) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (t->rows < 0 || t->max_pages <= 0 || t->num_pages <= 0 || t->page_size <= 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: page table sizes must be positive");
+    }
+    if ((t->page_size != 16 && t->page_size != 32 && t->page_size != 64 && t->page_size != 128) || t->rows > psx::kMostPageRows ||
+        t->num_pages > (1 << 30) || t->max_pages > (1 << 30) / t->page_size) {
+        return fail(PSX_ERR_UNSUPPORTED,
+                    "psx_b200: a cache in pages has pages of 16, 32, 64 or 128 positions, at most 4096 rows, 2^30 pages and 2^30 positions of a row");
+    }
+    if (t->rows > 0 && (!t->pages || !t->lengths || !t->references)) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    const int size = (int)t->page_size;
+    *view = {t->pages, t->lengths, t->references, (int32_t)t->rows, (int32_t)t->max_pages, (int32_t)t->num_pages, size,
+             size == 16 ? 4 : size == 32 ? 5 : size == 64 ? 6 : 7};
+    return PSX_OK;
+}
+
+// The bytes that a call on pools touches, none of them twice.
+psx_status check_page_pools(const psx_page_table* t, const psx_page_pool* pools, int64_t count) {
+    if (count < 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the number of pools must not be negative");
+    if (count > 65536) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: at most 65,536 pools in a call");
+    if (count > 0 && !pools) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    std::vector<std::pair<uintptr_t, uintptr_t>> ranges;
+    ranges.reserve((size_t)count + 3);
+    for (int64_t i = 0; i < count; ++i) {
+        const psx_page_pool& p = pools[i];
+        if (p.heads <= 0 || p.position_bytes <= 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: pool sizes must be positive");
+        if (p.heads > 65536 || p.position_bytes > (1 << 30) / t->page_size / p.heads) {
+            return fail(PSX_ERR_UNSUPPORTED, "psx_b200: a page takes at most 65,536 heads and 2^30 bytes");
+        }
+        if (!p.data) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p.data);
+        ranges.emplace_back(at, at + (uintptr_t)(p.heads * p.position_bytes * t->page_size) * (uintptr_t)t->num_pages);
+    }
+    const auto add = [&](const void* p, int64_t bytes) {
+        ranges.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes);
+    };
+    add(t->pages, t->rows * t->max_pages * (int64_t)sizeof(int32_t));
+    add(t->lengths, t->rows * (int64_t)sizeof(int64_t));
+    add(t->references, t->num_pages * (int64_t)sizeof(int32_t));
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i) {
+        if (ranges[i].first < ranges[i - 1].second) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: pools overlap each other or the page table");
+    }
+    return PSX_OK;
+}
+
+// Runs `launch` for all pools, as many at a time as a launch takes; once at least where `always`.
+template <class Launch>
+cudaError_t for_pools(const psx_page_pool* pools, int64_t count, bool always, uint64_t& launches, Launch launch) {
+    psx::PagePools some;
+    some.count = 0;
+    bool first = true;
+    for (int64_t i = 0; i < count || (always && first); ++i) {
+        if (i < count) some.pool[some.count++] = {static_cast<char*>(pools[i].data), pools[i].heads, pools[i].position_bytes, 0};
+        if (some.count == psx::kPoolsPerLaunch || i + 1 >= count) {
+            if (const cudaError_t e = launch(some, first)) return e;
+            ++launches;
+            first = false;
+            some.count = 0;
+        }
+    }
+    return cudaSuccess;
+}
+}  // namespace
+
+extern "C" {
+
+psx_status psx_b200_extend_pages(psx_ctx* ctx, void* stream_ptr, const psx_page_table* table, const int64_t* added, const psx_page_pool* pools,
+                                 int64_t pool_count, int32_t* row_status) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    psx::ExtendPagesParams p{};
+    if (psx_status s = check_page_table(table, &p.table)) return s;
+    if (psx_status s = check_page_pools(table, pools, pool_count)) return s;
+    if (table->rows == 0) return PSX_OK;
+    if (!added) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    bool capturing;
+    if (psx_status s = is_capturing(stream, &capturing)) return s;
+    if (psx_status s = reserve_kept(ctx, capturing, ctx->page_copies, (size_t)table->rows * sizeof(psx::PageCopy))) return s;
+    p.added = added; p.row_status = row_status; p.copies = static_cast<psx::PageCopy*>(ctx->page_copies.ptr);
+    PSX_CUDA(psx::launch_extend_pages(p, stream));
+    ctx->launches += 1;
+    PSX_CUDA(for_pools(pools, pool_count, false, ctx->launches,
+                       [&](psx::PagePools& some, bool) { return psx::launch_copy_last_pages(p, some, ctx->sm_count, stream); }));
+    return PSX_OK;
+}
+
+psx_status psx_b200_fork_pages(psx_ctx* ctx, void* stream_ptr, const psx_page_table* table, const int64_t* parents, int64_t beams) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    psx::ForkPagesParams p{};
+    if (psx_status s = check_page_table(table, &p.table)) return s;
+    if (beams <= 0 || table->rows % beams != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the rows of a page table must be groups of beams");
+    if (beams > psx::kMostSharingBeams) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: pages follow at most 64 beams");
+    if (table->rows == 0) return PSX_OK;
+    if (!parents) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    p.parents = parents; p.beams = (int32_t)beams; p.groups = (int32_t)(table->rows / beams);
+    PSX_CUDA(psx::launch_fork_pages(p, static_cast<cudaStream_t>(stream_ptr)));
+    ctx->launches += 1;
+    return PSX_OK;
+}
+
+psx_status psx_b200_release_pages(psx_ctx* ctx, void* stream_ptr, const psx_page_table* table, const int64_t* keep) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    psx::ReleasePagesParams p{};
+    if (psx_status s = check_page_table(table, &p.table)) return s;
+    if (table->rows == 0) return PSX_OK;
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    p.keep = keep;
+    PSX_CUDA(psx::launch_release_pages(p, static_cast<cudaStream_t>(stream_ptr)));
+    ctx->launches += 1;
+    return PSX_OK;
+}
+
+psx_status psx_b200_compact_pages(psx_ctx* ctx, void* stream_ptr, const psx_page_table* table, const psx_page_pool* pools, int64_t pool_count,
+                                  int64_t* used) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    psx::CompactPagesParams p{};
+    if (psx_status s = check_page_table(table, &p.table)) return s;
+    if (psx_status s = check_page_pools(table, pools, pool_count)) return s;
+    if (!used) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (!table->references) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    bool capturing;
+    if (psx_status s = is_capturing(stream, &capturing)) return s;
+    if (psx_status s = reserve_kept(ctx, capturing, ctx->page_moves, psx::compact_scratch_bytes(table->num_pages))) return s;
+    p.used = used;
+    p.from = static_cast<int32_t*>(ctx->page_moves.ptr);
+    p.to = p.from + table->num_pages;
+    p.moved_to = p.to + table->num_pages;
+    p.moves = p.moved_to + table->num_pages;
+    PSX_CUDA(psx::launch_compact_pages(p, stream));
+    ctx->launches += 1;
+    PSX_CUDA(for_pools(pools, pool_count, true, ctx->launches,
+                       [&](psx::PagePools& some, bool first) { return psx::launch_move_pages(p, some, first, ctx->sm_count, stream); }));
     return PSX_OK;
 }
 

@@ -128,3 +128,13 @@ def test_beam_and_cache_entry_points_check_their_arguments_before_touching_a_gpu
     # as a C compiler lays out psx_beam_state and psx_cache_8bit
     assert C.sizeof(binding.BeamState) == 40 and C.sizeof(binding.Cache8bitLayout) == 72
     assert lib.psx_b200_prompt_attention(None, None, 0, None, None, None, None, 0, 0, 0, 0, 0, None, None, 0, 1, 1, 8, 1.0, 1, 0, None) == binding.ERR_BAD_ARGUMENT
+
+
+def test_page_entry_points_check_their_arguments_before_touching_a_gpu(lib):
+    table = binding.PageTableLayout()
+    at = C.addressof(table)
+    assert lib.psx_b200_extend_pages(None, None, at, None, None, 0, None) == binding.ERR_BAD_ARGUMENT
+    assert lib.psx_b200_fork_pages(None, None, at, None, 1) == binding.ERR_BAD_ARGUMENT
+    assert lib.psx_b200_release_pages(None, None, at, None) == binding.ERR_BAD_ARGUMENT
+    assert lib.psx_b200_compact_pages(None, None, at, None, 0, None) == binding.ERR_BAD_ARGUMENT
+    assert C.sizeof(binding.PageTableLayout) == 56  # (psx_page_table)
