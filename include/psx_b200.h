@@ -55,7 +55,7 @@ typedef enum psx_row_status {
                                 row is decided from the row itself */
     PSX_ROW_DEVICE_TIMEOUT = 32, /* a bounded device-side wait (a bulk copy of a piece of the row into
                                 shared memory) ran out; nothing was drawn for this row */
-    PSX_ROW_CACHE_FULL = 64,  /* psx_b200_store_cache_8bit, psx_b200_extend_pages: the row's new positions do not fit; none was stored, or
+    PSX_ROW_CACHE_FULL = 64,  /* psx_b200_store_cache_8bit, psx_b200_extend_pages, psx_b200_rotate_heads: the row's new positions do not fit; none was stored, or
                                  no room made */
     PSX_ROW_BAD_OFFSETS = 65  /* the same: the row's offsets, its filled length or the number of its new positions make no sense */
 } psx_row_status;
@@ -498,6 +498,37 @@ PSX_API psx_status psx_b200_release_pages(psx_ctx* ctx, void* stream, const psx_
  * needs scratch of 12 bytes per page (in a stream capture as psx_b200_beam_select). */
 PSX_API psx_status psx_b200_compact_pages(psx_ctx* ctx, void* stream, const psx_page_table* table, const psx_page_pool* pools,
                                           int64_t pool_count, int64_t* used);
+
+/* A layer's cache in pages: its table and its two pools, (num_pages, kv_heads, page_size, head_dim) each of the `dtype` that the call names,
+ * 16-byte aligned.  head_dim is a multiple of 8 up to 256 (else PSX_ERR_UNSUPPORTED). */
+typedef struct psx_paged_cache {
+    psx_page_table table;
+    void* key_pages;
+    void* value_pages;
+    int64_t kv_heads, head_dim;
+} psx_paged_cache;
+
+/* Queries and keys on their way from a projection into the attention, in one pass: what MultiHeadAttentionModule::forward_cached does between them
+ * (src/multihead_attention_module.cpp: norm of queries and keys per head, rotation, append to the cache), for packed rows of different lengths and
+ * a cache in pages.  q: device, `dtype`, (total, heads, head_dim), a position at q + i * q_stride elements, its heads contiguous; k, v: (total, kv_heads,
+ * head_dim), likewise (slices of one projection will do).  Row b's new positions are offsets[b] .. offsets[b + 1] (device int64, batch + 1,
+ * ascending), and they are positions first[b] onwards of the row (device int64, batch).
+ *   norm      with q_weight or k_weight (device, `dtype`, head_dim): x / sqrt(mean(x^2) + eps) * weight for every head; NULL: none.  Squares are
+ *             added in floats (magnitudes beyond 2^60 or so overflow).
+ *   rotation  of the first `rotated` dimensions: pair j, of dimensions (j, j + rotated / 2) or, `interleaved`, (2 j, 2 j + 1), turns by position *
+ *             frequencies[j] (device double, rotated / 2; NULL with rotated == 0), the angle taken in double precision.
+ *   results   q_out (total, heads, head_dim), contiguous, may be q itself if that is; k_out (total, kv_heads, head_dim), likewise, or NULL; with `cache` (a
+ *             row of its table for every row of the batch, the lengths already those that hold the new positions, see psx_b200_extend_pages) keys and
+ *             values go into its pages, too (v is not read otherwise).  Rounded once.  Positions of no row are left as they were.
+ * row_status: device int32 (batch), may be NULL: PSX_ROW_OK; PSX_ROW_CACHE_FULL: the row's last new position is beyond its length in the table; none was stored;
+ * PSX_ROW_BAD_OFFSETS: offsets or first make no sense; none was stored.  A page number outside the pool takes nothing.
+ * Pointers 16-byte aligned, strides a multiple of 16 bytes.  Limits: head_dim a multiple of 8 up to 256, rotated a multiple of 8 up to head_dim, batch <= 4096,
+ * total <= 2^29 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`. */
+PSX_API psx_status psx_b200_rotate_heads(psx_ctx* ctx, void* stream, int32_t dtype, const void* q, const void* k, const void* v, void* q_out,
+                                         void* k_out, int64_t total, int64_t q_stride, int64_t k_stride, int64_t v_stride, const int64_t* offsets,
+                                         const int64_t* first, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                         const void* q_weight, const void* k_weight, float eps, const double* frequencies, int64_t rotated,
+                                         int32_t interleaved, const psx_paged_cache* cache, int32_t* row_status);
 
 /* Replace DeviceBackend::softmax_rows, logsumexp_rows and gather_rows
  * (include/pulsatrix/device_backend.hpp:456,465,596; CUDA implementations src/cuda_backend.cu with

@@ -23,7 +23,7 @@ EXPORTS = [
     "psx_b200_exchange_sample", "psx_b200_exchange_results", "psx_b200_exchange_test_wait",
     "psx_b200_top_k_rows", "psx_b200_lm_head_logits", "psx_b200_lm_head_sample_rows", "psx_b200_softmax_rows", "psx_b200_logsumexp_rows", "psx_b200_gather_rows", "psx_b200_decode_attention",
     "psx_b200_beam_select", "psx_b200_reorder_states", "psx_b200_store_cache_8bit", "psx_b200_decode_attention_8bit", "psx_b200_prompt_attention",
-    "psx_b200_extend_pages", "psx_b200_fork_pages", "psx_b200_release_pages", "psx_b200_compact_pages",
+    "psx_b200_extend_pages", "psx_b200_fork_pages", "psx_b200_release_pages", "psx_b200_compact_pages", "psx_b200_rotate_heads",
     "psx_uniforms_mt19937_64", "psx_uniforms_portable",
 ]
 
@@ -93,6 +93,12 @@ class PageTableLayout(C.Structure):
 
     _fields_ = [("pages", C.c_void_p), ("lengths", C.c_void_p), ("references", C.c_void_p), ("rows", C.c_int64), ("max_pages", C.c_int64),
                 ("num_pages", C.c_int64), ("page_size", C.c_int64)]
+
+
+class PagedCacheLayout(C.Structure):
+    """psx_paged_cache."""
+
+    _fields_ = [("table", PageTableLayout), ("key_pages", C.c_void_p), ("value_pages", C.c_void_p), ("kv_heads", C.c_int64), ("head_dim", C.c_int64)]
 
 
 _lib = None
@@ -170,6 +176,8 @@ def library():
         lib.psx_b200_fork_pages.argtypes = [ptr, ptr, ptr, ptr, i64]
         lib.psx_b200_release_pages.argtypes = [ptr, ptr, ptr, ptr]
         lib.psx_b200_compact_pages.argtypes = [ptr, ptr, ptr, ptr, i64, ptr]
+        lib.psx_b200_rotate_heads.argtypes = [ptr, ptr, C.c_int32, ptr, ptr, ptr, ptr, ptr, i64, i64, i64, i64, ptr, ptr, i64, i64, i64, i64, ptr, ptr,
+                                              C.c_float, ptr, i64, C.c_int32, ptr, ptr]
         lib.psx_uniforms_mt19937_64.argtypes = [ptr, i64, ptr]
         lib.psx_uniforms_portable.argtypes = [ptr, i64, ptr]
         from . import _native as native
@@ -346,6 +354,29 @@ class PageTable:
         import torch
         return cls(torch.full((rows, max_pages), -1, dtype=torch.int32, device=device), torch.zeros(rows, dtype=torch.int64, device=device),
                    torch.zeros(num_pages, dtype=torch.int32, device=device), page_size)
+
+
+class PagedCache:
+    """A layer's cache in pages (psx_paged_cache): a PageTable and two tensors of the caller's, keys and values (num_pages, kv_heads, page_size,
+    head_dim), float32, bfloat16 or float16, contiguous."""
+
+    def __init__(self, table, key_pages, value_pages):
+        shape = key_pages.shape
+        if len(shape) != 4 or shape[0] != table.num_pages or shape[2] != table.page_size:
+            raise ValueError("pages are (num_pages, kv_heads, page_size, head_dim)")
+        if not (value_pages.shape == shape and key_pages.dtype is value_pages.dtype and key_pages.is_contiguous() and value_pages.is_contiguous()):
+            raise ValueError("keys and values are contiguous tensors of one shape and type")
+        if not table.device == key_pages.get_device() == value_pages.get_device():
+            raise ValueError("a cache lies on one device")
+        self.dtype_code = _dtype_code(key_pages)
+        self.table, self.key_pages, self.value_pages = table, key_pages, value_pages
+        self.device, self.kv_heads, self.head_dim = table.device, shape[1], shape[3]
+        self._layout = PagedCacheLayout(table._layout, key_pages.data_ptr(), value_pages.data_ptr(), shape[1], shape[3])
+        self._address = C.addressof(self._layout)
+
+    def pools(self):
+        """Its tensors as Context.extend_pages and compact_pages take them."""
+        return [self.key_pages, self.value_pages]
 
 
 class Context:
@@ -831,6 +862,62 @@ class Context:
         if code:
             _check(code)
         return used
+
+    def rotate_heads(self, q, k, v=None, *, offsets, first, frequencies=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, cache=None,
+                     keys_too=None, stream=None):
+        """Queries and keys on their way into the attention (psx_b200_rotate_heads): norm per head (q_weight, k_weight: (head_dim)), rotation by the
+        position (frequencies: float64, one per pair of dimensions), keys and values into a PagedCache.  q: float32, bfloat16 or float16 (total, heads,
+        head_dim); k, v: (total, kv_heads, head_dim); heads and dimensions of a position contiguous; offsets: int64 (batch + 1); first: int64
+        (batch), the position of a row's first new one.  Returns q and k as they are then (k only with keys_too, which is so without a cache) and the
+        rows' statuses, int32."""
+        torch = _torch or _torch_module()
+        if keys_too is None:
+            keys_too = cache is None
+        q_shape, k_shape = q.shape, k.shape
+        total, heads, head_dim = q_shape
+        kv_heads = k_shape[1]
+        if not (k_shape == (total, kv_heads, head_dim) and q.dtype is k.dtype):
+            raise ValueError("q and k are (total, heads, head_dim) of one type")
+        q_stride, k_stride, v_stride = q.stride(), k.stride(), k.stride()
+        here = self.device
+        if cache is not None:
+            if v is None or v.shape != k_shape or v.dtype is not k.dtype or cache.dtype_code != _dtype_code(k):
+                raise ValueError("what a cache stores is k and v of one shape and of its type")
+            v_stride = v.stride()
+            if not cache.device == here == v.get_device():
+                self._here(cache.key_pages, v)
+        if total and not (q_stride[2] == k_stride[2] == v_stride[2] == 1 and (heads == 1 or q_stride[1] == head_dim) and
+                          (kv_heads == 1 or k_stride[1] == v_stride[1] == head_dim)):
+            raise ValueError("heads and dimensions of a position are contiguous")
+        batch = offsets.numel() - 1
+        if not (offsets.dtype is first.dtype is torch.int64 and batch >= 0 and first.numel() == batch and offsets.is_contiguous() and first.is_contiguous()):
+            raise ValueError("offsets are int64 (batch + 1), first is int64 (batch)")
+        if not q.get_device() == here == k.get_device() == offsets.get_device() == first.get_device():
+            self._here(q, k, offsets, first)
+        rotated = 0
+        if frequencies is not None:
+            if not (frequencies.dtype is torch.float64 and frequencies.is_contiguous()):
+                raise ValueError("frequencies are contiguous float64")
+            self._here(frequencies)
+            rotated = 2 * frequencies.numel()
+        for weight in (q_weight, k_weight):
+            if weight is not None:
+                if not (weight.dtype is q.dtype and weight.numel() == head_dim and weight.is_contiguous()):
+                    raise ValueError("a norm's weight is (head_dim), of q's type")
+                self._here(weight)
+        q_out = torch.empty_like(q) if q.is_contiguous() else self._empty((total, heads, head_dim), q.dtype)
+        k_out = self._empty((total, kv_heads, head_dim), k.dtype) if keys_too else None
+        status = self._empty((batch,), torch.int32)
+        many = total > 1
+        width = kv_heads * head_dim
+        code = _native.rotate_heads(self._handle, _stream_of(q) if stream is None else stream, _dtype_code(q), q.data_ptr(), k.data_ptr(),
+                                    None if v is None else v.data_ptr(), q_out.data_ptr(), None if k_out is None else k_out.data_ptr(), total,
+                                    q_stride[0] if many else heads * head_dim, k_stride[0] if many else width, v_stride[0] if many else width,
+                                    offsets.data_ptr(), first.data_ptr(), batch, heads, kv_heads, head_dim, _ptr(q_weight), _ptr(k_weight), eps,
+                                    _ptr(frequencies), rotated, 1 if interleaved else 0, None if cache is None else cache._address, status.data_ptr())
+        if code:
+            _check(code)
+        return q_out, k_out, status
 
     # ---- vocabulary-sharded -----------------------------------------------------------------------------
     def shard_record_bytes(self, config) -> int:

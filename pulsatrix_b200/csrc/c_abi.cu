@@ -22,6 +22,7 @@
 #include "process_rows.cuh"
 #include "prompt_attention.cuh"
 #include "reorder_states.cuh"
+#include "rotate_heads.cuh"
 #include "row_prefix.cuh"
 #include "row_ops.cuh"
 #include "sample_plan.cuh"
@@ -1470,6 +1471,25 @@ psx_status check_page_pools(const psx_page_table* t, const psx_page_pool* pools,
     return PSX_OK;
 }
 
+psx_status check_paged_cache(const psx_paged_cache* c, int32_t dtype, psx::PagedCacheView* view) {
+    if (!c) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (psx_status s = check_page_table(&c->table, &view->table)) return s;
+    if (c->kv_heads <= 0 || c->head_dim <= 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: cache sizes must be positive");
+    if (c->head_dim % 8 != 0 || c->head_dim > 256 || c->kv_heads > 65536 ||
+        c->kv_heads * c->head_dim * c->table.page_size * psx::element_bytes(dtype) > (1 << 30)) {
+        return fail(PSX_ERR_UNSUPPORTED, "psx_b200: a cache in pages has a head dimension that is a multiple of 8 up to 256, and pages of at most 2^30 bytes");
+    }
+    if (!c->key_pages || !c->value_pages) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if ((reinterpret_cast<uintptr_t>(c->key_pages) | reinterpret_cast<uintptr_t>(c->value_pages)) % 16 != 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the cache must start on a 16-byte boundary");
+    }
+    view->keys = static_cast<char*>(c->key_pages);
+    view->values = static_cast<char*>(c->value_pages);
+    view->kv_heads = (int32_t)c->kv_heads;
+    view->head_dim = (int32_t)c->head_dim;
+    return PSX_OK;
+}
+
 // Runs `launch` for all pools, as many at a time as a launch takes; once at least where `always`.
 template <class Launch>
 cudaError_t for_pools(const psx_page_pool* pools, int64_t count, bool always, uint64_t& launches, Launch launch) {
@@ -1565,6 +1585,50 @@ psx_status psx_b200_compact_pages(psx_ctx* ctx, void* stream_ptr, const psx_page
     ctx->launches += 1;
     PSX_CUDA(for_pools(pools, pool_count, true, ctx->launches,
                        [&](psx::PagePools& some, bool first) { return psx::launch_move_pages(p, some, first, ctx->sm_count, stream); }));
+    return PSX_OK;
+}
+
+psx_status psx_b200_rotate_heads(psx_ctx* ctx, void* stream_ptr, int32_t dtype, const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                                 int64_t total, int64_t q_stride, int64_t k_stride, int64_t v_stride, const int64_t* offsets, const int64_t* first,
+                                 int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, const void* q_weight, const void* k_weight, float eps,
+                                 const double* frequencies, int64_t rotated, int32_t interleaved, const psx_paged_cache* cache, int32_t* row_status) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
+    if (batch < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || total < 0 || rotated < 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: sizes of heads must be positive");
+    }
+    if (rotated > head_dim || rotated % 2 != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: pairs of at most head_dim dimensions are rotated");
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: eps must be finite and not negative");
+    if (head_dim % 8 != 0 || head_dim > 256 || rotated % 8 != 0 || batch > psx::kMostPageRows || total > (1 << 29) || heads > 65536 || kv_heads > 65536) {
+        return fail(PSX_ERR_UNSUPPORTED,
+                    "psx_b200: heads have a dimension that is a multiple of 8 up to 256, a multiple of 8 of it rotated; at most 4096 rows and 2^29 positions");
+    }
+    if (q_stride < heads * head_dim || k_stride < kv_heads * head_dim || (cache && v_stride < kv_heads * head_dim)) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: a position's stride is at least its heads times head_dim");
+    }
+    if (total > 0 && !cache && !k_out) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: keys go to k_out, into a cache, or both");
+    psx::RotateHeadsParams p{};
+    if (cache) {
+        if (psx_status s = check_paged_cache(cache, dtype, &p.cache)) return s;
+        if (cache->table.rows != batch || cache->kv_heads != kv_heads || cache->head_dim != head_dim) {
+            return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the cache has other rows, heads or dimensions");
+        }
+    }
+    if (batch == 0) return PSX_OK;
+    if (!offsets || !first || (rotated > 0 && !frequencies)) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (total > 0 && (!q || !k || !q_out || (cache && !v))) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    const uintptr_t lies = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | (cache ? reinterpret_cast<uintptr_t>(v) : 0) |
+                           reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(q_weight) |
+                           reinterpret_cast<uintptr_t>(k_weight) | (uintptr_t)((q_stride | k_stride | (cache ? v_stride : 0)) * psx::element_bytes(dtype));
+    if (lies % 16 != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: operands and their positions must start on 16-byte boundaries");
+    p.q = q; p.k = k; p.v = v; p.q_out = q_out; p.k_out = k_out; p.q_weight = q_weight; p.k_weight = k_weight; p.frequencies = frequencies;
+    p.offsets = offsets; p.first = first; p.row_status = row_status; p.total = total; p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride;
+    p.batch = (int32_t)batch; p.heads = (int32_t)heads; p.kv_heads = (int32_t)kv_heads; p.head_dim = (int32_t)head_dim; p.rotated = (int32_t)rotated;
+    p.interleaved = interleaved ? 1 : 0; p.type = dtype; p.eps = eps;
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    PSX_CUDA(psx::launch_rotate_heads(p, ctx->sm_count, static_cast<cudaStream_t>(stream_ptr)));
+    ctx->launches += 1;
     return PSX_OK;
 }
 

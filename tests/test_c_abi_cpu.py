@@ -138,3 +138,5 @@ def test_page_entry_points_check_their_arguments_before_touching_a_gpu(lib):
     assert lib.psx_b200_release_pages(None, None, at, None) == binding.ERR_BAD_ARGUMENT
     assert lib.psx_b200_compact_pages(None, None, at, None, 0, None) == binding.ERR_BAD_ARGUMENT
     assert C.sizeof(binding.PageTableLayout) == 56  # (psx_page_table)
+    assert lib.psx_b200_rotate_heads(None, None, 0, None, None, None, None, None, 0, 0, 0, 0, None, None, 0, 1, 1, 8, None, None, 0.0, None, 0, 0, None, None) == binding.ERR_BAD_ARGUMENT
+    assert C.sizeof(binding.PagedCacheLayout) == 88  # (psx_paged_cache)
