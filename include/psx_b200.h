@@ -530,6 +530,19 @@ PSX_API psx_status psx_b200_rotate_heads(psx_ctx* ctx, void* stream, int32_t dty
                                          const void* q_weight, const void* k_weight, float eps, const double* frequencies, int64_t rotated,
                                          int32_t interleaved, const psx_paged_cache* cache, int32_t* row_status);
 
+/* Attention of the new positions over a cache in pages, for rows of different lengths: what psx_b200_decode_attention_8bit does, for a
+ * cache of `dtype`.  q and context: device, `dtype`, (rows * q_len, heads, head_dim), contiguous, 16-byte aligned, a row's q_len new positions
+ * one behind the other (as psx_b200_rotate_heads leaves them); context apart from q.  Row b sees positions 0 .. lengths[b] - 1 of the
+ * cache's table, its new positions being the last of them (already stored).  New position i is position p = lengths[b] - q_len + i: with `causal` it
+ * sees no key j > p and, with window > 0, no key j + window <= p.  A query that sees nothing has the context 0; one whose visible scores are all -inf, as
+ * in any softmax, NaN; positions in a page number outside the pool have the score -inf.  Positions that no query of a row sees are not read; a
+ * NaN in a position that one of a row's new positions sees may reach the others.  Softmax statistics and sums are floats; bf16 and fp16: weights carry
+ * 16 and 22 bits (fp16's end at 2^-39 of the largest); fp32: products are exact to about 2^-22 (an infinity counts as NaN).
+ * Limit: (heads / kv_heads) * q_len <= 16 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; scratch in a stream capture as
+ * psx_b200_beam_select. */
+PSX_API psx_status psx_b200_decode_attention_pages(psx_ctx* ctx, void* stream, const void* q, int32_t dtype, const psx_paged_cache* cache,
+                                                   void* context, int64_t heads, int64_t q_len, float scale, int32_t causal, int64_t window);
+
 /* Replace DeviceBackend::softmax_rows, logsumexp_rows and gather_rows
  * (include/pulsatrix/device_backend.hpp:456,465,596; CUDA implementations src/cuda_backend.cu with
  * the kernels src/gpu_kernels.cuh:315-365,665; CPU semantics src/cpu_backend.cpp:292-338,459-466)

@@ -23,7 +23,7 @@ EXPORTS = [
     "psx_b200_exchange_sample", "psx_b200_exchange_results", "psx_b200_exchange_test_wait",
     "psx_b200_top_k_rows", "psx_b200_lm_head_logits", "psx_b200_lm_head_sample_rows", "psx_b200_softmax_rows", "psx_b200_logsumexp_rows", "psx_b200_gather_rows", "psx_b200_decode_attention",
     "psx_b200_beam_select", "psx_b200_reorder_states", "psx_b200_store_cache_8bit", "psx_b200_decode_attention_8bit", "psx_b200_prompt_attention",
-    "psx_b200_extend_pages", "psx_b200_fork_pages", "psx_b200_release_pages", "psx_b200_compact_pages", "psx_b200_rotate_heads",
+    "psx_b200_extend_pages", "psx_b200_fork_pages", "psx_b200_release_pages", "psx_b200_compact_pages", "psx_b200_rotate_heads", "psx_b200_decode_attention_pages",
     "psx_uniforms_mt19937_64", "psx_uniforms_portable",
 ]
 
@@ -178,6 +178,7 @@ def library():
         lib.psx_b200_compact_pages.argtypes = [ptr, ptr, ptr, ptr, i64, ptr]
         lib.psx_b200_rotate_heads.argtypes = [ptr, ptr, C.c_int32, ptr, ptr, ptr, ptr, ptr, i64, i64, i64, i64, ptr, ptr, i64, i64, i64, i64, ptr, ptr,
                                               C.c_float, ptr, i64, C.c_int32, ptr, ptr]
+        lib.psx_b200_decode_attention_pages.argtypes = [ptr, ptr, ptr, C.c_int32, ptr, ptr, i64, i64, C.c_float, C.c_int32, i64]
         lib.psx_uniforms_mt19937_64.argtypes = [ptr, i64, ptr]
         lib.psx_uniforms_portable.argtypes = [ptr, i64, ptr]
         from . import _native as native
@@ -918,6 +919,24 @@ class Context:
         if code:
             _check(code)
         return q_out, k_out, status
+
+    def decode_attention_pages(self, q, cache, q_len=1, scale=None, causal=True, window=0, stream=None):
+        """Attention of the new positions over a PagedCache (psx_b200_decode_attention_pages).  q: of the cache's type, (rows * q_len, heads, head_dim), a
+        row's new positions one behind the other; what the rows see is the table's lengths.  Returns the context, like q."""
+        torch = _torch or _torch_module()
+        total, heads, head_dim = q.shape
+        if not (total == cache.table.rows * q_len and head_dim == cache.head_dim and q.dtype is cache.key_pages.dtype and q.is_contiguous()):
+            raise ValueError("q is a contiguous (rows * q_len, heads, head_dim) of the cache's type")
+        if not cache.device == self.device == q.get_device():
+            self._here(q, cache.key_pages)
+        if scale is None:
+            scale = head_dim ** -0.5
+        context = torch.empty_like(q)
+        code = _native.decode_attention_pages(self._handle, _stream_of(q) if stream is None else stream, q.data_ptr(), cache.dtype_code, cache._address,
+                                              context.data_ptr(), heads, q_len, scale, 1 if causal else 0, window)
+        if code:
+            _check(code)
+        return context
 
     # ---- vocabulary-sharded -----------------------------------------------------------------------------
     def shard_record_bytes(self, config) -> int:

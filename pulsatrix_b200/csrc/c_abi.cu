@@ -13,6 +13,7 @@
 
 #include "beam_select.cuh"
 #include "decode_attention_8bit.cuh"
+#include "decode_attention_pages.cuh"
 #include "elements.cuh"
 #include "lm_head.cuh"
 #include "merge_rows.cuh"
@@ -94,7 +95,7 @@ struct psx_ctx {
     // staging of the sharded path
     Buffer shard_uniform_scratch;
     // Scratch that captured graphs may hold: what a capture has used stays allocated until the context goes (see reserve_kept).
-    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts, page_copies, page_moves;
+    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts, page_copies, page_moves, attention_pages_pieces, attention_pages_arrived;
     std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
     bool timing = false;
@@ -452,7 +453,7 @@ void psx_b200_ctx_destroy(psx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Buffer* b : {&ctx->stats[0], &ctx->stats[1], &ctx->part_counts[0], &ctx->part_counts[1], &ctx->candidates[0], &ctx->candidates[1], &ctx->banned, &ctx->sort_keys, &ctx->head_logits, &ctx->attention_partial, &ctx->surv_cols, &ctx->surv_vals,
                       &ctx->surv_counts, &ctx->pl_tokens, &ctx->pl_log_probs, &ctx->pl_status, &ctx->h_logits, &ctx->h_inputs,
-                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts, &ctx->page_copies, &ctx->page_moves}) {
+                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts, &ctx->page_copies, &ctx->page_moves, &ctx->attention_pages_pieces, &ctx->attention_pages_arrived}) {
         if (b->ptr) cudaFree(b->ptr);
     }
     for (void* p : ctx->outgrown) cudaFree(p);
@@ -1628,6 +1629,44 @@ psx_status psx_b200_rotate_heads(psx_ctx* ctx, void* stream_ptr, int32_t dtype, 
     const OnDevice device(ctx->device);
     PSX_CUDA(device.error);
     PSX_CUDA(psx::launch_rotate_heads(p, ctx->sm_count, static_cast<cudaStream_t>(stream_ptr)));
+    ctx->launches += 1;
+    return PSX_OK;
+}
+
+psx_status psx_b200_decode_attention_pages(psx_ctx* ctx, void* stream_ptr, const void* q, int32_t dtype, const psx_paged_cache* cache, void* context,
+                                           int64_t heads, int64_t q_len, float scale, int32_t causal, int64_t window) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    psx::PagedAttentionParams p{};
+    if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
+    if (psx_status s = check_paged_cache(cache, dtype, &p.cache)) return s;
+    if (heads <= 0 || q_len <= 0 || window < 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: attention sizes must be positive");
+    if (heads % cache->kv_heads != 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: heads must be a multiple of kv_heads");
+    if (!std::isfinite(scale)) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: the score scale must be finite");
+    const int64_t group = heads / cache->kv_heads;
+    if (group > 16 || q_len > 16 || group * q_len > 16) {
+        return fail(PSX_ERR_UNSUPPORTED, "psx_b200: attention over a cache in pages takes at most 16 query rows per kv head (group x new positions)");
+    }
+    if (p.cache.table.rows == 0) return PSX_OK;
+    if (!q || !context) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(context)) % 16 != 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: queries and context must start on a 16-byte boundary");
+    }
+    p.q = q; p.context = context; p.heads = (int32_t)heads; p.group = (int32_t)group; p.q_len = (int32_t)q_len; p.rows = (int32_t)(group * q_len);
+    p.type = dtype; p.causal = causal ? 1 : 0; p.scale = scale;
+    p.window = std::min<int64_t>(window, p.cache.table.capacity());  // (a wider one hides nothing more, and sums with it stay in range)
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    psx::plan_paged_attention(p, ctx->sm_count);
+    if (p.pieces > 1) {
+        bool capturing;
+        if (psx_status s = is_capturing(stream, &capturing)) return s;
+        if (psx_status s = reserve_kept(ctx, capturing, ctx->attention_pages_pieces, psx::paged_attention_partial_bytes(p))) return s;
+        if (psx_status s = reserve_counters(ctx, stream, capturing, ctx->attention_pages_arrived, (size_t)psx::paged_attention_counters(p))) return s;
+        p.partial = static_cast<float*>(ctx->attention_pages_pieces.ptr);
+        p.arrived = static_cast<int32_t*>(ctx->attention_pages_arrived.ptr);
+    }
+    PSX_CUDA(psx::launch_paged_attention(p, stream));
     ctx->launches += 1;
     return PSX_OK;
 }

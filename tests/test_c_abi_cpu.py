@@ -140,3 +140,5 @@ def test_page_entry_points_check_their_arguments_before_touching_a_gpu(lib):
     assert C.sizeof(binding.PageTableLayout) == 56  # (psx_page_table)
     assert lib.psx_b200_rotate_heads(None, None, 0, None, None, None, None, None, 0, 0, 0, 0, None, None, 0, 1, 1, 8, None, None, 0.0, None, 0, 0, None, None) == binding.ERR_BAD_ARGUMENT
     assert C.sizeof(binding.PagedCacheLayout) == 88  # (psx_paged_cache)
+    cache = binding.PagedCacheLayout()
+    assert lib.psx_b200_decode_attention_pages(None, None, None, 0, C.addressof(cache), None, 1, 1, 1.0, 1, 0) == binding.ERR_BAD_ARGUMENT
