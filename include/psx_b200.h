@@ -57,7 +57,8 @@ typedef enum psx_row_status {
                                 shared memory) ran out; nothing was drawn for this row */
     PSX_ROW_CACHE_FULL = 64,  /* psx_b200_store_cache_8bit, psx_b200_extend_pages, psx_b200_rotate_heads: the row's new positions do not fit; none was stored, or
                                  no room made */
-    PSX_ROW_BAD_OFFSETS = 65  /* the same: the row's offsets, its filled length or the number of its new positions make no sense */
+    PSX_ROW_BAD_OFFSETS = 65, /* the same: the row's offsets, its filled length or the number of its new positions make no sense */
+    PSX_ROW_BAD_TOKEN = 66    /* psx_b200_token_log_probs: the token is not in the vocabulary */
 } psx_row_status;
 
 /* GenerationConfig (include/pulsatrix/generation.hpp:29-52) without the loop fields, plus the
@@ -542,6 +543,25 @@ PSX_API psx_status psx_b200_rotate_heads(psx_ctx* ctx, void* stream, int32_t dty
  * psx_b200_beam_select. */
 PSX_API psx_status psx_b200_decode_attention_pages(psx_ctx* ctx, void* stream, const void* q, int32_t dtype, const psx_paged_cache* cache,
                                                    void* context, int64_t heads, int64_t q_len, float scale, int32_t causal, int64_t window);
+
+/* Log-probabilities of given tokens under the raw logits, with the rows' entropies and their largest alternatives: what psx_b200_sample_rows gives for
+ * the token that it draws, for any token and any type (scoring of a prompt, of another model's draft, of beams; no counterpart in the reference).
+ *   logits         device, `dtype`, row r at logits + r * row_stride elements (row_stride >= vocab; any alignment of the type)
+ *   tokens         device int64 (rows), or NULL: no log_probs
+ *   log_probs      device fp32 (rows): logits[r][tokens[r]] - log sum_w exp(logits[r][w])
+ *   entropy        device fp32 (rows), or NULL: -sum p log p
+ *   top_log_probs  device fp32 (rows, top), top_tokens device int64 (rows, top): the `top` largest, best first, of equal logits the lowest token;
+ *                  places that no token is left for get -inf, -1; top may be 0
+ *   row_status     device int32 (rows), may be NULL: PSX_ROW_OK; PSX_ROW_NON_FINITE: a NaN or +inf among the logits (all results NaN, tokens -1);
+ *                  PSX_ROW_ALL_REMOVED: every logit is -inf (results NaN, alternatives -inf, -1); PSX_ROW_BAD_TOKEN: the token is not in the
+ *                  vocabulary (log_probs NaN, the rest as ever)
+ * Logits of -inf have the probability 0.  Sums run over all logits but the largest, so that log-probabilities near 0 have their digits: with r the others'
+ * sum relative to the largest, log(1 + r) is off by less than 200 * 2^-24 of r / (1 + r), the entropy by less than 400 * 2^-24 of it.  The same call gives the same bits.
+ * Limits: top <= 128, vocab <= 2^30 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; the outputs must not overlap the inputs.  Needs scratch of rows *
+ * ceil(vocab / 1024) * (top * 8 + 16) + 4 * rows bytes at most (far less where there are many rows; in a stream capture as psx_b200_beam_select). */
+PSX_API psx_status psx_b200_token_log_probs(psx_ctx* ctx, void* stream, int32_t dtype, const void* logits, int64_t rows, int64_t vocab,
+                                            int64_t row_stride, const int64_t* tokens, float* log_probs, float* entropy, int64_t top,
+                                            float* top_log_probs, int64_t* top_tokens, int32_t* row_status);
 
 /* Replace DeviceBackend::softmax_rows, logsumexp_rows and gather_rows
  * (include/pulsatrix/device_backend.hpp:456,465,596; CUDA implementations src/cuda_backend.cu with

@@ -11,7 +11,7 @@ from pathlib import Path
 import numpy as np
 
 PACKAGE = Path(__file__).resolve().parent
-ROW_OK, ROW_NON_FINITE, ROW_ALL_REMOVED, ROW_TOO_WIDE, ROW_DEVICE_TIMEOUT, ROW_CACHE_FULL, ROW_BAD_OFFSETS = 0, 4, 5, 16, 32, 64, 65
+ROW_OK, ROW_NON_FINITE, ROW_ALL_REMOVED, ROW_TOO_WIDE, ROW_DEVICE_TIMEOUT, ROW_CACHE_FULL, ROW_BAD_OFFSETS, ROW_BAD_TOKEN = 0, 4, 5, 16, 32, 64, 65, 66
 OK, ERR_BAD_ARGUMENT, ERR_CUDA, ERR_ROW_FAILED, ERR_UNSUPPORTED = range(5)
 
 EXPORTS = [
@@ -24,6 +24,7 @@ EXPORTS = [
     "psx_b200_top_k_rows", "psx_b200_lm_head_logits", "psx_b200_lm_head_sample_rows", "psx_b200_softmax_rows", "psx_b200_logsumexp_rows", "psx_b200_gather_rows", "psx_b200_decode_attention",
     "psx_b200_beam_select", "psx_b200_reorder_states", "psx_b200_store_cache_8bit", "psx_b200_decode_attention_8bit", "psx_b200_prompt_attention",
     "psx_b200_extend_pages", "psx_b200_fork_pages", "psx_b200_release_pages", "psx_b200_compact_pages", "psx_b200_rotate_heads", "psx_b200_decode_attention_pages",
+    "psx_b200_token_log_probs",
     "psx_uniforms_mt19937_64", "psx_uniforms_portable",
 ]
 
@@ -179,6 +180,7 @@ def library():
         lib.psx_b200_rotate_heads.argtypes = [ptr, ptr, C.c_int32, ptr, ptr, ptr, ptr, ptr, i64, i64, i64, i64, ptr, ptr, i64, i64, i64, i64, ptr, ptr,
                                               C.c_float, ptr, i64, C.c_int32, ptr, ptr]
         lib.psx_b200_decode_attention_pages.argtypes = [ptr, ptr, ptr, C.c_int32, ptr, ptr, i64, i64, C.c_float, C.c_int32, i64]
+        lib.psx_b200_token_log_probs.argtypes = [ptr, ptr, C.c_int32, ptr, i64, i64, i64, ptr, ptr, ptr, i64, ptr, ptr, ptr]
         lib.psx_uniforms_mt19937_64.argtypes = [ptr, i64, ptr]
         lib.psx_uniforms_portable.argtypes = [ptr, i64, ptr]
         from . import _native as native
@@ -937,6 +939,39 @@ class Context:
         if code:
             _check(code)
         return context
+
+    # ---- log-probabilities of given tokens ----------------------------------------------------------------
+    def token_log_probs(self, logits, tokens=None, top=0, entropy=False, vocab=None, stream=None):
+        """Log-probabilities of given tokens (psx_b200_token_log_probs).  logits: float32, bfloat16 or float16 (rows, vocab), rows contiguous; tokens:
+        int64 (rows) or None.  Returns {"log_probs" (rows), "entropy" (rows), "top_log_probs" and "top_tokens" (rows, top), "status" (rows)}; what is
+        not asked for is None."""
+        torch = _torch or _torch_module()
+        rows, columns = logits.shape
+        vocab = columns if vocab is None else vocab
+        if not 0 < vocab <= columns:
+            raise ValueError("a row holds `vocab` logits at least")
+        row_stride, column_stride = logits.stride()
+        if rows <= 1:
+            row_stride = columns
+        if column_stride != 1 and rows and vocab > 1:
+            raise ValueError("a row's logits are contiguous")
+        self._here(logits)
+        log_probs = entropies = top_log_probs = top_tokens = None
+        if tokens is not None:
+            if not (tokens.dtype is torch.int64 and tokens.numel() == rows and tokens.is_contiguous()):
+                raise ValueError("one int64 token per row")
+            self._here(tokens)
+            log_probs = self._empty((rows,), torch.float32)
+        if entropy:
+            entropies = self._empty((rows,), torch.float32)
+        if top > 0:
+            top_log_probs, top_tokens = self._empty((rows, top), torch.float32), self._empty((rows, top), torch.int64)
+        status = self._empty((rows,), torch.int32)
+        code = _native.token_log_probs(self._handle, _stream_of(logits) if stream is None else stream, _dtype_code(logits), logits.data_ptr(), rows, vocab,
+                                       row_stride, _ptr(tokens), _ptr(log_probs), _ptr(entropies), top, _ptr(top_log_probs), _ptr(top_tokens), status.data_ptr())
+        if code:
+            _check(code)
+        return {"log_probs": log_probs, "entropy": entropies, "top_log_probs": top_log_probs, "top_tokens": top_tokens, "status": status}
 
     # ---- vocabulary-sharded -----------------------------------------------------------------------------
     def shard_record_bytes(self, config) -> int:

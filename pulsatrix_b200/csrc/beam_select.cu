@@ -22,7 +22,7 @@
 
 #include <algorithm>
 
-#include "elements.cuh"
+#include "row_selection.cuh"
 
 namespace psx {
 namespace {
@@ -31,56 +31,6 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMostChunks = 8;  // of a part
 constexpr int kPartList = 1024, kGroupList = 1024;
 constexpr int kHeldEntries = 8;  // per thread, of the parts' lists
-constexpr float kNone = -__builtin_huge_valf();
-constexpr float kLog2e = 1.4426950408889634f;
-
-// Floats as integers of the same order (NaN aside); 0 is below every number.
-__device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u); }
-
-// -0 and +0 are equal: both as +0.
-__device__ __forceinline__ uint64_t entry_key(float logit, int token) {
-    return (uint64_t)ordered(logit + 0.0f) << 32 | (uint32_t)~token;
-}
-
-// A number that at least `keep` of the block's numbers reach, given every thread's largest (-inf where it has none): see
-// above.  Lanes of equal maxima leave together, which can only lower it.
-__device__ __forceinline__ uint32_t warp_bound(float largest, int keep, uint32_t* top) {
-    uint32_t key = ordered(largest), bound = 0;
-    for (int n = (keep + kWarps - 1) / kWarps; n > 0; --n) {
-        bound = __reduce_max_sync(0xffffffffu, key);
-        if (top) *top = bound, top = nullptr;
-        key = key == bound ? 0u : key;
-        if (bound <= ordered(kNone)) return 0;
-    }
-    return bound;
-}
-
-__device__ __forceinline__ uint64_t block_max(uint64_t key, uint64_t* shared) {
-    for (int step = 16; step > 0; step /= 2) key = max(key, __shfl_xor_sync(0xffffffffu, key, step));
-    if (threadIdx.x % 32 == 0) shared[threadIdx.x / 32] = key;
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) key = max(key, shared[w]);
-    __syncthreads();
-    return key;
-}
-
-// {a, b} + {x, x} and {a, b} * {x, x}, each rounded as alone.
-__device__ __forceinline__ float2 add_pair(float2 a, float2 x) {
-    float2 r;
-    asm("{\n\t.reg .b64 a, x, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tadd.rn.f32x2 r, a, x;\n\tmov.b64 {%0, %1}, r;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(x.x), "f"(x.y));
-    return r;
-}
-__device__ __forceinline__ float2 mul_pair(float2 a, float2 x) {
-    float2 r;
-    asm("{\n\t.reg .b64 a, x, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tmul.rn.f32x2 r, a, x;\n\tmov.b64 {%0, %1}, r;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(x.x), "f"(x.y));
-    return r;
-}
 
 struct PartShared {
     uint64_t list[kPartList], best_of[kWarps];
@@ -159,7 +109,7 @@ __device__ __forceinline__ void part_of_row(const BeamSelectParams& p, PartShare
     }
     // (A NaN or +inf among the logits makes the sum NaN: the maximum passes over a NaN, and inf - inf is one.)
     uint32_t warp_top_key;
-    const uint32_t mine = warp_bound(top, keep, &warp_top_key);
+    const uint32_t mine = warp_bound<kWarps>(top, keep, &warp_top_key);
     const float warp_level = from_ordered(warp_top_key);
     double total = sum * exp2_approx((top - (warp_level > kNone ? warp_level : 0.0f)) * kLog2e);
 #pragma unroll
@@ -221,7 +171,7 @@ __device__ __forceinline__ void part_of_row(const BeamSelectParams& p, PartShare
                     if (key < last) best = max(best, key);
                 }
             }
-            best = block_max(best, s.best_of);
+            best = block_max<kWarps>(best, s.best_of);
             if (best == 0) break;
             if (threadIdx.x == 0) entries[placed] = {from_ordered((uint32_t)(best >> 32)), (int)~(uint32_t)best};
             last = best;
@@ -245,21 +195,6 @@ __device__ __forceinline__ Candidate candidate_at(double value, uint64_t place) 
 
 __device__ __forceinline__ bool ahead(const Candidate& a, const Candidate& b) {
     return a.key > b.key || (a.key == b.key && a.place < b.place);
-}
-
-// The logarithm of a sum, in double precision: x = 2^e f with f between sqrt(1/2) and sqrt(2), log f = 2 atanh(z) with
-// z = (f - 1) / (f + 1), by its power series up to z^15 (|z| < 0.1716: what is left out is below 2^-44 of it).  A sum just above 1, a token that is
-// nearly certain, has its own logarithm, which a float's fraction would lose below 2^-24.
-__device__ __forceinline__ double log_of(double x) {
-    const int high = __double2hiint(x);
-    int exponent = (high >> 20) - 1023;
-    double f = __hiloint2double((high & 0xfffff) | 0x3ff00000, __double2loint(x));
-    if (f > 1.4142135623730951) f *= 0.5, ++exponent;
-    const double z = (f - 1.0) / (f + 1.0), w = z * z;
-    double series = 1.0 / 15.0;
-#pragma unroll
-    for (int n = 13; n > 0; n -= 2) series = fma(series, w, 1.0 / n);
-    return fma((double)exponent, 0.6931471805599453, 2.0 * z * series);
 }
 
 // The value as a float, in an order that rounding keeps; what is below the lowest float counts as that, so that it stays a candidate.
@@ -343,7 +278,7 @@ __device__ __forceinline__ void best_of_group(const BeamSelectParams& p, GroupSh
     for (int i = 0; i < kHeldEntries; ++i) {
         largest = fmaxf(largest, as_float(candidate_of(held_list[i], held[i]).value()));
     }
-    const uint32_t mine = warp_bound(largest, keep, nullptr);
+    const uint32_t mine = warp_bound<kWarps>(largest, keep, nullptr);
     if (lane == 0) s.bounds[warp] = mine;
     __syncthreads();
     uint32_t bound_key = s.bounds[0];

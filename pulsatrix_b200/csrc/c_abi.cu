@@ -30,6 +30,7 @@
 #include "scan_rows.cuh"
 #include "shard_records.cuh"
 #include "store_cache_8bit.cuh"
+#include "token_log_probs.cuh"
 #include "topk_rows.cuh"
 #include "whole_rows.cuh"
 
@@ -95,7 +96,8 @@ struct psx_ctx {
     // staging of the sharded path
     Buffer shard_uniform_scratch;
     // Scratch that captured graphs may hold: what a capture has used stays allocated until the context goes (see reserve_kept).
-    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts, page_copies, page_moves, attention_pages_pieces, attention_pages_arrived;
+    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts, page_copies, page_moves, attention_pages_pieces, attention_pages_arrived, log_prob_parts,
+        log_prob_arrived;
     std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
     bool timing = false;
@@ -453,7 +455,8 @@ void psx_b200_ctx_destroy(psx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Buffer* b : {&ctx->stats[0], &ctx->stats[1], &ctx->part_counts[0], &ctx->part_counts[1], &ctx->candidates[0], &ctx->candidates[1], &ctx->banned, &ctx->sort_keys, &ctx->head_logits, &ctx->attention_partial, &ctx->surv_cols, &ctx->surv_vals,
                       &ctx->surv_counts, &ctx->pl_tokens, &ctx->pl_log_probs, &ctx->pl_status, &ctx->h_logits, &ctx->h_inputs,
-                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts, &ctx->page_copies, &ctx->page_moves, &ctx->attention_pages_pieces, &ctx->attention_pages_arrived}) {
+                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts, &ctx->page_copies, &ctx->page_moves, &ctx->attention_pages_pieces, &ctx->attention_pages_arrived, &ctx->log_prob_parts,
+                      &ctx->log_prob_arrived}) {
         if (b->ptr) cudaFree(b->ptr);
     }
     for (void* p : ctx->outgrown) cudaFree(p);
@@ -1667,6 +1670,47 @@ psx_status psx_b200_decode_attention_pages(psx_ctx* ctx, void* stream_ptr, const
         p.arrived = static_cast<int32_t*>(ctx->attention_pages_arrived.ptr);
     }
     PSX_CUDA(psx::launch_paged_attention(p, stream));
+    ctx->launches += 1;
+    return PSX_OK;
+}
+
+// ---- log-probabilities of given tokens ------------------------------------------------------------------------------------
+
+psx_status psx_b200_token_log_probs(psx_ctx* ctx, void* stream_ptr, int32_t dtype, const void* logits, int64_t rows, int64_t vocab, int64_t row_stride,
+                                    const int64_t* tokens, float* log_probs, float* entropy, int64_t top, float* top_log_probs, int64_t* top_tokens,
+                                    int32_t* row_status) {
+    if (!ctx) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: context is null");
+    if (dtype < psx::kFloat32 || dtype > psx::kFloat16) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: unknown element type");
+    if (rows < 0 || vocab <= 0 || top < 0) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: sizes of rows must be positive");
+    if (row_stride < vocab) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: row_stride is smaller than the vocabulary");
+    if (top > psx::kMostTop || vocab > (int64_t(1) << 30)) {
+        return fail(PSX_ERR_UNSUPPORTED, "psx_b200: log-probabilities come with at most 128 alternatives, of at most 2^30 tokens");
+    }
+    if (rows == 0) return PSX_OK;
+    if (!logits || (tokens && !log_probs) || (top > 0 && (!top_log_probs || !top_tokens))) return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: null pointer");
+    if (reinterpret_cast<uintptr_t>(logits) % psx::element_bytes(dtype) != 0) {
+        return fail(PSX_ERR_BAD_ARGUMENT, "psx_b200: logits must be aligned to their type");
+    }
+    psx::TokenLogProbsParams p{};
+    p.logits = logits; p.tokens = tokens; p.log_probs = log_probs; p.entropy = entropy; p.top_log_probs = top_log_probs; p.top_tokens = top_tokens;
+    p.row_status = row_status; p.rows = rows; p.row_stride = row_stride; p.vocab = (int32_t)vocab; p.top = (int32_t)top; p.type = dtype;
+    if (rows > 0x7fffffff) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many rows for one call");
+    psx::plan_token_log_probs(p, ctx->sm_count);
+    if (rows * p.parts > 0x7fffffff) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many rows for one call");
+    const OnDevice device(ctx->device);
+    PSX_CUDA(device.error);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    const size_t lists = (size_t)(rows * p.parts), stats_bytes = lists * sizeof(psx::LogProbPart);
+    bool capturing;
+    if (psx_status s = is_capturing(stream, &capturing)) return s;
+    if (psx_status s = reserve_kept(ctx, capturing, ctx->log_prob_parts, stats_bytes + lists * (size_t)top * sizeof(psx::LogProbEntry))) return s;
+    p.stats = static_cast<psx::LogProbPart*>(ctx->log_prob_parts.ptr);
+    p.entries = reinterpret_cast<psx::LogProbEntry*>(static_cast<char*>(ctx->log_prob_parts.ptr) + stats_bytes);
+    if (p.parts > 1) {
+        if (psx_status s = reserve_counters(ctx, stream, capturing, ctx->log_prob_arrived, (size_t)rows)) return s;
+        p.arrived = static_cast<int32_t*>(ctx->log_prob_arrived.ptr);
+    }
+    PSX_CUDA(psx::launch_token_log_probs(p, stream));
     ctx->launches += 1;
     return PSX_OK;
 }

@@ -82,7 +82,7 @@ PyObject* invoke(psx_status (*fn)(A...), PyObject* const* args, Py_ssize_t count
     X(exchange_sample) X(top_k_rows) X(lm_head_logits) X(lm_head_sample_rows) X(softmax_rows) X(logsumexp_rows)         \
     X(gather_rows) X(decode_attention) X(beam_select) X(reorder_states) X(store_cache_8bit) X(decode_attention_8bit)    \
     X(prompt_attention) X(extend_pages) X(fork_pages) X(release_pages) X(compact_pages) X(rotate_heads)         \
-    X(decode_attention_pages)
+    X(decode_attention_pages) X(token_log_probs)
 
 #define PSX_DEFINE(name)                                                                                         \
     decltype(&psx_b200_##name) g_##name = nullptr;                                                               \

@@ -142,3 +142,7 @@ def test_page_entry_points_check_their_arguments_before_touching_a_gpu(lib):
     assert C.sizeof(binding.PagedCacheLayout) == 88  # (psx_paged_cache)
     cache = binding.PagedCacheLayout()
     assert lib.psx_b200_decode_attention_pages(None, None, None, 0, C.addressof(cache), None, 1, 1, 1.0, 1, 0) == binding.ERR_BAD_ARGUMENT
+
+
+def test_log_probabilities_check_their_arguments_before_touching_a_gpu(lib):
+    assert lib.psx_b200_token_log_probs(None, None, 0, None, 1, 1, 1, None, None, None, 0, None, None, None) == binding.ERR_BAD_ARGUMENT
