@@ -22,8 +22,10 @@ namespace psx {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMostChunks = 8;  // of a part
+constexpr int kMostChunks = 32;  // of a part
 constexpr int kLongVectors = 4;
+constexpr int kBlocks = 4;  // that an SM holds
+constexpr int kMostMaxima = (kMostTop + kWarps - 1) / kWarps + 2;  // of a warp
 constexpr int kPartList = 1024, kRowList = 1024;
 constexpr int kHeldEntries = 8;  // per thread, of the parts' lists
 constexpr float kLeast = -200.0f;  // 2^-200 is 0 as a float; the logarithm of a weight is never less (0 times -inf would be NaN)
@@ -52,6 +54,7 @@ __device__ __forceinline__ float warp_largest(float x) {
 template <class T>
 struct Word {
     static constexpr int elements = 4 / sizeof(T);
+    static constexpr float lowest = std::is_same<T, __half>::value ? -65504.0f : -0x1.fep127f;
     uint32_t bits;
 
     __device__ __forceinline__ static Word none() {
@@ -69,6 +72,23 @@ struct Word {
             return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xffff0000u));
         }
     }
+    // Both numbers and `minus`, as floats.
+    __device__ __forceinline__ float2 plus(float minus) const {
+        float2 r;
+        if constexpr (sizeof(T) == 4) r = make_float2(__uint_as_float(bits) + minus, kNone);
+        else if constexpr (std::is_same<T, __half>::value)
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %3;\n\tadd.rn.f32.f16 %1, h, %3;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(bits), "f"(minus));
+        else
+            asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %3;\n\tadd.rn.f32.bf16 %1, h, %3;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(bits), "f"(minus));
+        return r;
+    }
+    __device__ __forceinline__ static Word both(float x) {  // rounded
+        if constexpr (sizeof(T) == 4) return {__float_as_uint(x)};
+        const T two[2] = {from_float<T>(x), from_float<T>(x)};
+        Word r;
+        __builtin_memcpy(&r.bits, two, 4);
+        return r;
+    }
     __device__ __forceinline__ Word max_with(Word o) const {
         Word r;
         if constexpr (sizeof(T) == 4) asm("max.NaN.f32 %0, %1, %2;" : "=r"(r.bits) : "r"(bits), "r"(o.bits));
@@ -85,12 +105,52 @@ struct Word {
     }
 };
 
+// A bound that at least `keep` of the block's numbers reach, each thread giving its largest: the `keep`-th largest of what the warps' largest few make
+// (two more than an equal share; where one warp has more of the largest than that the bound is lower than it could be), 0 where there are not so many.
+__device__ __forceinline__ int maxima_of(int keep) { return (keep + kWarps - 1) / kWarps + (keep > 1 ? 2 : 0); }
+__device__ __forceinline__ void warp_maxima(float largest, int keep, uint32_t* maxima) {
+    const int each = maxima_of(keep), lane = threadIdx.x % 32;
+    uint32_t key = largest > kNone ? ordered(largest) : 0;
+    for (int i = 0; i < each;) {
+        const uint32_t next = __reduce_max_sync(0xffffffffu, key);
+        const int held = next == 0 ? each : __popc(__ballot_sync(0xffffffffu, key == next)), to = min(each, i + held);
+        for (int k = i + lane; k < to; k += 32) maxima[threadIdx.x / 32 * each + k] = next;
+        if (key == next) key = 0;
+        i = to;
+    }
+}
+__device__ __forceinline__ void bound_of(const uint32_t* maxima, int keep, uint32_t& bound) {  // (every thread but one of several equal ones counts)
+    const int count = maxima_of(keep) * kWarps;
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t mine = maxima[i];
+        int place = 0;
+#pragma unroll 4
+        for (int k = 0; k < count; ++k) place += maxima[k] > mine || (maxima[k] == mine && k < i);
+        if (place == keep - 1) bound = mine;
+    }
+}
+
 struct PartShared {
     uint64_t list[kPartList], best_of[kWarps];
-    uint32_t bounds[kWarps];
+    uint32_t maxima[kWarps * kMostMaxima], bound;
     float tops[kWarps], sums[kWarps], weighted[kWarps];
+    float chunk_top[kMostChunks][kThreads];  // a thread's own
     int listed;
 };
+
+// The vector of 16 bytes that an end of the row cuts: elements first .. end of it, one by one, and -inf for the others.
+template <class T>
+__device__ __noinline__ uint4 cut_vector(const T* at, int first, int end) {
+    uint4 x = make_uint4(Word<T>::none().bits, Word<T>::none().bits, Word<T>::none().bits, Word<T>::none().bits);
+    T e[16 / sizeof(T)];
+    __builtin_memcpy(e, &x, 16);
+#pragma unroll
+    for (int i = 0; i < (int)(16 / sizeof(T)); ++i) {
+        if (i >= first && i < end) e[i] = at[i];
+    }
+    __builtin_memcpy(&x, e, 16);
+    return x;
+}
 
 // Of several holders of (m, sums), all lanes of a warp taking part: the sums relative to `high`, the largest m, of which `first` is one holder.
 __device__ __forceinline__ void relative_to(float high, bool first, float m, float& sum, float& weighted) {
@@ -100,8 +160,49 @@ __device__ __forceinline__ void relative_to(float high, bool first, float m, flo
     sum = (1.0f + sum) * f;
 }
 
-template <class T, int vectors, bool picks>
-__device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartShared& s) {
+// What a row's alternatives are relative to: the largest logit and log(1 + r).
+struct Outcome {
+    double top, lse;
+    int status;
+};
+
+// By one lane: the row's own results.
+template <class T>
+__device__ __forceinline__ void finish_row(const TokenLogProbsParams& p, Outcome& o, int64_t row, float high, double r, double weighted, int64_t token, float logit) {
+    const bool wrong = !(high < -kNone), none = high == kNone, real = token >= 0 && token < p.vocab;
+    const double lse = log_of_one_and(r);
+    const float nan = __int_as_float(0x7fffffff);
+    o.top = high;
+    o.lse = lse;
+    o.status = wrong ? kRowNonFinite : none ? kRowAllRemoved : p.tokens && !real ? kRowBadToken : kRowOk;
+    if (p.tokens) p.log_probs[row] = wrong || none || !real ? nan : (float)(((double)logit - (double)high) - lse);
+    if (p.entropy) p.entropy[row] = wrong || none ? nan : (float)(lse - weighted * 0.69314718055994530942 / (1.0 + r));
+    if (p.row_status) p.row_status[row] = o.status;
+}
+
+__device__ __forceinline__ void put_alternative(const TokenLogProbsParams& p, const Outcome& o, int64_t row, int place, uint64_t key) {
+    p.top_log_probs[row * p.top + place] = (float)(((double)from_ordered((uint32_t)(key >> 32)) - o.top) - o.lse);
+    p.top_tokens[row * p.top + place] = (int64_t)~(uint32_t)key;
+}
+__device__ __forceinline__ void put_none(const TokenLogProbsParams& p, int64_t row, int place) {
+    p.top_log_probs[row * p.top + place] = kNone;
+    p.top_tokens[row * p.top + place] = -1;
+}
+__device__ __forceinline__ void put_wrong(const TokenLogProbsParams& p, int64_t row, int place) {
+    p.top_log_probs[row * p.top + place] = __int_as_float(0x7fffffff);
+    p.top_tokens[row * p.top + place] = -1;
+}
+
+// The given token of a row and its logit (0 where there is none).
+template <class T>
+__device__ __forceinline__ float given_logit(const TokenLogProbsParams& p, int64_t row, int64_t& token) {
+    token = p.tokens ? p.tokens[row] : 0;
+    return p.tokens && token >= 0 && token < p.vocab ? to_float(static_cast<const T*>(p.logits)[row * p.row_stride + token]) : 0.0f;
+}
+
+// `whole`: the part is the row.
+template <class T, int vectors, bool picks, bool whole>
+__device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartShared& s, Outcome& o) {
     constexpr int E = 16 / sizeof(T), kChunk = kThreads * vectors * E, kWords = vectors * 4;
     using W = Word<T>;
     const int64_t part_row = blockIdx.x;
@@ -112,70 +213,75 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
     const T* from = static_cast<const T*>(p.logits) + row * p.row_stride;
     const int shift = (int)(reinterpret_cast<uintptr_t>(from) % 16 / sizeof(T));
     from -= shift;
-    const int64_t all = (int64_t)shift + p.vocab;
-    const int64_t begin = (int64_t)part * p.chunks * kChunk, end = min(begin + (int64_t)p.chunks * kChunk, all);
-    const auto column = [&](int chunk, int v) { return begin + (int64_t)chunk * kChunk + (v * kThreads + (int)threadIdx.x) * E; };
+    const int begin = part * p.chunks * kChunk, end = (int)min((int64_t)begin + p.chunks * kChunk, (int64_t)shift + p.vocab);
+    const auto column = [&](int chunk, int v) { return begin + chunk * kChunk + (v * kThreads + (int)threadIdx.x) * E; };
     const auto load = [&](int chunk, W (&w)[kWords], bool again) {
 #pragma unroll
         for (int v = 0; v < vectors; ++v) {
-            const int64_t at = column(chunk, v);
+            const int at = column(chunk, v);
             uint4 x = make_uint4(W::none().bits, W::none().bits, W::none().bits, W::none().bits);
-            if (at >= shift && at + E <= end) {
-                x = again ? __ldcg(reinterpret_cast<const uint4*>(from + at)) : __ldcs(reinterpret_cast<const uint4*>(from + at));
-            } else if (at < end && at + E > shift) {  // (an end of the row)
-                T e[E];
-                __builtin_memcpy(e, &x, 16);
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    if (at + i >= shift && at + i < end) e[i] = from[at + i];
-                }
-                __builtin_memcpy(&x, e, 16);
-            }
+            if (at >= shift && at <= end - E) x = again ? __ldcg(reinterpret_cast<const uint4*>(from + at)) : __ldcs(reinterpret_cast<const uint4*>(from + at));
+            else if (at < end && at > shift - E) x = cut_vector(from + at, shift - at, end - at);
             w[4 * v].bits = x.x, w[4 * v + 1].bits = x.y, w[4 * v + 2].bits = x.z, w[4 * v + 3].bits = x.w;
         }
     };
 
-    W w[2][kWords], best = W::none();  // (best: the largest so far, of even and of odd places for 16-bit logits)
-    float chunk_top[picks ? kMostChunks : 1], level = kNone;
+    W best = W::none();  // (the largest so far, of even and of odd places for 16-bit logits)
+    float level = kNone;
     float2 sum = {0.0f, 0.0f}, weighted = {0.0f, 0.0f};
-    load(0, w[0], false);
+    const auto take = [&](int c, W (&x)[kWords]) {
+        if constexpr (picks) {
+            W high[2] = {x[0], x[1]};
 #pragma unroll
-    for (int c = 0; c < kMostChunks; ++c) {
-        if constexpr (picks) chunk_top[c] = kNone;
-        if (c < p.chunks) {
-            if (c + 1 < kMostChunks && c + 1 < p.chunks) load(c + 1, w[(c + 1) % 2], false);
-            W(&x)[kWords] = w[c % 2];
-            if constexpr (picks) {
-                W high[2] = {x[0], x[1]};
+            for (int i = 2; i < kWords; ++i) high[i % 2] = high[i % 2].max_with(x[i]);
+            const float2 two = high[0].max_with(high[1]).floats();
+            s.chunk_top[c][threadIdx.x] = larger(two.x, two.y);
+        }
 #pragma unroll
-                for (int i = 2; i < kWords; ++i) high[i % 2] = high[i % 2].max_with(x[i]);
-                const float2 two = high[0].max_with(high[1]).floats();
-                chunk_top[c] = larger(two.x, two.y);
-            }
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) {  // the larger one is kept aside
-                const W lower = best.min_with(x[i]);
-                best = best.max_with(x[i]);
-                x[i] = lower;
-            }
-            const float2 two = best.floats();
-            const float next = fmaxf(two.x, two.y), base = next > kNone ? next : 0.0f;
-            const float less = fmaxf((level - base) * kLog2e, kLeast), factor = exp2_approx(less);
-            weighted = mul_pair(fma_pair(make_float2(less, less), sum, weighted), make_float2(factor, factor));
-            sum = mul_pair(sum, make_float2(factor, factor));
-            level = base;
-            const float2 minus = make_float2(-base, -base), log2e = make_float2(kLog2e, kLog2e);
+        for (int i = 0; i < kWords; ++i) {  // the larger one is kept aside
+            const W lower = best.min_with(x[i]);
+            best = best.max_with(x[i]);
+            x[i] = lower;
+        }
+        const float2 two = best.floats();
+        const float next = fmaxf(two.x, two.y), base = next > kNone ? next : 0.0f;
+        const float less = fmaxf((level - base) * kLog2e, kLeast), factor = exp2_approx(less);
+        weighted = mul_pair(fma_pair(make_float2(less, less), sum, weighted), make_float2(factor, factor));
+        sum = mul_pair(sum, make_float2(factor, factor));
+        level = base;
+        const auto add_up = [&](bool clamp) {
 #pragma unroll
             for (int i = 0; i < kWords; i += W::elements == 1 ? 2 : 1) {
-                float2 y = x[i].floats();
-                if constexpr (W::elements == 1) y.y = x[i + 1].floats().x;
-                y = mul_pair(add_pair(y, minus), log2e);
-                y = make_float2(fmaxf(y.x, kLeast), fmaxf(y.y, kLeast));
+                float2 y = x[i].plus(-base);
+                if constexpr (W::elements == 1) y.y = x[i + 1].plus(-base).x;
+                y = mul_pair(y, make_float2(kLog2e, kLog2e));
+                if (clamp) y = make_float2(fmaxf(y.x, kLeast), fmaxf(y.y, kLeast));
                 const float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
                 sum = add_pair(sum, e);
                 weighted = fma_pair(y, e, weighted);
             }
+        };
+        // 16-bit logits are brought up to where their weights are 0 in pairs (150 nats below the largest, or a 32nd of that where it is larger, which
+        // the type's rounding leaves below 118), but for a largest so low that nothing of the type is.
+        const float least = base - fmaxf(150.0f, fabsf(base) * 0x1p-5f);
+        if (W::elements == 2 && least > W::lowest) {
+            const W floor = W::both(least);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) x[i] = x[i].max_with(floor);
+            add_up(false);
+        } else {
+            add_up(true);
         }
+    };
+    // (Two chunks a turn, one in work and one on its way; unrolled further, the instructions come too late.)
+    W w[2][kWords];
+    load(0, w[0], false);
+#pragma unroll 1
+    for (int c = 0; c < p.chunks; c += 2) {
+        if (c + 1 < p.chunks) load(c + 1, w[1], false);
+        take(c, w[0]);
+        if (c + 2 < p.chunks) load(c + 2, w[0], false);
+        if (c + 1 < p.chunks) take(c + 1, w[1]);
     }
     // The thread's own: the smaller of the two that are aside joins the sums.
     const float2 aside = best.floats();
@@ -194,11 +300,17 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
         own += __shfl_xor_sync(0xffffffffu, own, step);
         own_weighted += __shfl_xor_sync(0xffffffffu, own_weighted, step);
     }
-    uint32_t mine = 0;
-    if constexpr (picks) mine = warp_bound<kWarps>(top, p.top, nullptr);
-    if (lane == 0) s.bounds[warp] = mine, s.tops[warp] = warp_top, s.sums[warp] = own, s.weighted[warp] = own_weighted;
+    if (lane == 0) s.tops[warp] = warp_top, s.sums[warp] = own, s.weighted[warp] = own_weighted;
+    if constexpr (picks) warp_maxima(top, p.top, s.maxima);
     __syncthreads();
+    if constexpr (picks) {
+        bound_of(s.maxima, p.top, s.bound);
+        __syncthreads();
+    }
     if (warp == kWarps - 1) {  // the part's record
+        int64_t token = 0;
+        float logit = 0.0f;
+        if (whole && lane == 0) logit = given_logit<T>(p, row, token);
         const float m = lane < kWarps ? s.tops[lane] : kNone;
         const float high = warp_largest(m);
         float part_sum = lane < kWarps ? s.sums[lane] : 0.0f, part_weighted = lane < kWarps ? s.weighted[lane] : 0.0f;
@@ -209,23 +321,23 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
             part_sum += __shfl_xor_sync(0xffffffffu, part_sum, step);
             part_weighted += __shfl_xor_sync(0xffffffffu, part_weighted, step);
         }
-        if (lane == 0) __stcg(reinterpret_cast<float4*>(p.stats + part_row), make_float4(high, part_sum, part_weighted, 0.0f));
+        if (lane == 0) {
+            if (whole) finish_row<T>(p, o, row, high, part_sum, part_weighted, token, logit);
+            else __stcg(reinterpret_cast<float4*>(p.stats + part_row), make_float4(high, part_sum, part_weighted, 0.0f));
+        }
     }
     if constexpr (picks) {
         const int keep = p.top;
         LogProbEntry* entries = p.entries + part_row * keep;
         const auto put = [&](int place, uint64_t key) {
-            __stcg(reinterpret_cast<float2*>(entries + place), make_float2(from_ordered((uint32_t)(key >> 32)), __int_as_float((int)~(uint32_t)key)));
+            if constexpr (whole) put_alternative(p, o, row, place, key);
+            else __stcg(reinterpret_cast<float2*>(entries + place), make_float2(from_ordered((uint32_t)(key >> 32)), __int_as_float((int)~(uint32_t)key)));
         };
-        uint32_t bound_key = s.bounds[0];
-#pragma unroll
-        for (int i = 1; i < kWarps; ++i) bound_key = min(bound_key, s.bounds[i]);
-        const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
+        const float bound = s.bound == 0 ? kNone : from_ordered(s.bound);
         uint32_t hits = 0;  // the chunks that reach the bound; they are read again, out of L2
-#pragma unroll
-        for (int c = 0; c < kMostChunks; ++c) hits |= (chunk_top[c] >= bound && chunk_top[c] > kNone) ? 1u << c : 0u;
+        for (int c = 0; c < p.chunks; ++c) hits |= (s.chunk_top[c][threadIdx.x] >= bound && s.chunk_top[c][threadIdx.x] > kNone) ? 1u << c : 0u;
         // every logit of those chunks that reaches the bound, with its token
-        const auto look = [&](auto take) {
+        const auto look = [&](auto use) {
             for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
                 const int c = __ffs(rest) - 1;
                 load(c, w[0], true);
@@ -233,9 +345,9 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
                 for (int i = 0; i < kWords; ++i) {
                     const float2 x = w[0][i].floats();
                     const int token = (int)(column(c, i / 4) - shift) + i % 4 * W::elements;
-                    if (x.x >= bound && x.x > kNone) take(x.x, token);
+                    if (x.x >= bound && x.x > kNone) use(x.x, token);
                     if constexpr (W::elements == 2) {
-                        if (x.y >= bound && x.y > kNone) take(x.y, token + 1);
+                        if (x.y >= bound && x.y > kNone) use(x.y, token + 1);
                     }
                 }
             }
@@ -269,15 +381,21 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
                 last = next;
             }
         }
-        for (int i = placed + threadIdx.x; i < keep; i += kThreads) __stcg(reinterpret_cast<float2*>(entries + i), make_float2(kNone, __int_as_float(-1)));
+        for (int i = placed + threadIdx.x; i < keep; i += kThreads) {
+            if constexpr (whole) put_none(p, row, i);
+            else __stcg(reinterpret_cast<float2*>(entries + i), make_float2(kNone, __int_as_float(-1)));
+        }
+        if (whole && o.status == kRowNonFinite) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < keep; i += kThreads) put_wrong(p, row, i);
+        }
     }
 }
 
 struct RowShared {
     uint64_t list[kRowList], best_of[kWarps];
-    uint32_t bounds[kWarps];
-    double top, lse;  // the row's largest logit and log(1 + r)
-    int listed, status;
+    uint32_t maxima[kWarps * kMostMaxima], bound;
+    int listed;
 };
 
 // What the parts' blocks have written: out of L2.
@@ -287,7 +405,7 @@ __device__ __forceinline__ uint64_t key_of(const LogProbEntry* at) {
 }
 
 template <class T, bool picks>
-__device__ __forceinline__ void whole_row(const TokenLogProbsParams& p, RowShared& s, int64_t row) {
+__device__ __forceinline__ void whole_row(const TokenLogProbsParams& p, RowShared& s, Outcome& o, int64_t row) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, parts = p.parts, keep = p.top;
     const LogProbEntry* entries = p.entries + row * parts * keep;
     // The lists' first entries, then the second ones and so on, are asked for ahead of the sums and kept; neighbours go to different warps.
@@ -303,14 +421,12 @@ __device__ __forceinline__ void whole_row(const TokenLogProbsParams& p, RowShare
     }
     if (warp == 0) {
         const float4* stats = reinterpret_cast<const float4*>(p.stats + row * parts);
-        const int64_t token = p.tokens ? p.tokens[row] : 0;
-        const bool real = token >= 0 && token < p.vocab;
+        int64_t token = 0;
         float logit = 0.0f;
-        if (p.tokens && real && lane == 0) logit = to_float(static_cast<const T*>(p.logits)[row * p.row_stride + token]);
+        if (lane == 0) logit = given_logit<T>(p, row, token);
         float high = kNone;
         for (int i = lane; i < parts; i += 32) high = larger(high, __ldcg(stats + i).x);
         high = warp_largest(high);
-        const bool wrong = !(high < -kNone), none = high == kNone;
         double r = 0.0, weighted = 0.0;
         bool found = false;  // the part that holds the row's largest, the first of them
         for (int first = 0; first < parts; first += 32) {
@@ -328,26 +444,17 @@ __device__ __forceinline__ void whole_row(const TokenLogProbsParams& p, RowShare
             r += __shfl_xor_sync(0xffffffffu, r, step);
             weighted += __shfl_xor_sync(0xffffffffu, weighted, step);
         }
-        if (lane == 0) {
-            const double lse = log_of_one_and(r);
-            const float nan = __int_as_float(0x7fffffff);
-            s.top = high;
-            s.lse = lse;
-            s.status = wrong ? kRowNonFinite : none ? kRowAllRemoved : p.tokens && !real ? kRowBadToken : kRowOk;
-            if (p.tokens) p.log_probs[row] = wrong || none || !real ? nan : (float)(((double)logit - (double)high) - lse);
-            if (p.entropy) p.entropy[row] = wrong || none ? nan : (float)(lse - weighted * 0.69314718055994530942 / (1.0 + r));
-            if (p.row_status) p.row_status[row] = s.status;
-        }
+        if (lane == 0) finish_row<T>(p, o, row, high, r, weighted, token, logit);
     }
     if constexpr (picks) {
         uint64_t largest = 0;
 #pragma unroll
         for (int i = 0; i < kHeldEntries; ++i) largest = max(largest, held[i]);
-        const uint32_t mine = warp_bound<kWarps>(largest ? from_ordered((uint32_t)(largest >> 32)) : kNone, keep, nullptr);
-        if (lane == 0) s.bounds[warp] = mine;
+        warp_maxima(largest ? from_ordered((uint32_t)(largest >> 32)) : kNone, keep, s.maxima);
         __syncthreads();
-        uint32_t bound = s.bounds[0];
-        for (int w = 1; w < kWarps; ++w) bound = min(bound, s.bounds[w]);
+        bound_of(s.maxima, keep, s.bound);
+        __syncthreads();
+        const uint32_t bound = s.bound;
         const auto offer = [&](uint64_t key) {
             if (key == 0 || (uint32_t)(key >> 32) < bound) return false;
             const int at = atomicAdd(&s.listed, 1);
@@ -364,12 +471,9 @@ __device__ __forceinline__ void whole_row(const TokenLogProbsParams& p, RowShare
         }
         __syncthreads();
         const int count = s.listed;
-        const bool wrong = s.status == kRowNonFinite;
+        const bool wrong = o.status == kRowNonFinite;
         int placed = wrong ? 0 : min(count, keep);
-        const auto put = [&](int place, uint64_t key) {
-            p.top_log_probs[row * keep + place] = (float)(((double)from_ordered((uint32_t)(key >> 32)) - s.top) - s.lse);
-            p.top_tokens[row * keep + place] = (int64_t)~(uint32_t)key;
-        };
+        const auto put = [&](int place, uint64_t key) { put_alternative(p, o, row, place, key); };
         if (wrong) {
         } else if (count <= kRowList) {
             for (int e = threadIdx.x; e < count; e += kThreads) {
@@ -394,24 +498,25 @@ __device__ __forceinline__ void whole_row(const TokenLogProbsParams& p, RowShare
             }
         }
         for (int i = placed + threadIdx.x; i < keep; i += kThreads) {
-            p.top_log_probs[row * keep + i] = wrong ? __int_as_float(0x7fffffff) : kNone;
-            p.top_tokens[row * keep + i] = -1;
+            if (wrong) put_wrong(p, row, i);
+            else put_none(p, row, i);
         }
     }
 }
 
-template <class T, int vectors, bool picks>
-__global__ void __launch_bounds__(kThreads, vectors == 1 ? 2 : 4) token_log_probs_kernel(const __grid_constant__ TokenLogProbsParams p) {
+template <class T, int vectors, bool picks, bool whole>
+__global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(const __grid_constant__ TokenLogProbsParams p) {
     __shared__ union Shared {
         PartShared part;
         RowShared row;
         __device__ Shared() {}
     } shared;
+    __shared__ Outcome outcome;
     __shared__ int is_last;
-    part_of_row<T, vectors, picks>(p, shared.part);
-    const int64_t row = blockIdx.x / (unsigned)p.parts;
-    __syncthreads();
-    if (p.parts > 1) {
+    part_of_row<T, vectors, picks, whole>(p, shared.part, outcome);
+    if constexpr (!whole) {
+        const int64_t row = blockIdx.x / (unsigned)p.parts;
+        __syncthreads();
         if (threadIdx.x == 0) {  // (release: the block's part, ordered before by the barrier; acquire: the others')
             int before;
             asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + row) : "memory");
@@ -419,22 +524,22 @@ __global__ void __launch_bounds__(kThreads, vectors == 1 ? 2 : 4) token_log_prob
             if (is_last) p.arrived[row] = 0;
         }
         __syncthreads();
-        if (!is_last) return;
+        if (is_last) whole_row<T, picks>(p, shared.row, outcome, row);
     }
-    whole_row<T, picks>(p, shared.row, row);
+}
+
+template <class T, int vectors, bool picks>
+cudaError_t launch_with(const TokenLogProbsParams& p, cudaStream_t stream) {
+    const unsigned blocks = (unsigned)(p.rows * p.parts);
+    if (p.parts == 1) token_log_probs_kernel<T, vectors, picks, true><<<blocks, kThreads, 0, stream>>>(p);
+    else token_log_probs_kernel<T, vectors, picks, false><<<blocks, kThreads, 0, stream>>>(p);
+    return cudaGetLastError();
 }
 
 template <class T>
 cudaError_t launch_type(const TokenLogProbsParams& p, cudaStream_t stream) {
-    const unsigned blocks = (unsigned)(p.rows * p.parts);
-    if (p.vectors == 1) {
-        if (p.top > 0) token_log_probs_kernel<T, 1, true><<<blocks, kThreads, 0, stream>>>(p);
-        else token_log_probs_kernel<T, 1, false><<<blocks, kThreads, 0, stream>>>(p);
-    } else {
-        if (p.top > 0) token_log_probs_kernel<T, kLongVectors, true><<<blocks, kThreads, 0, stream>>>(p);
-        else token_log_probs_kernel<T, kLongVectors, false><<<blocks, kThreads, 0, stream>>>(p);
-    }
-    return cudaGetLastError();
+    if (p.vectors == 1) return p.top > 0 ? launch_with<T, 1, true>(p, stream) : launch_with<T, 1, false>(p, stream);
+    return p.top > 0 ? launch_with<T, kLongVectors, true>(p, stream) : launch_with<T, kLongVectors, false>(p, stream);
 }
 
 }  // namespace
@@ -446,9 +551,14 @@ void plan_token_log_probs(TokenLogProbsParams& p, int sm_count) {
     const auto chunks = [&](int vectors) { return ((int64_t)p.vocab + E - 1 + kThreads * vectors * E - 1) / (kThreads * vectors * E); };
     p.vectors = p.rows * chunks(kLongVectors) < sm_count ? 1 : kLongVectors;
     const int64_t all = chunks(p.vectors);
-    p.chunks = kMostChunks;
-    while (p.chunks > 1 && p.rows * ((all + p.chunks - 1) / p.chunks) < 2 * sm_count) --p.chunks;
-    p.parts = (int)((all + p.chunks - 1) / p.chunks);
+    // Of the numbers of parts that the chunks allow, the one whose rounds of blocks are done first, a part costing some chunks besides its own.
+    constexpr int kBesides = 3;
+    int64_t least = 0;
+    for (int64_t each = std::min<int64_t>(all, kMostChunks); each > 0; --each) {
+        const int64_t parts = (all + each - 1) / each, rounds = (p.rows * parts + sm_count * kBlocks - 1) / (sm_count * kBlocks);
+        const int64_t cost = rounds * ((all + parts - 1) / parts + kBesides);
+        if (least == 0 || cost < least) least = cost, p.parts = (int)parts;
+    }
     p.chunks = (int)((all + p.parts - 1) / p.parts);  // (no part much shorter than the others)
 }
 
