@@ -96,8 +96,7 @@ struct psx_ctx {
     // staging of the sharded path
     Buffer shard_uniform_scratch;
     // Scratch that captured graphs may hold: what a capture has used stays allocated until the context goes (see reserve_kept).
-    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts, page_copies, page_moves, attention_pages_pieces, attention_pages_arrived, log_prob_parts,
-        log_prob_arrived;
+    Buffer beam_scratch, beam_arrived, attention_8bit_pieces, attention_8bit_arrived, prompt_parts, page_copies, page_moves, attention_pages_pieces, attention_pages_arrived;
     std::vector<void*> outgrown;
     // optional per-kernel timing: (before row pass, between, after survivor stage) per call
     bool timing = false;
@@ -455,8 +454,7 @@ void psx_b200_ctx_destroy(psx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     for (Buffer* b : {&ctx->stats[0], &ctx->stats[1], &ctx->part_counts[0], &ctx->part_counts[1], &ctx->candidates[0], &ctx->candidates[1], &ctx->banned, &ctx->sort_keys, &ctx->head_logits, &ctx->attention_partial, &ctx->surv_cols, &ctx->surv_vals,
                       &ctx->surv_counts, &ctx->pl_tokens, &ctx->pl_log_probs, &ctx->pl_status, &ctx->h_logits, &ctx->h_inputs,
-                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts, &ctx->page_copies, &ctx->page_moves, &ctx->attention_pages_pieces, &ctx->attention_pages_arrived, &ctx->log_prob_parts,
-                      &ctx->log_prob_arrived}) {
+                      &ctx->h_results, &ctx->shard_uniform_scratch, &ctx->beam_scratch, &ctx->beam_arrived, &ctx->attention_8bit_pieces, &ctx->attention_8bit_arrived, &ctx->prompt_parts, &ctx->page_copies, &ctx->page_moves, &ctx->attention_pages_pieces, &ctx->attention_pages_arrived}) {
         if (b->ptr) cudaFree(b->ptr);
     }
     for (void* p : ctx->outgrown) cudaFree(p);
@@ -1699,18 +1697,7 @@ psx_status psx_b200_token_log_probs(psx_ctx* ctx, void* stream_ptr, int32_t dtyp
     if (rows * p.parts > 0x7fffffff) return fail(PSX_ERR_UNSUPPORTED, "psx_b200: too many rows for one call");
     const OnDevice device(ctx->device);
     PSX_CUDA(device.error);
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    const size_t lists = (size_t)(rows * p.parts), stats_bytes = lists * sizeof(psx::LogProbPart);
-    bool capturing;
-    if (psx_status s = is_capturing(stream, &capturing)) return s;
-    if (psx_status s = reserve_kept(ctx, capturing, ctx->log_prob_parts, stats_bytes + lists * (size_t)top * sizeof(psx::LogProbEntry))) return s;
-    p.stats = static_cast<psx::LogProbPart*>(ctx->log_prob_parts.ptr);
-    p.entries = reinterpret_cast<psx::LogProbEntry*>(static_cast<char*>(ctx->log_prob_parts.ptr) + stats_bytes);
-    if (p.parts > 1) {
-        if (psx_status s = reserve_counters(ctx, stream, capturing, ctx->log_prob_arrived, (size_t)rows)) return s;
-        p.arrived = static_cast<int32_t*>(ctx->log_prob_arrived.ptr);
-    }
-    PSX_CUDA(psx::launch_token_log_probs(p, stream));
+    PSX_CUDA(psx::launch_token_log_probs(p, static_cast<cudaStream_t>(stream_ptr)));
     ctx->launches += 1;
     return PSX_OK;
 }

@@ -6,28 +6,32 @@
 // thread keeps the largest of its logits aside, and whatever is not larger than it (or the one that it replaces) joins the sums, relative to
 // the thread's largest so far.  16-bit logits are compared in pairs as they come.
 //
-// A block takes a part of a row, in chunks of up to 16 vectors of 16 bytes per thread, the next one on its way; the part leaves m, its two sums
-// and its `top` best logits in order.  They are found as beam_select.cu finds them: a bound that at least `top` logits reach from the
-// threads' largest, a second look, out of L2, at the few chunks that reach it, and an entry's place is the number of keys above its own.  The block
-// of a row that ends last goes on with the row.  Rows need not be aligned: vectors are those of memory, and where one is cut by an end of the row its
-// elements are read one by one.  Bound by HBM: the logits, once.
+// The row is cut into 1 to 16 parts, the CTAs of a cluster; a thread takes up to four vectors of 16 bytes at a time, with the next ones on their way.
+// The `top` best are found by a bound that at least `top` logits reach: each part's is the top-th largest of its threads' largest, the row's the largest
+// of those.  A thread whose largest of some chunks reaches it looks at them again, out of L2, and puts what reaches the bound on a list in
+// the first CTA's shared memory; an entry's place is the number of keys above its own.  A list that overflows (thousands of equal logits) is replaced
+// by `top` sweeps.  Records, bounds and lists go through the cluster's shared memory: there is no scratch and nothing to be zero before a call.
+// (Lists and records in global memory, joined by the part that ends last: 64 rows of 8000 logits, 20 alternatives, 10.4 us instead of TIME.)
+// Rows need not be aligned: vectors are those of memory, and where one is cut by an end of the row its elements are read one by one.  Bound by HBM:
+// the logits, once; and nearly so by instructions for 16-bit logits, 9.4 for each.
 #include "token_log_probs.cuh"
 
 #include <algorithm>
 #include <type_traits>
 
+#include "once_per_device.hpp"
 #include "row_selection.cuh"
 
 namespace psx {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMostChunks = 32;  // of a part
+constexpr int kMostGroups = 32;  // of a part's chunks
 constexpr int kLongVectors = 4;
 constexpr int kBlocks = 4;  // that an SM holds
 constexpr int kMostMaxima = (kMostTop + kWarps - 1) / kWarps + 2;  // of a warp
-constexpr int kPartList = 1024, kRowList = 1024;
-constexpr int kHeldEntries = 8;  // per thread, of the parts' lists
+constexpr int kList = 1024;
+constexpr int kMostParts = 16;  // of a row: a cluster's CTAs
 constexpr float kLeast = -200.0f;  // 2^-200 is 0 as a float; the logarithm of a weight is never less (0 times -inf would be NaN)
 constexpr int kRowOk = 0, kRowNonFinite = 4, kRowAllRemoved = 5, kRowBadToken = 66;  // (psx_row_status)
 
@@ -130,12 +134,23 @@ __device__ __forceinline__ void bound_of(const uint32_t* maxima, int keep, uint3
     }
 }
 
-struct PartShared {
-    uint64_t list[kPartList], best_of[kWarps];
+// What a row's alternatives are relative to: the largest logit and log(1 + r).
+struct Outcome {
+    double top, lse;
+    int status;
+};
+
+struct Shared {
+    uint64_t list[kList];  // the first part's holds the row's
+    uint64_t best_of[kWarps], best[2];
+    float4 record;         // the part's largest logit and its two sums
+    Outcome outcome;       // the first part's, and the given token and its logit
+    int64_t token;
+    float given;
     uint32_t maxima[kWarps * kMostMaxima], bound;
     float tops[kWarps], sums[kWarps], weighted[kWarps];
-    float chunk_top[kMostChunks][kThreads];  // a thread's own
-    int listed;
+    float group_top[kMostGroups][kThreads];  // a thread's own
+    uint32_t listed;
 };
 
 // The vector of 16 bytes that an end of the row cuts: elements first .. end of it, one by one, and -inf for the others.
@@ -160,12 +175,6 @@ __device__ __forceinline__ void relative_to(float high, bool first, float m, flo
     sum = (1.0f + sum) * f;
 }
 
-// What a row's alternatives are relative to: the largest logit and log(1 + r).
-struct Outcome {
-    double top, lse;
-    int status;
-};
-
 // By one lane: the row's own results.
 template <class T>
 __device__ __forceinline__ void finish_row(const TokenLogProbsParams& p, Outcome& o, int64_t row, float high, double r, double weighted, int64_t token, float logit) {
@@ -184,14 +193,6 @@ __device__ __forceinline__ void put_alternative(const TokenLogProbsParams& p, co
     p.top_log_probs[row * p.top + place] = (float)(((double)from_ordered((uint32_t)(key >> 32)) - o.top) - o.lse);
     p.top_tokens[row * p.top + place] = (int64_t)~(uint32_t)key;
 }
-__device__ __forceinline__ void put_none(const TokenLogProbsParams& p, int64_t row, int place) {
-    p.top_log_probs[row * p.top + place] = kNone;
-    p.top_tokens[row * p.top + place] = -1;
-}
-__device__ __forceinline__ void put_wrong(const TokenLogProbsParams& p, int64_t row, int place) {
-    p.top_log_probs[row * p.top + place] = __int_as_float(0x7fffffff);
-    p.top_tokens[row * p.top + place] = -1;
-}
 
 // The given token of a row and its logit (0 where there is none).
 template <class T>
@@ -200,14 +201,61 @@ __device__ __forceinline__ float given_logit(const TokenLogProbsParams& p, int64
     return p.tokens && token >= 0 && token < p.vocab ? to_float(static_cast<const T*>(p.logits)[row * p.row_stride + token]) : 0.0f;
 }
 
-// `whole`: the part is the row.
-template <class T, int vectors, bool picks, bool whole>
-__device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartShared& s, Outcome& o) {
+// ---- the cluster's shared memory --------------------------------------------------------------------------------------------
+// `alone`: a cluster of one CTA.  All threads of the CTAs meet, each by itself.
+template <bool alone>
+struct Cluster {
+    __device__ __forceinline__ static void meets() {
+        if constexpr (alone) __syncthreads();
+        else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    }
+    // Where CTA `rank` has what this CTA has at p.
+    __device__ __forceinline__ static uint32_t at(const void* p, int rank) {
+        const uint32_t here = (uint32_t)__cvta_generic_to_shared(p);
+        if constexpr (alone) return here;
+        uint32_t there;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
+        return there;
+    }
+    __device__ __forceinline__ static uint32_t load_u32(uint32_t at) {
+        uint32_t x;
+        if constexpr (alone) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+        else asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+        return x;
+    }
+    __device__ __forceinline__ static uint64_t load_u64(uint32_t at) {
+        uint64_t x;
+        if constexpr (alone) asm volatile("ld.shared.u64 %0, [%1];" : "=l"(x) : "r"(at) : "memory");
+        else asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(at) : "memory");
+        return x;
+    }
+    __device__ __forceinline__ static float4 load_f4(uint32_t at) {
+        float4 x;
+        if constexpr (alone) asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+        else asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+        return x;
+    }
+    __device__ __forceinline__ static void store_u64(uint32_t at, uint64_t x) {
+        if constexpr (alone) asm volatile("st.shared.u64 [%0], %1;" ::"r"(at), "l"(x) : "memory");
+        else asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(x) : "memory");
+    }
+    __device__ __forceinline__ static uint32_t add_u32(uint32_t at, uint32_t x) {
+        uint32_t before;
+        if constexpr (alone) asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(before) : "r"(at), "r"(x) : "memory");
+        else asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(before) : "r"(at), "r"(x) : "memory");
+        return before;
+    }
+};
+
+template <class T, int vectors, bool picks, bool alone>
+__global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(const __grid_constant__ TokenLogProbsParams p) {
     constexpr int E = 16 / sizeof(T), kChunk = kThreads * vectors * E, kWords = vectors * 4;
     using W = Word<T>;
-    const int64_t part_row = blockIdx.x;
-    const int64_t row = part_row / p.parts;
-    const int part = (int)(part_row % p.parts), warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    using C = Cluster<alone>;
+    __shared__ Shared s;
+    const int parts = alone ? 1 : p.parts;
+    const int64_t row = blockIdx.x / (unsigned)parts;
+    const int part = alone ? 0 : (int)(blockIdx.x % (unsigned)parts), warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (threadIdx.x == 0) s.listed = 0;
     // Elements are counted from the 16-byte boundary that is not behind the row's first one.
     const T* from = static_cast<const T*>(p.logits) + row * p.row_stride;
@@ -235,7 +283,13 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
 #pragma unroll
             for (int i = 2; i < kWords; ++i) high[i % 2] = high[i % 2].max_with(x[i]);
             const float2 two = high[0].max_with(high[1]).floats();
-            s.chunk_top[c][threadIdx.x] = larger(two.x, two.y);
+            const float chunk_top = larger(two.x, two.y);
+            if (p.group == 1) {
+                s.group_top[c][threadIdx.x] = chunk_top;
+            } else {
+                float& held = s.group_top[c / p.group][threadIdx.x];
+                held = c % p.group == 0 ? chunk_top : larger(held, chunk_top);
+            }
         }
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {  // the larger one is kept aside
@@ -276,6 +330,11 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
     // (Two chunks a turn, one in work and one on its way; unrolled further, the instructions come too late.)
     W w[2][kWords];
     load(0, w[0], false);
+    if (part == 0 && threadIdx.x == 0) {  // (here its two trips to memory are nobody's)
+        int64_t token;
+        s.given = given_logit<T>(p, row, token);
+        s.token = token;
+    }
 #pragma unroll 1
     for (int c = 0; c < p.chunks; c += 2) {
         if (c + 1 < p.chunks) load(c + 1, w[1], false);
@@ -308,9 +367,6 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
         __syncthreads();
     }
     if (warp == kWarps - 1) {  // the part's record
-        int64_t token = 0;
-        float logit = 0.0f;
-        if (whole && lane == 0) logit = given_logit<T>(p, row, token);
         const float m = lane < kWarps ? s.tops[lane] : kNone;
         const float high = warp_largest(m);
         float part_sum = lane < kWarps ? s.sums[lane] : 0.0f, part_weighted = lane < kWarps ? s.weighted[lane] : 0.0f;
@@ -321,219 +377,121 @@ __device__ __forceinline__ void part_of_row(const TokenLogProbsParams& p, PartSh
             part_sum += __shfl_xor_sync(0xffffffffu, part_sum, step);
             part_weighted += __shfl_xor_sync(0xffffffffu, part_weighted, step);
         }
-        if (lane == 0) {
-            if (whole) finish_row<T>(p, o, row, high, part_sum, part_weighted, token, logit);
-            else __stcg(reinterpret_cast<float4*>(p.stats + part_row), make_float4(high, part_sum, part_weighted, 0.0f));
-        }
+        if (lane == 0) s.record = make_float4(high, part_sum, part_weighted, 0.0f);
     }
-    if constexpr (picks) {
-        const int keep = p.top;
-        LogProbEntry* entries = p.entries + part_row * keep;
-        const auto put = [&](int place, uint64_t key) {
-            if constexpr (whole) put_alternative(p, o, row, place, key);
-            else __stcg(reinterpret_cast<float2*>(entries + place), make_float2(from_ordered((uint32_t)(key >> 32)), __int_as_float((int)~(uint32_t)key)));
-        };
-        const float bound = s.bound == 0 ? kNone : from_ordered(s.bound);
-        uint32_t hits = 0;  // the chunks that reach the bound; they are read again, out of L2
-        for (int c = 0; c < p.chunks; ++c) hits |= (s.chunk_top[c][threadIdx.x] >= bound && s.chunk_top[c][threadIdx.x] > kNone) ? 1u << c : 0u;
-        // every logit of those chunks that reaches the bound, with its token
-        const auto look = [&](auto use) {
-            for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
-                const int c = __ffs(rest) - 1;
+    C::meets();
+    if (part == 0 && warp == 0) {  // the row's
+        const float4 x = lane < parts ? C::load_f4(C::at(&s.record, lane)) : make_float4(kNone, 0.0f, 0.0f, 0.0f);
+        const float high = warp_largest(x.x);
+        const unsigned holds = __ballot_sync(0xffffffffu, lane < parts && x.x == high);
+        float sum = x.y, w = x.z;
+        relative_to(high, lane == __ffs(holds) - 1, x.x, sum, w);
+        double r = sum, all_weighted = w;
+#pragma unroll
+        for (int step = kMostParts / 2; step > 0; step /= 2) {
+            r += __shfl_xor_sync(0xffffffffu, r, step);
+            all_weighted += __shfl_xor_sync(0xffffffffu, all_weighted, step);
+        }
+        if (lane == 0) finish_row<T>(p, s.outcome, row, high, r, all_weighted, s.token, s.given);
+    }
+    if constexpr (!picks) {
+        if (!alone) C::meets();  // (the records are read until then)
+        return;
+    }
+
+    const uint32_t bound_key = __reduce_max_sync(0xffffffffu, lane < parts ? C::load_u32(C::at(&s.bound, lane)) : 0u);
+    const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
+    const int groups = (p.chunks + p.group - 1) / p.group;
+    uint32_t hits = 0;  // the groups of chunks that reach the bound; they are read again, out of L2
+    for (int g = 0; g < groups; ++g) hits |= (s.group_top[g][threadIdx.x] >= bound && s.group_top[g][threadIdx.x] > kNone) ? 1u << g : 0u;
+    // every logit of those that reaches the bound, with its token
+    const auto look = [&](auto use) {
+        for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
+            const int g = __ffs(rest) - 1, last = min((g + 1) * p.group, p.chunks);
+            for (int c = g * p.group; c < last; ++c) {
                 load(c, w[0], true);
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
                     const float2 x = w[0][i].floats();
-                    const int token = (int)(column(c, i / 4) - shift) + i % 4 * W::elements;
+                    const int token = column(c, i / 4) - shift + i % 4 * W::elements;
                     if (x.x >= bound && x.x > kNone) use(x.x, token);
                     if constexpr (W::elements == 2) {
                         if (x.y >= bound && x.y > kNone) use(x.y, token + 1);
                     }
                 }
             }
-        };
-        look([&](float x, int token) {
-            const int at = atomicAdd(&s.listed, 1);
-            if (at < kPartList) s.list[at] = entry_key(x, token);
-        });
-        __syncthreads();
-        const int count = s.listed;
-        int placed = min(count, keep);
-        if (count <= kPartList) {
+        }
+    };
+    const uint32_t listed_at = C::at(&s.listed, 0), list_at = C::at(s.list, 0);
+    look([&](float x, int token) {
+        const uint32_t at = C::add_u32(listed_at, 1);
+        if (at < kList) C::store_u64(list_at + at * (uint32_t)sizeof(uint64_t), entry_key(x, token));
+    });
+    C::meets();
+    const int count = (int)C::load_u32(listed_at), keep = p.top;
+    const bool wrong = part == 0 && s.outcome.status == kRowNonFinite;
+    int placed = min(count, keep);
+    if (count <= kList) {
+        if (part == 0 && !wrong) {
             for (int e = threadIdx.x; e < count; e += kThreads) {
                 const uint64_t key = s.list[e];
                 int place = 0;
 #pragma unroll 4
                 for (int k = 0; k < count; ++k) place += s.list[k] > key;
-                if (place < keep) put(place, key);
-            }
-        } else {  // (thousands that tie at the bound)
-            uint64_t last = ~0ull;
-            for (placed = 0; placed < keep; ++placed) {
-                uint64_t next = 0;
-                look([&](float x, int token) {
-                    const uint64_t key = entry_key(x, token);
-                    if (key < last) next = max(next, key);
-                });
-                next = block_max<kWarps>(next, s.best_of);
-                if (next == 0) break;
-                if (threadIdx.x == 0) put(placed, next);
-                last = next;
+                if (place < keep) put_alternative(p, s.outcome, row, place, key);
             }
         }
-        for (int i = placed + threadIdx.x; i < keep; i += kThreads) {
-            if constexpr (whole) put_none(p, row, i);
-            else __stcg(reinterpret_cast<float2*>(entries + i), make_float2(kNone, __int_as_float(-1)));
-        }
-        if (whole && o.status == kRowNonFinite) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < keep; i += kThreads) put_wrong(p, row, i);
-        }
-    }
-}
-
-struct RowShared {
-    uint64_t list[kRowList], best_of[kWarps];
-    uint32_t maxima[kWarps * kMostMaxima], bound;
-    int listed;
-};
-
-// What the parts' blocks have written: out of L2.
-__device__ __forceinline__ uint64_t key_of(const LogProbEntry* at) {
-    const float2 two = __ldcg(reinterpret_cast<const float2*>(at));
-    return two.x > kNone ? entry_key(two.x, __float_as_int(two.y)) : 0;
-}
-
-template <class T, bool picks>
-__device__ __forceinline__ void whole_row(const TokenLogProbsParams& p, RowShared& s, Outcome& o, int64_t row) {
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, parts = p.parts, keep = p.top;
-    const LogProbEntry* entries = p.entries + row * parts * keep;
-    // The lists' first entries, then the second ones and so on, are asked for ahead of the sums and kept; neighbours go to different warps.
-    uint64_t held[kHeldEntries];
-    constexpr int kHeld = kHeldEntries * kThreads;
-    if constexpr (picks) {
-        if (threadIdx.x == 0) s.listed = 0;
-#pragma unroll
-        for (int i = 0; i < kHeldEntries; ++i) {
-            const int x = i * kThreads + lane * kWarps + warp;
-            held[i] = x < parts * keep ? key_of(entries + (int64_t)(x % parts) * keep + x / parts) : 0;
+    } else {  // thousands that tie at the bound: sweep after sweep, the best that is behind the last one
+        uint64_t last = ~0ull;
+        for (placed = 0; placed < keep; ++placed) {
+            uint64_t next = 0;
+            look([&](float x, int token) {
+                const uint64_t key = entry_key(x, token);
+                if (key < last) next = max(next, key);
+            });
+            next = block_max<kWarps>(next, s.best_of);
+            uint64_t& mine = s.best[placed % 2];  // (two that take turns: one meeting a sweep is enough)
+            if (threadIdx.x == 0) mine = next;
+            C::meets();
+            for (int i = 0; i < parts; ++i) next = max(next, C::load_u64(C::at(&mine, i)));
+            if (next == 0) break;
+            if (part == 0 && !wrong && threadIdx.x == 0) put_alternative(p, s.outcome, row, placed, next);
+            last = next;
         }
     }
-    if (warp == 0) {
-        const float4* stats = reinterpret_cast<const float4*>(p.stats + row * parts);
-        int64_t token = 0;
-        float logit = 0.0f;
-        if (lane == 0) logit = given_logit<T>(p, row, token);
-        float high = kNone;
-        for (int i = lane; i < parts; i += 32) high = larger(high, __ldcg(stats + i).x);
-        high = warp_largest(high);
-        double r = 0.0, weighted = 0.0;
-        bool found = false;  // the part that holds the row's largest, the first of them
-        for (int first = 0; first < parts; first += 32) {
-            const int i = first + lane;
-            const float4 x = i < parts ? __ldcg(stats + i) : make_float4(kNone, 0.0f, 0.0f, 0.0f);
-            const unsigned holders = __ballot_sync(0xffffffffu, x.x == high);
-            float sum = x.y, w = x.z;
-            relative_to(high, !found && lane == __ffs(holders) - 1, x.x, sum, w);
-            found |= holders != 0;
-            r += sum;
-            weighted += w;
-        }
-#pragma unroll
-        for (int step = 16; step > 0; step /= 2) {
-            r += __shfl_xor_sync(0xffffffffu, r, step);
-            weighted += __shfl_xor_sync(0xffffffffu, weighted, step);
-        }
-        if (lane == 0) finish_row<T>(p, o, row, high, r, weighted, token, logit);
-    }
-    if constexpr (picks) {
-        uint64_t largest = 0;
-#pragma unroll
-        for (int i = 0; i < kHeldEntries; ++i) largest = max(largest, held[i]);
-        warp_maxima(largest ? from_ordered((uint32_t)(largest >> 32)) : kNone, keep, s.maxima);
-        __syncthreads();
-        bound_of(s.maxima, keep, s.bound);
-        __syncthreads();
-        const uint32_t bound = s.bound;
-        const auto offer = [&](uint64_t key) {
-            if (key == 0 || (uint32_t)(key >> 32) < bound) return false;
-            const int at = atomicAdd(&s.listed, 1);
-            if (at < kRowList) s.list[at] = key;
-            return true;
-        };
-#pragma unroll
-        for (int i = 0; i < kHeldEntries; ++i) offer(held[i]);
-        if (kHeld < parts * keep) {  // lists are in order: each from where it is not held on, as far as it reaches the bound
-            for (int q = threadIdx.x; q < parts; q += kThreads) {
-                for (int slot = max(kHeld - q + parts - 1, 0) / parts; slot < keep && offer(key_of(entries + (int64_t)q * keep + slot)); ++slot) {
-                }
-            }
-        }
-        __syncthreads();
-        const int count = s.listed;
-        const bool wrong = o.status == kRowNonFinite;
-        int placed = wrong ? 0 : min(count, keep);
-        const auto put = [&](int place, uint64_t key) { put_alternative(p, o, row, place, key); };
-        if (wrong) {
-        } else if (count <= kRowList) {
-            for (int e = threadIdx.x; e < count; e += kThreads) {
-                const uint64_t key = s.list[e];
-                int place = 0;
-#pragma unroll 4
-                for (int k = 0; k < count; ++k) place += s.list[k] > key;
-                if (place < keep) put(place, key);
-            }
-        } else {  // more that tie at the bound than the list holds: sweep after sweep, the best that is behind the last one
-            uint64_t last = ~0ull;
-            for (placed = 0; placed < keep; ++placed) {
-                uint64_t next = 0;
-                for (int64_t e = threadIdx.x; e < (int64_t)parts * keep; e += kThreads) {
-                    const uint64_t key = key_of(entries + e);
-                    if (key < last) next = max(next, key);
-                }
-                next = block_max<kWarps>(next, s.best_of);
-                if (next == 0) break;
-                if (threadIdx.x == 0) put(placed, next);
-                last = next;
-            }
-        }
-        for (int i = placed + threadIdx.x; i < keep; i += kThreads) {
-            if (wrong) put_wrong(p, row, i);
-            else put_none(p, row, i);
+    if (part == 0) {
+        for (int i = (wrong ? 0 : placed) + threadIdx.x; i < keep; i += kThreads) {
+            p.top_log_probs[row * keep + i] = wrong ? __int_as_float(0x7fffffff) : kNone;
+            p.top_tokens[row * keep + i] = -1;
         }
     }
-}
-
-template <class T, int vectors, bool picks, bool whole>
-__global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(const __grid_constant__ TokenLogProbsParams p) {
-    __shared__ union Shared {
-        PartShared part;
-        RowShared row;
-        __device__ Shared() {}
-    } shared;
-    __shared__ Outcome outcome;
-    __shared__ int is_last;
-    part_of_row<T, vectors, picks, whole>(p, shared.part, outcome);
-    if constexpr (!whole) {
-        const int64_t row = blockIdx.x / (unsigned)p.parts;
-        __syncthreads();
-        if (threadIdx.x == 0) {  // (release: the block's part, ordered before by the barrier; acquire: the others')
-            int before;
-            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + row) : "memory");
-            is_last = before == p.parts - 1;
-            if (is_last) p.arrived[row] = 0;
-        }
-        __syncthreads();
-        if (is_last) whole_row<T, picks>(p, shared.row, outcome, row);
-    }
+    if (!alone) C::meets();  // (the count of the list, and the sweeps' best, are read until then)
 }
 
 template <class T, int vectors, bool picks>
 cudaError_t launch_with(const TokenLogProbsParams& p, cudaStream_t stream) {
-    const unsigned blocks = (unsigned)(p.rows * p.parts);
-    if (p.parts == 1) token_log_probs_kernel<T, vectors, picks, true><<<blocks, kThreads, 0, stream>>>(p);
-    else token_log_probs_kernel<T, vectors, picks, false><<<blocks, kThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    if (p.parts == 1) {
+        token_log_probs_kernel<T, vectors, picks, true><<<(unsigned)p.rows, kThreads, 0, stream>>>(p);
+        return cudaGetLastError();
+    }
+    const auto kernel = token_log_probs_kernel<T, vectors, picks, false>;
+    if (p.parts > 8) {  // (more than any device must hold)
+        static OncePerDevice raised;
+        int device = 0;
+        if (const cudaError_t e = cudaGetDevice(&device)) return e;
+        const cudaError_t e = raised.run(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(p.rows * p.parts));
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = (unsigned)p.parts, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, p);
 }
 
 template <class T>
@@ -546,20 +504,23 @@ cudaError_t launch_type(const TokenLogProbsParams& p, cudaStream_t stream) {
 
 void plan_token_log_probs(TokenLogProbsParams& p, int sm_count) {
     const int E = 16 / element_bytes(p.type);
-    // Long parts cost least per logit (what a part costs besides is shared by up to eight chunks); where they would be fewer than the
-    // GPU holds at once, shorter ones spread the rows further.
-    const auto chunks = [&](int vectors) { return ((int64_t)p.vocab + E - 1 + kThreads * vectors * E - 1) / (kThreads * vectors * E); };
-    p.vectors = p.rows * chunks(kLongVectors) < sm_count ? 1 : kLongVectors;
-    const int64_t all = chunks(p.vectors);
-    // Of the numbers of parts that the chunks allow, the one whose rounds of blocks are done first, a part costing some chunks besides its own.
-    constexpr int kBesides = 3;
-    int64_t least = 0;
-    for (int64_t each = std::min<int64_t>(all, kMostChunks); each > 0; --each) {
-        const int64_t parts = (all + each - 1) / each, rounds = (p.rows * parts + sm_count * kBlocks - 1) / (sm_count * kBlocks);
-        const int64_t cost = rounds * ((all + parts - 1) / parts + kBesides);
-        if (least == 0 || cost < least) least = cost, p.parts = (int)parts;
+    // The cluster size and the vectors of a chunk that a row takes least time with.  In us, as measured with 8 alternatives: one CTA by itself takes `chain`
+    // for its steps and `chunk` for each of its chunks, which come one behind the other; every further one on its SM adds what its instructions and
+    // bytes take there.  (64 x 151,936 bf16 in 1, 2, 4, 8, 16 parts: 21.2, 15.5, 13.2, 14.2, 27.5; 2000 x 4000 in one: 23.1 with one vector, 28.7 with
+    // four; 700 x 128,256 fp32 in 1, 2, 4: 84, 79, 91.)  Clusters of 16 are for few rows: they leave SMs idle where there are many.
+    double least = 0.0;
+    for (const int vectors : {kLongVectors, 1}) {
+        const double chunk = vectors == 1 ? 0.375 : 0.79, chain = vectors == 1 ? 4.3 : 5.2, further = vectors == 1 ? 1.2 : 1.7, further_chunk = 0.09 * vectors;
+        const int64_t elements = kThreads * vectors * E, all = (p.vocab + E - 1 + elements - 1) / elements;
+        for (int parts = 1; parts <= kMostParts; parts *= 2) {
+            const int64_t each = (all + parts - 1) / parts;
+            const double beside = std::max(1.0, (double)(p.rows * parts) / sm_count);
+            if (parts > 1 && (each * (parts - 1) >= all || (parts == kMostParts && beside > 1.0))) continue;  // (a part would be empty)
+            const double cost = each * chunk + chain + (parts > 1 ? 1.0 : 0.0) + (beside - 1.0) * (further + further_chunk * each);
+            if (least == 0.0 || cost < least) least = cost, p.parts = parts, p.vectors = vectors, p.chunks = (int)each;
+        }
     }
-    p.chunks = (int)((all + p.parts - 1) / p.parts);  // (no part much shorter than the others)
+    p.group = (p.chunks + kMostGroups - 1) / kMostGroups;
 }
 
 cudaError_t launch_token_log_probs(const TokenLogProbsParams& p, cudaStream_t stream) {
