@@ -15,7 +15,7 @@ struct RotateHeadsParams {
     int64_t total, q_stride, k_stride, v_stride;
     PagedCacheView cache;             // keys == nullptr: none
     int32_t batch, heads, kv_heads, head_dim, rotated, interleaved, type;
-    float eps;
+    float eps, inverse_dims;
     int32_t slabs, slab_rows;         // shares of a position's heads: how many, and heads of one
 };
 
