@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kAhead = 2;  // heads of a lane that are on their way at once
-constexpr int kBlocks = 5;  // that an SM holds, by registers
+constexpr int kBlocks = 6;  // that an SM holds, by registers
 constexpr int kMostPairs = 128;
 constexpr int kRowOk = 0, kRowCacheFull = 64, kRowBadOffsets = 65;  // (psx_row_status)
 
@@ -47,7 +47,7 @@ struct Run {
         __builtin_memcpy(&r.bits, e, sizeof(e));
         return r;
     }
-    __device__ __forceinline__ static Run at(const T* p) { return {__ldcs(reinterpret_cast<const Bits*>(p))}; }
+    __device__ __forceinline__ static Run at(const T* p) { return {__ldg(reinterpret_cast<const Bits*>(p))}; }
     __device__ __forceinline__ void put(T* p) const { *reinterpret_cast<Bits*>(p) = bits; }
 };
 
@@ -233,7 +233,8 @@ template <class T, int run, int lanes>
 cudaError_t launch_lanes(RotateHeadsParams& p, int sm_count, cudaStream_t stream) {
     constexpr int slots = 32 / lanes;
     const int all = p.heads + p.kv_heads + (p.cache.keys ? p.kv_heads : 0);
-    // A warp per position where that fills the GPU, or as many as there are heads to share out.
+    // A warp per position where that fills the GPU, or as many as there are heads to share out.  (Two a position: 108 us instead of 98 in the case
+    // below; a warp for two to five positions one after the other: 144 to 182.)
     const int64_t wanted = std::max<int64_t>(1, (int64_t)sm_count * 32 / std::max<int64_t>(p.total, 1));
     const int64_t most = (all + slots - 1) / slots;
     p.slabs = (int)std::min(wanted, most);
@@ -259,7 +260,7 @@ template <class T>
 cudaError_t launch(RotateHeadsParams& p, int sm_count, cudaStream_t stream) {
     p.inverse_dims = 1.0f / (float)p.head_dim;
     if constexpr (sizeof(T) == 2) {
-        // (12 prompts of up to 2111, 40 heads of 128 and 8 more for the values: MEASURED us with runs of 16 bytes, 213 with 8)
+        // (12 prompts of up to 2111, 40 heads of 128 and 8 more for the values: 98 us with runs of 16 bytes, 213 with 8)
         if (p.rotated % 16 == 0) return launch_run<T, 8>(p, sm_count, stream);
     }
     return launch_run<T, 4>(p, sm_count, stream);
