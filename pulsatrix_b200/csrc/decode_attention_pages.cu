@@ -17,6 +17,7 @@
 #include "decode_attention_pages.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "elements.cuh"
@@ -25,6 +26,7 @@ namespace psx {
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4, kTile = 16;
+constexpr double kSplitRate = 4.0;  // pieces squared for a tile where few pairs are cut to fill the GPU: more are longer in joining than they save
 constexpr int kMostShare = 64;  // tiles that a block takes where shorter pieces only balance
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
@@ -118,12 +120,13 @@ __host__ __device__ constexpr int words_of(int dims, int bytes) { return dims * 
 
 // Blocks that an SM holds, by registers.
 __host__ __device__ constexpr int blocks_of(int dims, int bytes, int tiles_of_rows) {
-    return dims == 256 || (dims == 128 && tiles_of_rows == 2) ? 2 : words_of(dims, bytes) <= 32 && tiles_of_rows == 1 ? 4 : 3;
+    if (dims == 256 || (tiles_of_rows == 2 && bytes == 4)) return 2;
+    return dims == 128 || tiles_of_rows == 2 ? 3 : 4;
 }
 
-// Query rows' parts (fp32) in shared memory, then the warps' contexts.
+// Query rows in shared memory, then the warps' contexts.
 __host__ __device__ constexpr size_t shared_of(int dims, int tiles_of_rows, bool precise) {
-    const size_t meet = (size_t)kWarps * 8 * tiles_of_rows * dims * sizeof(float), parts = precise ? (size_t)tiles_of_rows * dims / 8 * 32 * sizeof(uint4) : 0;
+    const size_t meet = (size_t)kWarps * 8 * tiles_of_rows * dims * sizeof(float), parts = (size_t)tiles_of_rows * dims / (precise ? 8 : 16) * 32 * (precise ? sizeof(uint4) : sizeof(uint2));
     return meet > parts ? meet : parts;
 }
 
@@ -171,29 +174,24 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
     const auto page_of = [&](int tile) { return tile < to_tile ? __ldg(pages + ((tile0 + tile) * kTile >> t.shift)) : -1; };
     int page = page_of(from_tile + warp), next_page = page_of(from_tile + warp + kWarps);
 
-    // The query rows as the right-hand operand: lane (gid, tig) holds row gid's words of the dimensions that it holds of a key.
-    uint32_t held[precise ? 1 : tiles_of_rows][precise ? 1 : kSteps][4];
-    uint4* parts = reinterpret_cast<uint4*>(shared);  // fp32: both parts of two words, by (tile of rows, step, half, lane)
-#pragma unroll
-    for (int n = 0; n < tiles_of_rows; ++n) {
-        const int r = n * 8 + gid;
-        const T* q = static_cast<const T*>(p.q) + element_of(min(r, rows - 1));
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int d = s * 4 * E + tig * E;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (precise && (s & (kWarps - 1)) != warp) continue;  // (the warps share the work)
-            if (r < rows && d < head_dim) x = __ldg(reinterpret_cast<const uint4*>(q + d));
-            if constexpr (precise) {
-                const uint32_t h[4] = {eleven_bits(x.x), eleven_bits(x.y), eleven_bits(x.z), eleven_bits(x.w)};
-                parts[((n * kSteps + s) * 2) * 32 + lane] = make_uint4(h[0], h[1], left_of(x.x, h[0]), left_of(x.y, h[1]));
-                parts[((n * kSteps + s) * 2 + 1) * 32 + lane] = make_uint4(h[2], h[3], left_of(x.z, h[2]), left_of(x.w, h[3]));
-            } else {
-                held[n][s][0] = x.x, held[n][s][1] = x.y, held[n][s][2] = x.z, held[n][s][3] = x.w;
-            }
+    // The query rows as the right-hand operand, in shared memory: for each step of two products, by (tile of rows, step, product, lane), the words
+    // of row gid that lane (gid, tig) wants; fp32's in two parts.  The warps share the work.
+    using Words = typename std::conditional<precise, uint4, uint2>::type;
+    Words* parts = reinterpret_cast<Words*>(shared);
+    for (int i = warp; i < tiles_of_rows * kSteps; i += kWarps) {
+        const int r = i / kSteps * 8 + gid, d = i % kSteps * 4 * E + tig * E;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < rows && d < head_dim) x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + element_of(r) + d));
+        if constexpr (precise) {
+            const uint32_t h[4] = {eleven_bits(x.x), eleven_bits(x.y), eleven_bits(x.z), eleven_bits(x.w)};
+            parts[2 * i * 32 + lane] = make_uint4(h[0], h[1], left_of(x.x, h[0]), left_of(x.y, h[1]));
+            parts[(2 * i + 1) * 32 + lane] = make_uint4(h[2], h[3], left_of(x.z, h[2]), left_of(x.w, h[3]));
+        } else {
+            parts[2 * i * 32 + lane] = make_uint2(x.x, x.y);
+            parts[(2 * i + 1) * 32 + lane] = make_uint2(x.z, x.w);
         }
     }
-    if constexpr (precise) __syncthreads();
+    __syncthreads();
 
     float out[tiles_of_rows][kBlocks][4], top[tiles_of_rows][2], total[tiles_of_rows][2];
     int first[tiles_of_rows][2], last[tiles_of_rows][2];
@@ -214,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
 
     for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
         const int position = (tile0 + tile) * kTile;
-        const bool real = t.real(page), whole = real && position >= seen && position + kTile <= length;
+        const bool real = t.real(page), whole = real && position >= seen && position + kTile <= length, plain = whole && head_dim == dims;
         // What no row sees, and pages that are none, arrive as zeros, whatever lies there.
         const char* k_at = keys + (real ? page : 0) * page_bytes + (position & (t.page_size - 1)) * row_bytes;
         const char* v_at = k_at + apart;
@@ -224,6 +222,17 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
 
         uint4 v[kBlocks / K::tiles][4];
         const auto load_values = [&]() {
+            if (plain) {  // (one address, and distances that are known)
+                const char* at = v_at + ((precise ? tig : 2 * tig) * dims + gid * E) * (int)sizeof(T);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int m = 0; m < kBlocks / K::tiles; ++m) {
+                        v[m][i] = load_once(at + ((precise ? 4 * i : (i & 1) + (i >> 1) * 8) * dims + m * 8 * E) * (int)sizeof(T));
+                    }
+                }
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = precise ? tig + 4 * i : 2 * tig + (i & 1) + (i >> 1) * 8;
@@ -239,16 +248,25 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
         float score[tiles_of_rows][4];
 #pragma unroll
         for (int n = 0; n < tiles_of_rows; ++n) score[n][0] = score[n][1] = score[n][2] = score[n][3] = 0.0f;
-        const bool low_there = there(gid), high_there = there(gid + 8);
 #pragma unroll
         for (int s0 = 0; s0 < kSteps; s0 += kSegment) {
             uint4 k[kSegment][2];
+            if (plain) {
+                const char* at = k_at + (gid * dims + tig * E) * (int)sizeof(T);
 #pragma unroll
-            for (int s = 0; s < kSegment; ++s) {
-                const int d = (s0 + s) * 4 * E + tig * E;
-                k[s][0] = k[s][1] = make_uint4(0, 0, 0, 0);
-                if (low_there && d < head_dim) k[s][0] = load_once(k_at + gid * row_bytes + d * (int)sizeof(T));
-                if (high_there && d < head_dim) k[s][1] = load_once(k_at + (gid + 8) * row_bytes + d * (int)sizeof(T));
+                for (int s = 0; s < kSegment; ++s) {
+                    k[s][0] = load_once(at + (s0 + s) * 4 * E * (int)sizeof(T));
+                    k[s][1] = load_once(at + (8 * dims + (s0 + s) * 4 * E) * (int)sizeof(T));
+                }
+            } else {
+                const bool low_there = there(gid), high_there = there(gid + 8);
+#pragma unroll
+                for (int s = 0; s < kSegment; ++s) {
+                    const int d = (s0 + s) * 4 * E + tig * E;
+                    k[s][0] = k[s][1] = make_uint4(0, 0, 0, 0);
+                    if (low_there && d < head_dim) k[s][0] = load_once(k_at + gid * row_bytes + d * (int)sizeof(T));
+                    if (high_there && d < head_dim) k[s][1] = load_once(k_at + (gid + 8) * row_bytes + d * (int)sizeof(T));
+                }
             }
             if (together) load_values();
 #pragma unroll
@@ -263,7 +281,10 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
                         add_to(score[n], some);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) multiply(score[n], a[j], held[n][s0 + s][2 * j], held[n][s0 + s][2 * j + 1], T{});
+                        for (int j = 0; j < 2; ++j) {
+                            const Words q = parts[((n * kSteps + s0 + s) * 2 + j) * 32 + lane];
+                            multiply(score[n], a[j], q.x, q.y, T{});
+                        }
                     }
                 }
             }
@@ -513,7 +534,7 @@ void plan_paged_attention(PagedAttentionParams& p, int sm_count) {
     const int64_t blocks = (int64_t)sm_count * blocks_of(dims, width, tiles_of_rows(p));
     // The pieces of a pair have their maxima and sums in shared memory when they are joined.
     const int64_t most = std::min<int64_t>((tiles + kWarps - 1) / kWarps, shared_of(dims, tiles_of_rows(p), width == 4) / (8 * tiles_of_rows(p) * sizeof(float2)));
-    const int64_t spread = std::max<int64_t>(1, blocks / units);
+    const int64_t spread = std::max<int64_t>(1, std::min(blocks / units, (int64_t)std::sqrt(kSplitRate * tiles)));
     const int64_t balanced = std::min((tiles + kMostShare - 1) / kMostShare, 16 * blocks / units);  // (blocks that find nothing to do cost time too)
     p.spread = (int)std::min(spread, most);
     p.pieces = (int)std::min(std::max(spread, balanced), most);
