@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
     constexpr int E = K::elements, kSteps = dims / (4 * E);  // 16 bytes of a lane for every so many dimensions of a key
     constexpr int kBlocks = dims / 16, kRows = 8 * tiles_of_rows;
     constexpr int kSegment = kSteps < 64 / 8 ? kSteps : 64 / 8;  // of steps whose two rows a lane holds at once
-    constexpr bool together = words_of(dims, sizeof(T)) <= 32;   // keys and values of a tile are asked for at once
+    constexpr bool keys_ahead = words_of(dims, sizeof(T)) <= 32;      // the next tile's keys are on their way while this one's values are in work
     extern __shared__ __align__(16) uint8_t shared[];
     __shared__ float tops[kWarps][kRows], totals[kWarps][kRows];
     __shared__ int is_last;
@@ -210,65 +210,80 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
     const int all_from = sight.first(p.q_len - 1), all_to = sight.last(0, p.causal != 0);  // every row sees those between
     const float factor = p.scale * kLog2e;
 
-    for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
-        const int position = (tile0 + tile) * kTile;
-        const bool real = t.real(page), whole = real && position >= seen && position + kTile <= length, plain = whole && head_dim == dims;
-        // What no row sees, and pages that are none, arrive as zeros, whatever lies there.
-        const char* k_at = keys + (real ? page : 0) * page_bytes + (position & (t.page_size - 1)) * row_bytes;
-        const char* v_at = k_at + apart;
-        const auto there = [&](int r) { return whole || (real && position + r >= seen && position + r < length); };
-        page = next_page;
-        next_page = page_of(tile + 2 * kWarps);
-
-        uint4 v[kBlocks / K::tiles][4];
-        const auto load_values = [&]() {
-            if (plain) {  // (one address, and distances that are known)
-                const char* at = v_at + ((precise ? tig : 2 * tig) * dims + gid * E) * (int)sizeof(T);
+    // A tile, and where its positions lie.  What no row sees, and pages that are none, arrive as zeros, whatever lies there.
+    struct Place {
+        int position;
+        bool real, whole, plain;  // its page is one of the pool; all of its positions are seen by some row; and its rows are as long as the kernel's
+        const char* keys;
+    };
+    const auto place_of = [&](int tile, int page) {
+        Place at;
+        at.position = (tile0 + tile) * kTile;
+        at.real = t.real(page);  // (a tile that is not there has the page -1)
+        at.whole = at.real && at.position >= seen && at.position + kTile <= length;
+        at.plain = at.whole && head_dim == dims;
+        at.keys = keys + (at.real ? page : 0) * page_bytes + (at.position & (t.page_size - 1)) * row_bytes;
+        return at;
+    };
+    const auto there = [&](const Place& at, int r) { return at.whole || (at.real && at.position + r >= seen && at.position + r < length); };
+    uint4 k[kSegment][2], v[kBlocks / K::tiles][4];
+    const auto load_keys = [&](const Place& place, int s0) {
+        if (place.plain) {  // (one address, and distances that are known)
+            const char* at = place.keys + (gid * dims + tig * E) * (int)sizeof(T);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (int m = 0; m < kBlocks / K::tiles; ++m) {
-                        v[m][i] = load_once(at + ((precise ? 4 * i : (i & 1) + (i >> 1) * 8) * dims + m * 8 * E) * (int)sizeof(T));
-                    }
-                }
-                return;
+            for (int s = 0; s < kSegment; ++s) {
+                k[s][0] = load_once(at + (s0 + s) * 4 * E * (int)sizeof(T));
+                k[s][1] = load_once(at + (8 * dims + (s0 + s) * 4 * E) * (int)sizeof(T));
             }
+        } else {
+            const bool low_there = there(place, gid), high_there = there(place, gid + 8);
+#pragma unroll
+            for (int s = 0; s < kSegment; ++s) {
+                const int d = (s0 + s) * 4 * E + tig * E;
+                k[s][0] = k[s][1] = make_uint4(0, 0, 0, 0);
+                if (low_there && d < head_dim) k[s][0] = load_once(place.keys + gid * row_bytes + d * (int)sizeof(T));
+                if (high_there && d < head_dim) k[s][1] = load_once(place.keys + (gid + 8) * row_bytes + d * (int)sizeof(T));
+            }
+        }
+    };
+    const auto load_values = [&](const Place& place) {
+        if (place.plain) {
+            const char* at = place.keys + apart + ((precise ? tig : 2 * tig) * dims + gid * E) * (int)sizeof(T);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int m = 0; m < kBlocks / K::tiles; ++m) {
+                    v[m][i] = load_once(at + ((precise ? 4 * i : (i & 1) + (i >> 1) * 8) * dims + m * 8 * E) * (int)sizeof(T));
+                }
+            }
+        } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = precise ? tig + 4 * i : 2 * tig + (i & 1) + (i >> 1) * 8;
-                const bool real_row = there(r);
+                const bool real_row = there(place, r);
 #pragma unroll
                 for (int m = 0; m < kBlocks / K::tiles; ++m) {
                     const int d = m * 8 * E + gid * E;
                     v[m][i] = make_uint4(0, 0, 0, 0);
-                    if (real_row && d < head_dim) v[m][i] = load_once(v_at + r * row_bytes + d * (int)sizeof(T));
+                    if (real_row && d < head_dim) v[m][i] = load_once(place.keys + apart + r * row_bytes + d * (int)sizeof(T));
                 }
             }
-        };
+        }
+    };
+    Place now = place_of(from_tile + warp, page);
+    if (keys_ahead) load_keys(now, 0);
+    for (int tile = from_tile + warp; tile < to_tile; tile += kWarps) {
+        const Place next = place_of(tile + kWarps, next_page);
+        next_page = page_of(tile + 2 * kWarps);
+        const int position = now.position;
+        const bool real = now.real;
+        if (keys_ahead) load_values(now);
         float score[tiles_of_rows][4];
 #pragma unroll
         for (int n = 0; n < tiles_of_rows; ++n) score[n][0] = score[n][1] = score[n][2] = score[n][3] = 0.0f;
 #pragma unroll
         for (int s0 = 0; s0 < kSteps; s0 += kSegment) {
-            uint4 k[kSegment][2];
-            if (plain) {
-                const char* at = k_at + (gid * dims + tig * E) * (int)sizeof(T);
-#pragma unroll
-                for (int s = 0; s < kSegment; ++s) {
-                    k[s][0] = load_once(at + (s0 + s) * 4 * E * (int)sizeof(T));
-                    k[s][1] = load_once(at + (8 * dims + (s0 + s) * 4 * E) * (int)sizeof(T));
-                }
-            } else {
-                const bool low_there = there(gid), high_there = there(gid + 8);
-#pragma unroll
-                for (int s = 0; s < kSegment; ++s) {
-                    const int d = (s0 + s) * 4 * E + tig * E;
-                    k[s][0] = k[s][1] = make_uint4(0, 0, 0, 0);
-                    if (low_there && d < head_dim) k[s][0] = load_once(k_at + gid * row_bytes + d * (int)sizeof(T));
-                    if (high_there && d < head_dim) k[s][1] = load_once(k_at + (gid + 8) * row_bytes + d * (int)sizeof(T));
-                }
-            }
-            if (together) load_values();
+            if (!keys_ahead) load_keys(now, s0);
 #pragma unroll
             for (int s = 0; s < kSegment; ++s) {
                 const uint32_t a[2][4] = {{k[s][0].x, k[s][1].x, k[s][0].y, k[s][1].y}, {k[s][0].z, k[s][1].z, k[s][0].w, k[s][1].w}};
@@ -289,7 +304,9 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
                 }
             }
         }
-        if (!together) load_values();
+        if (keys_ahead) load_keys(next, 0);
+        else load_values(now);
+        now = next;
         // score[n][2 o + i]: position 8 o + gid, query row 8 n + 2 tig + i
         const bool masked = !real || position < all_from || position + kTile - 1 > all_to;
 #pragma unroll
