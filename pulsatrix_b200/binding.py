@@ -336,10 +336,10 @@ class PageTable:
 
     def __init__(self, pages, lengths, references, page_size=64):
         torch = _torch or _torch_module()
-        shape = pages.shape
-        if len(shape) != 2 or pages.dtype is not torch.int32 or not pages.is_contiguous():
+        if pages.dim() != 2 or pages.dtype is not torch.int32 or not pages.is_contiguous():
             raise ValueError("pages are contiguous int32 (rows, max_pages)")
-        rows, max_pages = shape
+        rows, max_pages = pages.shape
+        num_pages = references.numel()
         if not (lengths.dtype is torch.int64 and lengths.numel() == rows and lengths.is_contiguous() and references.dtype is torch.int32 and
                 references.is_contiguous()):
             raise ValueError("lengths are int64 (rows), references int32 (num_pages)")
@@ -347,9 +347,10 @@ class PageTable:
         if not device == lengths.get_device() == references.get_device():
             raise ValueError("a page table lies on one device")
         self.pages, self.lengths, self.references = pages, lengths, references
-        self.rows, self.max_pages, self.num_pages, self.page_size = rows, max_pages, references.numel(), page_size
-        self._layout = PageTableLayout(pages.data_ptr(), lengths.data_ptr(), references.data_ptr(), rows, max_pages, self.num_pages, page_size)
-        self._address = C.addressof(self._layout)
+        self.rows, self.max_pages, self.num_pages, self.page_size = rows, max_pages, num_pages, page_size
+        # (PageTableLayout's words: an array is made in a third of the time)
+        self._layout = array.array("q", (pages.data_ptr(), lengths.data_ptr(), references.data_ptr(), rows, max_pages, num_pages, page_size))
+        self._address = self._layout.buffer_info()[0]
 
     @classmethod
     def empty(cls, rows, max_pages, num_pages, page_size=64, device="cuda"):
@@ -369,13 +370,15 @@ class PagedCache:
             raise ValueError("pages are (num_pages, kv_heads, page_size, head_dim)")
         if not (value_pages.shape == shape and key_pages.dtype is value_pages.dtype and key_pages.is_contiguous() and value_pages.is_contiguous()):
             raise ValueError("keys and values are contiguous tensors of one shape and type")
-        if not table.device == key_pages.get_device() == value_pages.get_device():
+        self.device = device = table.device
+        if not device == key_pages.get_device() == value_pages.get_device():
             raise ValueError("a cache lies on one device")
         self.dtype_code = _dtype_code(key_pages)
         self.table, self.key_pages, self.value_pages = table, key_pages, value_pages
-        self.device, self.kv_heads, self.head_dim = table.device, shape[1], shape[3]
-        self._layout = PagedCacheLayout(table._layout, key_pages.data_ptr(), value_pages.data_ptr(), shape[1], shape[3])
-        self._address = C.addressof(self._layout)
+        _, self.kv_heads, _, self.head_dim = shape
+        self._layout = layout = table._layout[:]  # (PagedCacheLayout's words)
+        layout.extend((key_pages.data_ptr(), value_pages.data_ptr(), self.kv_heads, self.head_dim))
+        self._address = layout.buffer_info()[0]
 
     def pools(self):
         """Its tensors as Context.extend_pages and compact_pages take them."""
@@ -866,6 +869,13 @@ class Context:
             _check(code)
         return used
 
+    def _norm_weight(self, weight, kind, head_dim):
+        if not (weight.dtype is kind and weight.numel() == head_dim and weight.is_contiguous()):
+            raise ValueError("a norm's weight is (head_dim), of q's type")
+        if weight.get_device() != self.device:
+            self._here(weight)
+        return weight.data_ptr()
+
     def rotate_heads(self, q, k, v=None, *, offsets, first, frequencies=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, cache=None,
                      keys_too=None, stream=None):
         """Queries and keys on their way into the attention (psx_b200_rotate_heads): norm per head (q_weight, k_weight: (head_dim)), rotation by the
@@ -874,50 +884,51 @@ class Context:
         (batch), the position of a row's first new one.  Returns q and k as they are then (k only with keys_too, which is so without a cache) and the
         rows' statuses, int32."""
         torch = _torch or _torch_module()
-        if keys_too is None:
-            keys_too = cache is None
-        q_shape, k_shape = q.shape, k.shape
-        total, heads, head_dim = q_shape
+        total, heads, head_dim = q.shape
+        k_shape, kind, here = k.shape, q.dtype, self.device
         kv_heads = k_shape[1]
-        if not (k_shape == (total, kv_heads, head_dim) and q.dtype is k.dtype):
+        if not (k_shape == (total, kv_heads, head_dim) and kind is k.dtype):
             raise ValueError("q and k are (total, heads, head_dim) of one type")
-        q_stride, k_stride, v_stride = q.stride(), k.stride(), k.stride()
-        here = self.device
+        q_stride, q_head, q_dim = q.stride()
+        k_stride, k_head, k_dim = k.stride()
+        v_stride, v_head, v_dim, v_at, cache_at = k_stride, k_head, 1, None, None
         if cache is not None:
-            if v is None or v.shape != k_shape or v.dtype is not k.dtype or cache.dtype_code != _dtype_code(k):
+            if v is None or v.shape != k_shape or v.dtype is not kind or kind is not cache.key_pages.dtype:
                 raise ValueError("what a cache stores is k and v of one shape and of its type")
-            v_stride = v.stride()
+            v_stride, v_head, v_dim = v.stride()
+            v_at, cache_at = v.data_ptr(), cache._address
             if not cache.device == here == v.get_device():
                 self._here(cache.key_pages, v)
-        if total and not (q_stride[2] == k_stride[2] == v_stride[2] == 1 and (heads == 1 or q_stride[1] == head_dim) and
-                          (kv_heads == 1 or k_stride[1] == v_stride[1] == head_dim)):
+        elif keys_too is None:
+            keys_too = True
+        if total and not (q_dim == k_dim == v_dim == 1 and (heads == 1 or q_head == head_dim) and (kv_heads == 1 or k_head == v_head == head_dim)):
             raise ValueError("heads and dimensions of a position are contiguous")
         batch = offsets.numel() - 1
         if not (offsets.dtype is first.dtype is torch.int64 and batch >= 0 and first.numel() == batch and offsets.is_contiguous() and first.is_contiguous()):
             raise ValueError("offsets are int64 (batch + 1), first is int64 (batch)")
         if not q.get_device() == here == k.get_device() == offsets.get_device() == first.get_device():
             self._here(q, k, offsets, first)
-        rotated = 0
+        rotated, frequencies_at, q_weight_at, k_weight_at = 0, None, None, None
         if frequencies is not None:
             if not (frequencies.dtype is torch.float64 and frequencies.is_contiguous()):
                 raise ValueError("frequencies are contiguous float64")
-            self._here(frequencies)
-            rotated = 2 * frequencies.numel()
-        for weight in (q_weight, k_weight):
-            if weight is not None:
-                if not (weight.dtype is q.dtype and weight.numel() == head_dim and weight.is_contiguous()):
-                    raise ValueError("a norm's weight is (head_dim), of q's type")
-                self._here(weight)
-        q_out = torch.empty_like(q) if q.is_contiguous() else self._empty((total, heads, head_dim), q.dtype)
-        k_out = self._empty((total, kv_heads, head_dim), k.dtype) if keys_too else None
+            if frequencies.get_device() != here:
+                self._here(frequencies)
+            rotated, frequencies_at = 2 * frequencies.numel(), frequencies.data_ptr()
+        if q_weight is not None:
+            q_weight_at = self._norm_weight(q_weight, kind, head_dim)
+        if k_weight is not None:
+            k_weight_at = self._norm_weight(k_weight, kind, head_dim)
+        width, key_width = heads * head_dim, kv_heads * head_dim
+        q_out = torch.empty_like(q) if q_stride == width and q.is_contiguous() else self._empty((total, heads, head_dim), kind)
+        k_out = self._empty((total, kv_heads, head_dim), kind) if keys_too else None
         status = self._empty((batch,), torch.int32)
-        many = total > 1
-        width = kv_heads * head_dim
-        code = _native.rotate_heads(self._handle, _stream_of(q) if stream is None else stream, _dtype_code(q), q.data_ptr(), k.data_ptr(),
-                                    None if v is None else v.data_ptr(), q_out.data_ptr(), None if k_out is None else k_out.data_ptr(), total,
-                                    q_stride[0] if many else heads * head_dim, k_stride[0] if many else width, v_stride[0] if many else width,
-                                    offsets.data_ptr(), first.data_ptr(), batch, heads, kv_heads, head_dim, _ptr(q_weight), _ptr(k_weight), eps,
-                                    _ptr(frequencies), rotated, 1 if interleaved else 0, None if cache is None else cache._address, status.data_ptr())
+        if total <= 1:
+            q_stride, k_stride, v_stride = width, key_width, key_width
+        code = _native.rotate_heads(self._handle, _stream_of(q) if stream is None else stream, _dtype_code(q), q.data_ptr(), k.data_ptr(), v_at,
+                                    q_out.data_ptr(), None if k_out is None else k_out.data_ptr(), total, q_stride, k_stride, v_stride, offsets.data_ptr(),
+                                    first.data_ptr(), batch, heads, kv_heads, head_dim, q_weight_at, k_weight_at, eps, frequencies_at, rotated,
+                                    1 if interleaved else 0, cache_at, status.data_ptr())
         if code:
             _check(code)
         return q_out, k_out, status
@@ -947,7 +958,8 @@ class Context:
         not asked for is None."""
         torch = _torch or _torch_module()
         rows, columns = logits.shape
-        vocab = columns if vocab is None else vocab
+        if vocab is None:
+            vocab = columns
         if not 0 < vocab <= columns:
             raise ValueError("a row holds `vocab` logits at least")
         row_stride, column_stride = logits.stride()
@@ -955,20 +967,28 @@ class Context:
             row_stride = columns
         if column_stride != 1 and rows and vocab > 1:
             raise ValueError("a row's logits are contiguous")
-        self._here(logits)
-        log_probs = entropies = top_log_probs = top_tokens = None
+        here = self.device
+        if logits.get_device() != here:
+            self._here(logits)
+        log_probs = entropies = top_log_probs = top_tokens = tokens_at = log_probs_at = entropies_at = top_log_probs_at = top_tokens_at = None
+        of_rows = (rows,)
         if tokens is not None:
             if not (tokens.dtype is torch.int64 and tokens.numel() == rows and tokens.is_contiguous()):
                 raise ValueError("one int64 token per row")
-            self._here(tokens)
-            log_probs = self._empty((rows,), torch.float32)
+            if tokens.get_device() != here:
+                self._here(tokens)
+            log_probs = self._empty(of_rows, torch.float32)
+            tokens_at, log_probs_at = tokens.data_ptr(), log_probs.data_ptr()
         if entropy:
-            entropies = self._empty((rows,), torch.float32)
+            entropies = self._empty(of_rows, torch.float32)
+            entropies_at = entropies.data_ptr()
         if top > 0:
-            top_log_probs, top_tokens = self._empty((rows, top), torch.float32), self._empty((rows, top), torch.int64)
-        status = self._empty((rows,), torch.int32)
+            of_top = (rows, top)
+            top_log_probs, top_tokens = self._empty(of_top, torch.float32), self._empty(of_top, torch.int64)
+            top_log_probs_at, top_tokens_at = top_log_probs.data_ptr(), top_tokens.data_ptr()
+        status = self._empty(of_rows, torch.int32)
         code = _native.token_log_probs(self._handle, _stream_of(logits) if stream is None else stream, _dtype_code(logits), logits.data_ptr(), rows, vocab,
-                                       row_stride, _ptr(tokens), _ptr(log_probs), _ptr(entropies), top, _ptr(top_log_probs), _ptr(top_tokens), status.data_ptr())
+                                       row_stride, tokens_at, log_probs_at, entropies_at, top, top_log_probs_at, top_tokens_at, status.data_ptr())
         if code:
             _check(code)
         return {"log_probs": log_probs, "entropy": entropies, "top_log_probs": top_log_probs, "top_tokens": top_tokens, "status": status}
