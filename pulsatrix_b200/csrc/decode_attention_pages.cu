@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "elements.cuh"
+#include "psx_device.cuh"
 
 namespace psx {
 namespace {
@@ -146,6 +147,8 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
     const int head_dim = p.cache.head_dim, kv_heads = p.cache.kv_heads;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, gid = lane / 4, tig = lane % 4;
 
+    grid_dependency_wait();
+    grid_dependents_may_launch();
     // This block's pair (beyond 128 dimensions eight of its query rows), and its tiles of the pair's.
     const int unit = (int)(blockIdx.x / (unsigned)p.pieces), number = (int)(blockIdx.x % (unsigned)p.pieces);
     const int pair = dims == 256 ? unit / p.row_groups : unit, first_row = dims == 256 ? unit % p.row_groups * kRows : 0;
@@ -525,12 +528,11 @@ int tiles_of_rows(const PagedAttentionParams& p) { return p.rows <= 8 || padded_
 template <class T, int dims, int tiles_of_rows>
 cudaError_t launch(const PagedAttentionParams& p, cudaStream_t stream) {
     constexpr size_t shared = shared_of(dims, tiles_of_rows, sizeof(T) == 4);
-    const auto kernel = decode_attention_pages_kernel<T, dims, tiles_of_rows>;
+    void (*const kernel)(const PagedAttentionParams) = decode_attention_pages_kernel<T, dims, tiles_of_rows>;
     if (shared > 40 << 10) {
         if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared)) return e;
     }
-    kernel<<<(unsigned)(paged_attention_counters(p) * p.pieces), kThreads, shared, stream>>>(p);
-    return cudaGetLastError();
+    return launch_overlapping(kernel, dim3((unsigned)(paged_attention_counters(p) * p.pieces)), dim3(kThreads), shared, stream, p);
 }
 
 template <class T>

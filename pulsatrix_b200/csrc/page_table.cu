@@ -61,11 +61,12 @@ __device__ __forceinline__ int4 four_references(const PageTableView& t, int at) 
 // the number of free pages, as far as they are asked for, and once to give them out.
 __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid_constant__ ExtendPagesParams p) {
     extern __shared__ __align__(16) char shared[];
-    __shared__ int64_t carry[kPlanWarps];
+    __shared__ uint64_t carry[kPlanWarps];
     const PageTableView& t = p.table;
     const int rows = t.rows;
     int* ends = reinterpret_cast<int*>(shared);  // pages that rows 0 .. row ask for together (more than there are: one more than those)
-    int* goes_on = ends + rows;                  // the shared page that a row goes on in; then only of those that copy it; else -1
+    int* goes_on = ends + (rows + 3) / 4 * 4;    // the shared page that a row goes on in; then only of those that copy it; else -1
+    grid_dependency_wait();
     grid_dependents_may_launch();
 
     int status[kRowsPerThread], length[kRowsPerThread], added[kRowsPerThread], held_by[kRowsPerThread];
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
         shares |= page >= 0;
         goes_on[row] = page;
     }
+    if (threadIdx.x < 4) goes_on[rows + threadIdx.x] = -1;
     bool copies[kRowsPerThread] = {};
     if (__syncthreads_or(shares)) {
 #pragma unroll
@@ -101,8 +103,12 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
             if (i >= count || goes_on[first + i] < 0) continue;
             const int page = goes_on[first + i];
             int going = 0, last = 0;
-            for (int row = 0; row < rows; ++row) {
-                if (goes_on[row] == page) ++going, last = row;
+            for (int row = 0; row < (rows + 3) / 4 * 4; row += 4) {  // (behind the last row: -1)
+                const int4 four = *reinterpret_cast<const int4*>(goes_on + row);
+                if (four.x == page) ++going, last = row;
+                if (four.y == page) ++going, last = row + 1;
+                if (four.z == page) ++going, last = row + 2;
+                if (four.w == page) ++going, last = row + 3;
             }
             copies[i] = !(going == held_by[i] && last == first + i);
         }
@@ -112,13 +118,16 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
             if (i < count && !copies[i]) goes_on[first + i] = -1;
         }
     }
-    int64_t mine = 0, need[kRowsPerThread];
+    int64_t mine = 0;
+    int need[kRowsPerThread];
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
         need[i] = t.pages_of(length[i] + added[i]) - t.pages_of(length[i]) + copies[i];
         mine += need[i];
     }
-    int64_t asked, before = sum_before(mine, carry, asked);
+    uint64_t all;
+    int64_t before = (int64_t)sum_before((uint64_t)mine, carry, all);
+    const int asked = (int)min((int64_t)all, (int64_t)t.num_pages + 1);
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
         before += need[i];
@@ -127,22 +136,27 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
             p.copies[first + i].filled = 0;
         }
     }
-    int64_t available = 0;
+    int available = 0;
     if (asked > 0) {
-        constexpr int kRead = 4;  // of four references, of a thread at a time
-        for (int64_t base = 0; base < t.num_pages && available < asked; base += kRead * 4 * kPlanThreads) {
-            int free = 0;
+        constexpr int kRead = 4;                               // of four references, of a thread at a time
+        constexpr int kStretch = kRead * 4 * kPlanThreads;     // of pages
+        int4 held[kRead];
+        uint64_t ahead = 0, totals = 0;  // free pages before this thread's, and in all, of each of the four: 16 bits each
+        const auto read = [&](int base) {
+            uint64_t free = 0;
 #pragma unroll
             for (int k = 0; k < kRead; ++k) {
-                const int64_t at = base + (k * kPlanThreads + (int)threadIdx.x) * 4;
-                if (at < t.num_pages) {
-                    const int4 r = four_references(t, (int)at);
-                    free += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
-                }
+                const int64_t at = (int64_t)base + (k * kPlanThreads + (int)threadIdx.x) * 4;
+                held[k] = at < t.num_pages ? four_references(t, (int)at) : make_int4(1, 1, 1, 1);
+                free |= (uint64_t)((held[k].x == 0) + (held[k].y == 0) + (held[k].z == 0) + (held[k].w == 0)) << (16 * k);
             }
-            int64_t of_all;
-            sum_before((int64_t)free, carry, of_all);
-            available += of_all;
+            ahead = sum_before(free, carry, totals);
+            return (int)((totals & 0xffff) + (totals >> 16 & 0xffff) + (totals >> 32 & 0xffff) + (totals >> 48));
+        };
+        int base = 0;
+        for (; base < t.num_pages; base += kStretch) {
+            available += read(base);
+            if (available >= asked) break;
         }
         // Rows in order, until one asks for more than there is: the pages of those before it.
         int low = 0, high = rows;  // the first row whose end is beyond what is there
@@ -151,36 +165,39 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
             if (ends[middle] > available) high = middle;
             else low = middle + 1;
         }
-        const int64_t given = low > 0 ? ends[low - 1] : 0;
-        int64_t rank = 0;
-        for (int64_t base = 0; base < t.num_pages && rank < given; base += 4 * kPlanThreads) {
-            const int at = (int)(base + threadIdx.x * 4);
-            const int4 r = base + threadIdx.x * 4 < t.num_pages ? four_references(t, at) : make_int4(1, 1, 1, 1);
-            const int here[4] = {r.x == 0, r.y == 0, r.z == 0, r.w == 0};
-            int64_t of_all, next = rank + sum_before((int64_t)(here[0] + here[1] + here[2] + here[3]), carry, of_all);
+        const int given = low > 0 ? ends[low - 1] : 0;
+        int rank = 0;
+        bool at_hand = base == 0;  // (the first stretch was enough, and is still there)
+        for (base = 0; base < t.num_pages && rank < given; base += kStretch) {
+            if (!at_hand) read(base);
+            at_hand = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (!here[k]) continue;
-                if (next < given) {
-                    const int page = at + k;
-                    int from = 0, to = rows - 1;  // the row that the page is for: the first that ends behind it
-                    while (from < to) {
-                        const int middle = (from + to) / 2;
-                        if (ends[middle] > next) to = middle;
-                        else from = middle + 1;
+            for (int k = 0; k < kRead; ++k) {
+                const int here[4] = {held[k].x == 0, held[k].y == 0, held[k].z == 0, held[k].w == 0};
+                int next = rank + (int)(ahead >> (16 * k) & 0xffff);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (here[j] && next < given) {
+                        const int page = base + (k * kPlanThreads + (int)threadIdx.x) * 4 + j;
+                        int from = 0, to = rows - 1;  // the row that the page is for: the first that ends behind it
+                        while (from < to) {
+                            const int middle = (from + to) / 2;
+                            if (ends[middle] > next) to = middle;
+                            else from = middle + 1;
+                        }
+                        const int slot = next - (from > 0 ? ends[from - 1] : 0), length_of = (int)t.lengths[from], old = goes_on[from];
+                        t.references[page] = 1;
+                        const int entry = old >= 0 && slot == 0 ? length_of >> t.shift : t.pages_of(length_of) + slot - (old >= 0);
+                        t.pages[(int64_t)from * t.max_pages + entry] = page;
+                        if (old >= 0 && slot == 0) {
+                            p.copies[from] = {old, page, length_of & (t.page_size - 1), 0};
+                            atomicSub(t.references + old, 1);  // (another row holds it still: it does not become free meanwhile)
+                        }
                     }
-                    const int slot = (int)(next - (from > 0 ? ends[from - 1] : 0)), held = (int)t.lengths[from], old = goes_on[from];
-                    t.references[page] = 1;
-                    const int entry = old >= 0 && slot == 0 ? held >> t.shift : t.pages_of(held) + slot - (old >= 0);
-                    t.pages[(int64_t)from * t.max_pages + entry] = page;
-                    if (old >= 0 && slot == 0) {
-                        p.copies[from] = {old, page, held & (t.page_size - 1), 0};
-                        atomicSub(t.references + old, 1);  // (another row holds it still: it does not become free meanwhile)
-                    }
+                    next += here[j];
                 }
-                ++next;
+                rank += (int)(totals >> (16 * k) & 0xffff);
             }
-            rank += of_all;
         }
         __syncthreads();  // (lengths are read until here)
     }
@@ -251,6 +268,8 @@ __global__ void __launch_bounds__(kForkThreads) fork_pages_kernel(const __grid_c
     __shared__ int most;
     const PageTableView& t = p.table;
     const int threads = blockDim.x;
+    grid_dependency_wait();
+    grid_dependents_may_launch();
     const int64_t row0 = (int64_t)blockIdx.x * p.beams;
     if (threadIdx.x == 0) most = 0;
     __syncthreads();
@@ -283,6 +302,8 @@ constexpr int kReleaseThreads = 128;
 
 __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const __grid_constant__ ReleasePagesParams p) {
     const PageTableView& t = p.table;
+    grid_dependency_wait();
+    grid_dependents_may_launch();
     const int row = blockIdx.x, length = t.length(row);
     const int kept = p.keep ? (int)min(max(p.keep[row], (int64_t)0), (int64_t)length) : 0;
     __syncthreads();  // (every thread has read the length)
@@ -297,28 +318,31 @@ __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const __
 // With `used` pages in use, those behind the first `used` places move into the free ones among them, both in ascending order.  No page is
 // read and written, so the moves need no order.
 __global__ void __launch_bounds__(kPlanThreads) compact_pages_kernel(const __grid_constant__ CompactPagesParams p) {
-    __shared__ int64_t carry[kPlanWarps];
+    __shared__ uint64_t carry[kPlanWarps];
     const PageTableView& t = p.table;
+    grid_dependency_wait();
     grid_dependents_may_launch();
     int in_use = 0;
     for (int64_t at = threadIdx.x * 4; at < t.num_pages; at += 4 * kPlanThreads) {
         const int4 r = four_references(t, (int)at);
         in_use += (r.x > 0) + (r.y > 0 && at + 1 < t.num_pages) + (r.z > 0 && at + 2 < t.num_pages) + (r.w > 0 && at + 3 < t.num_pages);
     }
-    int64_t used, free_found = 0, moved = 0;
-    sum_before((int64_t)in_use, carry, used);
+    uint64_t all;
+    int64_t free_found = 0, moved = 0;
+    sum_before((uint64_t)in_use, carry, all);
+    const int64_t used = (int64_t)all;
     for (int64_t base = 0; base < t.num_pages; base += 4 * kPlanThreads) {
         const int64_t at = base + threadIdx.x * 4;
         const int4 r = at < t.num_pages ? four_references(t, (int)at) : make_int4(1, 1, 1, 1);
         const int held[4] = {r.x, r.y, r.z, r.w};
-        int64_t counts = 0, of_all;  // goals in the low half, movers in the high one
+        uint64_t counts = 0, of_all;  // goals in the low half, movers in the high one
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (at + k < used) counts += held[k] <= 0;
-            else if (at + k < t.num_pages) counts += held[k] > 0 ? int64_t(1) << 32 : 0;
+            else if (at + k < t.num_pages) counts += held[k] > 0 ? uint64_t(1) << 32 : 0;
         }
-        const int64_t before = sum_before(counts, carry, of_all);
-        int64_t goal = free_found + (before & 0xffffffff), mover = moved + (before >> 32);
+        const uint64_t before = sum_before(counts, carry, of_all);
+        int64_t goal = free_found + (int64_t)(before & 0xffffffff), mover = moved + (int64_t)(before >> 32);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (at + k < used) {
@@ -327,8 +351,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_pages_kernel(const __gri
                 if (held[k] > 0) p.from[mover++] = (int)at + k;
             }
         }
-        free_found += of_all & 0xffffffff;
-        moved += of_all >> 32;
+        free_found += (int64_t)(of_all & 0xffffffff);
+        moved += (int64_t)(of_all >> 32);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < moved; i += kPlanThreads) {
@@ -385,8 +409,7 @@ void set_widths(PagePools& pools) {
 }  // namespace
 
 cudaError_t launch_extend_pages(const ExtendPagesParams& p, cudaStream_t stream) {
-    extend_pages_kernel<<<1, kPlanThreads, (size_t)p.table.rows * 2 * sizeof(int), stream>>>(p);
-    return cudaGetLastError();
+    return launch_overlapping(extend_pages_kernel, dim3(1), dim3(kPlanThreads), ((size_t)p.table.rows * 2 + 16) * sizeof(int), stream, p);
 }
 
 cudaError_t launch_copy_last_pages(const ExtendPagesParams& p, PagePools& pools, int sm_count, cudaStream_t stream) {
@@ -403,18 +426,15 @@ cudaError_t launch_copy_last_pages(const ExtendPagesParams& p, PagePools& pools,
 
 cudaError_t launch_fork_pages(const ForkPagesParams& p, cudaStream_t stream) {
     const int threads = p.beams > kForkColumns / kForkThreads ? kForkThreads / 2 : kForkThreads;
-    fork_pages_kernel<<<(unsigned)p.groups, threads, (size_t)p.beams * threads * sizeof(int), stream>>>(p);
-    return cudaGetLastError();
+    return launch_overlapping(fork_pages_kernel, dim3((unsigned)p.groups), dim3(threads), (size_t)p.beams * threads * sizeof(int), stream, p);
 }
 
 cudaError_t launch_release_pages(const ReleasePagesParams& p, cudaStream_t stream) {
-    release_pages_kernel<<<(unsigned)p.table.rows, kReleaseThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch_overlapping(release_pages_kernel, dim3((unsigned)p.table.rows), dim3(kReleaseThreads), 0, stream, p);
 }
 
 cudaError_t launch_compact_pages(const CompactPagesParams& p, cudaStream_t stream) {
-    compact_pages_kernel<<<1, kPlanThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch_overlapping(compact_pages_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p);
 }
 
 cudaError_t launch_move_pages(const CompactPagesParams& p, PagePools& pools, bool entries, int sm_count, cudaStream_t stream) {

@@ -258,21 +258,28 @@ inline cudaError_t allow_all_dynamic_shared_once(OncePerDevice& done, Kernel ker
 }
 
 // Launches `kernel` so that it may begin while the kernel before it in `stream` is still running
-// (see grid_dependency_wait above); PSX_B200_NO_PDL=1 in the environment launches the ordinary way.
+// (see grid_dependency_wait above); PSX_B200_NO_PDL=1 in the environment launches the ordinary way.  `cluster`: blocks
+// of a cluster where it is more than one.
 template <class Params>
 inline cudaError_t launch_overlapping(void (*kernel)(Params), dim3 grid, dim3 block, size_t shared, cudaStream_t stream,
-                                      const Params& params) {
+                                      const Params& params, unsigned cluster = 1) {
     static const bool plain = [] { const char* e = getenv("PSX_B200_NO_PDL"); return e && e[0] == '1'; }();
     cudaLaunchConfig_t config = {};
     config.gridDim = grid;
     config.blockDim = block;
     config.dynamicSmemBytes = shared;
     config.stream = stream;
-    cudaLaunchAttribute attribute[1];
-    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attribute[2];
     config.attrs = attribute;
-    config.numAttrs = plain ? 0 : 1;
+    if (!plain) {
+        attribute[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        cudaLaunchAttribute& a = attribute[config.numAttrs++];
+        a.id = cudaLaunchAttributeClusterDimension;
+        a.val.clusterDim.x = cluster, a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    }
     return cudaLaunchKernelEx(&config, kernel, params);
 }
 

@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "elements.cuh"
+#include "psx_device.cuh"
 
 namespace psx {
 namespace {
@@ -90,6 +91,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_heads_kernel(const _
     constexpr int kPairs = run;         // of a lane
     __shared__ __align__(16) float2 turned[kWarps][kMostPairs];  // cosine and sine of every pair
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, l = lane % lanes, slot = lane / lanes;
+    grid_dependency_wait();
+    grid_dependents_may_launch();
     if (p.row_status) {
         for (int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x; row < p.batch; row += (int64_t)gridDim.x * kThreads) p.row_status[row] = row_status(p, (int)row);
     }
@@ -241,8 +244,7 @@ cudaError_t launch_lanes(RotateHeadsParams& p, int sm_count, cudaStream_t stream
     p.slab_rows = ((all + p.slabs - 1) / p.slabs + slots - 1) / slots * slots;
     const int64_t blocks = std::max<int64_t>(1, (p.total * p.slabs + kWarps - 1) / kWarps);
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-    rotate_heads_kernel<T, run, lanes><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch_overlapping(rotate_heads_kernel<T, run, lanes>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
 }
 
 template <class T, int run>

@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "once_per_device.hpp"
+#include "psx_device.cuh"
 #include "row_selection.cuh"
 
 namespace psx {
@@ -256,6 +257,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
     const int parts = alone ? 1 : p.parts;
     const int64_t row = blockIdx.x / (unsigned)parts;
     const int part = alone ? 0 : (int)(blockIdx.x % (unsigned)parts), warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    grid_dependency_wait();
+    grid_dependents_may_launch();
     if (threadIdx.x == 0) s.listed = 0;
     // Elements are counted from the 16-byte boundary that is not behind the row's first one.
     const T* from = static_cast<const T*>(p.logits) + row * p.row_stride;
@@ -471,8 +474,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
 template <class T, int vectors, bool picks>
 cudaError_t launch_with(const TokenLogProbsParams& p, cudaStream_t stream) {
     if (p.parts == 1) {
-        token_log_probs_kernel<T, vectors, picks, true><<<(unsigned)p.rows, kThreads, 0, stream>>>(p);
-        return cudaGetLastError();
+        return launch_overlapping(token_log_probs_kernel<T, vectors, picks, true>, dim3((unsigned)p.rows), dim3(kThreads), 0, stream, p);
     }
     const auto kernel = token_log_probs_kernel<T, vectors, picks, false>;
     if (p.parts > 8) {  // (more than any device must hold)
@@ -482,16 +484,7 @@ cudaError_t launch_with(const TokenLogProbsParams& p, cudaStream_t stream) {
         const cudaError_t e = raised.run(device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); });
         if (e != cudaSuccess) return e;
     }
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(p.rows * p.parts));
-    config.blockDim = dim3(kThreads);
-    config.stream = stream;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = (unsigned)p.parts, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, p);
+    return launch_overlapping(kernel, dim3((unsigned)(p.rows * p.parts)), dim3(kThreads), 0, stream, p, (unsigned)p.parts);
 }
 
 template <class T>
