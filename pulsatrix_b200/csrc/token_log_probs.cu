@@ -8,8 +8,8 @@
 //
 // The row is cut into 1 to 16 parts, the CTAs of a cluster; a thread takes up to four vectors of 16 bytes at a time, with the next ones on their way.
 // The `top` best are found by a bound that at least `top` logits reach: each part's is the top-th largest of its threads' largest, the row's the largest
-// of those.  A thread whose largest of some chunks reaches it looks at them again, out of L2, and puts what reaches the bound on a list in
-// the first CTA's shared memory; an entry's place is the number of keys above its own.  A list that overflows (thousands of equal logits) is replaced
+// of those, or the smallest of what each part's share of them reaches.  A thread whose largest of some chunks reaches it looks at them again, out of L2, and puts what reaches the bound on its CTA's list; the first
+// CTA brings the lists together, and an entry's place is the number of keys above its own.  A list that overflows (thousands of equal logits) is replaced
 // by `top` sweeps.  Records, bounds and lists go through the cluster's shared memory: there is no scratch and nothing to be zero before a call.
 // (Lists and records in global memory, joined by the part that ends last: 64 rows of 8000 logits, 20 alternatives, 10.4 us instead of TIME.)
 // Rows need not be aligned: vectors are those of memory, and where one is cut by an end of the row its elements are read one by one.  Bound by HBM:
@@ -124,7 +124,8 @@ __device__ __forceinline__ void warp_maxima(float largest, int keep, uint32_t* m
         i = to;
     }
 }
-__device__ __forceinline__ void bound_of(const uint32_t* maxima, int keep, uint32_t& bound) {  // (every thread but one of several equal ones counts)
+// `share`: the same for its `share_of`-th largest.
+__device__ __forceinline__ void bound_of(const uint32_t* maxima, int keep, int share_of, uint32_t& bound, uint32_t& share) {
     const int count = maxima_of(keep) * kWarps;
     for (int i = threadIdx.x; i < count; i += kThreads) {
         const uint32_t mine = maxima[i];
@@ -132,6 +133,7 @@ __device__ __forceinline__ void bound_of(const uint32_t* maxima, int keep, uint3
 #pragma unroll 4
         for (int k = 0; k < count; ++k) place += maxima[k] > mine || (maxima[k] == mine && k < i);
         if (place == keep - 1) bound = mine;
+        if (place == share_of - 1) share = mine;
     }
 }
 
@@ -142,15 +144,15 @@ struct Outcome {
 };
 
 struct Shared {
-    uint64_t list[kList];  // the first part's holds the row's
+    alignas(16) uint64_t list[kList];  // what reaches the bound
     uint64_t best_of[kWarps], best[2];
     float4 record;         // the part's largest logit and its two sums
     Outcome outcome;       // the first part's, and the given token and its logit
     int64_t token;
     float given;
-    uint32_t maxima[kWarps * kMostMaxima], bound;
+    uint32_t maxima[kWarps * kMostMaxima], bound, share;
     float tops[kWarps], sums[kWarps], weighted[kWarps];
-    float group_top[kMostGroups][kThreads];  // a thread's own
+    alignas(16) float group_top[kMostGroups][kThreads];  // a thread's own
     uint32_t listed;
 };
 
@@ -236,16 +238,6 @@ struct Cluster {
         else asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
         return x;
     }
-    __device__ __forceinline__ static void store_u64(uint32_t at, uint64_t x) {
-        if constexpr (alone) asm volatile("st.shared.u64 [%0], %1;" ::"r"(at), "l"(x) : "memory");
-        else asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(x) : "memory");
-    }
-    __device__ __forceinline__ static uint32_t add_u32(uint32_t at, uint32_t x) {
-        uint32_t before;
-        if constexpr (alone) asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(before) : "r"(at), "r"(x) : "memory");
-        else asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(before) : "r"(at), "r"(x) : "memory");
-        return before;
-    }
 };
 
 template <class T, int vectors, bool picks, bool alone>
@@ -266,12 +258,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
     from -= shift;
     const int begin = part * p.chunks * kChunk, end = (int)min((int64_t)begin + p.chunks * kChunk, (int64_t)shift + p.vocab);
     const auto column = [&](int chunk, int v) { return begin + chunk * kChunk + (v * kThreads + (int)threadIdx.x) * E; };
-    const auto load = [&](int chunk, W (&w)[kWords], bool again) {
+    const auto load = [&](int chunk, W (&w)[kWords]) {
 #pragma unroll
         for (int v = 0; v < vectors; ++v) {
             const int at = column(chunk, v);
             uint4 x = make_uint4(W::none().bits, W::none().bits, W::none().bits, W::none().bits);
-            if (at >= shift && at <= end - E) x = again ? __ldcg(reinterpret_cast<const uint4*>(from + at)) : __ldcs(reinterpret_cast<const uint4*>(from + at));
+            if (at >= shift && at <= end - E) x = __ldcg(reinterpret_cast<const uint4*>(from + at));
             else if (at < end && at > shift - E) x = cut_vector(from + at, shift - at, end - at);
             w[4 * v].bits = x.x, w[4 * v + 1].bits = x.y, w[4 * v + 2].bits = x.z, w[4 * v + 3].bits = x.w;
         }
@@ -332,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
     };
     // (Two chunks a turn, one in work and one on its way; unrolled further, the instructions come too late.)
     W w[2][kWords];
-    load(0, w[0], false);
+    load(0, w[0]);
     if (part == 0 && threadIdx.x == 0) {  // (here its two trips to memory are nobody's)
         int64_t token;
         s.given = given_logit<T>(p, row, token);
@@ -340,9 +332,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
     }
 #pragma unroll 1
     for (int c = 0; c < p.chunks; c += 2) {
-        if (c + 1 < p.chunks) load(c + 1, w[1], false);
+        if (c + 1 < p.chunks) load(c + 1, w[1]);
         take(c, w[0]);
-        if (c + 2 < p.chunks) load(c + 2, w[0], false);
+        if (c + 2 < p.chunks) load(c + 2, w[0]);
         if (c + 1 < p.chunks) take(c + 1, w[1]);
     }
     // The thread's own: the smaller of the two that are aside joins the sums.
@@ -366,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
     if constexpr (picks) warp_maxima(top, p.top, s.maxima);
     __syncthreads();
     if constexpr (picks) {
-        bound_of(s.maxima, p.top, s.bound);
+        bound_of(s.maxima, p.top, (p.top + parts - 1) / parts, s.bound, s.share);
         __syncthreads();
     }
     if (warp == kWarps - 1) {  // the part's record
@@ -402,7 +394,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
         return;
     }
 
-    const uint32_t bound_key = __reduce_max_sync(0xffffffffu, lane < parts ? C::load_u32(C::at(&s.bound, lane)) : 0u);
+    // At least `top` logits reach the largest of the parts' bounds; and, each part giving its share of them, the smallest of those.
+    const uint32_t reached = __reduce_max_sync(0xffffffffu, lane < parts ? C::load_u32(C::at(&s.bound, lane)) : 0u);
+    const uint32_t shared_out = __reduce_min_sync(0xffffffffu, lane < parts ? C::load_u32(C::at(&s.share, lane)) : 0xffffffffu);
+    const uint32_t bound_key = max(reached, shared_out);
     const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
     const int groups = (p.chunks + p.group - 1) / p.group;
     uint32_t hits = 0;  // the groups of chunks that reach the bound; they are read again, out of L2
@@ -412,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
         for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
             const int g = __ffs(rest) - 1, last = min((g + 1) * p.group, p.chunks);
             for (int c = g * p.group; c < last; ++c) {
-                load(c, w[0], true);
+                load(c, w[0]);
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
                     const float2 x = w[0][i].floats();
@@ -425,22 +420,44 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
             }
         }
     };
-    const uint32_t listed_at = C::at(&s.listed, 0), list_at = C::at(s.list, 0);
     look([&](float x, int token) {
-        const uint32_t at = C::add_u32(listed_at, 1);
-        if (at < kList) C::store_u64(list_at + at * (uint32_t)sizeof(uint64_t), entry_key(x, token));
+        const uint32_t at = atomicAdd(&s.listed, 1u);
+        if (at < kList) s.list[at] = entry_key(x, token);
     });
     C::meets();
-    const int count = (int)C::load_u32(listed_at), keep = p.top;
+    // How many the parts have listed; the first CTA brings them together, behind what its threads kept of their groups, which is done with.
+    const int listed = lane < parts ? (int)C::load_u32(C::at(&s.listed, lane)) : 0;
+    int listed_to = listed;
+#pragma unroll
+    for (int step = 1; step < kMostParts; step *= 2) {
+        const int other = __shfl_up_sync(0xffffffffu, listed_to, step);
+        if (lane >= step) listed_to += other;
+    }
+    const int keep = p.top, count = min(__shfl_sync(0xffffffffu, listed_to, parts - 1), kList + 1);
     const bool wrong = part == 0 && s.outcome.status == kRowNonFinite;
     int placed = min(count, keep);
-    if (count <= kList) {
+    if (!__any_sync(0xffffffffu, listed > kList || count > kList)) {  // (the same in all warps)
         if (part == 0 && !wrong) {
+            const uint64_t* list = s.list;
+            if constexpr (!alone) {
+                uint64_t* together = reinterpret_cast<uint64_t*>(s.group_top);
+                for (int i = 0; i < parts; ++i) {
+                    const int end = __shfl_sync(0xffffffffu, listed_to, i), begin = end - __shfl_sync(0xffffffffu, listed, i);
+                    if (i % kWarps != warp) continue;
+                    for (int e = begin + lane; e < end; e += 32) together[e] = C::load_u64(C::at(&s.list[e - begin], i));
+                }
+                __syncthreads();
+                list = together;
+            }
             for (int e = threadIdx.x; e < count; e += kThreads) {
-                const uint64_t key = s.list[e];
+                const uint64_t key = list[e];
                 int place = 0;
 #pragma unroll 4
-                for (int k = 0; k < count; ++k) place += s.list[k] > key;
+                for (int k = 0; k < count / 2; ++k) {
+                    const ulonglong2 two = reinterpret_cast<const ulonglong2*>(list)[k];
+                    place += (two.x > key) + (two.y > key);
+                }
+                if (count % 2) place += list[count - 1] > key;
                 if (place < keep) put_alternative(p, s.outcome, row, place, key);
             }
         }
