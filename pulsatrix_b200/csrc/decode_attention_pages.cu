@@ -100,10 +100,10 @@ __device__ __forceinline__ void store_four(T* to, float4 x, float factor) {
     else *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(four);
 }
 
-// Cached positions are read once.
+// Cached positions are read once.  (Coherent, as all loads here: the kernel begins while the one that wrote them may be at its end.)
 __device__ __forceinline__ uint4 load_once(const void* at) {
     uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(at));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(at));
     return r;
 }
 
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
     const int64_t row_bytes = (int64_t)head_dim * sizeof(T), head_bytes = row_bytes * t.page_size, page_bytes = head_bytes * kv_heads;
     const char* keys = p.cache.keys + head * head_bytes;
     const int64_t apart = p.cache.values - p.cache.keys;
-    const auto page_of = [&](int tile) { return tile < to_tile ? __ldg(pages + ((tile0 + tile) * kTile >> t.shift)) : -1; };
+    const auto page_of = [&](int tile) { return tile < to_tile ? pages[(tile0 + tile) * kTile >> t.shift] : -1; };
     int page = page_of(from_tile + warp), next_page = page_of(from_tile + warp + kWarps);
 
     // The query rows as the right-hand operand, in shared memory: for each step of two products, by (tile of rows, step, product, lane), the words
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
     for (int i = warp; i < tiles_of_rows * kSteps; i += kWarps) {
         const int r = i / kSteps * 8 + gid, d = i % kSteps * 4 * E + tig * E;
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < rows && d < head_dim) x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + element_of(r) + d));
+        if (r < rows && d < head_dim) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + element_of(r) + d);
         if constexpr (precise) {
             const uint32_t h[4] = {eleven_bits(x.x), eleven_bits(x.y), eleven_bits(x.z), eleven_bits(x.w)};
             parts[2 * i * 32 + lane] = make_uint4(h[0], h[1], left_of(x.x, h[0]), left_of(x.y, h[1]));

@@ -48,7 +48,7 @@ struct Run {
         __builtin_memcpy(&r.bits, e, sizeof(e));
         return r;
     }
-    __device__ __forceinline__ static Run at(const T* p) { return {__ldg(reinterpret_cast<const Bits*>(p))}; }
+    __device__ __forceinline__ static Run at(const T* p) { return {*reinterpret_cast<const Bits*>(p)}; }
     __device__ __forceinline__ void put(T* p) const { *reinterpret_cast<Bits*>(p) = bits; }
 };
 

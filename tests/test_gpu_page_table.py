@@ -210,6 +210,20 @@ def test_many_pages(num_pages):
         book.check(table, pools)
 
 
+def test_references_that_start_anywhere():
+    import torch
+    rng = np.random.RandomState(9)
+    for shift in (1, 2, 3):
+        book, _, pools = _both(rng, 3, 6, 5000 + shift, 16, ((1, 1, np.uint8),))
+        table = psx.PageTable(torch.full((3, 6), -1, dtype=torch.int32, device="cuda"), _whole([0, 0, 0]), _whole([9] * shift + [0] * (5000 + shift), "int32")[shift:], 16)
+        ctx = gh.ctx()
+        for added in ([40, 3, 0], [1, 60, 17]):
+            assert ctx.extend_pages(table, _whole(added), pools).tolist() == book.extend(added)
+        ctx.release_pages(table, _whole([0, 30, 17])), book.release([0, 30, 17])
+        assert int(ctx.compact_pages(table, pools)) == book.compact()
+        book.check(table, pools)
+
+
 def test_as_many_rows_as_there_may_be():
     rng = np.random.RandomState(1)
     book, table, pools = _both(rng, 4096, 2, 9000, 16, ((1, 4, np.uint8),))
