@@ -28,7 +28,8 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = 4, kTile = 16;
 constexpr double kSplitRate = 4.0;  // pieces squared for a tile where few pairs are cut to fill the GPU: more are longer in joining than they save
-constexpr int kMostShare = 64;  // tiles that a block takes where shorter pieces only balance
+// Tiles that a block takes where shorter pieces only balance.
+__host__ __device__ constexpr int most_share(int dims) { return dims == 256 ? 32 : 64; }
 constexpr float kNone = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(dims, sizeof(T), tiles_of_
     const int length = t.length(row);
     const Sight sight{length, length - p.q_len, p.causal ? (int)p.window : 0};
     const int tile0 = sight.first_tile(), tiles = max(sight.end_tile() - tile0, 0);
-    const int share = max(max(kWarps, (tiles + p.pieces - 1) / p.pieces), min((tiles + p.spread - 1) / p.spread, kMostShare));
+    const int share = max(max(kWarps, (tiles + p.pieces - 1) / p.pieces), min((tiles + p.spread - 1) / p.spread, most_share(dims)));
     const int from_tile = number * share, to_tile = min(tiles, from_tile + share);
     // Row r of the pair is new position r / group, head r % group of the kv head's.
     const auto element_of = [&](int r) {
@@ -554,7 +555,7 @@ void plan_paged_attention(PagedAttentionParams& p, int sm_count) {
     // The pieces of a pair have their maxima and sums in shared memory when they are joined.
     const int64_t most = std::min<int64_t>((tiles + kWarps - 1) / kWarps, shared_of(dims, tiles_of_rows(p), width == 4) / (8 * tiles_of_rows(p) * sizeof(float2)));
     const int64_t spread = std::max<int64_t>(1, std::min(blocks / units, (int64_t)std::sqrt(kSplitRate * tiles)));
-    const int64_t balanced = std::min((tiles + kMostShare - 1) / kMostShare, 16 * blocks / units);  // (blocks that find nothing to do cost time too)
+    const int64_t balanced = std::min((tiles + most_share(dims) - 1) / most_share(dims), 16 * blocks / units);  // (blocks that find nothing to do cost time too)
     p.spread = (int)std::min(spread, most);
     p.pieces = (int)std::min(std::max(spread, balanced), most);
 }
