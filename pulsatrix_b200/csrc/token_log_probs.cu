@@ -156,7 +156,7 @@ struct Shared {
     uint32_t maxima[kWarps * kMostMaxima], bound, share;
     float tops[kWarps], sums[kWarps], weighted[kWarps];
     alignas(16) float group_top[kMostGroups][kThreads];  // a thread's own
-    uint32_t listed;
+    uint32_t listed, together;
 };
 
 // The vector of 16 bytes that an end of the row cuts: elements first .. end of it, one by one, and -inf for the others.
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
     const int part = alone ? 0 : (int)(blockIdx.x % (unsigned)parts), warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     grid_dependency_wait();
     grid_dependents_may_launch();
-    if (threadIdx.x == 0) s.listed = 0;
+    if (threadIdx.x == 0) s.listed = 0, s.together = 0;
     // Elements are counted from the 16-byte boundary that is not behind the row's first one.
     const T* from = static_cast<const T*>(p.logits) + row * p.row_stride;
     const int shift = (int)(reinterpret_cast<uintptr_t>(from) % 16 / sizeof(T));
@@ -377,6 +377,39 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
         }
         if (lane == 0) s.record = make_float4(high, part_sum, part_weighted, 0.0f);
     }
+    float bound = kNone;
+    uint32_t hits = 0;  // the groups of chunks that reach it; they are read again, out of L2
+    const auto look_from = [&](uint32_t key) {
+        bound = key == 0 ? kNone : from_ordered(key);
+        const int groups = (p.chunks + p.group - 1) / p.group;
+        hits = 0;
+        for (int g = 0; g < groups; ++g) hits |= (s.group_top[g][threadIdx.x] >= bound && s.group_top[g][threadIdx.x] > kNone) ? 1u << g : 0u;
+    };
+    // every logit of those that reaches the bound, with its token
+    const auto look = [&](auto use) {
+        for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
+            const int g = __ffs(rest) - 1, last = min((g + 1) * p.group, p.chunks);
+            for (int c = g * p.group; c < last; ++c) {
+                load(c, w[0]);
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const float2 x = w[0][i].floats();
+                    const int token = column(c, i / 4) - shift + i % 4 * W::elements;
+                    if (x.x >= bound && x.x > kNone) use(x.x, token);
+                    if constexpr (W::elements == 2) {
+                        if (x.y >= bound && x.y > kNone) use(x.y, token + 1);
+                    }
+                }
+            }
+        }
+    };
+    if constexpr (picks) {
+        look_from(s.bound);
+        look([&](float x, int token) {
+            const uint32_t at = atomicAdd(&s.listed, 1u);
+            if (at < kList) s.list[at] = entry_key(x, token);
+        });
+    }
     C::meets();
     if (part == 0 && warp == 0) {  // the row's
         const float4 x = lane < parts ? C::load_f4(C::at(&s.record, lane)) : make_float4(kNone, 0.0f, 0.0f, 0.0f);
@@ -397,62 +430,36 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
         return;
     }
 
-    // At least `top` logits reach the largest of the parts' bounds; and, each part giving its share of them, the smallest of those.
+    // What the parts have listed, and the row's bound: at least `top` logits reach the largest of theirs; and, each part giving its share of them, the
+    // smallest of those.
+    const int listed = lane < parts ? (int)C::load_u32(C::at(&s.listed, lane)) : 0;
     const uint32_t reached = __reduce_max_sync(0xffffffffu, lane < parts ? C::load_u32(C::at(&s.bound, lane)) : 0u);
     const uint32_t shared_out = __reduce_min_sync(0xffffffffu, lane < parts ? C::load_u32(C::at(&s.share, lane)) : 0xffffffffu);
     const uint32_t bound_key = max(reached, shared_out);
-    const float bound = bound_key == 0 ? kNone : from_ordered(bound_key);
-    const int groups = (p.chunks + p.group - 1) / p.group;
-    uint32_t hits = 0;  // the groups of chunks that reach the bound; they are read again, out of L2
-    for (int g = 0; g < groups; ++g) hits |= (s.group_top[g][threadIdx.x] >= bound && s.group_top[g][threadIdx.x] > kNone) ? 1u << g : 0u;
-    // every logit of those that reaches the bound, with its token
-    const auto look = [&](auto use) {
-        for (uint32_t rest = hits; rest != 0; rest &= rest - 1) {
-            const int g = __ffs(rest) - 1, last = min((g + 1) * p.group, p.chunks);
-            for (int c = g * p.group; c < last; ++c) {
-                load(c, w[0]);
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    const float2 x = w[0][i].floats();
-                    const int token = column(c, i / 4) - shift + i % 4 * W::elements;
-                    if (x.x >= bound && x.x > kNone) use(x.x, token);
-                    if constexpr (W::elements == 2) {
-                        if (x.y >= bound && x.y > kNone) use(x.y, token + 1);
-                    }
-                }
-            }
-        }
-    };
-    look([&](float x, int token) {
-        const uint32_t at = atomicAdd(&s.listed, 1u);
-        if (at < kList) s.list[at] = entry_key(x, token);
-    });
-    C::meets();
-    // How many the parts have listed; the first CTA brings them together, behind what its threads kept of their groups, which is done with.
-    const int listed = lane < parts ? (int)C::load_u32(C::at(&s.listed, lane)) : 0;
-    int listed_to = listed;
-#pragma unroll
-    for (int step = 1; step < kMostParts; step *= 2) {
-        const int other = __shfl_up_sync(0xffffffffu, listed_to, step);
-        if (lane >= step) listed_to += other;
-    }
-    const int keep = p.top, count = min(__shfl_sync(0xffffffffu, listed_to, parts - 1), kList + 1);
-    const bool wrong = part == 0 && s.outcome.status == kRowNonFinite;
-    int placed = min(count, keep);
-    if (!__any_sync(0xffffffffu, listed > kList || count > kList)) {  // (the same in all warps)
-        if (part == 0 && !wrong) {
+    const int keep = p.top;
+    int placed;
+    if (!__any_sync(0xffffffffu, listed > kList) && (int)__reduce_add_sync(0xffffffffu, (unsigned)listed) <= 2 * kList) {  // (the same in all warps)
+        if (part == 0) {
             const uint64_t* list = s.list;
-            if constexpr (!alone) {
+            int count = listed;
+            if constexpr (alone) {
+                count = __shfl_sync(0xffffffffu, listed, 0);
+                __syncthreads();  // (the row's outcome)
+            } else {  // the first CTA brings them together, where its threads kept their groups', which are done with
                 uint64_t* together = reinterpret_cast<uint64_t*>(s.group_top);
-                for (int i = 0; i < parts; ++i) {
-                    const int end = __shfl_sync(0xffffffffu, listed_to, i), begin = end - __shfl_sync(0xffffffffu, listed, i);
-                    if (i % kWarps != warp) continue;
-                    for (int e = begin + lane; e < end; e += 32) together[e] = C::load_u64(C::at(&s.list[e - begin], i));
+                for (int i = warp; i < parts; i += kWarps) {
+                    const int of_part = __shfl_sync(0xffffffffu, listed, i);
+                    for (int e = lane; e < of_part; e += 32) {
+                        const uint64_t key = C::load_u64(C::at(&s.list[e], i));
+                        if ((uint32_t)(key >> 32) >= bound_key) together[atomicAdd(&s.together, 1u)] = key;
+                    }
                 }
                 __syncthreads();
                 list = together;
+                count = (int)s.together;
             }
-            for (int e = threadIdx.x; e < count; e += kThreads) {
+            const bool wrong = s.outcome.status == kRowNonFinite;
+            for (int e = threadIdx.x; e < (wrong ? 0 : count); e += kThreads) {
                 const uint64_t key = list[e];
                 int place = 0;
 #pragma unroll 4
@@ -463,8 +470,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
                 if (count % 2) place += list[count - 1] > key;
                 if (place < keep) put_alternative(p, s.outcome, row, place, key);
             }
+            placed = min(count, keep);
         }
     } else {  // thousands that tie at the bound: sweep after sweep, the best that is behind the last one
+        look_from(bound_key);
         uint64_t last = ~0ull;
         for (placed = 0; placed < keep; ++placed) {
             uint64_t next = 0;
@@ -478,17 +487,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
             C::meets();
             for (int i = 0; i < parts; ++i) next = max(next, C::load_u64(C::at(&mine, i)));
             if (next == 0) break;
-            if (part == 0 && !wrong && threadIdx.x == 0) put_alternative(p, s.outcome, row, placed, next);
+            if (part == 0 && threadIdx.x == 0) put_alternative(p, s.outcome, row, placed, next);
             last = next;
         }
     }
     if (part == 0) {
+        const bool wrong = s.outcome.status == kRowNonFinite;
+        if (wrong) __syncthreads();  // (what the sweeps have put is put over)
         for (int i = (wrong ? 0 : placed) + threadIdx.x; i < keep; i += kThreads) {
             p.top_log_probs[row * keep + i] = wrong ? __int_as_float(0x7fffffff) : kNone;
             p.top_tokens[row * keep + i] = -1;
         }
     }
-    if (!alone) C::meets();  // (the count of the list, and the sweeps' best, are read until then)
+    if (!alone) C::meets();  // (records, lists and the sweeps' best are read until then)
 }
 
 template <class T, int vectors, bool picks>
