@@ -186,3 +186,53 @@ def test_a_step_is_captured_as_a_whole():
         torch.cuda.synchronize()
         for x, y in zip(buffers + [scored["log_probs"], scored["entropy"]], expected):
             assert (x == y).all()
+
+
+def test_pools_of_more_than_two_to_the_31_elements():
+    """The same pages at the end of a pool of 4.4 GB and in a small one: every call leaves the same in both."""
+    import torch
+    ctx, gen = gh.ctx(), torch.Generator(device="cuda").manual_seed(6)
+    size, kv_heads, dim, heads, many, few = 128, 8, 256, 16, 8400, 12
+    normal = lambda *shape: torch.randn(shape, generator=gen, device="cuda").bfloat16()
+    lengths = torch.tensor([300, 300, 130, 1], device="cuda")
+    small = torch.tensor([[9, 4, 11, 0], [9, 4, 11, 0], [7, 5, 0, 0], [10, 0, 0, 0]], dtype=torch.int32, device="cuda")  # (rows 0 and 1 share theirs)
+    caches = []
+    for pages, shift in ((few, 0), (many, many - few)):
+        table = psx.PageTable(small + shift, lengths.clone(), torch.zeros(pages, dtype=torch.int32, device="cuda"), size)
+        used = [9, 9, 4, 4, 11, 11, 7, 5, 10]
+        table.references.index_add_(0, torch.tensor(used, device="cuda") + shift, torch.ones(len(used), dtype=torch.int32, device="cuda"))
+        table.references[:shift] = 1  # (what lies below is taken)
+        caches.append(psx.PagedCache(table, *[torch.empty(pages, kv_heads, size, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)]))
+    assert caches[1].key_pages.numel() > 2 ** 31
+    for p in range(few):
+        page = [normal(kv_heads, size, dim) for _ in range(2)]
+        for cache in caches:
+            cache.key_pages[p - few], cache.value_pages[p - few] = page[0], page[1]
+
+    def same():
+        torch.cuda.synchronize()
+        a, b = caches
+        assert (a.table.lengths == b.table.lengths).all() and (a.table.references == b.table.references[many - few:]).all()
+        assert ((a.table.pages + (many - few) == b.table.pages)[:, :3] | (a.table.lengths[:, None] <= torch.arange(3, device="cuda") * size)).all()
+        assert (a.key_pages == b.key_pages[many - few:]).all() and (a.value_pages == b.value_pages[many - few:]).all()
+
+    one, qkv = torch.ones(4, dtype=torch.int64, device="cuda"), normal(4, heads + 2 * kv_heads, dim)
+    results = []
+    for cache in caches:
+        first = cache.table.lengths.clone()
+        status = ctx.extend_pages(cache.table, one, cache.pools())  # (row 0 gets a page of its own)
+        q, _, stored = ctx.rotate_heads(qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:], offsets=torch.arange(5, device="cuda"), first=first,
+                                        frequencies=torch.rand(dim // 2, generator=torch.Generator().manual_seed(1), dtype=torch.float64).cuda(), cache=cache)
+        results.append((status, stored, ctx.decode_attention_pages(q, cache)))
+    assert not results[0][0].any() and not results[0][1].any() and torch.isfinite(results[0][2]).all()
+    assert all((x == y).all() for x, y in zip(*results))
+    same()
+    big = caches[1]
+    big.table.references[:many - few] = 0
+    kept = [(big.key_pages[p.long()].clone(), big.value_pages[p.long()].clone()) for p in big.table.pages[:, :2]]
+    assert int(ctx.compact_pages(big.table, big.pools())) == 7
+    again = ctx.decode_attention_pages(q, big)
+    assert (again == results[0][2]).all()
+    for b in range(3):
+        now = big.table.pages[b, :2].long()
+        assert (now < 7).all() and (big.key_pages[now] == kept[b][0]).all() and (big.value_pages[now] == kept[b][1]).all()
