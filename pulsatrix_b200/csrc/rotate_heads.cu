@@ -25,7 +25,6 @@ namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kAhead = 2;  // heads of a lane that are on their way at once
-constexpr int kBlocks = 6;  // that an SM holds, by registers
 constexpr int kMostPairs = 128;
 constexpr int kRowOk = 0, kRowCacheFull = 64, kRowBadOffsets = 65;  // (psx_row_status)
 
@@ -68,6 +67,13 @@ __device__ __forceinline__ int row_status(const RotateHeadsParams& p, int row) {
     return first > length || end - begin > length - first ? kRowCacheFull : kRowOk;
 }
 
+// Heads of one operand on their way into L2, their lines shared out over the warp's lanes.
+template <class T>
+__device__ __forceinline__ void ask_for(const T* from, int heads, int dims) {
+    const char* at = reinterpret_cast<const char*>(from);
+    for (int line = (threadIdx.x % 32) * 128; line < heads * dims * (int)sizeof(T); line += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + line));
+}
+
 // The row that position `at` of the packed ones belongs to; -1: none.  The warp looks at 32 offsets at a time.
 __device__ __forceinline__ int row_of(const int64_t* offsets, int batch, int64_t at) {
     const int lane = threadIdx.x % 32;
@@ -85,7 +91,7 @@ __device__ __forceinline__ int row_of(const int64_t* offsets, int batch, int64_t
 }
 
 template <class T, int run, int lanes>
-__global__ void __launch_bounds__(kThreads, kBlocks) rotate_heads_kernel(const __grid_constant__ RotateHeadsParams p) {
+__global__ void __launch_bounds__(kThreads, run == 8 ? 5 : 6) rotate_heads_kernel(const __grid_constant__ RotateHeadsParams p) {
     using R = Run<T, run>;
     constexpr int kSlots = 32 / lanes;  // heads of a warp at once
     constexpr int kPairs = run;         // of a lane
@@ -96,14 +102,29 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_heads_kernel(const _
     if (p.row_status) {
         for (int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x; row < p.batch; row += (int64_t)gridDim.x * kThreads) p.row_status[row] = row_status(p, (int)row);
     }
-    const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
-    if (unit >= p.total * p.slabs) return;
-    const int64_t token = unit / p.slabs;
+    const unsigned unit = blockIdx.x * kWarps + warp, position_of = p.slabs == 1 ? unit : unit / (unsigned)p.slabs;
+    if (position_of >= (unsigned)p.total) return;
+    const int64_t token = position_of;
     const int dims = p.head_dim, all = p.heads + p.kv_heads + (p.cache.keys ? p.kv_heads : 0);
-    const int begin = (int)(unit % p.slabs) * p.slab_rows, end = min(begin + p.slab_rows, all);
+    const int begin = (int)(unit - position_of * (unsigned)p.slabs) * p.slab_rows, end = min(begin + p.slab_rows, all);
     const bool turns = 2 * run * l < p.rotated, halves = turns && !p.interleaved;
     const int low = halves ? run * l : 2 * run * l, high = halves ? run * l + p.rotated / 2 : 2 * run * l + run;
     const bool low_here = low < dims && 2 * run * l < dims, high_here = high < dims && 2 * run * l < dims;
+
+    // What does not depend on the row is asked for before it is known: the position's heads on their way into L2, the frequencies into registers.
+    const T* const q_at = static_cast<const T*>(p.q) + token * p.q_stride;
+    const T* const k_at = static_cast<const T*>(p.k) + token * p.k_stride;
+    const T* const v_at = static_cast<const T*>(p.v) + (p.cache.keys ? token * p.v_stride : 0);
+    const int first_key = max(begin - p.heads, 0), last_key = min(end - p.heads, p.kv_heads);
+    const int first_value = max(begin - p.heads - p.kv_heads, 0), last_value = end - p.heads - p.kv_heads;
+    if constexpr (sizeof(T) == 2) {  // (fp32 has twice the bytes of a lane on their way as it is: 172 us become 205)
+        ask_for(q_at + begin * dims, min(end, p.heads) - begin, dims);
+        ask_for(k_at + first_key * dims, last_key - first_key, dims);
+        ask_for(v_at + first_value * dims, last_value - first_value, dims);
+    }
+    double frequency[kMostPairs / 32];
+#pragma unroll
+    for (int i = 0; i < kMostPairs / 32; ++i) frequency[i] = i * 32 + lane < p.rotated / 2 ? p.frequencies[i * 32 + lane] : 0.0;
 
     const int row = row_of(p.offsets, p.batch, token);
     if (row < 0) return;
@@ -116,8 +137,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_heads_kernel(const _
     }
     const int64_t head_step = (int64_t)p.cache.table.page_size * dims;
 
-    for (int j = lane; j < p.rotated / 2; j += 32) {
-        const double quarters = (double)position * (p.frequencies[j] * 0.63661977236758134308);
+#pragma unroll
+    for (int i = 0; i < kMostPairs / 32; ++i) {
+        const int j = i * 32 + lane;
+        if (j >= p.rotated / 2) continue;
+        const double quarters = (double)position * (frequency[i] * 0.63661977236758134308);
         const double whole = rint(quarters);
         float sine, cosine;
         sincospif((float)(quarters - whole) * 0.5f, &sine, &cosine);
@@ -156,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_heads_kernel(const _
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
+                if (h0 + i * kSlots >= last) continue;  // (the warp together)
                 const int h = h0 + i * kSlots + slot;
                 float x[run], y[run];
                 a[i].to_floats(x);
@@ -198,21 +223,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotate_heads_kernel(const _
     };
     if (begin < p.heads) {
         T* to = static_cast<T*>(p.q_out) + token * p.heads * dims;
-        heads_of(static_cast<const T*>(p.q) + token * p.q_stride, begin, min(end, p.heads), static_cast<const T*>(p.q_weight),
+        heads_of(q_at, begin, min(end, p.heads), static_cast<const T*>(p.q_weight),
                  [&](int h, const R& a, const R& b) { put_at(to + h * dims, a, b); });
     }
-    const int first_key = max(begin - p.heads, 0), last_key = min(end - p.heads, p.kv_heads);
     if (first_key < last_key) {
         T* to = static_cast<T*>(p.k_out) + token * p.kv_heads * dims;
         T* pages = reinterpret_cast<T*>(p.cache.keys) + place;
-        heads_of(static_cast<const T*>(p.k) + token * p.k_stride, first_key, last_key, static_cast<const T*>(p.k_weight), [&](int h, const R& a, const R& b) {
+        heads_of(k_at, first_key, last_key, static_cast<const T*>(p.k_weight), [&](int h, const R& a, const R& b) {
             if (p.k_out) put_at(to + h * dims, a, b);
             if (place >= 0) put_at(pages + h * head_step, a, b);
         });
     }
-    const int first_value = max(begin - p.heads - p.kv_heads, 0), last_value = end - p.heads - p.kv_heads;
     if (place >= 0 && first_value < last_value) {  // (bit by bit)
-        const T* from = static_cast<const T*>(p.v) + token * p.v_stride;
+        const T* from = v_at;
         T* pages = reinterpret_cast<T*>(p.cache.values) + place;
 #pragma unroll 1
         for (int h0 = first_value; h0 < last_value; h0 += kAhead * kSlots) {
@@ -243,7 +266,7 @@ cudaError_t launch_lanes(RotateHeadsParams& p, int sm_count, cudaStream_t stream
     p.slabs = (int)std::min(wanted, most);
     p.slab_rows = ((all + p.slabs - 1) / p.slabs + slots - 1) / slots * slots;
     const int64_t blocks = std::max<int64_t>(1, (p.total * p.slabs + kWarps - 1) / kWarps);
-    if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+    if (blocks * kWarps > 0x7fffffff) return cudaErrorInvalidValue;
     return launch_overlapping(rotate_heads_kernel<T, run, lanes>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
 }
 
