@@ -4,7 +4,7 @@
 //     y = x / sqrt(mean(x^2) + eps) * w,   (u, v) -> (u cos a - v sin a, v cos a + u sin a) for pair j with a = position * frequency_j
 //
 // in floats, rounded once at the end.  The angle is taken in double precision, in quarter turns: position * frequency * 2 / pi less the
-// nearest whole number is what is left for sincospif, an eighth of a turn at most, so that its rounding to a float counts 2^-26 quarter turns
+// nearest whole number is what is left, an eighth of a turn at most, so that its rounding to a float counts 2^-26 quarter turns
 // however far the position is (in floats, an angle of 100,000 is off by up to 4e-3).
 //
 // A lane holds two runs of 16 bytes of a head (of 8, where half of the rotated dimensions is not a multiple of 16 bytes): one of both halves where pairs are
@@ -65,6 +65,13 @@ __device__ __forceinline__ int row_status(const RotateHeadsParams& p, int row) {
     if (!p.cache.keys) return kRowOk;
     const int64_t length = p.cache.table.length(row);
     return first > length || end - begin > length - first ? kRowCacheFull : kRowOk;
+}
+
+// Sine and cosine of an eighth of a turn at most, by their power series: what is left out is below 2.2e-9 and 1.2e-10.
+__device__ __forceinline__ void sine_and_cosine(float x, float& sine, float& cosine) {
+    const float z = x * x;
+    sine = fmaf(x, z * fmaf(z, fmaf(z, fmaf(z, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), x);
+    cosine = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
 }
 
 // Heads of one operand on their way into L2, their lines shared out over the warp's lanes.
@@ -141,11 +148,12 @@ __global__ void __launch_bounds__(kThreads, run == 8 ? 5 : 6) rotate_heads_kerne
     for (int i = 0; i < kMostPairs / 32; ++i) {
         const int j = i * 32 + lane;
         if (j >= p.rotated / 2) continue;
-        const double quarters = (double)position * (frequency[i] * 0.63661977236758134308);
-        const double whole = rint(quarters);
+        // Quarter turns and the nearest whole number of them: added to 1.5 * 2^52 it is rounded to a whole number, and its last bits are the sum's (for less
+        // than 2^51 of them).
+        const double quarters = (double)position * (frequency[i] * 0.63661977236758134308), shifted = quarters + 6755399441055744.0;
+        const int quadrant = __double2loint(shifted);
         float sine, cosine;
-        sincospif((float)(quarters - whole) * 0.5f, &sine, &cosine);
-        const int quadrant = (int)((long long)whole & 3);
+        sine_and_cosine((float)((quarters - (shifted - 6755399441055744.0)) * 1.57079632679489661923), sine, cosine);
         float2 turn = quadrant & 1 ? make_float2(-sine, cosine) : make_float2(cosine, sine);
         if (quadrant & 2) turn = make_float2(-turn.x, -turn.y);
         turned[warp][j] = turn;

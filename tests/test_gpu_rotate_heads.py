@@ -2,7 +2,7 @@
 
 Tolerance, in units of 2^-24 of |x| + |y|, the normed elements of a pair: a square and its sum over a lane's eight and five steps between lanes
 are off by at most 15, the root of it by half of that; mean, eps, root, quotient and the two products by one each: 13.5.  Cosine and sine: the angle
-is off by 2^-26 quarter turns (0.4), the functions by 2 (they err by an ulp, of numbers up to 1); product and sum 2.  Together less than 20.  The result is
+is off by 2^-26 quarter turns (0.4), the functions by 2 (two roundings of numbers up to 1, and 2.2e-9); product and sum 2.  Together less than 20.  The result is
 rounded to its type: half a step of it, 2^-25 at least in fp16's subnormal range."""
 import numpy as np
 import pytest
