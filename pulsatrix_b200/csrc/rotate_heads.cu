@@ -11,7 +11,7 @@
 // (j, j + rotated / 2), neighbours where they are (2 j, 2 j + 1) and where dimensions are not rotated; so both elements of a pair are in one
 // lane, and four to 32 lanes have a head.  A warp has a position, or some heads of one where positions are few: the row that it belongs to, its page and
 // its angles, which the lanes share out and pass on through shared memory, are found once for all of its heads.  Bound by HBM for prompts, by latency for
-// single positions: 12 prompts of up to 2111 positions, 32 + 8 + 8 heads of 128, take 98 us in bf16 (5.5 TB/s), 172 in fp32 (6.2 TB/s).
+// single positions: 12 prompts of up to 2111 positions, 32 + 8 + 8 heads of 128, take 94 us in bf16 (5.7 TB/s), 171 in fp32 (6.3 TB/s).
 #include "rotate_heads.cuh"
 
 #include <algorithm>
@@ -124,7 +124,9 @@ __global__ void __launch_bounds__(kThreads, run == 8 ? 5 : 6) rotate_heads_kerne
     const T* const v_at = static_cast<const T*>(p.v) + (p.cache.keys ? token * p.v_stride : 0);
     const int first_key = max(begin - p.heads, 0), last_key = min(end - p.heads, p.kv_heads);
     const int first_value = max(begin - p.heads - p.kv_heads, 0), last_value = end - p.heads - p.kv_heads;
-    if constexpr (sizeof(T) == 2) {  // (fp32 has twice the bytes of a lane on their way as it is: 172 us become 205)
+    // (Not for fp32, which has twice the bytes of a lane on their way as it is, 172 us would become 205 below; nor for few heads, 16 + 4 + 4 of 64 dimensions 21 us and
+    // 23; but 32 + 8 + 8 of them 58 without and 52.)
+    if (sizeof(T) == 2 && (end - begin) * dims >= 2048) {
         ask_for(q_at + begin * dims, min(end, p.heads) - begin, dims);
         ask_for(k_at + first_key * dims, last_key - first_key, dims);
         ask_for(v_at + first_value * dims, last_value - first_value, dims);
@@ -267,7 +269,7 @@ template <class T, int run, int lanes>
 cudaError_t launch_lanes(RotateHeadsParams& p, int sm_count, cudaStream_t stream) {
     constexpr int slots = 32 / lanes;
     const int all = p.heads + p.kv_heads + (p.cache.keys ? p.kv_heads : 0);
-    // A warp per position where that fills the GPU, or as many as there are heads to share out.  (Two a position: 108 us instead of 98 in the case
+    // A warp per position where that fills the GPU, or as many as there are heads to share out.  (Two a position: 108 us instead of 101 in the case
     // below; a warp for two to five positions one after the other: 144 to 182.)
     const int64_t wanted = std::max<int64_t>(1, (int64_t)sm_count * 32 / std::max<int64_t>(p.total, 1));
     const int64_t most = (all + slots - 1) / slots;
