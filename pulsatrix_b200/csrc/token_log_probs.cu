@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
         const float less = fmaxf((level - base) * kLog2e, kLeast), factor = exp2_approx(less);
         weighted = mul_pair(fma_pair(make_float2(less, less), sum, weighted), make_float2(factor, factor));
         sum = mul_pair(sum, make_float2(factor, factor));
-        level = base;
+        level = next;  // (not `base`: behind logits of -inf alone the factor of the empty sums is 0, where 0 less a base of -89 would make it infinite)
         const auto add_up = [&](bool clamp) {
 #pragma unroll
             for (int i = 0; i < kWords; i += W::elements == 1 ? 2 : 1) {

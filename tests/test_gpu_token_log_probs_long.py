@@ -1,0 +1,96 @@
+"""Log-probabilities of given tokens (psx_b200_token_log_probs) for rows that a thread takes in many steps: stretches that are masked ahead of low logits.
+Against the formula in double precision.
+
+Tolerance: that of test_gpu_token_log_probs.py."""
+import numpy as np
+import pytest
+
+import gpu_harness as gh
+import test_gpu_token_log_probs as score_test
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = score_test.TYPES
+
+
+def _check(logits, tokens, top):
+    """score_test._check, on the device, a row at a time."""
+    import torch
+    out = gh.ctx().token_log_probs(logits, tokens, top=top, entropy=True)
+    assert not out["status"].any()
+    for row in range(logits.shape[0]):
+        x = logits[row].double() + 0.0
+        (high, second), at = torch.topk(x, 2)[0].tolist(), int(x.argmax())
+        weight = torch.exp(x - high)
+        weight[at] = 0.0
+        r = float(weight.sum())
+        gap = (x - high).masked_fill_(x == -np.inf, 0.0)
+        entropy = np.log1p(r) - float((weight * gap).sum()) / (1 + r)
+        g, lost = min(high - second, 104.0), len(x) * 2.0 ** -126
+        slack = ((200 + 2 * g) * U * r + lost) / (1 + r)
+        want = float(x[tokens[row]]) - high - np.log1p(r)
+        assert abs(float(out["log_probs"][row]) - want) <= (slack + U * abs(want)) * (1 + 1e-9) + 1e-45 or want == float(out["log_probs"][row])
+        assert abs(float(out["entropy"][row]) - entropy) <= (401 + 4 * g) * U * entropy + 91 * lost + 1e-45
+        if top:
+            values, best = torch.sort(x, descending=True, stable=True)
+            values, best = values[:top], best[:top].masked_fill(values[:top] == -np.inf, -1)
+            assert (out["top_tokens"][row] == best).all()
+            want = (values - high - np.log1p(r)).cpu().numpy()
+            got = out["top_log_probs"][row].double().cpu().numpy()
+            finite = np.isfinite(want)
+            assert (got[~finite] == want[~finite]).all()
+            assert (np.abs(got[finite] - want[finite]) <= (slack + U * np.abs(want[finite])) * (1 + 1e-9) + 1e-45).all()
+
+
+def _plan(rows, vocab, dtype):
+    """Chunks of a part and parts of a row, restated for 148 SMs: what the cases below are to reach."""
+    elements, least = 4 if dtype == "float32" else 8, None
+    for vectors in (4, 1):
+        chunk, chain, further = (0.375, 4.3, 1.2) if vectors == 1 else (0.79, 5.2, 1.7)
+        steps = -(-(vocab + elements - 1) // (256 * vectors * elements))
+        for parts in (1, 2, 4, 8, 16):
+            each, beside = -(-steps // parts), max(1.0, rows * parts / 148)
+            if parts > 1 and (each * (parts - 1) >= steps or (parts == 16 and beside > 1.0)):
+                continue
+            cost = each * chunk + chain + (parts > 1) + (beside - 1.0) * (further + 0.09 * vectors * each)
+            if least is None or cost < least[0]:
+                least = cost, each, parts
+    return least[1:]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(300, 50257), (600, 40000), (40, 100000), (1, 262144)])
+@pytest.mark.parametrize("low", [-89.0, -100.0, -1000.0, -60000.0])
+def test_masked_stretches_ahead_of_low_logits(dtype, rows, vocab, low):
+    # every thread's first steps hold nothing but masked logits, and what comes then lies far below 0; with an ordinary largest one elsewhere, and without
+    import torch
+    steps, parts = _plan(rows, vocab, dtype)
+    assert steps > 1
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x = (low * (1 + 0.05 * torch.rand(rows, vocab, generator=gen, device="cuda"))).to(getattr(torch, dtype))
+    begin = -(-vocab // parts) // 2
+    for part in range(parts):
+        at = part * (-(-vocab // parts))
+        x[:, at:at + begin + 5000] = -np.inf
+    x[:, vocab - 3:] = low
+    x[rows // 2:, vocab // 2] = 1.0 if rows > 1 else low
+    tokens = torch.randint(vocab - 3, vocab, (rows,), generator=gen, device="cuda")
+    some = torch.tensor(sorted({0, rows // 2, rows - 1}), device="cuda")
+    out = gh.ctx().token_log_probs(x, tokens, top=5, entropy=True)
+    assert not out["status"].any() and not any(bool(torch.isnan(out[k]).any()) for k in ("log_probs", "entropy", "top_log_probs"))
+    _check(x[some].contiguous(), tokens[some], 5)
+    _check(x, tokens, 0) if rows == 1 else None
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 200])
+def test_a_few_tokens_that_a_grammar_allows(dtype, rows):
+    import torch
+    rng, vocab = np.random.RandomState(rows), 128256
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    for row in range(rows):
+        allowed = rng.choice(vocab, 50, replace=False)
+        x[row, allowed] = rng.uniform(-400, -90, 50)
+    logits = score_test._tensor(x, dtype)
+    tokens = torch.from_numpy(x.argmax(1)).cuda()
+    _check(logits, tokens, 60)
