@@ -477,8 +477,9 @@ typedef struct psx_page_pool {
 /* Room for new positions: lengths[b] += added[b] (device int64, rows), with the pages that this takes.  Rows come in order, the
  * lowest free page first.  A row that goes on in a last page which other rows hold too gets a page of its own for it, and what the row
  * holds of it is copied in all `pools` (a host array, read during the call); where all who hold the page go on in it, the last of
- * them keeps it.  What a page holds behind that is left as it was.  row_status (device int32, rows, may be NULL): PSX_ROW_OK;
- * PSX_ROW_CACHE_FULL: the row would need more than max_pages, or this row or one before it asked for more pages than were free;
+ * them keeps it, unless one of them gets no page and holds more of it.  What a page holds behind that is left as it was.  row_status (device int32, rows, may be NULL): PSX_ROW_OK;
+ * PSX_ROW_CACHE_FULL: the row would need more than max_pages, or this row or one before it asked for more pages than were free, or the row
+ * would have to write over positions of such a row;
  * PSX_ROW_BAD_OFFSETS: added[b] or lengths[b] is negative, the length beyond max_pages * page_size, or the last page not one of the pool.  Such
  * rows are left alone, their positions from lengths[b] on have no room.  pool_count may be 0 where no page is shared.  The pools must
  * overlap neither each other nor the table (PSX_ERR_BAD_ARGUMENT); page bytes of a pool <= 2^30 (else PSX_ERR_UNSUPPORTED).  Asynchronous on

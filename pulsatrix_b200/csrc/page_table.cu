@@ -5,7 +5,7 @@
 // use that do.  That count is all there is to know about a page; it is free where it is 0, so there is no list of free pages to keep, and
 // which pages a row gets depends on the table alone: the lowest free ones, row after row.  A row that goes on in a last page which others
 // hold too gets a page of its own and a copy of what it sees of the old one (the last of the rows that go on in it keeps it where nobody else
-// holds it).  So beams share their prompt's pages, and following a beam moves table entries, four bytes per page and row, instead of the
+// holds it, unless that would write over what one of them holds that got no page).  So beams share their prompt's pages, and following a beam moves table entries, four bytes per page and row, instead of the
 // cache.
 //
 // Bound by latency but for the copies, which run at HBM's rate (a thousand pages of 64 KB that move in four pools: 80 us, 6.7 TB/s).
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
         goes_on[row] = page;
     }
     if (threadIdx.x < 4) goes_on[rows + threadIdx.x] = -1;
-    bool copies[kRowsPerThread] = {};
+    bool copies[kRowsPerThread] = {}, keeps[kRowsPerThread] = {};
     if (__syncthreads_or(shares)) {
 #pragma unroll
         for (int i = 0; i < kRowsPerThread; ++i) {
@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
                 if (four.z == page) ++going, last = row + 2;
                 if (four.w == page) ++going, last = row + 3;
             }
-            copies[i] = !(going == held_by[i] && last == first + i);
+            keeps[i] = going == held_by[i] && last == first + i;
+            copies[i] = !keeps[i];
         }
         __syncthreads();
 #pragma unroll
@@ -201,13 +202,24 @@ __global__ void __launch_bounds__(kPlanThreads) extend_pages_kernel(const __grid
                 rank += (int)(totals >> (16 * k) & 0xffff);
             }
         }
+        // A row that would keep its page in place is refused like those before it where one of them, left in the page without a copy, holds more of it.
+        if (available < asked) {
+#pragma unroll
+            for (int i = 0; i < kRowsPerThread; ++i) {
+                if (!keeps[i]) continue;
+                const int page = t.pages[(int64_t)(first + i) * t.max_pages + (length[i] >> t.shift)], filled = length[i] & (t.page_size - 1);
+                for (int row = 0; row < first + i; ++row) {
+                    if (goes_on[row] == page && ends[row] > available && ((int)t.lengths[row] & (t.page_size - 1)) > filled) status[i] = kRowCacheFull;
+                }
+            }
+        }
         __syncthreads();  // (lengths are read until here)
     }
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
         if (i >= count) continue;
         if (need[i] > 0 && ends[first + i] > available) status[i] = kRowCacheFull;
-        else if (added[i] > 0) t.lengths[first + i] = length[i] + added[i];
+        if (added[i] > 0 && status[i] == kRowOk) t.lengths[first + i] = length[i] + added[i];
         if (p.row_status) p.row_status[first + i] = status[i];
     }
 }
