@@ -296,11 +296,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
             x[i] = lower;
         }
         const float2 two = best.floats();
-        const float next = fmaxf(two.x, two.y), base = next > kNone ? next : 0.0f;
+        // (Behind logits of -inf alone the lowest number, so that the factor of the empty sums is never above 1: 0 would make it infinite before a first logit of -89.)
+        const float base = fmaxf(fmaxf(two.x, two.y), -0x1.fffffep127f);
         const float less = fmaxf((level - base) * kLog2e, kLeast), factor = exp2_approx(less);
         weighted = mul_pair(fma_pair(make_float2(less, less), sum, weighted), make_float2(factor, factor));
         sum = mul_pair(sum, make_float2(factor, factor));
-        level = next;  // (not `base`: behind logits of -inf alone the factor of the empty sums is 0, where 0 less a base of -89 would make it infinite)
+        level = base;
         const auto add_up = [&](bool clamp) {
 #pragma unroll
             for (int i = 0; i < kWords; i += W::elements == 1 ? 2 : 1) {
