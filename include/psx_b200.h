@@ -557,8 +557,9 @@ PSX_API psx_status psx_b200_decode_attention_pages(psx_ctx* ctx, void* stream, c
  *                  PSX_ROW_ALL_REMOVED: every logit is -inf (results NaN, alternatives -inf, -1); PSX_ROW_BAD_TOKEN: the token is not in the
  *                  vocabulary (log_probs NaN, the rest as ever)
  * Logits of -inf have the probability 0.  Sums run over all logits but the largest, so that log-probabilities near 0 have their digits: with r the others'
- * sum relative to the largest and g nats between it and the second one, log(1 + r) is off by less than (200 + 2 g) 2^-24 of r / (1 + r), the entropy
- * by less than (400 + 4 g) 2^-24 of it; what is more than 87 nats below the largest counts nothing.  The same call gives the same bits.  Needs no scratch.
+ * sum relative to the largest and g nats between it and the second one, log(1 + r) is off by less than (100 + vocab / 400 + 2 g) 2^-24 of r / (1 + r), and by no more
+ * than (800 + 2 g) 2^-24 of it for any vocabulary, the entropy by less than twice as much of it; what is more than 87 nats below the largest counts nothing.  The same
+ * call gives the same bits.  Needs no scratch.
  * Limits: top <= 128, vocab <= 2^30 (else PSX_ERR_UNSUPPORTED).  Asynchronous on `stream`; the outputs must not overlap the inputs. */
 PSX_API psx_status psx_b200_token_log_probs(psx_ctx* ctx, void* stream, int32_t dtype, const void* logits, int64_t rows, int64_t vocab,
                                             int64_t row_stride, const int64_t* tokens, float* log_probs, float* entropy, int64_t top,

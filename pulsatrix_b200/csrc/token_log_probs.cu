@@ -33,6 +33,10 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMostGroups = 32;  // of a part's chunks
 constexpr int kLongVectors = 4;
 constexpr int kBlocks = 4;  // that an SM holds
+constexpr int kMostShort = 32;  // chunks of one vector
+// Chunks whose sums a thread holds as floats: of 294,912 logits, so that the vocabularies of today have no use for more (handing on costs 2 to 4 % of a row's time).
+template <class T>
+constexpr int kHandOn = 18 * sizeof(T);
 constexpr int kMostMaxima = (kMostTop + kWarps - 1) / kWarps + 2;  // of a warp
 constexpr int kList = 1024;
 constexpr int kMostParts = 16;  // of a row: a cluster's CTAs
@@ -146,8 +150,17 @@ struct Outcome {
     int status;
 };
 
+// A thread's sums of all chunks but the last few, relative to `level`.
+struct Held {
+    double sum[kThreads], weighted[kThreads];
+    float level[kThreads];
+};
+
 struct Shared {
-    alignas(16) uint64_t list[kList];  // what reaches the bound
+    union {
+        alignas(16) uint64_t list[kList];  // what reaches the bound
+        Held held;                         // before there is a list
+    };
     uint64_t best_of[kWarps], best[2];
     float4 record;         // the part's largest logit and its two sums
     Outcome outcome;       // the first part's, and the given token and its logit
@@ -179,6 +192,15 @@ __device__ __forceinline__ void relative_to(float high, bool first, float m, flo
     const float y = fmaxf((m - high) * kLog2e, kLeast), f = m > kNone ? exp2_approx(y) : 0.0f;
     weighted = (weighted + y * (1.0f + sum)) * f;
     sum = (1.0f + sum) * f;
+}
+
+// A thread's sums of some chunks, relative to `level`, go to those that it holds in double precision.
+__device__ __noinline__ void hand_on(Held& held, float level, float sum, float weighted) {
+    const int i = threadIdx.x;
+    const double less = fmax(((double)held.level[i] - (double)level) * 1.4426950408889634, -2000.0), factor = exp2(less);  // (2^-2000 is 0)
+    held.weighted[i] = (held.weighted[i] + less * held.sum[i]) * factor + (double)weighted;
+    held.sum[i] = held.sum[i] * factor + (double)sum;
+    held.level[i] = level;
 }
 
 // By one lane: the row's own results.
@@ -243,7 +265,8 @@ struct Cluster {
     }
 };
 
-template <class T, int vectors, bool picks, bool alone>
+// `many`: a part has more than kHandOn<T> chunks.
+template <class T, int vectors, bool picks, bool alone, bool many>
 __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(const __grid_constant__ TokenLogProbsParams p) {
     constexpr int E = 16 / sizeof(T), kChunk = kThreads * vectors * E, kWords = vectors * 4;
     using W = Word<T>;
@@ -326,6 +349,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
             add_up(true);
         }
     };
+    // Sums of floats lose a unit with every addition and two with every new largest: in rows of many chunks they go to sums in double precision time after time.
+    if constexpr (many) s.held.sum[threadIdx.x] = s.held.weighted[threadIdx.x] = 0.0, s.held.level[threadIdx.x] = kNone;
     // (Two chunks a turn, one in work and one on its way; unrolled further, the instructions come too late.)
     W w[2][kWords];
     load(0, w[0]);
@@ -340,11 +365,21 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
         take(c, w[0]);
         if (c + 2 < p.chunks) load(c + 2, w[0]);
         if (c + 1 < p.chunks) take(c + 1, w[1]);
+        if constexpr (many) {
+            if ((c + 2) % kHandOn<T> == 0) {
+                hand_on(s.held, level, sum.x + sum.y, weighted.x + weighted.y);
+                sum = weighted = make_float2(0.0f, 0.0f);
+            }
+        }
     }
     // The thread's own: the smaller of the two that are aside joins the sums.
     const float2 aside = best.floats();
     const float top = larger(aside.x, aside.y);
     float own = sum.x + sum.y, own_weighted = weighted.x + weighted.y;
+    if constexpr (many) {
+        hand_on(s.held, level, own, own_weighted);
+        own = (float)s.held.sum[threadIdx.x], own_weighted = (float)s.held.weighted[threadIdx.x];
+    }
     if constexpr (W::elements == 2) {
         const float y = fmaxf((smaller(aside.x, aside.y) - level) * kLog2e, kLeast), e = exp2_approx(y);
         own += e;
@@ -503,12 +538,12 @@ __global__ void __launch_bounds__(kThreads, kBlocks) token_log_probs_kernel(cons
     if (!alone) C::meets();  // (records, lists and the sweeps' best are read until then)
 }
 
-template <class T, int vectors, bool picks>
+template <class T, int vectors, bool picks, bool many>
 cudaError_t launch_with(const TokenLogProbsParams& p, cudaStream_t stream) {
     if (p.parts == 1) {
-        return launch_overlapping(token_log_probs_kernel<T, vectors, picks, true>, dim3((unsigned)p.rows), dim3(kThreads), 0, stream, p);
+        return launch_overlapping(token_log_probs_kernel<T, vectors, picks, true, many>, dim3((unsigned)p.rows), dim3(kThreads), 0, stream, p);
     }
-    const auto kernel = token_log_probs_kernel<T, vectors, picks, false>;
+    const auto kernel = token_log_probs_kernel<T, vectors, picks, false, many>;
     if (p.parts > 8) {  // (more than any device must hold)
         static OncePerDevice raised;
         int device = 0;
@@ -521,8 +556,9 @@ cudaError_t launch_with(const TokenLogProbsParams& p, cudaStream_t stream) {
 
 template <class T>
 cudaError_t launch_type(const TokenLogProbsParams& p, cudaStream_t stream) {
-    if (p.vectors == 1) return p.top > 0 ? launch_with<T, 1, true>(p, stream) : launch_with<T, 1, false>(p, stream);
-    return p.top > 0 ? launch_with<T, kLongVectors, true>(p, stream) : launch_with<T, kLongVectors, false>(p, stream);
+    if (p.vectors == 1) return p.top > 0 ? launch_with<T, 1, true, false>(p, stream) : launch_with<T, 1, false, false>(p, stream);
+    if (p.chunks > kHandOn<T>) return p.top > 0 ? launch_with<T, kLongVectors, true, true>(p, stream) : launch_with<T, kLongVectors, false, true>(p, stream);
+    return p.top > 0 ? launch_with<T, kLongVectors, true, false>(p, stream) : launch_with<T, kLongVectors, false, false>(p, stream);
 }
 
 }  // namespace
@@ -539,6 +575,7 @@ void plan_token_log_probs(TokenLogProbsParams& p, int sm_count) {
         const int64_t elements = kThreads * vectors * E, all = (p.vocab + E - 1 + elements - 1) / elements;
         for (int parts = 1; parts <= kMostParts; parts *= 2) {
             const int64_t each = (all + parts - 1) / parts;
+            if (vectors == 1 && each > kMostShort) continue;
             const double beside = std::max(1.0, (double)(p.rows * parts) / sm_count);
             if (parts > 1 && (each * (parts - 1) >= all || (parts == kMostParts && beside > 1.0))) continue;  // (a part would be empty)
             const double cost = each * chunk + chain + (parts > 1 ? 1.0 : 0.0) + (beside - 1.0) * (further + further_chunk * each);

@@ -1,7 +1,10 @@
-"""Log-probabilities of given tokens (psx_b200_token_log_probs) for rows that a thread takes in many steps: stretches that are masked ahead of low logits.
-Against the formula in double precision.
+"""Log-probabilities of given tokens (psx_b200_token_log_probs) for rows that a thread takes in many steps: stretches that are masked ahead of low logits, rows of
+millions of logits, and rows so long that a thread keeps one maximum for several steps.  Against the formula in double precision.
 
-Tolerance: that of test_gpu_token_log_probs.py."""
+Tolerance, in units u = 2^-24, as in test_gpu_token_log_probs.py but for what grows with the row: a term is off by 2 d + 4, d < 18 + g, and by ten joins and the sum of
+a pair.  A thread adds a pair for every 512 logits of its part, one unit each, and takes a factor for every 4096, two each; both rounded up to whole steps,
+18: less than 100 + vocab / 400 + 2 g together.  After at most 294,912 logits of a part its sums are handed on to sums in double precision (2^-53 each): 576 additions, 72
+factors, 800 + 2 g at most.  The entropy's second sum is off by as much again."""
 import numpy as np
 import pytest
 
@@ -11,6 +14,10 @@ import test_gpu_token_log_probs as score_test
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 TYPES = score_test.TYPES
+
+
+def _units(vocab):
+    return min(100 + vocab / 400, 800)
 
 
 def _check(logits, tokens, top):
@@ -27,10 +34,10 @@ def _check(logits, tokens, top):
         gap = (x - high).masked_fill_(x == -np.inf, 0.0)
         entropy = np.log1p(r) - float((weight * gap).sum()) / (1 + r)
         g, lost = min(high - second, 104.0), len(x) * 2.0 ** -126
-        slack = ((200 + 2 * g) * U * r + lost) / (1 + r)
+        slack = ((_units(len(x)) + 2 * g) * U * r + lost) / (1 + r)
         want = float(x[tokens[row]]) - high - np.log1p(r)
         assert abs(float(out["log_probs"][row]) - want) <= (slack + U * abs(want)) * (1 + 1e-9) + 1e-45 or want == float(out["log_probs"][row])
-        assert abs(float(out["entropy"][row]) - entropy) <= (401 + 4 * g) * U * entropy + 91 * lost + 1e-45
+        assert abs(float(out["entropy"][row]) - entropy) <= (2 * _units(len(x)) + 1 + 4 * g) * U * entropy + 91 * lost + 1e-45
         if top:
             values, best = torch.sort(x, descending=True, stable=True)
             values, best = values[:top], best[:top].masked_fill(values[:top] == -np.inf, -1)
@@ -94,3 +101,23 @@ def test_a_few_tokens_that_a_grammar_allows(dtype, rows):
     logits = score_test._tensor(x, dtype)
     tokens = torch.from_numpy(x.argmax(1)).cuda()
     _check(logits, tokens, 60)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("kind", ["equal", "rising", "falling", "small"])
+def test_rows_of_tens_of_millions(dtype, kind):
+    # (sums of floats alone lose hundreds of units in a row of equal terms)
+    import torch
+    vocab = 1 << 26
+    if kind == "equal":
+        x = torch.full((1, vocab), -1.0, device="cuda")
+        x[0, 12345] = 0.0
+    elif kind == "small":  # all others at one distance
+        x = torch.full((1, vocab), -0.7, device="cuda")
+        x[0, vocab - 1] = 0.0
+    else:
+        x = torch.linspace(0.0, 3.0, vocab, device="cuda")[None]
+        if kind == "falling":
+            x = x.flip(1)
+    x = x.contiguous().to(getattr(torch, dtype))
+    _check(x, torch.tensor([vocab // 2], device="cuda"), 3 if kind == "small" else 0)
