@@ -103,6 +103,32 @@ def test_a_few_tokens_that_a_grammar_allows(dtype, rows):
     _check(logits, tokens, 60)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(300, 600000), (1000, 270000), (1200, 320000), (1, 8400001), (5, 4200000)])
+@pytest.mark.parametrize("top", [1, 20, 128])
+def test_more_steps_than_a_thread_keeps_maxima_of(dtype, rows, vocab, top):
+    import torch
+    steps, parts = _plan(rows, vocab, dtype)
+    assert steps > 32
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (torch.randn(rows, vocab, generator=gen, device="cuda") * 3).to(getattr(torch, dtype))
+    x[::3, -7:] = 30.0    # (the best ones in the last group, which may be a part of one)
+    x[1::3] = x[1::3].clamp(max=1.0)  # thousands that are equal: the list overflows
+    tokens = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    some = torch.tensor(sorted({0, min(1, rows - 1), min(2, rows - 1), rows - 1}), device="cuda")
+    out = gh.ctx().token_log_probs(x, tokens, top=top, entropy=True)
+    few = gh.ctx().token_log_probs(x[some].contiguous(), tokens[some], top=top, entropy=True)  # (other plans, the same row)
+    assert (out["top_tokens"][some] == few["top_tokens"]).all()
+    for row in some.tolist():
+        best = torch.sort(x[row].float() + 0.0, descending=True, stable=True)[1][:top]
+        assert (out["top_tokens"][row] == best).all()
+    _check(x[some].contiguous(), tokens[some], top)
+    if rows > 100:  # every row's sums
+        lse = torch.cat([torch.logsumexp(part.double(), 1) for part in x.split(30)])
+        want = x.gather(1, tokens[:, None])[:, 0].double() - lse
+        assert ((out["log_probs"].double() - want).abs() <= (_units(vocab) + 6) * U + U * want.abs()).all()  # (r / (1 + r) < 1, g < 3)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("kind", ["equal", "rising", "falling", "small"])
 def test_rows_of_tens_of_millions(dtype, kind):
