@@ -535,9 +535,7 @@ template <class T, int dims, int tiles_of_rows>
 cudaError_t launch(const PagedAttentionParams& p, cudaStream_t stream) {
     constexpr size_t shared = shared_of(dims, tiles_of_rows, sizeof(T) == 4);
     void (*const kernel)(const PagedAttentionParams) = decode_attention_pages_kernel<T, dims, tiles_of_rows>;
-    if (shared > 40 << 10) {
-        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared)) return e;
-    }
+    static_assert(shared <= 40 << 10, "more than a kernel gets unasked");
     return launch_overlapping(kernel, dim3((unsigned)(paged_attention_counters(p) * p.pieces)), dim3(kThreads), shared, stream, p);
 }
 
