@@ -8,7 +8,10 @@
 // holds it, unless that would write over what one of them holds that got no page).  So beams share their prompt's pages, and following a beam moves table entries, four bytes per page and row, instead of the
 // cache.
 //
-// Bound by latency but for the copies, which run at HBM's rate (a thousand pages of 64 KB that move in four pools: 80 us, 6.7 TB/s).
+// Bound by latency but for the copies, which run at HBM's rate (a thousand pages of 64 KB that move in four pools: 80 us, 6.7 TB/s).  One block gives pages out, and
+// one pairs movers and free places, reading the references of a pool half of which is free: release and extension of 64 rows that ask for a page each take 10 us
+// with 16,384 pages, 21 with 81,920 and 129 with a million, a plan of moves 10, 35 and 383; rows that ask for none 6 whatever the pool.  Rows that part are compared with
+// all rows: 16 us for 512 of them, 460 for 4096, and 100 more where they are refused.
 #include "page_table.cuh"
 
 #include <algorithm>

@@ -4,7 +4,7 @@
 //     y = x / sqrt(mean(x^2) + eps) * w,   (u, v) -> (u cos a - v sin a, v cos a + u sin a) for pair j with a = position * frequency_j
 //
 // in floats, rounded once at the end.  The angle is taken in double precision, in quarter turns: position * frequency * 2 / pi less the
-// nearest whole number is what is left, an eighth of a turn at most, so that its rounding to a float counts 2^-26 quarter turns
+// nearest whole number is what is left, an eighth of a turn at most, pi / 4 radians, so that its rounding to a float counts 2^-25 radians at most,
 // however far the position is (in floats, an angle of 100,000 is off by up to 4e-3).
 //
 // A lane holds two runs of 16 bytes of a head (of 8, where half of the rotated dimensions is not a multiple of 16 bytes): one of both halves where pairs are

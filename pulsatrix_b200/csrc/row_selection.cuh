@@ -1,4 +1,4 @@
-// What the kernels share that look for the largest logits of rows and sum their exponentials (beam_select.cu, token_log_probs.cu).
+// What the kernels share that look for the largest logits of rows and sum their exponentials (beam_select.cu, token_log_probs.cu; warp_bound is beam_select's).
 #pragma once
 
 #include <stdint.h>

@@ -7,7 +7,7 @@
 // the thread's largest so far.  16-bit logits are compared in pairs as they come.
 //
 // The row is cut into 1 to 16 parts, the CTAs of a cluster; a thread takes up to four vectors of 16 bytes at a time, with the next ones on their way (two
-// instead of four: 220 us instead of 121 for 2048 rows of 151,936 bf16 logits).  The `top` best are found by a bound that at least `top` logits reach: each
+// instead of four: 220 us instead of 120 for 2048 rows of 151,936 bf16 logits).  The `top` best are found by a bound that at least `top` logits reach: each
 // part's is the top-th largest of its threads' largest, the row's the largest of those, or the smallest of what each part's share of them reaches.
 // A thread whose largest of some chunks reaches it looks at them again, out of L2, and puts what reaches the bound on its CTA's list; the first CTA brings the
 // lists together, and an entry's place is the number of keys above its own.  A list that overflows (thousands of equal logits) is replaced by `top` sweeps.
@@ -15,8 +15,8 @@
 // memory, joined by the part that ends last: 64 rows of 8000 logits, 20 alternatives, 12.4 us instead of 8.3.)
 //
 // Rows need not be aligned: vectors are those of memory, and where one is cut by an end of the row its elements are read one by one.  Bound by HBM, the
-// logits once, and nearly so by instructions for 16-bit logits, 9.2 for each: 2048 rows of 151,936 bf16 logits take 121 us (5.2 TB/s, issue slots 61 % busy;
-// 107 without alternatives), 1000 of 128,256 fp32 logits 92 (5.6 TB/s).
+// logits once, and nearly so by instructions for 16-bit logits, 9.0 for each: 2048 rows of 151,936 bf16 logits take 120 us when replayed (5.2 TB/s, issue slots 58 % busy;
+// 107 without alternatives; 133 on other logits every time), 1000 of 128,256 fp32 logits 93 (5.5 TB/s).
 #include "token_log_probs.cuh"
 
 #include <algorithm>
@@ -33,7 +33,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMostGroups = 32;  // of a part's chunks
 constexpr int kLongVectors = 4;
 constexpr int kBlocks = 4;  // that an SM holds
-constexpr int kMostShort = 32;  // chunks of one vector
+constexpr int kMostShort = 32;  // chunks of one vector that a part has at most: more are slower than a quarter as many of four by far
 // Chunks whose sums a thread holds as floats: of 294,912 logits, so that the vocabularies of today have no use for more (handing on costs 2 to 4 % of a row's time).
 template <class T>
 constexpr int kHandOn = 18 * sizeof(T);
