@@ -33,7 +33,10 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMostGroups = 32;  // of a part's chunks
 constexpr int kLongVectors = 4;
 constexpr int kBlocks = 4;  // that an SM holds
-constexpr int kMostShort = 32;  // chunks of one vector that a part has at most: more are slower than a quarter as many of four by far
+// Chunks of one vector that a part has at most, and where rows come in several rounds of an SM's CTAs: there more are slower than a quarter as many of four vectors,
+// whatever their chains (in us, with chunks of one vector and of four: 600 rows of 12,000 fp32 logits, twelve chunks, 14.4 and 16.5; 2000 rows of 8000, eight, 26.8 and
+// 28.1, of 12,000, twelve, 37 and 33; 8000 rows of 16,000 164 and 132, of 50,257 453 and 271; 8000 of 32,000 bf16 logits, sixteen, 191 and 169, of 151,936 815 and 433).
+constexpr int kMostShort = 32, kMostShortInRounds = 8;
 // Chunks whose sums a thread holds as floats: of 294,912 logits, so that the vocabularies of today have no use for more (handing on costs 2 to 4 % of a row's time).
 template <class T>
 constexpr int kHandOn = 18 * sizeof(T);
@@ -575,8 +578,8 @@ void plan_token_log_probs(TokenLogProbsParams& p, int sm_count) {
         const int64_t elements = kThreads * vectors * E, all = (p.vocab + E - 1 + elements - 1) / elements;
         for (int parts = 1; parts <= kMostParts; parts *= 2) {
             const int64_t each = (all + parts - 1) / parts;
-            if (vectors == 1 && each > kMostShort) continue;
             const double beside = std::max(1.0, (double)(p.rows * parts) / sm_count);
+            if (vectors == 1 && each > (beside > 2.0 * kBlocks ? kMostShortInRounds : kMostShort)) continue;
             if (parts > 1 && (each * (parts - 1) >= all || (parts == kMostParts && beside > 1.0))) continue;  // (a part would be empty)
             const double cost = each * chunk + chain + (parts > 1 ? 1.0 : 0.0) + (beside - 1.0) * (further + further_chunk * each);
             if (least == 0.0 || cost < least) least = cost, p.parts = parts, p.vectors = vectors, p.chunks = (int)each;

@@ -57,7 +57,7 @@ def _plan(rows, vocab, dtype):
         steps = -(-(vocab + elements - 1) // (256 * vectors * elements))
         for parts in (1, 2, 4, 8, 16):
             each, beside = -(-steps // parts), max(1.0, rows * parts / 148)
-            if parts > 1 and (each * (parts - 1) >= steps or (parts == 16 and beside > 1.0)):
+            if vectors == 1 and each > (8 if beside > 8.0 else 32) or parts > 1 and (each * (parts - 1) >= steps or (parts == 16 and beside > 1.0)):
                 continue
             cost = each * chunk + chain + (parts > 1) + (beside - 1.0) * (further + 0.09 * vectors * each)
             if least is None or cost < least[0]:
