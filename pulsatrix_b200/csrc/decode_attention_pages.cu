@@ -17,8 +17,8 @@
 // while this one's values are in work (without: 283 us instead of 257 for 64 rows x 8 kv heads of up to 8191 positions of 128); the last block of
 // a pair to end joins the pieces, in order.  (Pieces as the CTAs of a cluster, joined over its shared memory: 12 x 16 fp32 pairs of up to 1999 positions 42 us
 // instead of 37, 13 x 4 of up to 5997 47 instead of 34.  Pieces of equal length over all rows, which every block works out from the lengths: 39 and 35.)
-// Bound by HBM, the keys and values that are seen, once: that call reads at 6.3 TB/s when it is replayed on the same inputs (258 us; a plain copy runs at 6.5), and at 5.9
-// on other inputs every time (275 us); short caches by the chain from a row's length over its pages to the join, some 9 us.
+// Bound by HBM, the keys and values that are seen, once: that call reads at 6.3 TB/s when it is replayed on the same inputs (258 us; a plain copy runs at 6.5), and at 5.9 to 6.3
+// on other inputs every time (260 to 275 us, by the machine); short caches by the chain from a row's length over its pages to the join, some 9 us.
 #include "decode_attention_pages.cuh"
 
 #include <algorithm>

@@ -16,7 +16,7 @@
 //
 // Rows need not be aligned: vectors are those of memory, and where one is cut by an end of the row its elements are read one by one.  Bound by HBM, the
 // logits once, and nearly so by instructions for 16-bit logits, 9.0 for each: 2048 rows of 151,936 bf16 logits take 120 us when replayed (5.2 TB/s, issue slots 58 % busy;
-// 107 without alternatives; 133 on other logits every time), 1000 of 128,256 fp32 logits 93 (5.5 TB/s).
+// 107 without alternatives; 124 to 133, by the machine, on other logits every time), 1000 of 128,256 fp32 logits 93 (5.5 TB/s).
 #include "token_log_probs.cuh"
 
 #include <algorithm>
